@@ -293,6 +293,31 @@ int rlxq_quantize_act_int8(rlxq_ctx* ctx, const void* x, int x_dtype,
                            int64_t m, int64_t k, int8_t* q, float* scales,
                            void* stream);
 
+/* Rows of floats to MXFP4 (RLXQ_MLX_MXFP4 operands, E8M0 scale bytes): x
+ * [m, k] f32 or bf16 -> codes [m, k/2], scales [m, k/32], by the reference
+ * encoder's rule (crates/rlx-models-core/src/mxfp4_pack.rs:64-128, 196-250):
+ * a block of 32 takes the smallest power of two whose sixfold reaches its
+ * largest magnitude, and each element the nearest E2M1 value of its quotient,
+ * ties to the even mantissa.  A block of zeros, or one with an infinity or a
+ * NaN, has scale 1; what is not finite becomes +-6.  K % 32 == 0; x and codes
+ * 16-byte aligned.  With m = 0 nothing is read or written. */
+int rlxq_quantize_mxfp4(rlxq_ctx* ctx, const void* x, int x_dtype, int64_t m,
+                        int64_t k, uint8_t* codes, uint8_t* scales,
+                        void* stream);
+
+/* MXFP4 x MXFP4 matmul (W4A4): y[m, n] = sum_k Q(x)[m, k] * W[n, k], W as
+ * MXFP4 codes [n, k/2] and E8M0 scales [n, k/32] with the values that
+ * rlxq_dequantize gives them, x quantised on the fly by the rule of
+ * rlxq_quantize_mxfp4, on the scaled FP4 MFMA with f32 accumulation.  The
+ * reference computes MXFP4 linears on float activations
+ * (rlxq_dequant_matmul); this is the form with 4-bit activations, beside
+ * rlxq_w8a8_gemm.  A row of x with an infinity or a NaN gives NaN outputs
+ * (rather than the +-6 its codes would hold).  K % 32 == 0, K <= 2^24; x and w
+ * 16-byte aligned. */
+int rlxq_mxfp4_gemm(rlxq_ctx* ctx, const void* x, int x_dtype,
+                    const uint8_t* w, const uint8_t* w_scales, int64_t m,
+                    int64_t k, int64_t n, void* y, int y_dtype, void* stream);
+
 /* Dequantize `rows` packed rows of K weights to f32 [rows, K] with the same
  * arithmetic the kernels use (bit-exact against the CPU codec).  GGUF and
  * MLX schemes; MLX takes scales/biases as in rlxq_dequant_matmul. */

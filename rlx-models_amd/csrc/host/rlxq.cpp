@@ -51,6 +51,7 @@ RLXQ_EMBED(rlxq_co_bsgemm0, "bsgemm0.co")
 RLXQ_EMBED(rlxq_co_bsgemm1, "bsgemm1.co")
 RLXQ_EMBED(rlxq_co_bsgemm2, "bsgemm2.co")
 RLXQ_EMBED(rlxq_co_mfgemv, "mfgemv.co")
+RLXQ_EMBED(rlxq_co_mxfp4, "mxfp4.co")
 
 namespace {
 
@@ -80,6 +81,7 @@ const Image kImages[] = {
     {rlxq_co_bsgemm1_begin, rlxq_co_bsgemm1_end, "bsgemm1"},
     {rlxq_co_bsgemm2_begin, rlxq_co_bsgemm2_end, "bsgemm2"},
     {rlxq_co_mfgemv_begin, rlxq_co_mfgemv_end, "mfgemv"},
+    {rlxq_co_mxfp4_begin, rlxq_co_mxfp4_end, "mxfp4"},
 };
 
 std::string hip_msg(hipError_t e) { return std::string(hipGetErrorName(e)) + ": " + hipGetErrorString(e); }

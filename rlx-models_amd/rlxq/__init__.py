@@ -89,6 +89,8 @@ def lib() -> C.CDLL:
         "rlxq_swiglu": (I, [P, P, I, I64, I64, P, I, P]),
         "rlxq_w8a8_gemm": (I, [P, P, I, P, P, I64, I64, I64, P, I, P]),
         "rlxq_quantize_act_int8": (I, [P, P, I, I64, I64, P, P, P]),
+        "rlxq_quantize_mxfp4": (I, [P, P, I, I64, I64, P, P, P]),
+        "rlxq_mxfp4_gemm": (I, [P, P, I, P, P, I64, I64, I64, P, I, P]),
         "rlxq_dequantize": (I, [P, I, I, P, P, P, I, I64, I64, P, P]),
         "rlxq_dm_try_new": (I, [I, C.POINTER(P)]),
         "rlxq_dm_free": (None, [P]),
@@ -336,6 +338,36 @@ def check_w8a8(x, wq, w_scale, n: int, *, y=None, device=None) -> None:
         _on_device(device, x=x, wq=wq, w_scale=w_scale, y=y)
 
 
+def check_quantize_mxfp4(x, codes, scales, *, device=None) -> None:
+    import torch
+
+    _tensor(x, "quantize_mxfp4: x", _act_dtypes(), 2)
+    m, k = x.shape
+    _need(k > 0 and k % 32 == 0, f"quantize_mxfp4: K = {k} is not a multiple of 32")
+    for nm, t, per in (("codes", codes, 2), ("scales", scales, 32)):
+        if t is not None:
+            _tensor(t, f"quantize_mxfp4: {nm}", (torch.uint8,), 2)
+            _need(tuple(t.shape) == (m, k // per), f"quantize_mxfp4: {nm} has shape {tuple(t.shape)}, expected {(m, k // per)}")
+    if device is not None:
+        _on_device(device, x=x, codes=codes, scales=scales)
+
+
+def check_mxfp4_gemm(x, w, w_scales, n: int, *, y=None, device=None) -> None:
+    import torch
+
+    _tensor(x, "mxfp4_gemm: x", _act_dtypes(), 2)
+    m, k = x.shape
+    _need(k > 0 and k % 32 == 0, f"mxfp4_gemm: K = {k} is not a multiple of 32")
+    for nm, t, per in (("w", w, 2), ("w_scales", w_scales, 32)):
+        _tensor(t, f"mxfp4_gemm: {nm}", (torch.uint8,))
+        _need(t.numel() >= n * (k // per),
+              f"mxfp4_gemm: {nm} has {t.numel()} B, [N={n}, {k // per}] needs {n * (k // per)}")
+    if y is not None:
+        _check_out(y, (m, n), "mxfp4_gemm")
+    if device is not None:
+        _on_device(device, x=x, w=w, w_scales=w_scales, y=y)
+
+
 class Context:
     """Owns an rlxq_ctx on one device (rlxq_init / rlxq_destroy)."""
 
@@ -529,6 +561,34 @@ class Context:
         rc = lib().rlxq_quantize_act_int8(self.h, _ptr(x), _dt(x), m, k, _ptr(q), _ptr(s), _stream(stream))
         self._check(rc, "quantize_act_int8")
         return q, s
+
+    def quantize_mxfp4(self, x, *, codes=None, scales=None, stream=None):
+        """x [m, k] as MXFP4: codes [m, k/2] and E8M0 scales [m, k/32] (uint8)."""
+        import torch
+
+        check_quantize_mxfp4(x, codes, scales, device=self.device)
+        m, k = x.shape
+        if codes is None:
+            codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
+        if scales is None:
+            scales = torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
+        rc = lib().rlxq_quantize_mxfp4(self.h, _ptr(x), _dt(x), m, k, _ptr(codes), _ptr(scales), _stream(stream))
+        self._check(rc, "quantize_mxfp4")
+        return codes, scales
+
+    def mxfp4_gemm(self, x, w, w_scales, n: int, *, y=None, y_dtype=None, stream=None):
+        """y[m, n] = Q(x) . W^T: MXFP4 weights on activations quantised to
+        MXFP4 in the call; returns y (allocated if not given)."""
+        import torch
+
+        check_mxfp4_gemm(x, w, w_scales, n, y=y, device=self.device)
+        m, k = x.shape
+        if y is None:
+            y = torch.empty((m, n), dtype=y_dtype or torch.float32, device=x.device)
+        rc = lib().rlxq_mxfp4_gemm(self.h, _ptr(x), _dt(x), _ptr(w), _ptr(w_scales), m, k, n, _ptr(y), _dt(y),
+                                   _stream(stream))
+        self._check(rc, "mxfp4_gemm")
+        return y
 
     def w8a8_gemm(self, x, wq, w_scale, n: int, *, y=None, y_dtype=None, stream=None):
         import torch

@@ -132,3 +132,21 @@ def test_packed_row_bytes():
     assert rlxq.packed_row_bytes(rlxq.MLX_MXFP4, 4096) == 2048
     assert rlxq.packed_row_bytes(rlxq.GGUF_Q4_K, 4096) == 2304
     assert rlxq.packed_row_bytes(Q4_1, 100) == -1
+
+
+def test_mxfp4_quantize_and_gemm_checks():
+    x = torch.zeros((2, 64))
+    rlxq.check_quantize_mxfp4(x, _u8(64).view(2, 32), _u8(4).view(2, 2))
+    rlxq.check_mxfp4_gemm(x, _u8(8 * 32), _u8(16), 8, y=torch.zeros((2, 8)))
+    for bad in ((x[:, :48].contiguous(), None, None), (x.half(), None, None), (x[:, ::2], None, None),
+                (x, _u8(60).view(2, 30), None), (x, None, _u8(6).view(2, 3)), (x, torch.zeros((2, 32)), None)):
+        with pytest.raises(ValueError):
+            rlxq.check_quantize_mxfp4(*bad)
+    for bad in ((x, _u8(8 * 32 - 1), _u8(16), 8), (x, _u8(8 * 32), _u8(15), 8), (x, _u8(8 * 32), None, 8),
+                (x, torch.zeros(256), _u8(16), 8), (x.view(128), _u8(256), _u8(16), 8)):
+        with pytest.raises(ValueError):
+            rlxq.check_mxfp4_gemm(*bad)
+    with pytest.raises(ValueError, match="y has shape"):
+        rlxq.check_mxfp4_gemm(x, _u8(8 * 32), _u8(16), 8, y=torch.zeros((2, 9)))
+    with pytest.raises(ValueError, match="context is on cuda:0"):
+        rlxq.check_mxfp4_gemm(x, _u8(8 * 32), _u8(16), 8, device=0)

@@ -272,6 +272,35 @@ int rlxq_moe_route(rlxq_ctx* ctx, const float* logits, int64_t rows,
                    int64_t num_experts, int64_t top_k, int renorm,
                    int32_t* ids, float* probs, void* stream);
 
+/* The whole routed-expert layer in one call, from the rows to the weighted
+ * sum (the layer of rlxq_moe_route and two rlxq_moe_grouped calls, with the
+ * router's own product in front):
+ *   l[r, e] = sum_h x[r, h] * router[e, h], summed in f64 and rounded to f32;
+ *   the top_k largest logits of a row (ties to the lower expert) with their
+ *     softmax weights over all experts, renormalised over the kept ones if
+ *     renorm (standard_decoder.rs:12612-12760);
+ *   y[r] = sum_j p[r, j] * down[e] . (silu(gate[e] . x[r]) * (up[e] . x[r])).
+ * x [rows, hidden]; router [num_experts, hidden] f32 or bf16, or NULL with
+ * logits [rows, num_experts] f32 of the caller's (exactly one of the two);
+ * gate_up: num_experts slabs of gate rows [0, inter) then up rows
+ * [inter, 2 inter) over hidden; down: slabs [hidden, inter], each of its own
+ * scheme: GGUF (scales NULL), or RLXQ_MLX_MXFP4 with E8M0 byte scales
+ * [num_experts, rows of a slab, K/32].  y [rows, hidden].  ids / probs
+ * [rows, top_k] receive the routing, or are NULL.
+ * A row whose logits hold a NaN or +inf, or nothing but -inf, has no softmax:
+ * its y is NaN (ids 0 .. top_k - 1, probs NaN); -inf alone masks an expert.
+ * num_experts <= 1024, top_k <= min(num_experts, 64); hidden and inter as the
+ * schemes' K; x and router 16-byte aligned.  With rows = 0 nothing is read or
+ * written. */
+int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype,
+                   const void* router, int router_dtype, const float* logits,
+                   int gate_up_scheme, const void* gate_up,
+                   const void* gate_up_scales, int down_scheme,
+                   const void* down, const void* down_scales, int64_t rows,
+                   int64_t hidden, int64_t inter, int64_t num_experts,
+                   int64_t top_k, int renorm, int32_t* ids, float* probs,
+                   void* y, int y_dtype, void* stream);
+
 /* SwiGLU between the fused gate|up projection and down: for each row,
  * out[i] = silu(gu[i]) * gu[inter + i], gu [rows, 2*inter] -> out [rows, inter]
  * (crates/rlx-laguna/src/device_matmul.rs:383-426 GroupedSwiglu graph). */

@@ -26,11 +26,14 @@ bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p
 
 // Table + grouped GEMV (+ combine).  `ids` (int32) or `idx` (f32) give the
 // expert of each of the n entries; entry i reads activation row i / x_div.
+// The call's scratch starts ws_base bytes into the workspace (a caller that
+// keeps data of its own there has sized the workspace for both: need != NULL
+// only reports the bytes behind ws_base, and launches nothing).
 int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const void* x, int x_dtype,
                 const void* bank, const void* scales, const void* biases, int sb_dtype, const int32_t* ids,
                 const float* idx, int64_t n_entries, int64_t x_rows, int32_t x_div, int64_t k, int64_t n,
                 int64_t num_experts, void* y, int y_dtype, const float* probs, int64_t rows, int32_t top_k,
-                bool swiglu, void* stream) {
+                bool swiglu, void* stream, size_t ws_base = 0, size_t* need = nullptr) {
   if (!x || !bank || !y || (!ids && !idx)) return fail(ctx, RLXQ_E_NULL, std::string(what) + ": null pointer");
   if (k <= 0 || n < 0 || n_entries < 0 || x_rows < 0) return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": bad sizes");
   if (num_experts <= 0 || num_experts > 1024)
@@ -177,6 +180,10 @@ int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const vo
   bool xc = combine && xr && fused && top_k <= 8 && x_div == 1 && rows <= 0x7fffffff;
   if (const char* ev = std::getenv("RLXQ_MOE_COMBINE"))
     if (!std::strcmp(ev, "launch") || !std::strcmp(ev, "fused")) xc = false;
+  if (xc && need) {
+    *need = 0;
+    return RLXQ_OK;
+  }
   if (xc) {
     int64_t tc = 128;
     if (const char* ev = std::getenv("RLXQ_MOE_XC_TILE")) tc = std::max<int64_t>(16, std::min<int64_t>(1024, std::atoi(ev)));
@@ -263,7 +270,12 @@ int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const vo
   const size_t sum_bytes = sk ? r256((size_t)sk_xr * (bs ? bs_nu * 8 : k / 32) * 4) : 0;   // block sums of the x16 rows
   const size_t total_ws = table_bytes + tmp_bytes + cmap_bytes + emap_bytes + x16_bytes + is_bytes + sum_bytes;
   void* ws = nullptr;
-  if (total_ws && (rc = workspace(ctx, total_ws, &ws, stream))) return rc;
+  if (need) {
+    *need = total_ws;
+    return RLXQ_OK;
+  }
+  if (total_ws && (rc = workspace(ctx, ws_base + total_ws, &ws, stream))) return rc;
+  if (ws) ws = static_cast<char*>(ws) + ws_base;
   int32_t* table = fused || sk ? nullptr : static_cast<int32_t*>(ws);
   float* tmp = combine ? reinterpret_cast<float*>(static_cast<char*>(ws) + table_bytes) : nullptr;
   char* skb = static_cast<char*>(ws) + table_bytes + tmp_bytes;
@@ -478,6 +490,110 @@ int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const vo
   return RLXQ_OK;
 }
 
+// ---- the whole expert layer (rlxq_moe_layer) ------------------------------
+struct LayerCall {
+  const void* x;
+  int x_dtype;
+  const void* router;
+  int router_dtype;
+  const float* logits;
+  int gu_scheme;
+  const void *gu, *gu_s;
+  int d_scheme;
+  const void *d, *d_s;
+  int64_t rows, hidden, inter, experts, top_k;
+  int renorm;
+  int32_t* ids;
+  float* probs;
+  void* y;
+  int y_dtype;
+};
+
+bool layer_scheme(int s) { return is_gguf(s) || kquant_bytes(s) > 0 || s == RLXQ_MLX_MXFP4; }
+
+// Logits of the router product (f64 sums): a wave per expert and four rows,
+// or per four experts and eight rows where that still gives a wave to each
+// SIMD (fewer reads per product).
+int layer_logits(rlxq_ctx* ctx, const LayerCall& c, float* logits, void* stream) {
+  rlxq_moe_logits_args a;
+  std::memset(&a, 0, sizeof a);
+  a.x = c.x;
+  a.router = c.router;
+  a.logits = logits;
+  a.rows = c.rows;
+  a.H = c.hidden;
+  a.E = (int32_t)c.experts;
+  const bool big = ((c.experts + 3) / 4) * ((c.rows + 7) / 8) >= 1024;
+  char name[64];
+  std::snprintf(name, sizeof name, "rlxq_moe_logits_%s_%s_%s", c.x_dtype == RLXQ_BF16 ? "bf16" : "f32",
+                c.router_dtype == RLXQ_BF16 ? "bf16" : "f32", big ? "e4r8" : "e1r4");
+  hipFunction_t fn;
+  int rc = get_fn(ctx, name, &fn);
+  if (rc) return rc;
+  const int64_t gx = big ? (c.experts + 3) / 4 : c.experts, gy = big ? (c.rows + 7) / 8 : (c.rows + 3) / 4;
+  void* args[] = {&a};
+  return launch(ctx, fn, dim3((unsigned)gx, (unsigned)gy), dim3(64), 0, stream, args, name);
+}
+
+int layer_pick(rlxq_ctx* ctx, const LayerCall& c, const float* logits, int32_t* ids, float* probs, void* stream) {
+  rlxq_moe_pick_args a;
+  std::memset(&a, 0, sizeof a);
+  a.logits = logits;
+  a.ids = ids;
+  a.probs = probs;
+  a.rows = c.rows;
+  a.E = (int32_t)c.experts;
+  a.top_k = (int32_t)c.top_k;
+  a.renorm = c.renorm;
+  const int nper = c.experts <= 64 ? 1 : c.experts <= 128 ? 2 : c.experts <= 256 ? 4 : 16;
+  char name[32];
+  std::snprintf(name, sizeof name, "rlxq_moe_pick_k%d", nper);
+  hipFunction_t fn;
+  int rc = get_fn(ctx, name, &fn);
+  if (rc) return rc;
+  void* args[] = {&a};
+  return launch(ctx, fn, dim3((unsigned)c.rows), dim3(64), 0, stream, args, name);
+}
+
+// The layer from the library's own calls: router product, top-k, grouped
+// gate|up + SwiGLU, grouped down + weighted sum.  The activations between the
+// two grouped products have x's type (bf16 ones are what the grouped register
+// and MFMA kernels take; the layer's few-token kernels keep them in f32).
+int layer_grouped(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
+  auto r256 = [](size_t b) { return (b + 255) & ~size_t(255); };
+  const size_t n = (size_t)(c.rows * c.top_k), xs = c.x_dtype == RLXQ_BF16 ? 2 : 4;
+  const size_t b_log = c.logits ? 0 : r256((size_t)(c.rows * c.experts) * 4), b_ids = r256(n * 4), b_pr = r256(n * 4);
+  const size_t b_act = r256(n * (size_t)c.inter * xs), base = b_log + b_ids + b_pr + b_act;
+  const char* what = "moe_layer";
+  auto gate_up = [&](void* act, const int32_t* ids, size_t* need) {
+    return grouped_run(ctx, what, c.gu_scheme, 32, c.x, c.x_dtype, c.gu, c.gu_s, nullptr, RLXQ_U8, ids, nullptr,
+                       (int64_t)n, c.rows, (int32_t)c.top_k, c.hidden, 2 * c.inter, c.experts, act, c.x_dtype, nullptr,
+                       c.rows, (int32_t)c.top_k, true, stream, base, need);
+  };
+  auto down = [&](const void* act, const int32_t* ids, const float* probs, size_t* need) {
+    return grouped_run(ctx, what, c.d_scheme, 32, act, c.x_dtype, c.d, c.d_s, nullptr, RLXQ_U8, ids, nullptr, (int64_t)n,
+                       (int64_t)n, 1, c.inter, c.hidden, c.experts, c.y, c.y_dtype, probs, c.rows, (int32_t)c.top_k,
+                       false, stream, base, need);
+  };
+  // (any non-null pointers: sizes only)
+  alignas(16) static const char dummy[16] = {};
+  size_t n1 = 0, n2 = 0;
+  int rc;
+  if ((rc = gate_up(const_cast<char*>(dummy), reinterpret_cast<const int32_t*>(dummy), &n1))) return rc;
+  if ((rc = down(dummy, reinterpret_cast<const int32_t*>(dummy), reinterpret_cast<const float*>(dummy), &n2))) return rc;
+  void* ws = nullptr;
+  if ((rc = workspace(ctx, base + std::max(n1, n2), &ws, stream))) return rc;
+  char* p = static_cast<char*>(ws);
+  float* logits = reinterpret_cast<float*>(p);
+  int32_t* ids = c.ids ? c.ids : reinterpret_cast<int32_t*>(p + b_log);
+  float* probs = c.probs ? c.probs : reinterpret_cast<float*>(p + b_log + b_ids);
+  void* act = p + b_log + b_ids + b_pr;
+  if (!c.logits && (rc = layer_logits(ctx, c, logits, stream))) return rc;
+  if ((rc = layer_pick(ctx, c, c.logits ? c.logits : logits, ids, probs, stream))) return rc;
+  if ((rc = gate_up(act, ids, nullptr))) return rc;
+  return down(act, ids, probs, nullptr);
+}
+
 }  // namespace
 
 }  // namespace rlxq
@@ -521,6 +637,45 @@ int rlxq_moe_grouped(rlxq_ctx* ctx, int scheme, int mode, const void* x, int x_d
                        false, stream);
   }
   return fail(ctx, RLXQ_E_SHAPE, "moe_grouped: mode must be EXPAND, COMBINE or EXPAND_SWIGLU");
+}
+
+int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype, const void* router, int router_dtype,
+                   const float* logits, int gate_up_scheme, const void* gate_up, const void* gate_up_scales,
+                   int down_scheme, const void* down, const void* down_scales, int64_t rows, int64_t hidden,
+                   int64_t inter, int64_t num_experts, int64_t top_k, int renorm, int32_t* ids, float* probs, void* y,
+                   int y_dtype, void* stream) {
+  if (!ctx) return RLXQ_E_NULL;
+  ctx->last_error.clear();
+  if ((router != nullptr) == (logits != nullptr))
+    return fail(ctx, RLXQ_E_NULL, "moe_layer: exactly one of router and logits");
+  // with no rows nothing is read or written: x and y may be NULL then
+  if (!gate_up || !down || (rows > 0 && (!x || !y))) return fail(ctx, RLXQ_E_NULL, "moe_layer: null pointer");
+  if (!layer_scheme(gate_up_scheme) || !layer_scheme(down_scheme))
+    return fail(ctx, RLXQ_E_SCHEME, "moe_layer: GGUF schemes and MXFP4 only");
+  if (rows < 0 || hidden <= 0 || inter <= 0 || hidden > (1 << 24) || inter > (1 << 24))
+    return fail(ctx, RLXQ_E_SHAPE, "moe_layer: need rows >= 0, 0 < hidden, inter <= 2^24");
+  if (num_experts <= 0 || num_experts > 1024 || top_k <= 0 || top_k > num_experts || top_k > 64)
+    return fail(ctx, RLXQ_E_SHAPE, "moe_layer: need 0 < top_k <= min(num_experts, 64), num_experts <= 1024");
+  if (rows * top_k > ((int64_t)1 << 28)) return fail(ctx, RLXQ_E_SHAPE, "moe_layer: too many rows");
+  if (x_dtype != RLXQ_F32 && x_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, "moe_layer: x_dtype");
+  if (y_dtype != RLXQ_F32 && y_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, "moe_layer: y_dtype");
+  if (router && router_dtype != RLXQ_F32 && router_dtype != RLXQ_BF16)
+    return fail(ctx, RLXQ_E_DTYPE, "moe_layer: router_dtype");
+  int64_t rb;
+  int rc;
+  if ((rc = check_weights(ctx, "moe_layer gate_up", gate_up_scheme, 32, gate_up, gate_up_scales, nullptr, RLXQ_U8, hidden,
+                          &rb)))
+    return rc;
+  if ((rc = check_weights(ctx, "moe_layer down", down_scheme, 32, down, down_scales, nullptr, RLXQ_U8, inter, &rb)))
+    return rc;
+  if (!aligned(x, 16) || !aligned(router, 16))
+    return fail(ctx, RLXQ_E_ALIGN, "moe_layer: x and router must be 16-byte aligned");
+  if (rows == 0) return RLXQ_OK;
+  DeviceGuard g(ctx->device);
+  if (!g.ok()) return fail(ctx, RLXQ_E_HIP, "moe_layer: hipSetDevice");
+  const LayerCall c{x,        x_dtype, router, router_dtype, logits, gate_up_scheme, gate_up, gate_up_scales, down_scheme,
+                    down,     down_scales, rows, hidden, inter, num_experts, top_k, renorm, ids, probs, y, y_dtype};
+  return layer_grouped(ctx, c, stream);
 }
 
 }  // extern "C"

@@ -52,6 +52,7 @@ RLXQ_EMBED(rlxq_co_bsgemm1, "bsgemm1.co")
 RLXQ_EMBED(rlxq_co_bsgemm2, "bsgemm2.co")
 RLXQ_EMBED(rlxq_co_mfgemv, "mfgemv.co")
 RLXQ_EMBED(rlxq_co_mxfp4, "mxfp4.co")
+RLXQ_EMBED(rlxq_co_moelayer, "moelayer.co")
 
 namespace {
 
@@ -82,6 +83,7 @@ const Image kImages[] = {
     {rlxq_co_bsgemm2_begin, rlxq_co_bsgemm2_end, "bsgemm2"},
     {rlxq_co_mfgemv_begin, rlxq_co_mfgemv_end, "mfgemv"},
     {rlxq_co_mxfp4_begin, rlxq_co_mxfp4_end, "mxfp4"},
+    {rlxq_co_moelayer_begin, rlxq_co_moelayer_end, "moelayer"},
 };
 
 std::string hip_msg(hipError_t e) { return std::string(hipGetErrorName(e)) + ": " + hipGetErrorString(e); }

@@ -90,4 +90,22 @@ typedef struct rlxq_moe_sk_args {
   const float* ssum;      /* block sums of x16 (min / bias formats)       */
 } rlxq_moe_sk_args;
 
+/* Whole expert layer (rlxq_moe_layer).  Router product: logits [rows, E].   */
+typedef struct rlxq_moe_logits_args {
+  const void* x;          /* [rows, H] f32 or bf16                         */
+  const void* router;     /* [E, H] f32 or bf16                            */
+  float* logits;
+  int64_t rows, H;
+  int32_t E, pad;
+} rlxq_moe_logits_args;
+
+/* Top-k of the logits and their softmax weights.                            */
+typedef struct rlxq_moe_pick_args {
+  const float* logits;
+  int32_t* ids;           /* [rows, top_k]                                 */
+  float* probs;           /* [rows, top_k]                                 */
+  int64_t rows;
+  int32_t E, top_k, renorm, pad;
+} rlxq_moe_pick_args;
+
 #endif

@@ -86,6 +86,7 @@ def lib() -> C.CDLL:
         "rlxq_dequant_grouped_matmul": (I, [P, I, I, P, I, P, P, P, I, P, I64, I64, I64, I64, P, I, P]),
         "rlxq_moe_grouped": (I, [P, I, I, P, I, P, P, P, I64, I64, I64, I64, I64, P, I, P]),
         "rlxq_moe_route": (I, [P, P, I64, I64, I64, I, P, P, P]),
+        "rlxq_moe_layer": (I, [P, P, I, P, I, P, I, P, P, I, P, P, I64, I64, I64, I64, I64, I, P, P, P, I, P]),
         "rlxq_swiglu": (I, [P, P, I, I64, I64, P, I, P]),
         "rlxq_w8a8_gemm": (I, [P, P, I, P, P, I64, I64, I64, P, I, P]),
         "rlxq_quantize_act_int8": (I, [P, P, I, I64, I64, P, P, P]),
@@ -338,6 +339,38 @@ def check_w8a8(x, wq, w_scale, n: int, *, y=None, device=None) -> None:
         _on_device(device, x=x, wq=wq, w_scale=w_scale, y=y)
 
 
+def check_moe_layer(x, router, gate_up, down, gate_up_scheme: int, down_scheme: int, top_k: int, inter: int,
+                    num_experts: int, *, logits=None, gate_up_scales=None, down_scales=None, ids=None, probs=None,
+                    y=None, device=None) -> None:
+    import torch
+
+    _tensor(x, "moe_layer: x", _act_dtypes(), 2)
+    rows, hidden = x.shape
+    _need((router is None) != (logits is None), "moe_layer: exactly one of router and logits")
+    _need(num_experts > 0 and 0 < top_k <= num_experts and inter > 0,
+          "moe_layer: need num_experts > 0, 0 < top_k <= num_experts, inter > 0")
+    if router is not None:
+        _tensor(router, "moe_layer: router", _act_dtypes(), 2)
+        _need(tuple(router.shape) == (num_experts, hidden), f"moe_layer: router has shape {tuple(router.shape)}")
+    else:
+        _tensor(logits, "moe_layer: logits", (torch.float32,), 2)
+        _need(tuple(logits.shape) == (rows, num_experts), f"moe_layer: logits have shape {tuple(logits.shape)}")
+    for nm, sch, w, sc, n, k in (("gate_up", gate_up_scheme, gate_up, gate_up_scales, 2 * inter, hidden),
+                                 ("down", down_scheme, down, down_scales, hidden, inter)):
+        _check_weights(sch, 32, w, sc, None, num_experts * n, k, f"moe_layer: {nm}")
+        if sch == MLX_MXFP4 and sc is not None:
+            _need(sc.dtype == torch.uint8, f"moe_layer: {nm} scales have dtype {sc.dtype}, E8M0 bytes are uint8")
+    for nm, t, dt in (("ids", ids, torch.int32), ("probs", probs, torch.float32)):
+        if t is not None:
+            _tensor(t, f"moe_layer: {nm}", (dt,), 2)
+            _need(tuple(t.shape) == (rows, top_k), f"moe_layer: {nm} has shape {tuple(t.shape)}")
+    if y is not None:
+        _check_out(y, (rows, hidden), "moe_layer")
+    if device is not None:
+        _on_device(device, x=x, router=router, logits=logits, gate_up=gate_up, down=down, gate_up_scales=gate_up_scales,
+                   down_scales=down_scales, ids=ids, probs=probs, y=y)
+
+
 def check_quantize_mxfp4(x, codes, scales, *, device=None) -> None:
     import torch
 
@@ -521,6 +554,28 @@ class Context:
         rc = lib().rlxq_moe_grouped(self.h, scheme, mode, _ptr(x), _dt(x), _ptr(bank), _ptr(ids), _ptr(probs),
                                     rows, top_k, k, n, num_experts, _ptr(y), _dt(y), _stream(stream))
         self._check(rc, "moe_grouped")
+        return y
+
+    def moe_layer(self, x, router, gate_up, down, gate_up_scheme: int, down_scheme: int, top_k: int, inter: int,
+                  num_experts: int, *, logits=None, gate_up_scales=None, down_scales=None, renorm: bool = True,
+                  ids=None, probs=None, y=None, y_dtype=None, stream=None):
+        """The routed-expert layer of x [rows, hidden]: router product (or the
+        caller's logits, router=None), top-k, gate|up + SwiGLU, down and the
+        weighted sum; returns y [rows, hidden].  ids / probs [rows, top_k]
+        receive the routing if given."""
+        import torch
+
+        check_moe_layer(x, router, gate_up, down, gate_up_scheme, down_scheme, top_k, inter, num_experts, logits=logits,
+                        gate_up_scales=gate_up_scales, down_scales=down_scales, ids=ids, probs=probs, y=y,
+                        device=self.device)
+        rows, hidden = x.shape
+        if y is None:
+            y = torch.empty((rows, hidden), dtype=y_dtype or torch.float32, device=x.device)
+        rc = lib().rlxq_moe_layer(self.h, _ptr(x), _dt(x), _ptr(router), _dt(router) if router is not None else F32,
+                                  _ptr(logits), gate_up_scheme, _ptr(gate_up), _ptr(gate_up_scales), down_scheme,
+                                  _ptr(down), _ptr(down_scales), rows, hidden, inter, num_experts, top_k, int(renorm),
+                                  _ptr(ids), _ptr(probs), _ptr(y), _dt(y), _stream(stream))
+        self._check(rc, "moe_layer")
         return y
 
     def moe_route(self, logits, top_k: int, renorm: bool, *, stream=None):

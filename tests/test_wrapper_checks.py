@@ -150,3 +150,26 @@ def test_mxfp4_quantize_and_gemm_checks():
         rlxq.check_mxfp4_gemm(x, _u8(8 * 32), _u8(16), 8, y=torch.zeros((2, 9)))
     with pytest.raises(ValueError, match="context is on cuda:0"):
         rlxq.check_mxfp4_gemm(x, _u8(8 * 32), _u8(16), 8, device=0)
+
+
+def test_moe_layer_checks():
+    mx, q41 = rlxq.MLX_MXFP4, rlxq.GGUF_Q4_1
+    x, r = torch.zeros((2, 64)), torch.zeros((4, 64))
+    g, gs, d = _u8(4 * 64 * 32), _u8(4 * 64 * 2), _u8(4 * 64 * 20)
+    ok = dict(gate_up_scales=gs)
+    rlxq.check_moe_layer(x, r, g, d, mx, q41, 2, 32, 4, y=torch.zeros((2, 64)), **ok)
+    rlxq.check_moe_layer(x, None, g, d, mx, q41, 2, 32, 4, logits=torch.zeros((2, 4)), **ok)
+    bad = [((x, None, g, d, mx, q41, 2, 32, 4), ok), ((x, r, g, d, mx, q41, 2, 32, 4), dict(logits=torch.zeros((2, 4)), **ok)),
+           ((x, r[:3], g, d, mx, q41, 2, 32, 4), ok), ((x, r.double(), g, d, mx, q41, 2, 32, 4), ok),
+           ((x, r, g[1:], d, mx, q41, 2, 32, 4), ok), ((x, r, g, d[1:], mx, q41, 2, 32, 4), ok),
+           ((x, r, g, d, mx, q41, 5, 32, 4), ok), ((x, r, g, d, mx, q41, 2, 64, 4), ok),
+           ((x, r, g, d, mx, q41, 2, 32, 4), dict(gate_up_scales=gs[1:])),
+           ((x, r, g, d, mx, q41, 2, 32, 4), dict(gate_up_scales=torch.zeros(512, dtype=torch.bfloat16))),
+           ((x, r, g, d, mx, q41, 2, 32, 4), dict(ids=torch.zeros((2, 2)), **ok)),
+           ((x, r, g, d, mx, q41, 2, 32, 4), dict(probs=torch.zeros((2, 3)), **ok)),
+           ((x, r, g, d, mx, q41, 2, 32, 4), dict(y=torch.zeros((2, 32)), **ok)),
+           ((x, None, g, d, mx, q41, 2, 32, 4), dict(logits=torch.zeros((2, 5)), **ok)),
+           ((x, r, g, d, mx, q41, 2, 32, 4), dict(device=0, **ok))]
+    for args, kw in bad:
+        with pytest.raises(ValueError):
+            rlxq.check_moe_layer(*args, **kw)

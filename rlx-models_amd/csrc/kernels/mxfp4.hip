@@ -102,26 +102,6 @@ RLXQ_DEV void mx_quant_rows(const rlxq_mx_quant_args& a) {
   if ((threadIdx.x & 3) == 0) a.scales[i >> 2] = (uint8_t)b;
 }
 
-// The matmul's activation fragments (mxfp4_args.h); the blocks past K of the
-// last span are zeros.
-template <bool BF16>
-RLXQ_DEV void mx_quant_frag(const rlxq_mx_quant_args& a) {
-  const int R = a.rows, G8 = 64 / R * 16;   // eights in a span
-  const int64_t per = (int64_t)a.spans * G8;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= a.M * per) return;
-  const int64_t m = i / per, e8 = i - m * per;
-  const int span = (int)(e8 / G8), t = (int)(e8 - (int64_t)span * G8);
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (e8 * 8 < a.K) mx_load8<BF16>(a.x, m * a.K + e8 * 8, v);   // (K is whole blocks: uniform over a quad)
-  uint32_t b;
-  const uint32_t c = mx_quant8<true>(v, b);
-  const int blk = t >> 2, lane = (blk >> 2) * R + (int)(m % R), j = blk & 3;
-  uint8_t* p = a.codes + ((m / R) * a.spans + span) * (int64_t)RLXQ_MX_CHUNK;
-  *reinterpret_cast<uint32_t*>(p + 1024 * j + 16 * lane + 4 * (t & 3)) = c;
-  if ((t & 3) == 0) p[4096 + 4 * lane + j] = (uint8_t)b;
-}
-
 // Four scale bytes of weights as the MFMA takes them: 255 reads as 2^127
 // (e8m0_to_f32), which is byte 254.
 RLXQ_DEV uint32_t mx_scales(uint32_t s) {
@@ -130,6 +110,69 @@ RLXQ_DEV uint32_t mx_scales(uint32_t s) {
 }
 // Whether one of the four bytes is 0 (a scale of zero).
 RLXQ_DEV bool mx_has_zero(uint32_t s) { return ((s - 0x01010101u) & ~s & 0x80808080u) != 0u; }
+
+// The scale bytes of 32 weight rows (one workgroup), a dword per lane and span
+// of 256 elements in the lane order of the fragments: the matmul then reads
+// whole lines of them.  255 becomes 254 (mx_scales), blocks past K get 127.
+// zero[rb] tells whether one of the row block's bytes is 0.
+RLXQ_DEV void mx_scale_frag(const rlxq_mx_quant_args& a, int rb) {
+  const int nb = (int)(a.K / 32);
+  bool zero = false;
+  for (int i = threadIdx.x; i < a.spans * 32; i += blockDim.x) {
+    const int span = i >> 5, row = i & 31;
+    int64_t n = (int64_t)rb * 32 + row;
+    n = n < a.N ? n : a.N - 1;
+    const uint8_t* p = a.ws + n * nb + 8 * span;
+    uint64_t v;   // the span's eight bytes of the row
+    if (8 * span + 8 <= nb) {
+      __builtin_memcpy(&v, p, 8);
+    } else {
+      v = 0x7f7f7f7f7f7f7f7full;
+      for (int j = 0; 8 * span + j < nb; j++) v = (v & ~(0xffull << (8 * j))) | ((uint64_t)p[j] << (8 * j));
+    }
+    const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    zero = zero || mx_has_zero(lo) || mx_has_zero(hi);
+    uint32_t* o = a.wsf + ((int64_t)rb * a.spans + span) * 64 + row;
+    o[0] = mx_scales(perm_b32(hi, lo, 0x05040100u));    // blocks 0, 1, 4, 5
+    o[32] = mx_scales(perm_b32(hi, lo, 0x07060302u));   // blocks 2, 3, 6, 7
+  }
+  const bool any = __syncthreads_or(zero) != 0;
+  if (threadIdx.x == 0) a.zero[rb] = any ? 1 : 0;
+}
+
+// The matmul's activation fragments (mxfp4_args.h), a workgroup per chunk: the
+// threads follow the chunk's code dwords, so a wave stores 256 consecutive
+// bytes and a quad reads a block.  Zeros for the blocks past K and the rows
+// past M.
+template <bool BF16>
+RLXQ_DEV void mx_quant_frag(const rlxq_mx_quant_args& a) {
+  if ((int)blockIdx.x < a.wblocks) {   // (the weights' scales beside them)
+    mx_scale_frag(a, blockIdx.x);
+    return;
+  }
+  const int R = a.rows, c = blockIdx.x - a.wblocks;
+  const int rb = c / a.spans, span = c - rb * a.spans;
+  const int lane = threadIdx.x >> 2, row = lane % R, g = lane / R;
+  const int64_t m = (int64_t)rb * R + row;
+  uint8_t* p = a.codes + (int64_t)c * RLXQ_MX_CHUNK;
+  float v[4][8];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int blk = R == 16 ? 4 * g + j : 4 * (j >> 1) + 2 * g + (j & 1);
+    const int64_t e = (int64_t)span * (64 / R * 128) + 32 * blk + 8 * (threadIdx.x & 3);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[j][i] = 0.f;
+    if (m < a.M && e < a.K) mx_load8<BF16>(a.x, m * a.K + e, v[j]);   // (K is whole blocks)
+  }
+  uint32_t sc = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    uint32_t b;
+    reinterpret_cast<uint32_t*>(p)[256 * j + threadIdx.x] = mx_quant8<true>(v[j], b);
+    sc |= b << (8 * j);
+  }
+  if ((threadIdx.x & 3) == 0) *reinterpret_cast<uint32_t*>(p + 4096 + threadIdx.x) = sc;
+}
 
 // The scale bytes of blocks b0 .. b0 + 3 of a row of nb blocks (blocks past
 // the end repeat the last one: their activations' codes are zero).
@@ -247,7 +290,378 @@ RLXQ_DEV void mx_dec_body(const rlxq_mx_gemm_args& a) {
   }
 }
 
+// ------------------------------------------------------------- many rows
+typedef float mx_f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t mx_u32x4_t __attribute__((ext_vector_type(4)));
+
+// c += a . b for 32 x 32 outputs and 64 elements, byte OP of the scales.  As the
+// instruction itself, so that it stays where it is written between the LDS
+// reads and the loads around it (the compiler moves the builtin past both).
+// The compiler then does not see what the instruction asks for: two wait
+// states behind a vector instruction that writes one of its operands (masked
+// weights straight in front of it gave wrong sums without them; behind another
+// MFMA they cost nothing), and mx_mfma_done() ahead of any other use of c.
+template <int OP>
+RLXQ_DEV void mx_mfma32(mx_f32x16_t& c, const uint4& a, const uint4& b, uint32_t sa, uint32_t sb) {
+  const mx_u32x4_t av = {a.x, a.y, a.z, a.w}, bv = {b.x, b.y, b.z, b.w};
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] "
+               "cbsz:4 blgp:4"
+               : "+a"(c)
+               : "v"(av), "v"(bv), "v"(sa), "v"(sb), "n"(OP & 1), "n"(OP >> 1));
+}
+RLXQ_DEV void mx_mfma_done() { asm volatile("s_nop 15\n\ts_nop 15"); }
+
+// 64 lanes x 16 (or 4) bytes from base + off + I into LDS at M0 + I (base and
+// M0 wave-uniform).  Written as the instruction itself: the compiler cannot
+// tell the buffer that is being filled from the one being read and would wait
+// for the fill ahead of every LDS read.  mx_loads_wait() waits for all but the
+// wave's last N loads; nothing else does.
+RLXQ_DEV void mx_lds_dst(uint32_t dst) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" : : "s"(dst) : "memory"); }
+template <int I>
+RLXQ_DEV void mx_to_lds16(const uint8_t* base, uint32_t off) {
+  asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" : : "v"(off), "s"(base), "n"(I) : "memory");
+}
+template <int I>
+RLXQ_DEV void mx_to_lds4(const uint8_t* base, uint32_t off) {
+  asm volatile("global_load_lds_dword %0, %1 offset:%2" : : "v"(off), "s"(base), "n"(I) : "memory");
+}
+template <int N>
+RLXQ_DEV void mx_loads_wait() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
+}
+// p, the same in every lane, in scalar registers.
+RLXQ_DEV const uint8_t* mx_uniform(const uint8_t* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = __builtin_amdgcn_readfirstlane((int)(u >> 32));
+  return reinterpret_cast<const uint8_t*>(((uint64_t)hi << 32) | lo);
+}
+RLXQ_DEV uint32_t mx_lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+
+// One output tile of 32 TM WGM activation rows x 32 TN WGN weight rows by
+// WGM x WGN waves, in stages of 128 elements (64 code bytes a row).  Both
+// operands go from memory straight into LDS, three stages ahead of the one
+// being multiplied, in a ring of four: the activations' fragments as they are
+// (a wave reads lane-consecutive 16 bytes), the weights as rows of four
+// 16-byte pieces, piece p of row r at slot p ^ (r >> 1 & 3), which spreads the
+// eight lanes that read one piece of eight rows over all banks.  Scales come a
+// span (two stages) at a time, a dword per lane and 32 rows.
+// A stage is two MFMA steps.  While one step's MFMAs run, the fragments of the
+// next are read and the loads of the stage three ahead are issued, one or two
+// between any two MFMAs; the workgroup meets once a stage, between the steps:
+// behind that barrier the next stage is in LDS and the last one has been read.
+// The weights are the MFMA's first operand, so that a lane's results are four
+// consecutive columns of y.
+// MASKED: weight blocks whose scale byte is 0 are read as zero codes.
+template <int WGM, int WGN, int TM, int TN, bool MASKED>
+RLXQ_DEV void mx_gemm_tile(const rlxq_mx_gemm_args& a, int tm, int tn, uint8_t* mx_lds) {
+  constexpr int BM = 32 * TM * WGM, BN = 32 * TN * WGN, NW = WGM * WGN;
+  constexpr int STAGE = (BM + BN) * 64, XB = BM / 32, WB = BN / 32, SCALES = (XB + WB) * 256;
+  constexpr int LX = BM * 64 / 1024 / NW, LW = BN * 64 / 1024 / NW;   // 1 KB loads per wave and stage
+  constexpr int LS = (XB + WB) / NW;   // 256 B scale loads per wave and span
+  static_assert(LX * NW * 1024 == BM * 64 && LW * NW * 1024 == BN * 64 && LS * NW == XB + WB, "whole loads per wave");
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wv / WGN, wn = wv % WGN;
+  const int row = lane & 31, g = lane >> 5;
+  const int nb = (int)(a.K / 32);
+  const int64_t kb = a.K / 2;
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int xb_last = (int)((a.M + 31) / 32) - 1, wb_last = (int)((a.N + 31) / 32) - 1;
+  const int per = (a.spans + a.splits - 1) / a.splits;
+  const int s0 = __builtin_amdgcn_readfirstlane((int)blockIdx.y * per);
+  const int s1 = __builtin_amdgcn_readfirstlane(s0 + per < a.spans ? s0 + per : a.spans);
+
+  // ---- loads.  A wave fills LX KB of the activations' part of a ring slot
+  // and LW KB of the weights', each one run of LDS: one M0 and immediate
+  // offsets, which move the source too (the lanes' offsets undo that).
+  // Its LX KB are whole halves of row blocks' fragments: 2 KB each.
+  static_assert(LX % 2 == 0, "whole row blocks per wave");
+  constexpr int XP = LX / 2;
+  const uint32_t l16 = 16 * lane, l4 = 4 * lane;
+  const uint8_t* xp[XP];   // row block q's fragments (its half-chunk of the next stage to load), less 2048 q
+#pragma unroll
+  for (int q = 0; q < XP; q++) {
+    const int rb = tm * XB + wv * XP + q;
+    xp[q] = mx_uniform(a.xf + ((int64_t)(rb < xb_last ? rb : xb_last) * a.spans + s0) * RLXQ_MX_CHUNK - 2048 * q);
+  }
+  // weight pieces of this lane (rows clamped to N): piece (lane & 3) ^ .. of
+  // row lane >> 2 of each 16; blocks past K read the row's last one (the
+  // activations are zero there): `back` in the stage that K ends in
+  // (offsets are unsigned: the base never passes that stage)
+  const int piece = (lane & 3) ^ ((lane >> 3) & 3), u_end = __builtin_amdgcn_readfirstlane((nb - 1) / 4);
+  uint32_t wo[LW];
+  const int over = 4 * u_end + piece - (nb - 1);
+  const uint32_t back = over > 0 ? 16 * over : 0;
+#pragma unroll
+  for (int i = 0; i < LW; i++) {
+    int64_t n = n0 + (wv * LW + i) * 16 + (lane >> 2);
+    n = n < a.N ? n : a.N - 1;
+    wo[i] = (uint32_t)((n - n0) * kb) + 16 * piece + 1024 * (LW - 1 - i);
+  }
+  const uint8_t* wbase = mx_uniform(a.w + n0 * kb - 1024 * (LW - 1));
+  // scales: the wave's run i of 256 B is row block wv LS + i of the
+  // activations, then of the weights
+  const uint8_t* sp_[LS];
+  int sstep[LS];
+#pragma unroll
+  for (int i = 0; i < LS; i++) {
+    const int c = wv * LS + i;
+    const bool sx = c < XB;
+    const int rb = sx ? tm * XB + c : tn * WB + c - XB, last = sx ? xb_last : wb_last;
+    sstep[i] = sx ? RLXQ_MX_CHUNK : 256;
+    const uint8_t* b = sx ? a.xf + 4096 : reinterpret_cast<const uint8_t*>(a.wsf);
+    sp_[i] = mx_uniform(b + (int64_t)(rb < last ? rb : last) * a.spans * sstep[i] - 256 * i);
+  }
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(mx_lds_addr(mx_lds));
+  const uint32_t x_dst = lds0 + 1024 * wv * LX, w_dst = lds0 + BM * 64 + 1024 * wv * LW;
+  const uint32_t s_dst = lds0 + 4 * STAGE + 256 * wv * LS;
+  const uint8_t* wp = wbase;   // of the next stage to load
+  bool w_end = false;          // that stage is the one K ends in
+  // before the loads of stage u (past the last stage: that one again)
+  const int u_last = 2 * s1 - 1;
+  auto stage_w = [&](int u) {
+    u = u < u_last ? u : u_last;
+    w_end = u >= u_end;
+    wp = wbase + 64 * (int64_t)(w_end ? u_end : u);
+  };
+  // load i (0 .. LX + LW - 1) of the stage into ring slot `slot`
+  auto load_codes = [&](auto ii, int slot) {
+    constexpr int i = decltype(ii)::value;
+    if constexpr (i < LX) {
+      if constexpr (i == 0) mx_lds_dst(x_dst + slot * STAGE);
+      mx_to_lds16<1024 * i>(xp[i / 2], l16);
+    } else {
+      if constexpr (i == LX) mx_lds_dst(w_dst + slot * STAGE);
+      mx_to_lds16<1024 * (i - LX)>(wp, wo[i - LX] - (w_end ? back : 0));
+    }
+  };
+  // the activations' pointers from a stage (half h of a span) to the next;
+  // past the last stage they stay
+  auto next_x = [&](int u, int h) {
+    const int d = u < u_last ? (h ? RLXQ_MX_CHUNK - 2048 : 2048) : 0;
+#pragma unroll
+    for (int q = 0; q < XP; q++) xp[q] += d;
+  };
+  auto load_scales = [&](auto ii, int sp) {   // run i of span sp's scales
+    constexpr int i = decltype(ii)::value;
+    if constexpr (i == 0) mx_lds_dst(s_dst + (sp & 1) * SCALES);
+    mx_to_lds4<256 * i>(sp_[i] + (int64_t)(sp < s1 ? sp : s1 - 1) * sstep[i], l4);
+  };
+  mx_f32x16_t acc[TN][TM];
+#pragma unroll
+  for (int j = 0; j < TN; j++)
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[j][i][r] = 0.f;
+
+  // ---- fragments.  Stages of even spans are in slots 0 and 1, of odd ones in
+  // 2 and 3: `half` is the byte offset of the span's pair of slots.
+  uint4 xf[2][TM], wf[2][TN];
+  uint32_t xc[TM], wc[TN], xn[TM], wn_[TN];
+  const uint8_t* xl = mx_lds + wm * TM * 2048 + l16;
+  const uint8_t* wl = mx_lds + BM * 64 + (wn * TN * 32 + row) * 64;
+  const uint32_t wpc[2] = {(uint32_t)(((2 * g) ^ ((row >> 1) & 3)) << 4), (uint32_t)(((2 * g + 1) ^ ((row >> 1) & 3)) << 4)};
+  // fragment q of MFMA step k (0..3) of a span
+  auto read_frag = [&](auto kk, auto qq, uint32_t half) {
+    constexpr int k = decltype(kk)::value, q = decltype(qq)::value;
+    constexpr int slot = (k >> 1) * STAGE;
+    if constexpr (q < TM) xf[k & 1][q] = *reinterpret_cast<const uint4*>(xl + half + (slot + q * 2048 + 1024 * (k & 1)));
+    else wf[k & 1][q - TM] = *reinterpret_cast<const uint4*>(wl + half + wpc[k & 1] + (slot + (q - TM) * 2048));
+  };
+  auto read_scale = [&](auto qq, int sp) {
+    constexpr int q = decltype(qq)::value;
+    const uint8_t* st = mx_lds + 4 * STAGE + (sp & 1) * SCALES + l4;
+    if constexpr (q < TM) xn[q] = *reinterpret_cast<const uint32_t*>(st + wm * TM * 256 + q * 256);
+    else wn_[q - TM] = *reinterpret_cast<const uint32_t*>(st + (XB + wn * TN) * 256 + (q - TM) * 256);
+  };
+  auto take_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < TM; i++) xc[i] = xn[i];
+#pragma unroll
+    for (int j = 0; j < TN; j++) wc[j] = wn_[j];
+  };
+  // The MFMAs of step k with `A` other actions spread between them.
+  auto step = [&](auto kk, auto nact, auto act) {
+    constexpr int k = decltype(kk)::value, A = decltype(nact)::value, Q = TM * TN;
+    static_for<Q>([&](auto qq) {
+      constexpr int q = decltype(qq)::value, j = q / TM, i = q % TM;
+      if constexpr (MASKED && i == 0) {
+        if (((wc[j] >> (8 * k)) & 0xffu) == 0u) wf[k & 1][j] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      mx_mfma32<k>(acc[j][i], wf[k & 1][j], xf[k & 1][i], wc[j], xc[i]);
+      static_for<A>([&](auto aa) {
+        constexpr int x = decltype(aa)::value;
+        if constexpr (x * Q / A == q) act(aa);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  constexpr int LC = LX + LW, F = TM + TN;
+
+  static_for<LS>([&](auto i) { load_scales(i, s0); });
+  static_for<3>([&](auto uu) {
+    constexpr int u = decltype(uu)::value;
+    if constexpr (u == 2) static_for<LS>([&](auto i) { load_scales(i, s0 + 1); });
+    stage_w(2 * s0 + u);
+    static_for<LC>([&](auto i) { load_codes(i, u); });
+    next_x(2 * s0 + u, u & 1);
+  });
+  mx_loads_wait<2 * LC + LS>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  static_for<F>([&](auto q) { read_scale(q, s0); });
+  static_for<F>([&](auto q) { read_frag(std::integral_constant<int, 0>{}, q, 0); });
+  take_scales();
+  for (int sp = s0; sp < s1; sp++) {
+    const uint32_t half = ((sp - s0) & 1) * (2 * STAGE);
+    const int slots = 2 * ((sp - s0) & 1);
+    static_for<2>([&](auto hh) {   // stage u = 2 sp + h, in slot slots + h
+      constexpr int h = decltype(hh)::value;
+      const int u = 2 * sp + h;
+      constexpr std::integral_constant<int, 2 * h> k0{};
+      constexpr std::integral_constant<int, 2 * h + 1> k1{};
+      constexpr std::integral_constant<int, h == 0 ? 2 : 0> k2{};
+      // first step; meanwhile the second's fragments, then the stage three on
+      stage_w(u + 3);
+      step(k0, std::integral_constant<int, F + LC>{}, [&](auto aa) {
+        constexpr int x = decltype(aa)::value;
+        if constexpr (x < F) read_frag(k1, aa, half);
+        else load_codes(std::integral_constant<int, x - F>{}, h == 0 ? (slots + 3) & 3 : slots);
+      });
+      next_x(u + 3, 1 - h);
+      if constexpr (h == 1) static_for<LS>([&](auto i) { load_scales(i, sp + 2); });
+      mx_loads_wait<2 * LC + LS>();   // stage u + 1 has landed; this wave has read stage u
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      // second step; meanwhile the first fragments (and scales) of the next stage
+      step(k1, std::integral_constant<int, F * (h + 1)>{}, [&](auto aa) {
+        constexpr int x = decltype(aa)::value;
+        if constexpr (x < F) read_frag(k2, aa, h == 0 ? half : half ^ (2 * STAGE));
+        else read_scale(std::integral_constant<int, x - F>{}, sp + 1);
+      });
+      if constexpr (h == 1) take_scales();
+    });
+  }
+  // (the loads past the last stage: none may land in another workgroup's LDS)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  mx_mfma_done();
+
+  // A lane holds activation row (column of the MFMA's result) lane & 31 and
+  // weight rows 8 q + 4 g .. + 3 of each tile: four consecutive outputs.  A
+  // whole tile goes out through the wave's own part of LDS, 32 rows at a time,
+  // as whole runs of 32 TN outputs (straight from the registers a store would
+  // hold 32 runs of 16 or 32 bytes).
+  const int64_t mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
+  const bool whole = m0 + BM <= a.M && n0 + BN <= a.N && a.vec;
+  const bool bf = a.splits == 1 && a.y_bf16;
+  uint8_t* yb = reinterpret_cast<uint8_t*>(a.splits > 1 ? a.part + (int64_t)blockIdx.y * a.M * a.N : a.y);
+  constexpr int EROW = 32 * TN * 4 + 16;   // bytes of a staged row (16 more: rows start in different banks)
+  static_assert(NW * 32 * EROW <= 4 * STAGE, "staging fits the ring");
+  uint8_t* est = mx_lds + wv * (32 * EROW);
+  __syncthreads();   // (every wave has read its last fragments)
+  auto tiles = [&](auto bfc) {
+    constexpr bool BF = decltype(bfc)::value;
+    constexpr int ES = BF ? 2 : 4;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        mx_f32x16_t v = acc[j][i];
+        asm volatile("" : "+v"(v) : : "memory");   // (one tile at a time out of the accumulators)
+        if (whole) {
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            uint8_t* d = est + row * EROW + (32 * j + 8 * q + 4 * g) * ES;
+            if constexpr (BF)
+              *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3]));
+            else
+              *reinterpret_cast<float4*>(d) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          }
+        } else if (mw + 32 * i + row < a.M) {
+          const int64_t o = (mw + 32 * i + row) * a.N + nw + 32 * j + 4 * g;
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int d = 8 * (r / 4) + r % 4;
+            if (nw + 32 * j + 4 * g + d >= a.N) continue;
+            if constexpr (BF) reinterpret_cast<uint16_t*>(yb)[o + d] = (uint16_t)f32_to_bf16_bits(v[r]);
+            else reinterpret_cast<float*>(yb)[o + d] = v[r];
+          }
+        }
+      }
+      if (whole) {
+        // (the wave's own LDS: its stores are done before its reads)
+        constexpr int PER = 32 * TN * ES / 16, RPI = 64 / PER;   // lanes per row, rows per store
+        static_assert(PER <= 64, "a row per store at least");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < 32 / RPI; q++) {
+          const int r = q * RPI + lane / PER, c = 16 * (lane % PER);
+          const uint4 v = *reinterpret_cast<const uint4*>(est + r * EROW + c);
+          *reinterpret_cast<uint4*>(yb + ((mw + 32 * i + r) * a.N + nw) * ES + c) = v;
+        }
+      }
+    }
+  };
+  if (bf) tiles(std::true_type{});
+  else tiles(std::false_type{});
+}
+
+template <int WGM, int WGN, int TM, int TN>
+RLXQ_DEV void mx_gemm_body(const rlxq_mx_gemm_args& a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t mx_lds[];
+  constexpr int BM = 32 * TM * WGM, BN = 32 * TN * WGN;
+  const int tiles_m = (int)((a.M + BM - 1) / BM), tiles_n = (int)((a.N + BN - 1) / BN);
+  int tm, tn;
+  if (!tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn)) return;
+  const int wb_last = (int)((a.N + 31) / 32) - 1;
+  bool zero = false;
+#pragma unroll
+  for (int j = 0; j < BN / 32; j++) {
+    const int rb = tn * (BN / 32) + j;
+    zero = zero || a.zero[rb < wb_last ? rb : wb_last] != 0;
+  }
+  if (__builtin_amdgcn_readfirstlane(zero ? 1 : 0)) mx_gemm_tile<WGM, WGN, TM, TN, true>(a, tm, tn, mx_lds);
+  else mx_gemm_tile<WGM, WGN, TM, TN, false>(a, tm, tn, mx_lds);
+}
+
+// y = the K splits' partial sums, added in split order.
+RLXQ_DEV void mx_reduce_body(const rlxq_mx_gemm_args& a) {
+  const int64_t total = a.M * a.N;
+  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4;
+  if (i >= total) return;
+  if (i + 4 <= total && a.vec) {
+    float4 s = *reinterpret_cast<const float4*>(a.part + i);
+    for (int p = 1; p < a.splits; p++) {
+      const float4 v = *reinterpret_cast<const float4*>(a.part + p * total + i);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    if (a.y_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.y) + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+    else *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.y) + i) = s;
+    return;
+  }
+  for (int64_t j = i; j < i + 4 && j < total; j++) {
+    float s = a.part[j];
+    for (int p = 1; p < a.splits; p++) s += a.part[p * total + j];
+    if (a.y_bf16) reinterpret_cast<uint16_t*>(a.y)[j] = (uint16_t)f32_to_bf16_bits(s);
+    else reinterpret_cast<float*>(a.y)[j] = s;
+  }
+}
+
 }  // namespace rlxq
+
+extern "C" __global__ __launch_bounds__(256) void rlxq_mx_reduce(rlxq_mx_gemm_args a) { rlxq::mx_reduce_body(a); }
+#define RLXQ_MX_GEMM(NAME, WGM, WGN, TM, TN)                                                             \
+  extern "C" __global__ __launch_bounds__(64 * WGM * WGN) void rlxq_mx_gemm_##NAME(rlxq_mx_gemm_args a) { \
+    rlxq::mx_gemm_body<WGM, WGN, TM, TN>(a);                                                             \
+  }
+RLXQ_MX_GEMM(m256n256, 2, 2, 4, 4)
+RLXQ_MX_GEMM(m256n256w8, 2, 4, 4, 2)
+RLXQ_MX_GEMM(m128n128, 2, 2, 2, 2)
+RLXQ_MX_GEMM(m128n256, 2, 2, 2, 4)
+RLXQ_MX_GEMM(m64n64, 1, 2, 2, 1)
+RLXQ_MX_GEMM(m64n128, 1, 2, 2, 2)
+RLXQ_MX_GEMM(m128n64, 2, 1, 2, 2)
+RLXQ_MX_GEMM(m32n64, 1, 1, 1, 2)
 
 extern "C" __global__ __launch_bounds__(256) void rlxq_mx_quant_bf16(rlxq_mx_quant_args a) { rlxq::mx_quant_rows<true>(a); }
 extern "C" __global__ __launch_bounds__(256) void rlxq_mx_quant_f32(rlxq_mx_quant_args a) { rlxq::mx_quant_rows<false>(a); }

@@ -162,7 +162,7 @@ def _stream(stream) -> int | None:
     if stream is None:
         import torch
 
-        return torch.cuda.current_stream().cuda_stream or None
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or None
     return int(stream)
 
 
@@ -208,26 +208,36 @@ def _nbytes(t) -> int:
 
 
 def _tensor(t, name: str, dtypes=None, ndim=None):
-    _need(t is not None, f"{name} is required")
-    _need(hasattr(t, "data_ptr") and hasattr(t, "is_contiguous"), f"{name} must be a tensor")
-    _need(t.is_contiguous(), f"{name} must be contiguous (got strides {tuple(t.stride())})")
-    if dtypes is not None:
-        _need(t.dtype in dtypes, f"{name} has dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
-    if ndim is not None:
-        _need(t.dim() == ndim, f"{name} must be {ndim}-D (got shape {tuple(t.shape)})")
+    # (messages are built for a failing check only: the wrappers of calls of a
+    # few microseconds run these checks every time)
+    if t is None:
+        raise ValueError(f"{name} is required")
+    if not (hasattr(t, "data_ptr") and hasattr(t, "is_contiguous")):
+        raise ValueError(f"{name} must be a tensor")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous (got strides {tuple(t.stride())})")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise ValueError(f"{name} has dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
+    if ndim is not None and t.dim() != ndim:
+        raise ValueError(f"{name} must be {ndim}-D (got shape {tuple(t.shape)})")
 
 
 def _on_device(device: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None:
-            _need(t.is_cuda and (t.device.index or 0) == device,
-                  f"{name} is on {t.device}, the context is on cuda:{device}")
+        if t is not None and not (t.is_cuda and t.get_device() == device):
+            raise ValueError(f"{name} is on {t.device}, the context is on cuda:{device}")
+
+
+_act_types = None
 
 
 def _act_dtypes():
-    import torch
+    global _act_types
+    if _act_types is None:
+        import torch
 
-    return (torch.float32, torch.bfloat16)
+        _act_types = (torch.float32, torch.bfloat16)
+    return _act_types
 
 
 def _check_weights(scheme: int, group: int, w, scales, biases, rows: int, k: int, what: str) -> None:
@@ -237,7 +247,7 @@ def _check_weights(scheme: int, group: int, w, scales, biases, rows: int, k: int
     dtypes, NULL slabs) is left to it, so its status codes reach the caller."""
     import torch
 
-    _tensor(w, f"{what}: w")
+    _tensor(w, what + ": w")
     if scheme == INT8_BLOCK:
         _need(w.dtype in (torch.int8, torch.uint8), f"{what}: Int8Block weights are int8 [K, N]")
         _need(_nbytes(w) >= k * rows, f"{what}: w holds {_nbytes(w)} B, [K={k}, N={rows}] int8 needs {k * rows}")
@@ -251,7 +261,8 @@ def _check_weights(scheme: int, group: int, w, scales, biases, rows: int, k: int
     rb = packed_row_bytes(scheme, k)
     if rb <= 0:
         return
-    _need(_nbytes(w) >= rows * rb, f"{what}: w holds {_nbytes(w)} B, {rows} rows of {rb} B need {rows * rb}")
+    if _nbytes(w) < rows * rb:
+        raise ValueError(f"{what}: w holds {_nbytes(w)} B, {rows} rows of {rb} B need {rows * rb}")
     if scheme in (MLX_AFFINE4, MLX_AFFINE8, MLX_MXFP4):
         g = 32 if scheme == MLX_MXFP4 else group
         if g <= 0 or k % g:
@@ -261,14 +272,16 @@ def _check_weights(scheme: int, group: int, w, scales, biases, rows: int, k: int
         for nm, t in slabs:
             if t is not None:
                 _tensor(t, f"{what}: {nm}")
-                _need(t.numel() >= per, f"{what}: {nm} has {t.numel()} elements, [{rows}, {k // g}] needs {per}")
+                if t.numel() < per:
+                    raise ValueError(f"{what}: {nm} has {t.numel()} elements, [{rows}, {k // g}] needs {per}")
         if scheme != MLX_MXFP4 and scales is not None and biases is not None:
             _need(scales.dtype == biases.dtype, f"{what}: scales and biases must share a dtype")
 
 
 def _check_out(y, shape, what: str) -> None:
-    _tensor(y, f"{what}: y", _act_dtypes())
-    _need(tuple(y.shape) == tuple(shape), f"{what}: y has shape {tuple(y.shape)}, expected {tuple(shape)}")
+    _tensor(y, what + ": y", _act_dtypes())
+    if tuple(y.shape) != tuple(shape):
+        raise ValueError(f"{what}: y has shape {tuple(y.shape)}, expected {tuple(shape)}")
 
 
 def check_dense(x, w, scheme: int, n: int, *, group: int = 32, scales=None, biases=None, y=None,
@@ -351,19 +364,22 @@ def check_moe_layer(x, router, gate_up, down, gate_up_scheme: int, down_scheme: 
           "moe_layer: need num_experts > 0, 0 < top_k <= num_experts, inter > 0")
     if router is not None:
         _tensor(router, "moe_layer: router", _act_dtypes(), 2)
-        _need(tuple(router.shape) == (num_experts, hidden), f"moe_layer: router has shape {tuple(router.shape)}")
+        if tuple(router.shape) != (num_experts, hidden):
+            raise ValueError(f"moe_layer: router has shape {tuple(router.shape)}, expected {(num_experts, hidden)}")
     else:
         _tensor(logits, "moe_layer: logits", (torch.float32,), 2)
-        _need(tuple(logits.shape) == (rows, num_experts), f"moe_layer: logits have shape {tuple(logits.shape)}")
-    for nm, sch, w, sc, n, k in (("gate_up", gate_up_scheme, gate_up, gate_up_scales, 2 * inter, hidden),
-                                 ("down", down_scheme, down, down_scales, hidden, inter)):
-        _check_weights(sch, 32, w, sc, None, num_experts * n, k, f"moe_layer: {nm}")
-        if sch == MLX_MXFP4 and sc is not None:
-            _need(sc.dtype == torch.uint8, f"moe_layer: {nm} scales have dtype {sc.dtype}, E8M0 bytes are uint8")
+        if tuple(logits.shape) != (rows, num_experts):
+            raise ValueError(f"moe_layer: logits have shape {tuple(logits.shape)}, expected {(rows, num_experts)}")
+    _check_weights(gate_up_scheme, 32, gate_up, gate_up_scales, None, num_experts * 2 * inter, hidden, "moe_layer: gate_up")
+    _check_weights(down_scheme, 32, down, down_scales, None, num_experts * hidden, inter, "moe_layer: down")
+    for sch, sc in ((gate_up_scheme, gate_up_scales), (down_scheme, down_scales)):
+        if sch == MLX_MXFP4 and sc is not None and sc.dtype != torch.uint8:
+            raise ValueError(f"moe_layer: MXFP4 scales have dtype {sc.dtype}, E8M0 bytes are uint8")
     for nm, t, dt in (("ids", ids, torch.int32), ("probs", probs, torch.float32)):
         if t is not None:
-            _tensor(t, f"moe_layer: {nm}", (dt,), 2)
-            _need(tuple(t.shape) == (rows, top_k), f"moe_layer: {nm} has shape {tuple(t.shape)}")
+            _tensor(t, "moe_layer: " + nm, (dt,), 2)
+            if tuple(t.shape) != (rows, top_k):
+                raise ValueError(f"moe_layer: {nm} has shape {tuple(t.shape)}, expected {(rows, top_k)}")
     if y is not None:
         _check_out(y, (rows, hidden), "moe_layer")
     if device is not None:
@@ -376,11 +392,13 @@ def check_quantize_mxfp4(x, codes, scales, *, device=None) -> None:
 
     _tensor(x, "quantize_mxfp4: x", _act_dtypes(), 2)
     m, k = x.shape
-    _need(k > 0 and k % 32 == 0, f"quantize_mxfp4: K = {k} is not a multiple of 32")
+    if k <= 0 or k % 32:
+        raise ValueError(f"quantize_mxfp4: K = {k} is not a multiple of 32")
     for nm, t, per in (("codes", codes, 2), ("scales", scales, 32)):
         if t is not None:
-            _tensor(t, f"quantize_mxfp4: {nm}", (torch.uint8,), 2)
-            _need(tuple(t.shape) == (m, k // per), f"quantize_mxfp4: {nm} has shape {tuple(t.shape)}, expected {(m, k // per)}")
+            _tensor(t, "quantize_mxfp4: " + nm, (torch.uint8,), 2)
+            if tuple(t.shape) != (m, k // per):
+                raise ValueError(f"quantize_mxfp4: {nm} has shape {tuple(t.shape)}, expected {(m, k // per)}")
     if device is not None:
         _on_device(device, x=x, codes=codes, scales=scales)
 
@@ -390,11 +408,12 @@ def check_mxfp4_gemm(x, w, w_scales, n: int, *, y=None, device=None) -> None:
 
     _tensor(x, "mxfp4_gemm: x", _act_dtypes(), 2)
     m, k = x.shape
-    _need(k > 0 and k % 32 == 0, f"mxfp4_gemm: K = {k} is not a multiple of 32")
+    if k <= 0 or k % 32:
+        raise ValueError(f"mxfp4_gemm: K = {k} is not a multiple of 32")
     for nm, t, per in (("w", w, 2), ("w_scales", w_scales, 32)):
-        _tensor(t, f"mxfp4_gemm: {nm}", (torch.uint8,))
-        _need(t.numel() >= n * (k // per),
-              f"mxfp4_gemm: {nm} has {t.numel()} B, [N={n}, {k // per}] needs {n * (k // per)}")
+        _tensor(t, "mxfp4_gemm: " + nm, (torch.uint8,))
+        if t.numel() < n * (k // per):
+            raise ValueError(f"mxfp4_gemm: {nm} has {t.numel()} B, [N={n}, {k // per}] needs {n * (k // per)}")
     if y is not None:
         _check_out(y, (m, n), "mxfp4_gemm")
     if device is not None:
@@ -516,7 +535,8 @@ class Context:
         if out is None:
             out = torch.empty((rows, k), dtype=torch.float32, device=w.device)
         _tensor(out, "dequantize: out", (torch.float32,))
-        _need(tuple(out.shape) == (rows, k), f"dequantize: out has shape {tuple(out.shape)}, expected {(rows, k)}")
+        if tuple(out.shape) != (rows, k):
+            raise ValueError(f"dequantize: out has shape {tuple(out.shape)}, expected {(rows, k)}")
         _on_device(self.device, w=w, scales=scales, biases=biases, out=out)
         sb = _dt(scales) if scales is not None else F32
         rc = lib().rlxq_dequantize(self.h, scheme, group, _ptr(w), _ptr(scales), _ptr(biases), sb, rows, k,

@@ -2,6 +2,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -46,20 +47,53 @@ int quant_frag(rlxq_ctx* ctx, const rlxq_mx_gemm_args& g, const void* x, int x_d
   return launch(ctx, fn, dim3((unsigned)grid), dim3(256), 0, stream, args, name);
 }
 
+// Compiled tilings (kernel rlxq_mx_gemm_<name>), and what they cost: `span` us
+// for 256 elements of one tile on a CU that is full of them, `solo` us where a
+// tile has the CU to itself, `over` us a tile (prologue and stores).  `occ`
+// tiles fit a CU (LDS).
 struct MxCfg {
   const char* name;
-  int BM, BN, waves;
+  int BM, BN, waves, occ;
+  double solo, span, over;
 };
-// Compiled tilings (kernel rlxq_mx_gemm_<name>).
-const MxCfg kMx[] = {{"m256n256", 256, 256, 4}, {"m256n256w8", 256, 256, 8}, {"m128n128", 128, 128, 4},
-                     {"m128n256", 128, 256, 4}, {"m64n64", 64, 64, 2},       {"m64n128", 64, 128, 2},
-                     {"m128n64", 128, 64, 2},   {"m32n64", 32, 64, 1}};
+const MxCfg kMx[] = {{"m256n256", 256, 256, 8, 1, 0.0, 1.18, 11.1},
+                     {"m128n128", 128, 128, 4, 2, 0.0, 0.52, 3.5},
+                     {"m128n64", 128, 64, 2, 3, 0.44, 0.34, 2.3},
+                     {"m64n64", 64, 64, 2, 4, 0.33, 0.25, 1.1}};
+
+int span_splits(int spans, int splits) {   // K splits that all have spans
+  if (splits > spans) splits = spans;
+  const int per = (spans + splits - 1) / splits;
+  return (spans + per - 1) / per;
+}
+
+// Tiling and K splits by the model above, the CUs filled evenly round by
+// round, plus 3.3 us and 8 bytes per partial sum at 8.8 TB/s where K is split.
+// Fitted to 1404 calls (33 to 4096 rows, K 1056 to 12288, N 2048 to 24576); its
+// choices are 1.4% behind the fastest of all tilings on average, 18% at worst
+// (384 x 4096 x 24576: 256 x 256 tiles 52 us, 128 x 128 ones 45).
+const MxCfg& pick_tiling(int64_t m, int64_t k, int64_t n, int cus, int* splits) {
+  const MxCfg* best = &kMx[0];
+  double best_t = 1e300;
+  const int spans = (int)((k + 255) / 256);
+  for (const MxCfg& c : kMx) {
+    const double tiles = (double)((m + c.BM - 1) / c.BM) * (double)((n + c.BN - 1) / c.BN);
+    for (int sp : {1, 2, 3, 4, 6}) {
+      if (sp > 1 && (sp > spans || tiles * sp > 4.0 * cus)) break;
+      const int real = span_splits(spans, sp), per = (spans + real - 1) / real;
+      const double n_cu = std::ceil(tiles * real / cus), full = std::floor(n_cu / c.occ), rest = n_cu - full * c.occ;
+      auto round = [&](double g) { return g > 0 ? std::max(c.solo, g * c.span) * per + c.over * (0.5 + 0.5 * g) : 0.0; };
+      double t = full * round(c.occ) + round(rest);
+      if (real > 1) t += 3.3 + real * (double)m * (double)n * 8.0 / 8.8e6;
+      if (t < best_t) best_t = t, best = &c, *splits = real;
+    }
+  }
+  return *best;
+}
 
 int gemm_tiled(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, const MxCfg& c, int splits, void* stream) {
   a.spans = (int)((a.K + 255) / 256);
-  if (splits > a.spans) splits = a.spans;
-  const int per = (a.spans + splits - 1) / splits;
-  a.splits = (a.spans + per - 1) / per;
+  a.splits = span_splits(a.spans, splits);
   const int64_t tiles_m = (a.M + c.BM - 1) / c.BM, tiles_n = (a.N + c.BN - 1) / c.BN;
   if (tiles_m * tiles_n > 0x7ffffff0) return fail(ctx, RLXQ_E_SHAPE, "mxfp4_gemm: too many tiles");
   const int64_t xb = (a.M + 31) / 32, wb = (a.N + 31) / 32;
@@ -93,6 +127,43 @@ int gemm_tiled(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, c
     ctx->last_kernel = name;
   }
   return RLXQ_OK;
+}
+
+// At most 32 rows: the kernel that streams the weights through registers.
+//   - 32 weight rows a workgroup where that still gives 192 of them, else 16
+//     (1 row, K = 4096, N = 6144: 5.8 us and 6.0; N = 4096: 5.6 and 4.9).
+//   - Eight waves; sixteen where the workgroups are no more than the CUs and K
+//     is long enough for them (4 rows, 12288 -> 4096: 11.4 and 10.6 us); four for
+//     more than 16 rows on 32 weight rows (32 rows, 4096 -> 24576: 24.9 and 20.3).
+//   - The activations quantised in the kernel up to 24576 of them: a launch less
+//     (1 row, 4096 -> 24576: 12.8 us against 15.6; 2 of 12288: 11.1 and 12.0; 4 of
+//     12288: 13.9 and 12.1).
+int gemm_decode(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, void* stream) {
+  a.spans = (int)((a.K + 511) / 512);
+  const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
+  const int mt = a.M > 16 ? 2 : 1;
+  const int nt = (a.N + 31) / 32 >= 3 * cus / 4 ? 2 : 1;
+  const bool fused = mt == 1 && a.M * a.K <= 24576;
+  int waves = nt == 2 && mt == 2 ? 4 : 8;
+  if (nt == 1 && (a.N + 15) / 16 <= cus && (fused || a.spans >= 16)) waves = 16;
+  char name[48];
+  if (fused) {
+    std::snprintf(name, sizeof name, "rlxq_mx_dec_n%d_f%s", nt, x_dtype == RLXQ_BF16 ? "bf16" : "f32");
+    a.x = x;
+  } else {
+    std::snprintf(name, sizeof name, "rlxq_mx_dec_n%dm%d", nt, mt);
+    void* ws = nullptr;
+    int rc = workspace(ctx, (size_t)mt * a.spans * RLXQ_MX_CHUNK, &ws, stream);
+    if (rc) return rc;
+    a.xf = static_cast<uint8_t*>(ws);
+    if ((rc = quant_frag(ctx, a, x, x_dtype, 16, static_cast<uint8_t*>(ws), 0, nullptr, nullptr, stream))) return rc;
+  }
+  hipFunction_t fn;
+  int rc = get_fn(ctx, name, &fn);
+  if (rc) return rc;
+  const size_t lds = (size_t)waves * nt * mt * 1024 + (fused ? (size_t)((a.spans * a.M * 272 + 15) & ~15) : 0);
+  void* args[] = {&a};
+  return launch(ctx, fn, dim3((unsigned)((a.N + 16 * nt - 1) / (16 * nt))), dim3(64 * waves), lds, stream, args, name);
 }
 
 }  // namespace
@@ -163,26 +234,21 @@ int rlxq_mxfp4_gemm(rlxq_ctx* ctx, const void* x, int x_dtype, const uint8_t* w,
   a.K = k;
   a.y_bf16 = y_dtype == RLXQ_BF16;
   a.vec = n % (y_dtype == RLXQ_BF16 ? 8 : 4) == 0 && aligned(y, 16);
-  int rc;
+  // RLXQ_MX_CFG=<tiling>[,<K splits>] selects a tiled kernel (tuning sweeps and
+  // the per-variant tests)
   if (const char* e = std::getenv("RLXQ_MX_CFG")) {
-    int i = -1, sp = 1;
-    if (std::sscanf(e, "%d,%d", &i, &sp) >= 1 && i >= 0 && i < 8) return gemm_tiled(ctx, a, x, x_dtype, kMx[i], sp, stream);
+    const std::string s(e), nm = s.substr(0, s.find(','));
+    const int sp = s.size() > nm.size() ? std::max(1, std::atoi(s.c_str() + nm.size() + 1)) : 1;
+    for (const auto& c : kMx)
+      if (nm == c.name) return gemm_tiled(ctx, a, x, x_dtype, c, sp, stream);
+    return fail(ctx, RLXQ_E_NOKERNEL, "mxfp4_gemm: RLXQ_MX_CFG names no compiled tiling");
   }
-  const int64_t tiles_n = (n + 15) / 16, tiles_m = (m + 15) / 16;
-  if (tiles_m > 65535) return fail(ctx, RLXQ_E_SHAPE, "mxfp4_gemm: too many rows");
-  a.spans = (int)((k + 511) / 512);
-  a.splits = 1;
-  void* ws = nullptr;
-  if ((rc = workspace(ctx, (size_t)tiles_m * a.spans * RLXQ_MX_CHUNK, &ws, stream))) return rc;
-  a.xf = static_cast<uint8_t*>(ws);
-  if ((rc = quant_frag(ctx, a, x, x_dtype, 16, static_cast<uint8_t*>(ws), 0, nullptr, nullptr, stream))) return rc;
-  hipFunction_t fn;
-  const char* name = "rlxq_mx_dec_n1m1";
-  if ((rc = get_fn(ctx, name, &fn))) return rc;
-  const int waves = 8;
-  void* args[] = {&a};
-  return launch(ctx, fn, dim3((unsigned)tiles_n, (unsigned)tiles_m), dim3(64 * waves), (size_t)waves * 1024, stream, args,
-                name);
+  // (17 to 32 rows too: the tiles' preparation and LDS ring start slower than
+  // the weights stream, 4096 -> 4096 8.2 us against 11.9)
+  if (m <= 32) return gemm_decode(ctx, a, x, x_dtype, stream);
+  int splits = 1;
+  const MxCfg& c = pick_tiling(m, k, n, ctx->cu_count > 0 ? ctx->cu_count : 256, &splits);
+  return gemm_tiled(ctx, a, x, x_dtype, c, splits, stream);
 }
 
 }  // extern "C"

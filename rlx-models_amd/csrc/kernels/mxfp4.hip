@@ -196,17 +196,23 @@ RLXQ_DEV mx_f32x4_t mx_mfma16(const uint4& a, const uint4& b, mx_f32x4_t c, uint
 }
 
 // Few rows: a wave takes NT tiles of 16 weight rows (the MFMA's first operand,
-// straight from memory to registers) and MT tiles of 16 activation rows; the
-// waves of the workgroup take the spans of 512 elements in turn and their sums
-// meet in LDS.  Grid: (weight tiles, activation tiles, K splits).
-template <int NT, int MT>
+// straight from memory to registers, the next span's while this one is
+// multiplied) and MT tiles of 16 activation rows; the waves of the workgroup
+// take the spans of 512 elements in turn and their sums meet in LDS.  Weight
+// bytes bound it: 64 consecutive code bytes and four scale bytes per lane and
+// span, four MFMAs per 4 KB.
+// FUSED (MT == 1): the workgroup quantises the activation rows itself, into
+// LDS, while its first weights are on the way (no launch ahead of this one);
+// else they come as fragments from the preparation launch.
+template <int NT, int MT, bool FUSED, bool XBF>
 RLXQ_DEV void mx_dec_body(const rlxq_mx_gemm_args& a) {
-  extern __shared__ float mx_red[];   // [waves][NT * MT][256]
+  extern __shared__ __attribute__((aligned(16))) uint8_t mx_dec_lds[];
+  float* red = reinterpret_cast<float*>(mx_dec_lds);   // [waves][NT * MT][256], behind the activations
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int row = lane & 15, g = lane >> 4;
   const int nb = (int)(a.K / 32);
   const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
-  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  const int M = FUSED ? (int)a.M : 0;
   const uint8_t* wr[NT];
   const uint8_t* sr[NT];
 #pragma unroll
@@ -216,59 +222,98 @@ RLXQ_DEV void mx_dec_body(const rlxq_mx_gemm_args& a) {
     wr[t] = a.w + n * (a.K / 2);
     sr[t] = a.ws + n * nb;
   }
+  struct Buf {
+    uint4 c[NT][4];
+    uint32_t s[NT];
+  };
+  auto load = [&](int s, Buf& w) {
+    const int b0 = 16 * s + 4 * g;
+    if (16 * s + 16 <= nb) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.c[t][j] = *reinterpret_cast<const uint4*>(wr[t] + 16 * (int64_t)(b0 + j));
+        __builtin_memcpy(&w.s[t], sr[t] + b0, 4);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          w.c[t][j] = *reinterpret_cast<const uint4*>(wr[t] + 16 * (int64_t)(b0 + j < nb ? b0 + j : nb - 1));
+        w.s[t] = mx_load_scales(sr[t], b0, nb);
+      }
+    }
+  };
+  Buf cur;
+  if (wv < a.spans) load(wv, cur);
+  if constexpr (FUSED) {
+    // row m, span s: 64 code bytes and a dword of scales per lane group g, at
+    // (s M + m) 272 + 68 g
+    const int per = a.spans * 64;   // eights of a row, whole spans
+    for (int i = threadIdx.x; i < M * per; i += blockDim.x) {
+      const int m = i / per, e8 = i - m * per, blk = e8 >> 2;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (e8 * 8 < a.K) mx_load8<XBF>(a.x, (int64_t)m * a.K + e8 * 8, v);
+      uint32_t b;
+      const uint32_t c = mx_quant8<true>(v, b);
+      uint8_t* p = mx_dec_lds + ((blk >> 4) * M + m) * 272 + 68 * ((blk >> 2) & 3);
+      *reinterpret_cast<uint32_t*>(p + 16 * (blk & 3) + 4 * (e8 & 3)) = c;
+      if ((e8 & 3) == 0) p[64 + (blk & 3)] = (uint8_t)b;
+    }
+    red = reinterpret_cast<float*>(mx_dec_lds + ((a.spans * M * 272 + 15) & ~15));
+    __syncthreads();
+  }
   mx_f32x4_t acc[NT][MT];
 #pragma unroll
   for (int t = 0; t < NT; t++)
 #pragma unroll
     for (int q = 0; q < MT; q++) acc[t][q] = mx_f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int per = (a.spans + a.splits - 1) / a.splits;
-  const int s0 = (int)blockIdx.z * per, s1 = s0 + per < a.spans ? s0 + per : a.spans;
-  for (int s = s0 + wv; s < s1; s += nw) {
-    const int b0 = 16 * s + 4 * g;
-    uint4 wc[NT][4];
-    uint32_t wsc[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int b = b0 + j < nb ? b0 + j : nb - 1;
-        wc[t][j] = *reinterpret_cast<const uint4*>(wr[t] + 16 * (int64_t)b);
-      }
-      wsc[t] = mx_load_scales(sr[t], b0, nb);
-    }
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-      if (mx_has_zero(wsc[t])) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (((wsc[t] >> (8 * j)) & 0xffu) == 0u) wc[t][j] = make_uint4(0u, 0u, 0u, 0u);
-      }
-      wsc[t] = mx_scales(wsc[t]);
-    }
+  for (int s = wv; s < a.spans; s += nw) {
+    Buf nxt;
+    if (s + nw < a.spans) load(s + nw, nxt);
+    uint4 xc[MT][4];
+    uint32_t xs[MT];
 #pragma unroll
     for (int q = 0; q < MT; q++) {
-      const uint8_t* xp = a.xf + ((m0 / 16 + q) * (int64_t)a.spans + s) * RLXQ_MX_CHUNK;
-      uint4 xc[4];
-      uint32_t xs = 0;
+      xs[q] = 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) xc[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (m0 + 16 * q + row < a.M) {
+      for (int j = 0; j < 4; j++) xc[q][j] = make_uint4(0u, 0u, 0u, 0u);
+      if (16 * q + row < a.M) {
+        if constexpr (FUSED) {
+          const uint32_t* p = reinterpret_cast<const uint32_t*>(mx_dec_lds + (s * M + row) * 272 + 68 * g);
 #pragma unroll
-        for (int j = 0; j < 4; j++) xc[j] = *reinterpret_cast<const uint4*>(xp + 1024 * j + 16 * lane);
-        xs = *reinterpret_cast<const uint32_t*>(xp + 4096 + 4 * lane);
-      }
+          for (int j = 0; j < 4; j++) xc[q][j] = make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+          xs[q] = p[16];
+        } else {
+          const uint8_t* xp = a.xf + (q * (int64_t)a.spans + s) * RLXQ_MX_CHUNK;
 #pragma unroll
-      for (int t = 0; t < NT; t++) {
-        acc[t][q] = mx_mfma16<0>(wc[t][0], xc[0], acc[t][q], wsc[t], xs);
-        acc[t][q] = mx_mfma16<1>(wc[t][1], xc[1], acc[t][q], wsc[t], xs);
-        acc[t][q] = mx_mfma16<2>(wc[t][2], xc[2], acc[t][q], wsc[t], xs);
-        acc[t][q] = mx_mfma16<3>(wc[t][3], xc[3], acc[t][q], wsc[t], xs);
+          for (int j = 0; j < 4; j++) xc[q][j] = *reinterpret_cast<const uint4*>(xp + 1024 * j + 16 * lane);
+          xs[q] = *reinterpret_cast<const uint32_t*>(xp + 4096 + 4 * lane);
+        }
       }
     }
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      if (mx_has_zero(cur.s[t])) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (((cur.s[t] >> (8 * j)) & 0xffu) == 0u) cur.c[t][j] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      const uint32_t sw = mx_scales(cur.s[t]);
+#pragma unroll
+      for (int q = 0; q < MT; q++) {
+        acc[t][q] = mx_mfma16<0>(cur.c[t][0], xc[q][0], acc[t][q], sw, xs[q]);
+        acc[t][q] = mx_mfma16<1>(cur.c[t][1], xc[q][1], acc[t][q], sw, xs[q]);
+        acc[t][q] = mx_mfma16<2>(cur.c[t][2], xc[q][2], acc[t][q], sw, xs[q]);
+        acc[t][q] = mx_mfma16<3>(cur.c[t][3], xc[q][3], acc[t][q], sw, xs[q]);
+      }
+    }
+    cur = nxt;
   }
-  // D: lane holds rows (weight rows) 4 g .. 4 g + 3 of column (activation row)
-  // lane & 15; word i of tile (t, q) is weight row i / 16, activation row i % 16
-  float* mine = mx_red + wv * (NT * MT * 256);
+  // D: lane holds weight rows 4 g .. 4 g + 3 of activation row lane & 15; word
+  // 16 n + m of tile (t, q) is weight row n, activation row m
+  float* mine = red + wv * (NT * MT * 256);
 #pragma unroll
   for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -279,13 +324,12 @@ RLXQ_DEV void mx_dec_body(const rlxq_mx_gemm_args& a) {
   for (int i = threadIdx.x; i < NT * MT * 256; i += blockDim.x) {
     // neighbouring threads take neighbouring columns of y
     const int q = i / (NT * 256), m = (i / (NT * 16)) & 15, n = i % (NT * 16);
-    const int64_t mm = m0 + 16 * q + m, nn = n0 + n;
+    const int64_t mm = 16 * q + m, nn = n0 + n;
     if (mm >= a.M || nn >= a.N) continue;
-    const float* p = mx_red + ((n >> 4) * MT + q) * 256 + (n & 15) * 16 + m;
+    const float* p = red + ((n >> 4) * MT + q) * 256 + (n & 15) * 16 + m;
     float s = 0.f;
     for (int v = 0; v < nw; v++) s += p[v * (NT * MT * 256)];
-    if (a.splits > 1) a.part[((int64_t)blockIdx.z * a.M + mm) * a.N + nn] = s;
-    else if (a.y_bf16) reinterpret_cast<uint16_t*>(a.y)[mm * a.N + nn] = (uint16_t)f32_to_bf16_bits(s);
+    if (a.y_bf16) reinterpret_cast<uint16_t*>(a.y)[mm * a.N + nn] = (uint16_t)f32_to_bf16_bits(s);
     else reinterpret_cast<float*>(a.y)[mm * a.N + nn] = s;
   }
 }
@@ -654,18 +698,27 @@ extern "C" __global__ __launch_bounds__(256) void rlxq_mx_reduce(rlxq_mx_gemm_ar
   extern "C" __global__ __launch_bounds__(64 * WGM * WGN) void rlxq_mx_gemm_##NAME(rlxq_mx_gemm_args a) { \
     rlxq::mx_gemm_body<WGM, WGN, TM, TN>(a);                                                             \
   }
-RLXQ_MX_GEMM(m256n256, 2, 2, 4, 4)
-RLXQ_MX_GEMM(m256n256w8, 2, 4, 4, 2)
+RLXQ_MX_GEMM(m256n256, 2, 4, 4, 2)
 RLXQ_MX_GEMM(m128n128, 2, 2, 2, 2)
-RLXQ_MX_GEMM(m128n256, 2, 2, 2, 4)
-RLXQ_MX_GEMM(m64n64, 1, 2, 2, 1)
-RLXQ_MX_GEMM(m64n128, 1, 2, 2, 2)
 RLXQ_MX_GEMM(m128n64, 2, 1, 2, 2)
-RLXQ_MX_GEMM(m32n64, 1, 1, 1, 2)
+RLXQ_MX_GEMM(m64n64, 1, 2, 2, 1)
 
 extern "C" __global__ __launch_bounds__(256) void rlxq_mx_quant_bf16(rlxq_mx_quant_args a) { rlxq::mx_quant_rows<true>(a); }
 extern "C" __global__ __launch_bounds__(256) void rlxq_mx_quant_f32(rlxq_mx_quant_args a) { rlxq::mx_quant_rows<false>(a); }
 extern "C" __global__ __launch_bounds__(256) void rlxq_mx_frag_bf16(rlxq_mx_quant_args a) { rlxq::mx_quant_frag<true>(a); }
 extern "C" __global__ __launch_bounds__(256) void rlxq_mx_frag_f32(rlxq_mx_quant_args a) { rlxq::mx_quant_frag<false>(a); }
 
-extern "C" __global__ __launch_bounds__(512) void rlxq_mx_dec_n1m1(rlxq_mx_gemm_args a) { rlxq::mx_dec_body<1, 1>(a); }
+
+// rlxq_mx_dec_<weight tiles>_<activation tiles>, _f<type>: quantising itself
+#define RLXQ_MX_DEC(NAME, NT, MT, FUSED, XBF, WAVES)                                                      \
+  extern "C" __global__ __launch_bounds__(64 * WAVES) void rlxq_mx_dec_##NAME(rlxq_mx_gemm_args a) {      \
+    rlxq::mx_dec_body<NT, MT, FUSED, XBF>(a);                                                      \
+  }
+RLXQ_MX_DEC(n1m1, 1, 1, false, false, 16)
+RLXQ_MX_DEC(n2m1, 2, 1, false, false, 8)
+RLXQ_MX_DEC(n1m2, 1, 2, false, false, 16)
+RLXQ_MX_DEC(n2m2, 2, 2, false, false, 8)
+RLXQ_MX_DEC(n1_fbf16, 1, 1, true, true, 16)
+RLXQ_MX_DEC(n2_fbf16, 2, 1, true, true, 8)
+RLXQ_MX_DEC(n1_ff32, 1, 1, true, false, 16)
+RLXQ_MX_DEC(n2_ff32, 2, 1, true, false, 8)

@@ -32,6 +32,7 @@ typedef struct rlxq_mx_quant_args {
 
 typedef struct rlxq_mx_gemm_args {
   const uint8_t* xf;  /* activation fragments                                */
+  const void* x;      /* kernels that quantise them themselves: [M, K]       */
   const uint8_t* w;   /* codes [N, K / 2]                                    */
   const uint8_t* ws;  /* E8M0 scales [N, K / 32]                             */
   void* y;            /* [M, N] f32 or bf16                                  */

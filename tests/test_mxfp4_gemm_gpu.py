@@ -130,7 +130,14 @@ def _want(orc, xv, codes, eb, n):
 
 def _check(y, want, s, k, bf16):
     tol = k * 2.0 ** -23 * s + (2.0 ** -8 * np.abs(want) if bf16 else 0.0)
-    err = np.abs(y - want)
+    # A true value past f32's largest, (2 - 2^-23) 2^127, has no finite f32: its
+    # output is the infinity of its sign.  Where only S passes it, a partial sum
+    # may, and no bound holds.
+    top = float(np.finfo(np.float32).max)
+    big = s > top
+    past = np.abs(want) > top * (1 + 2.0 ** -24) + tol
+    assert np.array_equal(y[past], np.sign(want[past]) * np.inf)
+    err = np.where(big, 0.0, np.abs(np.where(big, 0.0, y) - np.where(big, 0.0, want)))
     assert np.all(err <= tol), f"worst {np.max(err - tol):.3e} over the bound, max err {np.max(err):.3e}"
 
 
@@ -138,7 +145,10 @@ def _weights(rng, n, k, lo=110, hi=130):
     return rng.integers(0, 256, (n, k // 2), dtype=np.uint8), rng.integers(lo, hi, (n, k // 32), dtype=np.uint8)
 
 
-SHAPES = [(1, 32, 1), (1, 4096, 512), (2, 96, 33), (5, 480, 17), (16, 512, 64), (17, 544, 100), (33, 1056, 250),
+# (K in part of a span of 512 or 256 and of a stage of 128, more and fewer spans
+# than waves, 16 and 32 weight rows a workgroup, activations quantised inside
+# and ahead, one tile and many, edges in every direction)
+SHAPES = [(1, 32, 1), (2, 1056, 6200), (3, 8704, 40), (12, 2176, 6176), (20, 160, 6190), (31, 9216, 130), (9, 4096, 520), (1, 4096, 512), (2, 96, 33), (5, 480, 17), (16, 512, 64), (17, 544, 100), (33, 1056, 250),
           (64, 2048, 384), (130, 800, 301), (200, 4096, 96), (257, 320, 513), (300, 1536, 640), (512, 288, 1025)]
 
 
@@ -157,6 +167,64 @@ def test_gemm(ctx, orc, shape, xdt, ydt):
     assert ctx.last_kernel.startswith("rlxq_mx_")
     want, s = _want(orc, xv, codes, eb, n)
     _check(y.double().cpu().numpy(), want, s, k, ydt == "bf16")
+
+
+@pytest.mark.parametrize("cfg", ["m256n256", "m256n256,3", "m128n128", "m128n128,2", "m128n64", "m128n64,4", "m64n64",
+                                 "m64n64,2"])
+@pytest.mark.parametrize("shape", [(1, 32, 1), (33, 96, 70), (70, 2336, 264), (130, 800, 301), (256, 256, 256),
+                                   (300, 1536, 640), (512, 1152, 520)], ids=lambda s: "x".join(map(str, s)))
+def test_gemm_every_tiling(ctx, orc, monkeypatch, shape, cfg):
+    """Every tiling with and without K splits (an odd number of spans, of stages
+    within the last one, more splits than spans), and weight blocks of scale 0."""
+    import torch
+
+    m, k, n = shape
+    announce(f"mxfp4_gemm {cfg} {shape}")
+    monkeypatch.setenv("RLXQ_MX_CFG", cfg)
+    rng = np.random.default_rng(m + 3 * k + n)
+    codes, eb = _weights(rng, n, k)
+    for zeros, ydt in ((False, torch.bfloat16), (True, torch.float32)):
+        if zeros:
+            eb[rng.random(eb.shape) < 0.1] = 0
+            eb[n // 2, 0] = 255
+        x, xv = _as((rng.standard_normal((m, k)) * np.exp(rng.standard_normal(k))).astype(np.float32), "bf16")
+        y = ctx.mxfp4_gemm(x, _t(codes), _t(eb), n, y_dtype=ydt)
+        torch.cuda.synchronize()
+        assert ctx.last_kernel == "rlxq_mx_gemm_" + cfg.split(",")[0]
+        want, s = _want(orc, xv, codes, eb, n)
+        _check(y.double().cpu().numpy(), want, s, k, ydt == torch.bfloat16)
+
+
+def test_gemm_unknown_tiling(ctx, monkeypatch):
+    import rlxq
+    import torch
+
+    monkeypatch.setenv("RLXQ_MX_CFG", "m7n7")
+    w, s = torch.zeros((8, 32), dtype=torch.uint8, device="cuda"), torch.zeros((8, 2), dtype=torch.uint8, device="cuda")
+    with pytest.raises(rlxq.RlxqError) as e:
+        ctx.mxfp4_gemm(torch.zeros((2, 64), device="cuda"), w, s, 8)
+    assert e.value.status == rlxq.E_NOKERNEL
+
+
+def test_gemm_unaligned_output_and_scales(ctx, orc):
+    """y and the scales at addresses that allow no wide access."""
+    import torch
+
+    for m, k, n in ((3, 352, 40), (200, 352, 264)):
+        announce(f"mxfp4_gemm unaligned {m}x{k}x{n}")
+        rng = np.random.default_rng(11)
+        codes, eb = _weights(rng, n, k)
+        buf = torch.zeros(n * k // 32 + 3, dtype=torch.uint8, device="cuda")
+        s = buf[3:].view(n, k // 32)
+        s.copy_(_t(eb))
+        x, xv = _as(rng.standard_normal((m, k)).astype(np.float32), "f32")
+        out = torch.full((m * n + 3,), 7.0, device="cuda")
+        y = out[1:1 + m * n].view(m, n)
+        ctx.mxfp4_gemm(x, _t(codes), s, n, y=y)
+        torch.cuda.synchronize()
+        want, sm = _want(orc, xv, codes, eb, n)
+        _check(y.double().cpu().numpy(), want, sm, k, False)
+        assert out[0] == 7.0 and torch.all(out[1 + m * n:] == 7.0)
 
 
 @pytest.mark.parametrize("m", [1, 3, 40, 300])

@@ -20,6 +20,10 @@ namespace {
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
+// Groups of elements per thread of the row kernels: four once they still give
+// 16 workgroups a CU (mx_quant_rows' figures).
+int rows_ilp(int64_t groups) { return groups >= (int64_t)4096 * 1024 ? 4 : 1; }
+
 // The activations as fragments of `rows` rows (mxfp4_args.h); wblocks > 0:
 // the weights' scales in the lane order of 32-row fragments beside them.
 int quant_frag(rlxq_ctx* ctx, const rlxq_mx_gemm_args& g, const void* x, int x_dtype, int rows, uint8_t* xf,
@@ -168,6 +172,24 @@ int gemm_decode(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, 
 
 }  // namespace
 
+// Values of MXFP4 rows with E8M0 scales (rlxq_dequantize).
+int mx_dequantize(rlxq_ctx* ctx, const void* codes, const void* scales, int64_t rows, int64_t k, float* out, void* stream) {
+  rlxq_mx_quant_args a;
+  std::memset(&a, 0, sizeof a);
+  a.codes = static_cast<uint8_t*>(const_cast<void*>(codes));
+  a.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  a.M = rows;
+  a.K = k;
+  hipFunction_t fn;
+  const int u = rows_ilp(rows * (k / 4));
+  int rc = get_fn(ctx, u == 1 ? "rlxq_mx_dequant_u1" : "rlxq_mx_dequant_u4", &fn);
+  if (rc) return rc;
+  const int64_t grid = (rows * (k / 4) + 256 * u - 1) / (256 * u);
+  if (grid > 0x7fffffff) return fail(ctx, RLXQ_E_SHAPE, "dequantize: too many weights");
+  void* args[] = {&a, &out};
+  return launch(ctx, fn, dim3((unsigned)grid), dim3(256), 0, stream, args, "dequantize");
+}
+
 }  // namespace rlxq
 
 using namespace rlxq;
@@ -196,12 +218,14 @@ int rlxq_quantize_mxfp4(rlxq_ctx* ctx, const void* x, int x_dtype, int64_t m, in
   a.scales = scales;
   a.M = m;
   a.K = k;
-  const char* name = x_dtype == RLXQ_BF16 ? "rlxq_mx_quant_bf16" : "rlxq_mx_quant_f32";
+  const int u = rows_ilp(m * (k / 8));
+  char name[32];
+  std::snprintf(name, sizeof name, "rlxq_mx_quant_%s_u%d", x_dtype == RLXQ_BF16 ? "bf16" : "f32", u);
   hipFunction_t fn;
   int rc = get_fn(ctx, name, &fn);
   if (rc) return rc;
-  const int64_t grid = (m * (k / 8) + 255) / 256;
-  if (grid > 0x7fffffff) return fail(ctx, RLXQ_E_SHAPE, "quantize_mxfp4: more than 2^42 elements");
+  const int64_t grid = (m * (k / 8) + 256 * u - 1) / (256 * u);
+  if (grid > 0x7fffffff) return fail(ctx, RLXQ_E_SHAPE, "quantize_mxfp4: more than 2^43 elements");
   void* args[] = {&a};
   return launch(ctx, fn, dim3((unsigned)grid), dim3(256), 0, stream, args, name);
 }

@@ -687,6 +687,10 @@ int rlxq_dequantize(rlxq_ctx* ctx, int scheme, int group_size, const void* w, co
   if (rc) return rc;
   if (rows == 0) return RLXQ_OK;
   DeviceGuard g(ctx->device);
+  // MXFP4 with E8M0 scales: the kernel beside its quantiser (24576 x 4096:
+  // 124 us here) where the rows can leave in 16-byte stores
+  if (scheme == RLXQ_MLX_MXFP4 && sb_dtype == RLXQ_U8 && aligned(out, 16))
+    return mx_dequantize(ctx, w, scales, rows, k, out, stream);
   hipFunction_t fn;
   if ((rc = get_fn(ctx, "rlxq_dequant_rows", &fn))) return rc;
   int sch = scheme, sb = sb_code(sb_dtype), grp = is_mlx(scheme) ? group_size : 32, K = (int)k;

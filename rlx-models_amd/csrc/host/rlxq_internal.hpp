@@ -170,5 +170,7 @@ int bs_dispatch(rlxq_ctx* ctx, int scheme, const float* x, const void* w, int64_
 int i8b_dispatch(rlxq_ctx* ctx, int group, const void* x, int x_dtype, const void* w, const void* scales,
                  const void* zp, int sb_dtype, int64_t m, int64_t k, int64_t n, void* y, int y_dtype,
                  void* stream);
+int mx_dequantize(rlxq_ctx* ctx, const void* codes, const void* scales, int64_t rows, int64_t k, float* out,
+                  void* stream);
 
 }  // namespace rlxq

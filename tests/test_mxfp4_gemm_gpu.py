@@ -100,6 +100,30 @@ def test_quantize_not_finite(ctx, orc, xdt):
     np.testing.assert_array_equal(codes.cpu().numpy(), wc)
 
 
+@pytest.mark.parametrize("xdt", ["bf16", "f32"])
+def test_quantize_and_dequantize_large(ctx, orc, xdt):
+    """The kernels of large matrices (several groups of elements per thread, the
+    last workgroup part filled): sampled rows, the last ones among them."""
+    import rlxq
+    import torch
+
+    m, k = 8201, 4128
+    announce(f"quantize_mxfp4, dequantize {m}x{k} {xdt}")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    x = torch.randn((m, k), device="cuda", generator=gen).to(torch.bfloat16 if xdt == "bf16" else torch.float32)
+    codes, scales = ctx.quantize_mxfp4(x)
+    v = ctx.dequantize(codes, rlxq.MLX_MXFP4, m, k, scales=scales)
+    torch.cuda.synchronize()
+    rows = np.unique(np.concatenate([np.arange(4), np.arange(m - 4, m), np.random.default_rng(2).integers(0, m, 60)]))
+    at = torch.from_numpy(rows).cuda()
+    wc, wb = orc.mxfp4_quantize(x[at].float().cpu().numpy())
+    np.testing.assert_array_equal(scales[at].cpu().numpy(), wb)
+    np.testing.assert_array_equal(codes[at].cpu().numpy(), wc)
+    want = orc.mxfp4_dequantize(wc, wb, len(rows), k).astype(np.float32)
+    np.testing.assert_array_equal(v[at].cpu().numpy(), want)
+
+
 def test_quantize_then_dequantize_and_matmul(ctx, orc):
     """Together: rows packed on the device, decoded, and used as the weights of
     the dense op."""

@@ -33,7 +33,7 @@ HIPCC = str(ROCM / "bin" / "hipcc")
 # <name><i>.co; the parts build in parallel).  A name without a source file is
 # embedded empty and skipped at load time.
 CODE_OBJECTS = (("gemv", 6), ("misc", 1), ("gemm", 1), ("moe", 5), ("int8", 1), ("skinny", 1), ("bsgemm", 3),
-                ("mfgemv", 1), ("mxfp4", 1), ("moelayer", 1))
+                ("mfgemv", 1), ("mxfp4", 1), ("moelayer", 6))
 
 HIP_FLAGS = [
     "--genco", "--offload-arch=gfx950", "-O3", "-std=c++17",

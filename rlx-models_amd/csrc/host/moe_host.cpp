@@ -555,6 +555,115 @@ int layer_pick(rlxq_ctx* ctx, const LayerCall& c, const float* logits, int32_t* 
   return launch(ctx, fn, dim3((unsigned)c.rows), dim3(64), 0, stream, args, name);
 }
 
+// Lanes (2^log2l) and units per lane (NU) that spread a row of `units` over a
+// wave with the fewest idle lanes; false if no compiled shape holds it.
+bool few_shape(int scheme, int64_t k, int* log2l, int* nu) {
+  const int blocks = scheme == RLXQ_GGUF_Q4_0 || scheme == RLXQ_GGUF_Q8_0 || scheme == RLXQ_GGUF_Q4_K ||
+                     scheme == RLXQ_GGUF_Q5_K ? 2 : 1;
+  const int64_t units = k / 32 / blocks;
+  const int most = blocks == 2 ? 2 : 4;
+  int64_t best = 0;
+  for (int l = 6; l >= 2; l--)   // (ties: more lanes per row, fewer registers)
+    for (int u = 1; u <= most; u++) {
+      const int64_t cap = ((int64_t)u) << l;
+      if (cap >= units && (best == 0 || cap < best)) best = cap, *log2l = l, *nu = u;
+    }
+  return best != 0;
+}
+
+size_t few_down_lds(const LayerCall& c, int64_t tile) {
+  return (size_t)(c.top_k * (c.inter * 4 + c.inter / 32 * 16 + tile * 4));
+}
+
+// Whether the few-token kernels hold the call: entries and expert choices fit a
+// workgroup, rows fit a wave's registers, the down launch's planes its LDS.
+bool few_holds(const rlxq_ctx* ctx, const LayerCall& c) {
+  int l, u;
+  return c.rows * c.top_k <= 256 && c.hidden <= 8192 && c.inter <= 8192 && few_shape(c.gu_scheme, c.hidden, &l, &u) &&
+         few_shape(c.d_scheme, c.inter, &l, &u) && few_down_lds(c, 256) <= std::min<size_t>(ctx->max_lds, 160 * 1024);
+}
+
+// Three launches: router product and prepared rows; routing, gate|up and
+// SwiGLU; down and the weighted sum.  The activations in between are f32.
+int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
+  auto r256 = [](size_t b) { return (b + 255) & ~size_t(255); };
+  const size_t n = (size_t)(c.rows * c.top_k), xn = (size_t)(c.rows * c.hidden);
+  const bool xbf = c.x_dtype == RLXQ_BF16;
+  const size_t b_log = c.logits ? 0 : r256((size_t)(c.rows * c.experts) * 4), b_ids = r256(n * 4), b_pr = r256(n * 4);
+  const size_t b_hi = r256(xn * 2), b_lo = xbf ? 0 : r256(xn * 2), b_meta = r256(xn / 32 * 16), b_act = r256(n * (size_t)c.inter * 4);
+  void* ws = nullptr;
+  int rc;
+  if ((rc = workspace(ctx, b_log + b_ids + b_pr + b_hi + b_lo + b_meta + b_act, &ws, stream))) return rc;
+  char* p = static_cast<char*>(ws);
+  const int64_t cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
+
+  rlxq_moe_prep_args pa;
+  std::memset(&pa, 0, sizeof pa);
+  pa.r.x = c.x;
+  pa.r.router = c.router;
+  pa.r.logits = reinterpret_cast<float*>(p);
+  pa.r.rows = c.rows;
+  pa.r.H = c.hidden;
+  pa.r.E = (int32_t)c.experts;
+  pa.hi = reinterpret_cast<uint16_t*>(p + b_log + b_ids + b_pr);
+  pa.lo = xbf ? nullptr : reinterpret_cast<uint16_t*>(p + b_log + b_ids + b_pr + b_hi);
+  pa.meta = reinterpret_cast<float*>(p + b_log + b_ids + b_pr + b_hi + b_lo);
+  pa.lblocks = c.logits ? 0 : (int32_t)(c.experts * ((c.rows + 3) / 4));
+  char name[64];
+  std::snprintf(name, sizeof name, "rlxq_moe_prep_%s_%s", xbf ? "bf16" : "f32", c.router_dtype == RLXQ_BF16 ? "bf16" : "f32");
+  hipFunction_t fn;
+  if ((rc = get_fn(ctx, name, &fn))) return rc;
+  void* pargs[] = {&pa};
+  if ((rc = launch(ctx, fn, dim3((unsigned)(pa.lblocks + (xn / 4 + 63) / 64)), dim3(64), 0, stream, pargs, name))) return rc;
+
+  rlxq_moe_few_args a;
+  std::memset(&a, 0, sizeof a);
+  a.hi = pa.hi;
+  a.lo = pa.lo;
+  a.meta = pa.meta;
+  a.logits = c.logits ? c.logits : pa.r.logits;
+  a.ids = reinterpret_cast<int32_t*>(p + b_log);
+  a.probs = reinterpret_cast<float*>(p + b_log + b_ids);
+  a.act = reinterpret_cast<float*>(p + b_log + b_ids + b_pr + b_hi + b_lo + b_meta);
+  a.ids2 = c.ids;
+  a.probs2 = c.probs;
+  a.y = c.y;
+  a.rows = (int32_t)c.rows;
+  a.H = (int32_t)c.hidden;
+  a.I = (int32_t)c.inter;
+  a.E = (int32_t)c.experts;
+  a.top_k = (int32_t)c.top_k;
+  a.renorm = c.renorm;
+  a.y_bf16 = c.y_dtype == RLXQ_BF16;
+  int nu = 0;
+  few_shape(c.gu_scheme, c.hidden, &a.log2l, &nu);
+  a.bank = static_cast<const uint8_t*>(c.gu);
+  a.scales = static_cast<const uint8_t*>(c.gu_s);
+  if ((rc = check_weights(ctx, "moe_layer gate_up", c.gu_scheme, 32, c.gu, c.gu_s, nullptr, RLXQ_U8, c.hidden, &a.rb))) return rc;
+  std::snprintf(name, sizeof name, "rlxq_moefew_gu_%s_u%d_p%d", scheme_name(c.gu_scheme), nu, xbf ? 1 : 2);
+  if ((rc = get_fn(ctx, name, &fn))) return rc;
+  void* args[] = {&a};
+  // one round of workgroups
+  const int per_cu = std::min(2, blocks_per_cu(ctx, name, fn, 512, 0));
+  const int64_t steps = (int64_t)n * ((c.inter + (64 >> a.log2l) - 1) / (64 >> a.log2l));
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(cus * per_cu, (steps + 7) / 8));
+  if ((rc = launch(ctx, fn, dim3((unsigned)grid), dim3(512), 0, stream, args, name))) return rc;
+
+  few_shape(c.d_scheme, c.inter, &a.log2l, &nu);
+  a.bank = static_cast<const uint8_t*>(c.d);
+  a.scales = static_cast<const uint8_t*>(c.d_s);
+  if ((rc = check_weights(ctx, "moe_layer down", c.d_scheme, 32, c.d, c.d_s, nullptr, RLXQ_U8, c.inter, &a.rb))) return rc;
+  // column tiles: two workgroups a CU, whole steps of the waves of a slot
+  const int64_t rp = 64 >> a.log2l, unit = rp * std::max<int64_t>(1, 8 / c.top_k);
+  int64_t tile = (c.rows * c.hidden + 2 * cus - 1) / (2 * cus);
+  tile = std::min<int64_t>(256, std::max<int64_t>(unit, (tile + unit - 1) / unit * unit));
+  a.tile = (int32_t)tile;
+  a.tiles = (int32_t)((c.hidden + tile - 1) / tile);
+  std::snprintf(name, sizeof name, "rlxq_moefew_dn_%s_u%d", scheme_name(c.d_scheme), nu);
+  if ((rc = get_fn(ctx, name, &fn))) return rc;
+  return launch(ctx, fn, dim3((unsigned)(c.rows * a.tiles)), dim3(512), few_down_lds(c, tile), stream, args, name);
+}
+
 // The layer from the library's own calls: router product, top-k, grouped
 // gate|up + SwiGLU, grouped down + weighted sum.  The activations between the
 // two grouped products have x's type (bf16 ones are what the grouped register
@@ -675,7 +784,9 @@ int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype, const void* router
   if (!g.ok()) return fail(ctx, RLXQ_E_HIP, "moe_layer: hipSetDevice");
   const LayerCall c{x,        x_dtype, router, router_dtype, logits, gate_up_scheme, gate_up, gate_up_scales, down_scheme,
                     down,     down_scales, rows, hidden, inter, num_experts, top_k, renorm, ids, probs, y, y_dtype};
-  return layer_grouped(ctx, c, stream);
+  bool few = few_holds(ctx, c);
+  if (const char* e = std::getenv("RLXQ_MOE_LAYER")) few = few && std::strcmp(e, "grouped") != 0;
+  return few ? layer_few(ctx, c, stream) : layer_grouped(ctx, c, stream);
 }
 
 }  // extern "C"

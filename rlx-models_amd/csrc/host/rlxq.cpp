@@ -52,7 +52,12 @@ RLXQ_EMBED(rlxq_co_bsgemm1, "bsgemm1.co")
 RLXQ_EMBED(rlxq_co_bsgemm2, "bsgemm2.co")
 RLXQ_EMBED(rlxq_co_mfgemv, "mfgemv.co")
 RLXQ_EMBED(rlxq_co_mxfp4, "mxfp4.co")
-RLXQ_EMBED(rlxq_co_moelayer, "moelayer.co")
+RLXQ_EMBED(rlxq_co_moelayer0, "moelayer0.co")
+RLXQ_EMBED(rlxq_co_moelayer1, "moelayer1.co")
+RLXQ_EMBED(rlxq_co_moelayer2, "moelayer2.co")
+RLXQ_EMBED(rlxq_co_moelayer3, "moelayer3.co")
+RLXQ_EMBED(rlxq_co_moelayer4, "moelayer4.co")
+RLXQ_EMBED(rlxq_co_moelayer5, "moelayer5.co")
 
 namespace {
 
@@ -83,7 +88,12 @@ const Image kImages[] = {
     {rlxq_co_bsgemm2_begin, rlxq_co_bsgemm2_end, "bsgemm2"},
     {rlxq_co_mfgemv_begin, rlxq_co_mfgemv_end, "mfgemv"},
     {rlxq_co_mxfp4_begin, rlxq_co_mxfp4_end, "mxfp4"},
-    {rlxq_co_moelayer_begin, rlxq_co_moelayer_end, "moelayer"},
+    {rlxq_co_moelayer0_begin, rlxq_co_moelayer0_end, "moelayer0"},
+    {rlxq_co_moelayer1_begin, rlxq_co_moelayer1_end, "moelayer1"},
+    {rlxq_co_moelayer2_begin, rlxq_co_moelayer2_end, "moelayer2"},
+    {rlxq_co_moelayer3_begin, rlxq_co_moelayer3_end, "moelayer3"},
+    {rlxq_co_moelayer4_begin, rlxq_co_moelayer4_end, "moelayer4"},
+    {rlxq_co_moelayer5_begin, rlxq_co_moelayer5_end, "moelayer5"},
 };
 
 std::string hip_msg(hipError_t e) { return std::string(hipGetErrorName(e)) + ": " + hipGetErrorString(e); }

@@ -108,4 +108,38 @@ typedef struct rlxq_moe_pick_args {
   int32_t E, top_k, renorm, pad;
 } rlxq_moe_pick_args;
 
+/* Few-token expert layer.  The activation rows as f16 planes ("prepared"):
+ * of each 32-element block, scaled by the power of two that brings its largest
+ * magnitude into [2^14, 2^15), the rounded values (hi) and, for f32 rows, their
+ * rounded remainders (lo); and per block four floats: the factor that undoes
+ * the scaling, the sum of the block's elements, that of its first 16, 0.     */
+typedef struct rlxq_moe_prep_args {
+  rlxq_moe_logits_args r;   /* the router's part (r.router NULL: none)       */
+  uint16_t* hi;             /* [rows, H]                                     */
+  uint16_t* lo;             /* [rows, H], or NULL (bf16 rows)                */
+  float* meta;              /* [rows, H / 32, 4]                             */
+  int32_t lblocks, pad;     /* workgroups of the router's part, ahead        */
+} rlxq_moe_prep_args;
+
+typedef struct rlxq_moe_few_args {
+  /* gate|up: prepared rows in, act out.  down: act in, y out.               */
+  const uint16_t* hi;
+  const uint16_t* lo;
+  const float* meta;
+  const float* logits;      /* [rows, E]                                     */
+  float* act;               /* [rows * top_k, I] silu(g) * u                 */
+  int32_t* ids;             /* [rows, top_k], written by gate|up             */
+  float* probs;
+  int32_t* ids2;            /* the caller's copies, or NULL                  */
+  float* probs2;
+  const uint8_t* bank;      /* E slabs of packed rows                        */
+  const uint8_t* scales;    /* MXFP4: E8M0 bytes, else NULL                  */
+  void* y;                  /* [rows, H]                                     */
+  int64_t rb;               /* bytes of a packed row                         */
+  int32_t rows, H, I, E, top_k, renorm, y_bf16;
+  int32_t log2l;            /* lanes of a weight row: 4 .. 64                */
+  int32_t tile;             /* down: columns of a workgroup                  */
+  int32_t tiles;            /* down: column tiles                            */
+} rlxq_moe_few_args;
+
 #endif

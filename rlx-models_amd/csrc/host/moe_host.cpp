@@ -555,45 +555,63 @@ int layer_pick(rlxq_ctx* ctx, const LayerCall& c, const float* logits, int32_t* 
   return launch(ctx, fn, dim3((unsigned)c.rows), dim3(64), 0, stream, args, name);
 }
 
-// Lanes (2^log2l) and units per lane (NU) that spread a row of `units` over a
-// wave with the fewest idle lanes; false if no compiled shape holds it.
-bool few_shape(int scheme, int64_t k, int* log2l, int* nu) {
+// Lanes (2^log2l) a weight row of K elements is spread over.  Fewer lanes a row
+// take more rows at once, which share the reduction and the stores and read an
+// activation record together; the waves still want `cols` columns' worth of
+// steps each.  Of the widths that give it, the one with the fewest idle lanes.
+int few_log2l(int scheme, int64_t k, double cols) {
   const int blocks = scheme == RLXQ_GGUF_Q4_0 || scheme == RLXQ_GGUF_Q8_0 || scheme == RLXQ_GGUF_Q4_K ||
                      scheme == RLXQ_GGUF_Q5_K ? 2 : 1;
   const int64_t units = k / 32 / blocks;
-  const int most = blocks == 2 ? 2 : 4;
-  int64_t best = 0;
-  for (int l = 6; l >= 2; l--)   // (ties: more lanes per row, fewer registers)
-    for (int u = 1; u <= most; u++) {
-      const int64_t cap = ((int64_t)u) << l;
-      if (cap >= units && (best == 0 || cap < best)) best = cap, *log2l = l, *nu = u;
-    }
-  return best != 0;
+  int lo = 6;   // 64 / 2^lo rows at once
+  while (lo > 3 && (double)(64 >> (lo - 1)) <= cols) lo--;
+  if (const char* e = std::getenv("RLXQ_FEW_L")) lo = std::atoi(e);
+  int best = lo;
+  int64_t cap = ((units + (1 << lo) - 1) >> lo) << lo;
+  for (int l = lo - 1; l >= 3 && l >= lo - 1; l--) {
+    const int64_t c = ((units + (1 << l) - 1) >> l) << l;
+    if (c < cap) cap = c, best = l;
+  }
+  return best;
 }
-
+int few_order(int scheme) {   // of a block's codes (moe_args.h)
+  return scheme == RLXQ_MLX_MXFP4 ? 0 : scheme == RLXQ_GGUF_Q4_0 || scheme == RLXQ_GGUF_Q4_1 ? 1 : 2;
+}
 size_t few_down_lds(const LayerCall& c, int64_t tile) {
-  return (size_t)(c.top_k * (c.inter * 4 + c.inter / 32 * 16 + tile * 4));
+  return (size_t)(c.top_k * (c.inter / 32 * RLXQ_FEW_REC(2) + tile * 4));
+}
+constexpr int64_t kFewTile = 256;   // most columns of a down workgroup
+
+// Entries of one expert that share a pass over its weights, by the entries per
+// fired expert to expect of even routing (one row: every expert once).
+int few_mt(const LayerCall& c) {
+  if (c.rows == 1) return 1;
+  const double e = (double)c.experts, k = (double)c.top_k, r = (double)c.rows;
+  const double avg = r * k / (e * (1.0 - std::pow(1.0 - k / e, r)));
+  return avg < 1.1 ? 1 : avg < 2.2 ? 2 : 4;
 }
 
-// Whether the few-token kernels hold the call: entries and expert choices fit a
-// workgroup, rows fit a wave's registers, the down launch's planes its LDS.
+// Whether the few-token kernels hold the call: entries fit a workgroup's tables,
+// the activation rows its LDS.
 bool few_holds(const rlxq_ctx* ctx, const LayerCall& c) {
-  int l, u;
-  return c.rows * c.top_k <= 256 && c.hidden <= 8192 && c.inter <= 8192 && few_shape(c.gu_scheme, c.hidden, &l, &u) &&
-         few_shape(c.d_scheme, c.inter, &l, &u) && few_down_lds(c, 256) <= std::min<size_t>(ctx->max_lds, 160 * 1024);
+  const size_t lds = std::min<size_t>(ctx->max_lds, 160 * 1024) - 8192;   // (less the routing's tables)
+  return c.rows <= 32 && c.rows * c.top_k <= 256 &&
+         (size_t)few_mt(c) * (size_t)(c.hidden / 32 * RLXQ_FEW_REC(c.x_dtype == RLXQ_BF16 ? 1 : 2)) <= lds &&
+         few_down_lds(c, kFewTile) <= lds;
 }
 
 // Three launches: router product and prepared rows; routing, gate|up and
 // SwiGLU; down and the weighted sum.  The activations in between are f32.
 int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   auto r256 = [](size_t b) { return (b + 255) & ~size_t(255); };
-  const size_t n = (size_t)(c.rows * c.top_k), xn = (size_t)(c.rows * c.hidden);
-  const bool xbf = c.x_dtype == RLXQ_BF16;
+  const size_t n = (size_t)(c.rows * c.top_k);
+  const int planes = c.x_dtype == RLXQ_BF16 ? 1 : 2;
+  const size_t xrow = (size_t)(c.hidden / 32 * RLXQ_FEW_REC(planes));
   const size_t b_log = c.logits ? 0 : r256((size_t)(c.rows * c.experts) * 4), b_ids = r256(n * 4), b_pr = r256(n * 4);
-  const size_t b_hi = r256(xn * 2), b_lo = xbf ? 0 : r256(xn * 2), b_meta = r256(xn / 32 * 16), b_act = r256(n * (size_t)c.inter * 4);
+  const size_t b_rec = r256((size_t)c.rows * xrow), b_act = r256(n * (size_t)c.inter * 4);
   void* ws = nullptr;
   int rc;
-  if ((rc = workspace(ctx, b_log + b_ids + b_pr + b_hi + b_lo + b_meta + b_act, &ws, stream))) return rc;
+  if ((rc = workspace(ctx, b_log + b_ids + b_pr + b_rec + b_act, &ws, stream))) return rc;
   char* p = static_cast<char*>(ws);
   const int64_t cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
 
@@ -605,26 +623,25 @@ int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   pa.r.rows = c.rows;
   pa.r.H = c.hidden;
   pa.r.E = (int32_t)c.experts;
-  pa.hi = reinterpret_cast<uint16_t*>(p + b_log + b_ids + b_pr);
-  pa.lo = xbf ? nullptr : reinterpret_cast<uint16_t*>(p + b_log + b_ids + b_pr + b_hi);
-  pa.meta = reinterpret_cast<float*>(p + b_log + b_ids + b_pr + b_hi + b_lo);
+  pa.rec = reinterpret_cast<uint8_t*>(p + b_log + b_ids + b_pr);
   pa.lblocks = c.logits ? 0 : (int32_t)(c.experts * ((c.rows + 3) / 4));
+  pa.order = few_order(c.gu_scheme);
   char name[64];
-  std::snprintf(name, sizeof name, "rlxq_moe_prep_%s_%s", xbf ? "bf16" : "f32", c.router_dtype == RLXQ_BF16 ? "bf16" : "f32");
+  std::snprintf(name, sizeof name, "rlxq_moe_prep_%s_%s", planes == 1 ? "bf16" : "f32",
+                c.router && c.router_dtype == RLXQ_BF16 ? "bf16" : "f32");
   hipFunction_t fn;
   if ((rc = get_fn(ctx, name, &fn))) return rc;
   void* pargs[] = {&pa};
-  if ((rc = launch(ctx, fn, dim3((unsigned)(pa.lblocks + (xn / 4 + 63) / 64)), dim3(64), 0, stream, pargs, name))) return rc;
+  const int64_t pgrid = pa.lblocks + (c.rows * c.hidden / 4 + 255) / 256;
+  if ((rc = launch(ctx, fn, dim3((unsigned)pgrid), dim3(256), 0, stream, pargs, name))) return rc;
 
   rlxq_moe_few_args a;
   std::memset(&a, 0, sizeof a);
-  a.hi = pa.hi;
-  a.lo = pa.lo;
-  a.meta = pa.meta;
+  a.rec = pa.rec;
   a.logits = c.logits ? c.logits : pa.r.logits;
   a.ids = reinterpret_cast<int32_t*>(p + b_log);
   a.probs = reinterpret_cast<float*>(p + b_log + b_ids);
-  a.act = reinterpret_cast<float*>(p + b_log + b_ids + b_pr + b_hi + b_lo + b_meta);
+  a.act = reinterpret_cast<float*>(p + b_log + b_ids + b_pr + b_rec);
   a.ids2 = c.ids;
   a.probs2 = c.probs;
   a.y = c.y;
@@ -635,33 +652,36 @@ int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   a.top_k = (int32_t)c.top_k;
   a.renorm = c.renorm;
   a.y_bf16 = c.y_dtype == RLXQ_BF16;
-  int nu = 0;
-  few_shape(c.gu_scheme, c.hidden, &a.log2l, &nu);
   a.bank = static_cast<const uint8_t*>(c.gu);
   a.scales = static_cast<const uint8_t*>(c.gu_s);
   if ((rc = check_weights(ctx, "moe_layer gate_up", c.gu_scheme, 32, c.gu, c.gu_s, nullptr, RLXQ_U8, c.hidden, &a.rb))) return rc;
-  std::snprintf(name, sizeof name, "rlxq_moefew_gu_%s_u%d_p%d", scheme_name(c.gu_scheme), nu, xbf ? 1 : 2);
+  const int mt = few_mt(c);
+  std::snprintf(name, sizeof name, "rlxq_moefew_gu_%s_p%d_m%d", scheme_name(c.gu_scheme), planes, mt);
   if ((rc = get_fn(ctx, name, &fn))) return rc;
   void* args[] = {&a};
-  // one round of workgroups
-  const int per_cu = std::min(2, blocks_per_cu(ctx, name, fn, 512, 0));
+  // one round of workgroups: of four waves for up to four rows to route, else
+  // of eight
+  const size_t lds = (size_t)mt * xrow;
+  const int waves = c.rows <= 4 ? 4 : 8;
+  const int64_t wgs = cus * std::min(16 / waves, blocks_per_cu(ctx, name, fn, 64 * waves, lds));
+  a.log2l = few_log2l(c.gu_scheme, c.hidden, (double)n * (double)c.inter / (double)(wgs * waves));
   const int64_t steps = (int64_t)n * ((c.inter + (64 >> a.log2l) - 1) / (64 >> a.log2l));
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(cus * per_cu, (steps + 7) / 8));
-  if ((rc = launch(ctx, fn, dim3((unsigned)grid), dim3(512), 0, stream, args, name))) return rc;
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(wgs, (steps + waves - 1) / waves));
+  if ((rc = launch(ctx, fn, dim3((unsigned)grid), dim3(64 * waves), lds, stream, args, name))) return rc;
 
-  few_shape(c.d_scheme, c.inter, &a.log2l, &nu);
+  a.log2l = few_log2l(c.d_scheme, c.inter, (double)n * (double)c.hidden / (double)(cus * 16));
   a.bank = static_cast<const uint8_t*>(c.d);
   a.scales = static_cast<const uint8_t*>(c.d_s);
   if ((rc = check_weights(ctx, "moe_layer down", c.d_scheme, 32, c.d, c.d_s, nullptr, RLXQ_U8, c.inter, &a.rb))) return rc;
   // column tiles: two workgroups a CU, whole steps of the waves of a slot
-  const int64_t rp = 64 >> a.log2l, unit = rp * std::max<int64_t>(1, 8 / c.top_k);
+  const int64_t unit = (64 >> a.log2l) * std::max<int64_t>(1, 8 / c.top_k);
   int64_t tile = (c.rows * c.hidden + 2 * cus - 1) / (2 * cus);
-  tile = std::min<int64_t>(256, std::max<int64_t>(unit, (tile + unit - 1) / unit * unit));
+  tile = std::min<int64_t>(kFewTile, std::max<int64_t>(unit, (tile + unit - 1) / unit * unit));
   a.tile = (int32_t)tile;
   a.tiles = (int32_t)((c.hidden + tile - 1) / tile);
-  std::snprintf(name, sizeof name, "rlxq_moefew_dn_%s_u%d", scheme_name(c.d_scheme), nu);
+  std::snprintf(name, sizeof name, "rlxq_moefew_dn_%s", scheme_name(c.d_scheme));
   if ((rc = get_fn(ctx, name, &fn))) return rc;
-  return launch(ctx, fn, dim3((unsigned)(c.rows * a.tiles)), dim3(512), few_down_lds(c, tile), stream, args, name);
+  return launch(ctx, fn, dim3((unsigned)(c.rows * ((a.tiles + 7) / 8 * 8))), dim3(512), few_down_lds(c, tile), stream, args, name);
 }
 
 // The layer from the library's own calls: router product, top-k, grouped

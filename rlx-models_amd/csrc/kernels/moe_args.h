@@ -108,24 +108,24 @@ typedef struct rlxq_moe_pick_args {
   int32_t E, top_k, renorm, pad;
 } rlxq_moe_pick_args;
 
-/* Few-token expert layer.  The activation rows as f16 planes ("prepared"):
- * of each 32-element block, scaled by the power of two that brings its largest
- * magnitude into [2^14, 2^15), the rounded values (hi) and, for f32 rows, their
- * rounded remainders (lo); and per block four floats: the factor that undoes
- * the scaling, the sum of the block's elements, that of its first 16, 0.     */
+/* Few-token expert layer.  Activation rows as records ("prepared"), one per
+ * 32-element block: its elements, scaled by the power of two that brings their
+ * largest magnitude into [2^14, 2^15), rounded to f16 (64 bytes), for f32 rows
+ * their rounded remainders (64 bytes), both in the order in which the weight
+ * scheme's codes unpack (order: 0 element by element, 1 the GGUF nibbles', 2
+ * pairs two apart), and four floats: the factor that undoes the scaling, the
+ * sum of the block's elements, that of its first 16, 0.                      */
+#define RLXQ_FEW_REC(planes) (64 * (planes) + 16)
 typedef struct rlxq_moe_prep_args {
-  rlxq_moe_logits_args r;   /* the router's part (r.router NULL: none)       */
-  uint16_t* hi;             /* [rows, H]                                     */
-  uint16_t* lo;             /* [rows, H], or NULL (bf16 rows)                */
-  float* meta;              /* [rows, H / 32, 4]                             */
-  int32_t lblocks, pad;     /* workgroups of the router's part, ahead        */
+  rlxq_moe_logits_args r;   /* the router's part (lblocks > 0)               */
+  uint8_t* rec;             /* [rows, H / 32] records                        */
+  int32_t lblocks;          /* workgroups of the router's part, ahead        */
+  int32_t order;
 } rlxq_moe_prep_args;
 
 typedef struct rlxq_moe_few_args {
   /* gate|up: prepared rows in, act out.  down: act in, y out.               */
-  const uint16_t* hi;
-  const uint16_t* lo;
-  const float* meta;
+  const uint8_t* rec;
   const float* logits;      /* [rows, E]                                     */
   float* act;               /* [rows * top_k, I] silu(g) * u                 */
   int32_t* ids;             /* [rows, top_k], written by gate|up             */

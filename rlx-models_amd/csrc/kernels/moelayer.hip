@@ -30,10 +30,27 @@ RLXQ_DEV void load4(const void* p, int64_t i, double (&v)[4]) {
   }
 }
 
+// Sum over the wave (lanes of a row of 16 by DPP moves of the halves, the four
+// rows through readlane), the same in every lane.
+template <int CTRL>
+RLXQ_DEV double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+RLXQ_DEV double lane_f64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
 RLXQ_DEV double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+  v += dpp_f64<0xB1>(v);
+  v += dpp_f64<0x4E>(v);
+  v += dpp_f64<0x141>(v);
+  v += dpp_f64<0x140>(v);
+  return (lane_f64(v, 0) + lane_f64(v, 16)) + (lane_f64(v, 32) + lane_f64(v, 48));
 }
 
 // One wave: experts eb EB .., rows rb RB ...
@@ -82,6 +99,13 @@ RLXQ_DEV uint32_t wave_umax(uint32_t v) {
   return m(m(r0, r1), m(r2, r3));
 }
 
+RLXQ_DEV float wave_fmax(float v) {
+  v = group8_max(v);
+  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xF, 0xF, false)));
+  auto at = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
+  return fmaxf(fmaxf(at(0), at(16)), fmaxf(at(32), at(48)));
+}
+
 // Floats in their order as unsigned keys, all above 0 (-0 as 0).
 RLXQ_DEV uint32_t order_key(float f) {
   const uint32_t u = __float_as_uint(f + 0.f);
@@ -104,8 +128,7 @@ RLXQ_DEV void pick_row(const float* __restrict__ l, int E, int top_k, bool renor
     key[i] = e < E ? order_key(v[i]) : 0u;
     mx = fmaxf(mx, v[i]);
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  mx = wave_fmax(mx);
 #pragma unroll
   for (int i = 0; i < NPER; i++) s += expf(v[i] - mx);
   s = lane_group_sum<64>(s);
@@ -154,46 +177,90 @@ RLXQ_DEV void moe_pick_body(const rlxq_moe_pick_args& a) {
   }
 }
 
-// ------------------------------------------------------- rows as f16 planes
-// Four elements of a block per lane, eight lanes a block: the block's scale,
-// its planes and sums (moe_args.h).  v is zero where there is no element.
-struct PlaneQuad {
-  uint2 hi, lo;
-  float inv, sum, sum16;   // (the same in the block's eight lanes)
-};
-RLXQ_DEV PlaneQuad plane_quad(const float (&x)[4], bool want_lo) {
-  PlaneQuad r;
+// ------------------------------------------------------- rows as records
+// Order of a scheme's codes within a block (moe_args.h).
+template <int SCH>
+RLXQ_DEV constexpr int few_order() {
+  return SCH == SCH_MXFP4 ? 0 : (SCH == SCH_Q4_0 || SCH == SCH_Q4_1) ? 1 : 2;
+}
+
+// Four elements 4 q .. 4 q + 3 of a block per lane, eight lanes (q = lane & 7) a
+// block, into the block's record; all lanes of the wave take part.
+RLXQ_DEV void put_record(uint8_t* rec, const float (&x)[4], int planes, int order, bool active) {
+  const int q = threadIdx.x & 7;
   const float s = (x[0] + x[1]) + (x[2] + x[3]);
-  r.sum = group8_sum(s);
-  r.sum16 = group4_sum(s);   // (lanes 0..3: of the first 16 elements)
+  const float sum = group8_sum(s), sum16 = group4_sum(s);   // (lanes 0..3: of the first 16 elements)
   const float amax = group8_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-  // 2^e: amax 2^-e in [2^14, 2^15); the float's own exponent bits.  (An infinity
-  // or a NaN stays what it is under any scale.)
+  // 2^e: amax 2^-e in [2^14, 2^15), from the float's exponent bits (an infinity
+  // or a NaN stays what it is under any scale)
   int e = (int)(__float_as_uint(amax) >> 23) - 127 - 14;
   e = amax < INFINITY ? (e < -126 ? -126 : e) : 0;
   const float sc = __uint_as_float((uint32_t)(127 - e) << 23);
-  r.inv = __uint_as_float((uint32_t)(127 + e) << 23);
   uint32_t h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const float v = x[i] * sc;
     h[i] = f32_to_f16_bits(v);
-    l[i] = want_lo ? f32_to_f16_bits(v - f16_bits_to_f32(h[i])) : 0u;
+    l[i] = f32_to_f16_bits(v - f16_bits_to_f32(h[i]));
   }
-  r.hi = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-  r.lo = make_uint2(l[0] | (l[1] << 16), l[2] | (l[3] << 16));
-  return r;
+  if (!active) return;
+  // the lane's two pairs and their places among the block's 16
+  const int near = order == 0 ? 1 : 2;   // (4q, 4q + near)
+  const int t0 = order == 1 ? (q < 4 ? 4 * q : 4 * (q - 4) + 1) : 2 * q, t1 = order == 1 ? t0 + 2 : t0 + 1;
+  uint32_t* r = reinterpret_cast<uint32_t*>(rec);
+  r[t0] = h[0] | ((near == 1 ? h[1] : h[2]) << 16);
+  r[t1] = (near == 1 ? h[2] : h[1]) | (h[3] << 16);
+  if (planes == 2) {
+    r[16 + t0] = l[0] | ((near == 1 ? l[1] : l[2]) << 16);
+    r[16 + t1] = (near == 1 ? l[2] : l[1]) | (l[3] << 16);
+  }
+  if (q == 0) {
+    float* m = reinterpret_cast<float*>(rec + 64 * planes);
+    m[0] = __uint_as_float((uint32_t)(127 + e) << 23);
+    m[1] = sum;
+    m[2] = sum16;
+    m[3] = 0.f;
+  }
 }
 
-// Router logits (workgroups 0 .. lblocks - 1, one wave each) and, beside them,
-// the prepared rows.
+// Router logits (the first lblocks workgroups: an expert and four rows, H over
+// the four waves) and, beside them, the prepared rows.
 template <bool XBF, bool RBF>
 RLXQ_DEV void moe_prep_body(const rlxq_moe_prep_args& a) {
+  constexpr int RB = 4;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   if ((int)blockIdx.x < a.lblocks) {
-    moe_logits_body<XBF, RBF, 1, 4>(a.r, blockIdx.x % a.r.E, blockIdx.x / a.r.E);
+    __shared__ double part[4][RB];
+    const int e = blockIdx.x % a.r.E;
+    const int64_t r0 = (int64_t)(blockIdx.x / a.r.E) * RB;
+    double acc[RB] = {0., 0., 0., 0.};
+#pragma unroll 2
+    for (int64_t h = 4 * threadIdx.x; h < a.r.H; h += 1024) {
+      double w[4], v[RB][4];
+      load4<RBF>(a.r.router, (int64_t)e * a.r.H + h, w);
+#pragma unroll
+      for (int q = 0; q < RB; q++)
+        if (r0 + q < a.r.rows) load4<XBF>(a.r.x, (r0 + q) * a.r.H + h, v[q]);   // (uniform)
+#pragma unroll
+      for (int q = 0; q < RB; q++)
+        if (r0 + q < a.r.rows) {
+#pragma unroll
+          for (int c = 0; c < 4; c++) acc[q] = fma(w[c], v[q][c], acc[q]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < RB; q++) {
+      if (r0 + q >= a.r.rows) break;
+      const double s = wave_sum(acc[q]);
+      if (lane == 0) part[wv][q] = s;
+    }
+    __syncthreads();
+    const int q = threadIdx.x;
+    if (q < RB && r0 + q < a.r.rows)
+      a.r.logits[(r0 + q) * a.r.E + e] = (float)((part[0][q] + part[1][q]) + (part[2][q] + part[3][q]));
     return;
   }
-  const int64_t i = (int64_t)(blockIdx.x - a.lblocks) * 64 + threadIdx.x, n4 = a.r.rows * a.r.H / 4;
+  const int64_t i = (int64_t)(blockIdx.x - a.lblocks) * 256 + threadIdx.x, n4 = a.r.rows * a.r.H / 4;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (i < n4) {   // (H is whole blocks: uniform over a block's lanes)
     double d[4];
@@ -201,22 +268,19 @@ RLXQ_DEV void moe_prep_body(const rlxq_moe_prep_args& a) {
 #pragma unroll
     for (int q = 0; q < 4; q++) v[q] = (float)d[q];
   }
-  const PlaneQuad p = plane_quad(v, !XBF);
-  if (i >= n4) return;
-  reinterpret_cast<uint2*>(a.hi)[i] = p.hi;
-  if (!XBF) reinterpret_cast<uint2*>(a.lo)[i] = p.lo;
-  if ((threadIdx.x & 7) == 0) reinterpret_cast<float4*>(a.meta)[i >> 3] = make_float4(p.inv, p.sum, p.sum16, 0.f);
+  constexpr int P = XBF ? 1 : 2;
+  put_record(a.rec + (i >> 3) * RLXQ_FEW_REC(P), v, P, a.order, i < n4);
 }
 
 // ------------------------------------------------- products for few tokens
-// A weight row is spread over L = 2^log2l lanes of a wave, lane li holding units
-// li, li + L, ... (NU of them; a unit is one or two 32-weight blocks), the same
-// units of the activation row in its registers; 64 / L rows go at once.  Codes
-// become exact f16 integers (the offset of the bit pattern subtracted), so the
-// products with the f16 planes are exact in v_dot2_f32_f16 and a block's sum is
-// an f32 sum of its 32 (64 with the lo plane) products, which then takes the
-// block's scale (times the activation block's power of two) and, for formats
-// with a minimum, the minimum times the block's sum of activations.
+// A weight row is spread over L = 2^log2l lanes of a wave, lane li taking units
+// li, li + L, ... (a unit is one or two 32-weight blocks) against the activation
+// rows' records in LDS; 64 / L rows go at once.  Codes become exact f16 integers
+// (the offset of the bit pattern subtracted), so the products with the f16
+// planes are exact in v_dot2_f32_f16 and a block's sum is an f32 sum of its 32
+// (64 with the remainders) products, which then takes the block's scale (times
+// the activation block's power of two) and, for formats with a minimum, the
+// minimum times the block's sum of activations.
 
 // f16 pairs of block bl of a unit in the scheme's order, exact integers.
 template <int SCH>
@@ -243,116 +307,120 @@ RLXQ_DEV void block_f16(const uint32_t* dw, int bl, uint32_t* pw, const UnpackK&
   }
 }
 
-// Natural f16 pairs (x[2i], x[2i+1]) of a block in the scheme's pair order.
 template <int SCH>
-RLXQ_DEV void planes_from_raw(const uint32_t* R, uint32_t* X) {
-  // (byte codes and the 2 to 6-bit K-quants pair as Q4_K's nibbles do)
-  constexpr int AS = SCH == SCH_MXFP4 || SCH == SCH_Q4_0 || SCH == SCH_Q4_1 ? SCH : SCH_Q4_K;
-  pairs_from_raw<AS>(R, X);
-}
-
-template <int SCH, int NU, int NPL>
-struct FewX {
-  static constexpr int NB = NU * Unit<SCH>::BLOCKS;
-  uint32_t h[NB][16], l[NPL == 2 ? NB : 1][16];
-  float inv[NB], sum[NB], sum16[half_scales<SCH>() ? NB : 1];
-
-  // The lane's blocks of a row: planes hi / lo [K] and meta [K / 32][4].
-  RLXQ_DEV void load(const uint16_t* hi, const uint16_t* lo, const float* meta, const int* uc, const bool* uok) {
-#pragma unroll
-    for (int c = 0; c < NU; c++)
-#pragma unroll
-      for (int bl = 0; bl < Unit<SCH>::BLOCKS; bl++) {
-        const int i = c * Unit<SCH>::BLOCKS + bl, b = uc[c] * Unit<SCH>::BLOCKS + bl;
-        uint32_t R[16];
-        auto plane = [&](const uint16_t* p, uint32_t* X) {
-#pragma unroll
-          for (int q = 0; q < 4; q++) {
-            const uint4 v = reinterpret_cast<const uint4*>(p + 32 * b)[q];
-            R[4 * q] = v.x; R[4 * q + 1] = v.y; R[4 * q + 2] = v.z; R[4 * q + 3] = v.w;
-          }
-          planes_from_raw<SCH>(R, X);
-        };
-        plane(hi, h[i]);
-        if constexpr (NPL == 2) plane(lo, l[i]);
-        const float4 m = reinterpret_cast<const float4*>(meta)[b];
-        // (a unit past the row's end repeats the last one, times zero)
-        inv[i] = uok[c] ? m.x : 0.f;
-        sum[i] = uok[c] ? m.y : 0.f;
-        if constexpr (half_scales<SCH>()) sum16[i] = uok[c] ? m.z : 0.f;
-        if (!uok[c]) {
-#pragma unroll
-          for (int t = 0; t < 16; t++) {
-            h[i][t] = 0u;
-            if constexpr (NPL == 2) l[i][t] = 0u;
-          }
-        }
-      }
-  }
-};
-
-template <int SCH, int NU>
 struct FewW {
-  uint32_t dw[NU][Unit<SCH>::DW];
-  uint32_t sc[SCH == SCH_MXFP4 ? NU : 1];
+  uint32_t dw[Unit<SCH>::DW];
+  uint32_t sc;
+  // unit u of the packed row at p (MXFP4: its scale byte among those at s)
+  RLXQ_DEV void load(const uint8_t* p, const uint8_t* s, int u) {
+    load_unit_at<SCH>(dw, p, u);
+    if constexpr (SCH == SCH_MXFP4) sc = s[u];
+  }
+};
 
-  // A lane's units of the packed row at p (MXFP4: its scale bytes at s).
-  RLXQ_DEV void load(const uint8_t* p, const uint8_t* s, const int* uc) {
+// One block's record in registers.
+template <int NPL>
+struct FewRec {
+  uint32_t h[16], l[NPL == 2 ? 16 : 1];
+  float4 me;
+  RLXQ_DEV void load(const uint8_t* rec, bool uok) {
 #pragma unroll
-    for (int c = 0; c < NU; c++) {
-      load_unit_at<SCH>(dw[c], p, uc[c]);
-      if constexpr (SCH == SCH_MXFP4) sc[c] = s[uc[c]];
+    for (int q = 0; q < 4; q++) {
+      const uint4 v = reinterpret_cast<const uint4*>(rec)[q];
+      h[4 * q] = v.x; h[4 * q + 1] = v.y; h[4 * q + 2] = v.z; h[4 * q + 3] = v.w;
+      if constexpr (NPL == 2) {
+        const uint4 z = reinterpret_cast<const uint4*>(rec)[4 + q];
+        l[4 * q] = z.x; l[4 * q + 1] = z.y; l[4 * q + 2] = z.z; l[4 * q + 3] = z.w;
+      }
+    }
+    // (a unit past the row's end repeats the last one, times zero)
+    me = uok ? reinterpret_cast<const float4*>(rec)[4 * NPL] : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+};
+
+// A block of a weight row: exact f16 codes, multipliers of its code sum (of its
+// halves') and of its activations' sum (halves').
+template <int SCH>
+struct FewBlk {
+  uint32_t pw[16];
+  float d, d2, mn, m2;
+  RLXQ_DEV void decode(const FewW<SCH>& w, int bl, int u, const UnpackK& kc) {
+    block_f16<SCH>(w.dw, bl, pw, kc);
+    d2 = mn = m2 = 0.f;
+    if constexpr (SCH == SCH_MXFP4) d = e8m0_to_f32(w.sc);
+    else if constexpr (SCH == SCH_Q6_K) block_scales<SCH>(w.dw, bl, d, d2, u);
+    else if constexpr (half_scales<SCH>()) block_scales_half<SCH>(w.dw, d, d2, mn, m2);
+    else block_scales<SCH>(w.dw, bl, d, mn, u);
+  }
+  template <int NPL>
+  RLXQ_DEV void add(const FewRec<NPL>& x, float& s) const {
+    float c0 = 0.f, c1 = 0.f;   // (two chains: the halves, hi and lo, or even and odd pairs)
+#pragma unroll
+    for (int t = 0; t < 16; t++) {
+      if constexpr (half_scales<SCH>()) {
+        float& c = t < 8 ? c0 : c1;
+        c = dot2_f16(pw[t], x.h[t], c);
+        if constexpr (NPL == 2) c = dot2_f16(pw[t], x.l[t], c);
+      } else if constexpr (NPL == 2) {
+        c0 = dot2_f16(pw[t], x.h[t], c0);
+        c1 = dot2_f16(pw[t], x.l[t], c1);
+      } else {
+        float& c = t & 1 ? c1 : c0;
+        c = dot2_f16(pw[t], x.h[t], c);
+      }
+    }
+    if constexpr (half_scales<SCH>()) {
+      s = fmaf(d * x.me.x, c0, s);
+      s = fmaf(d2 * x.me.x, c1, s);
+      if constexpr (SCH == SCH_Q2_K) {
+        s = fmaf(mn, x.me.z, s);
+        s = fmaf(m2, x.me.y - x.me.z, s);
+      }
+    } else {
+      s = fmaf(d * x.me.x, c0 + c1, s);
+      if constexpr (SCH == SCH_Q4_1 || SCH == SCH_Q4_K || SCH == SCH_Q5_K) s = fmaf(mn, x.me.y, s);
     }
   }
 };
 
-// The lane's part of a weight row times the activation row.
-template <int SCH, int NU, int NPL>
-RLXQ_DEV float few_dot(const FewW<SCH, NU>& w, const FewX<SCH, NU, NPL>& x, const int* uc, const UnpackK& kc) {
-  constexpr int BLOCKS = Unit<SCH>::BLOCKS;
-  float acc = 0.f;
+// A unit's part of R weight rows (w[0 .. R - 1], unit u) times MT activation
+// rows (records of the unit's first block at x + m * xld).  One activation row:
+// its record stays in registers and the weight rows are decoded in turn; more:
+// the weight rows are decoded once and the records pass.  (The empty statements
+// keep the products where they stand: the compiler would gather them behind the
+// reads of all records, in as many registers, and run them for absent rows.)
+template <int SCH, int NPL, int R, int MT>
+RLXQ_DEV void few_unit(const FewW<SCH> (&w)[R], const uint8_t* x, int xld, int cnt, int u, bool uok, const UnpackK& kc,
+                       float (&acc)[R][MT]) {
 #pragma unroll
-  for (int c = 0; c < NU; c++)
+  for (int bl = 0; bl < Unit<SCH>::BLOCKS; bl++) {
+    if constexpr (MT == 1) {
+      FewRec<NPL> rec;
+      rec.load(x + bl * RLXQ_FEW_REC(NPL), uok);
 #pragma unroll
-    for (int bl = 0; bl < BLOCKS; bl++) {
-      const int i = c * BLOCKS + bl;
-      uint32_t pw[16];
-      block_f16<SCH>(w.dw[c], bl, pw, kc);
-      if constexpr (half_scales<SCH>()) {   // a scale (and minimum) per 16 weights
-        float d, d2, m = 0.f, m2 = 0.f;
-        if constexpr (SCH == SCH_Q6_K) block_scales<SCH>(w.dw[c], bl, d, d2, uc[c]);
-        else block_scales_half<SCH>(w.dw[c], d, d2, m, m2);
-        float c0 = 0.f, c1 = 0.f;
+      for (int r = 0; r < R; r++) {
+        FewBlk<SCH> b;
+        b.decode(w[r], bl, u, kc);
+        b.add(rec, acc[r][0]);
+        asm volatile("" : "+v"(acc[r][0]));
+      }
+    } else {
+      FewBlk<SCH> b[R];
 #pragma unroll
-        for (int t = 0; t < 8; t++) {
-          c0 = dot2_f16(pw[t], x.h[i][t], c0);
-          c1 = dot2_f16(pw[8 + t], x.h[i][8 + t], c1);
-          if constexpr (NPL == 2) {
-            c0 = dot2_f16(pw[t], x.l[i][t], c0);
-            c1 = dot2_f16(pw[8 + t], x.l[i][8 + t], c1);
-          }
+      for (int r = 0; r < R; r++) b[r].decode(w[r], bl, u, kc);
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        if (m > 0 && m >= cnt) break;   // (uniform)
+        FewRec<NPL> rec;
+        rec.load(x + m * xld + bl * RLXQ_FEW_REC(NPL), uok);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          b[r].add(rec, acc[r][m]);
+          asm volatile("" : "+v"(acc[r][m]));
         }
-        acc = fmaf(d * x.inv[i], c0, acc);
-        acc = fmaf(d2 * x.inv[i], c1, acc);
-        if constexpr (SCH == SCH_Q2_K) {
-          acc = fmaf(m, x.sum16[i], acc);
-          acc = fmaf(m2, x.sum[i] - x.sum16[i], acc);
-        }
-      } else {
-        float d, m = 0.f;
-        if constexpr (SCH == SCH_MXFP4) d = e8m0_to_f32(w.sc[c]);
-        else block_scales<SCH>(w.dw[c], bl, d, m, uc[c]);
-        float c0 = 0.f, c1 = 0.f;
-#pragma unroll
-        for (int t = 0; t < 16; t++) {
-          c0 = dot2_f16(pw[t], x.h[i][t], c0);
-          if constexpr (NPL == 2) c1 = dot2_f16(pw[t], x.l[i][t], c1);
-        }
-        acc = fmaf(d * x.inv[i], NPL == 2 ? c0 + c1 : c0, acc);
-        if constexpr (SCH == SCH_Q4_1 || SCH == SCH_Q4_K || SCH == SCH_Q5_K) acc = fmaf(m, x.sum[i], acc);
       }
     }
-  return acc;
+  }
 }
 
 // Sum over aligned groups of L = 2^log2l lanes (4 .. 64), in every lane of the
@@ -364,10 +432,8 @@ RLXQ_DEV float few_sum(float v, int log2l) {
   if (log2l == 3) return v;
   v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xF, 0xF, false));
   if (log2l == 4) return v;
-  const float r0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 0));
-  const float r1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16));
-  const float r2 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 32));
-  const float r3 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 48));
+  auto at = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
+  const float r0 = at(0), r1 = at(16), r2 = at(32), r3 = at(48);
   if (log2l == 5) return (threadIdx.x & 32) ? r2 + r3 : r0 + r1;
   return (r0 + r1) + (r2 + r3);
 }
@@ -378,17 +444,117 @@ RLXQ_DEV UnpackK f16_unpack_consts() {
   return k;
 }
 
-constexpr int FEW_ENTRIES = 256;   // most (row, slot) pairs of a call
+// Columns c_first, c_first + c_step, ... below c_end of a slab (64 / L columns at
+// each) times the rows whose records start at x (MT of them, xld apart, cnt in
+// use).  R = 2: a column is gate row col and up row col + up.  The steps (column,
+// unit) run as one sequence with the weights of D - 1 steps ahead in registers;
+// past the last step the loads repeat its column (a load under a condition would
+// make the compiler wait for all the others).  begin() requests the first; run()
+// needs the records in LDS.
+template <int SCH, int NPL, int R, int MT>
+struct FewCols {
+  static constexpr int D0 = 48 / (R * Unit<SCH>::DW), D = D0 < 1 ? 1 : D0 > 4 ? 4 : D0;   // (48 registers of weights)
+  FewW<SCH> ring[D][R];
+  const uint8_t* base;
+  const uint8_t* sbase;
+  int64_t rb;
+  int up, nbs, U, c_first, c_step, c_end, log2l, nchunk, S;
+  const uint8_t *lp[R], *ls[R];   // the rows of the column being loaded
+  int l_col, l_j;
+
+  RLXQ_DEV void load(FewW<SCH> (&w)[R]) {   // the next step's weights
+    if (l_j == 0) {
+      const int col = l_col < c_end ? l_col : c_end - 1;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const int64_t n = col + (r ? up : 0);
+        lp[r] = base + n * rb;
+        ls[r] = SCH == SCH_MXFP4 ? sbase + n * nbs : nullptr;
+      }
+    }
+    int u = (threadIdx.x & ((1 << log2l) - 1)) + (l_j << log2l);
+    u = u < U ? u : U - 1;
+#pragma unroll
+    for (int r = 0; r < R; r++) w[r].load(lp[r], ls[r], u);
+    if (++l_j == nchunk) {
+      l_j = 0;
+      l_col += c_step;
+    }
+  }
+  RLXQ_DEV void begin() {
+    nchunk = (U + (1 << log2l) - 1) >> log2l;
+    S = c_first < c_end ? (c_end - c_first + c_step - 1) / c_step * nchunk : 0;
+    l_col = c_first + ((threadIdx.x & 63) >> log2l);
+    l_j = 0;
+#pragma unroll
+    for (int d = 0; d < D - 1; d++) load(ring[d]);
+  }
+  template <class Emit>
+  RLXQ_DEV void run(const uint8_t* x, int xld, int cnt, const UnpackK& kc, Emit emit) {
+    const int lane = threadIdx.x & 63, li = lane & ((1 << log2l) - 1);
+    float acc[R][MT];
+    int col = c_first + (lane >> log2l), j = 0;
+    for (int s0 = 0; s0 < S; s0 += D) {
+#pragma unroll
+      for (int d = 0; d < D; d++) {
+        const int s = s0 + d;
+        load(ring[(d + D - 1) % D]);
+        if (s < S) {
+          if (j == 0) {
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+              for (int m = 0; m < MT; m++) acc[r][m] = 0.f;
+          }
+          const int u = li + (j << log2l);
+          const bool uok = u < U;
+          const int uc = uok ? u : U - 1;
+          few_unit<SCH, NPL, R, MT>(ring[d], x + uc * (Unit<SCH>::BLOCKS * RLXQ_FEW_REC(NPL)), xld, cnt, uc, uok, kc, acc);
+          if (++j == nchunk) {
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+              if (m > 0 && m >= cnt) break;
+              float v[R];
+#pragma unroll
+              for (int r = 0; r < R; r++) v[r] = few_sum(acc[r][m], log2l);
+              if (li == 0 && col < c_end) emit(m, col, v);
+            }
+            j = 0;
+            col += c_step;
+          }
+        }
+      }
+    }
+  }
+};
+
+constexpr int FEW_ENTRIES = 256;   // most (row, slot) pairs of a call (of at most 32 rows)
 
 // gate|up and SwiGLU.  Every workgroup routes all rows itself (a wave a row:
 // the grid is one round of workgroups, so the layer pays for it once, where a
-// launch of its own would cost more), then the waves share the (entry, group of
-// columns) steps evenly.  Workgroup 0 leaves the routing for the down launch.
-template <int SCH, int NU, int NPL>
+// launch of its own would cost more).  The entries of one expert are cut into
+// chunks of MT, and the workgroups share the (chunk, columns) evenly; a chunk's
+// rows are copied to LDS and its weights read once for all of them.  Workgroup
+// 0 leaves the routing for the down launch.
+template <int SCH, int NPL, int MT>
 RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
-  __shared__ int32_t ids[FEW_ENTRIES];
+  extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];   // MT rows of records
+  __shared__ __attribute__((aligned(16))) int32_t ids[FEW_ENTRIES];
+  // (MT > 1; a chunk holds at least one entry)
+  __shared__ uint32_t mask[MT > 1 ? 1024 : 1];
+  __shared__ int32_t first[MT > 1 ? 1024 : 1], member[MT > 1 ? FEW_ENTRIES * MT : 1], wsum[8];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-  const int n = a.rows * a.top_k;
+  const int n = a.rows * a.top_k, nb = a.H / 32, xld = nb * RLXQ_FEW_REC(NPL);
+  auto stage = [&](int m, int r) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.rec + (int64_t)r * xld);
+    uint4* dst = reinterpret_cast<uint4*>(few_lds + m * xld);
+    for (int i = threadIdx.x; i < xld / 16; i += blockDim.x) dst[i] = src[i];
+  };
+  if (a.rows == 1) stage(0, 0);   // (the only row: ahead of the routing)
+  if constexpr (MT > 1) {
+    for (int i = threadIdx.x; i < a.E; i += blockDim.x) mask[i] = 0u;
+    for (int i = threadIdx.x; i < n * MT; i += blockDim.x) member[i] = -1;
+  }
   for (int r = wv; r < a.rows; r += nw) {
     int id;
     float p;
@@ -408,101 +574,140 @@ RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
     }
   }
   __syncthreads();
-  const int L = 1 << a.log2l, RP = 64 >> a.log2l;
-  const int g = lane >> a.log2l, li = lane & (L - 1);
-  const int U = a.H / 32 / Unit<SCH>::BLOCKS;
-  int uc[NU];
-  bool uok[NU];
+  int chunks = n;
+  if constexpr (MT > 1) {
+    // a row takes an expert once: an expert's entries are the bits of a mask of
+    // rows, an entry's rank among them the bits below its row's
+    for (int i = threadIdx.x; i < n; i += blockDim.x) atomicOr(&mask[ids[i]], 1u << (i / a.top_k));
+    __syncthreads();
+    // chunk offsets: exclusive sum over the experts, four a thread
+    int c4[4], t = 0;
 #pragma unroll
-  for (int c = 0; c < NU; c++) {
-    const int u = li + L * c;
-    uok[c] = u < U;
-    uc[c] = uok[c] ? u : U - 1;
-  }
-  const UnpackK kc = f16_unpack_consts();
-  const int steps = (a.I + RP - 1) / RP;   // of an entry
-  const int64_t total = (int64_t)n * steps, waves = (int64_t)gridDim.x * nw, w = (int64_t)blockIdx.x * nw + wv;
-  int64_t s = total * w / waves;
-  const int64_t s_end = total * (w + 1) / waves;
-  while (s < s_end) {
-    const int ent = (int)(s / steps), c0 = (int)(s - (int64_t)ent * steps);
-    const int c1 = (int)(s_end - (int64_t)ent * steps < steps ? s_end - (int64_t)ent * steps : steps);
-    const int e = __builtin_amdgcn_readfirstlane(ids[ent]), r = ent / a.top_k;
-    const uint8_t* base = a.bank + (int64_t)e * 2 * a.I * a.rb;
-    const uint8_t* sbase = SCH == SCH_MXFP4 ? a.scales + (int64_t)e * 2 * a.I * (a.H / 32) : nullptr;
-    FewW<SCH, NU> gate[2], up[2];
-    auto load = [&](int c, int slot) {
-      int col = c * RP + g;
-      col = col < a.I ? col : a.I - 1;
-      gate[slot].load(base + (int64_t)col * a.rb, sbase + (int64_t)col * (a.H / 32), uc);
-      up[slot].load(base + (int64_t)(a.I + col) * a.rb, sbase + (int64_t)(a.I + col) * (a.H / 32), uc);
-    };
-    FewX<SCH, NU, NPL> x;
-    load(c0, 0);
-    x.load(a.hi + (int64_t)r * a.H, NPL == 2 ? a.lo + (int64_t)r * a.H : nullptr, a.meta + (int64_t)r * (a.H / 32) * 4, uc, uok);
-    auto step = [&](int c, int slot) {
-      const float gv = few_sum(few_dot<SCH, NU, NPL>(gate[slot], x, uc, kc), a.log2l);
-      const float uv = few_sum(few_dot<SCH, NU, NPL>(up[slot], x, uc, kc), a.log2l);
-      const int col = c * RP + g;
-      if (li == 0 && col < a.I) a.act[(int64_t)ent * a.I + col] = gv / (1.f + expf(-gv)) * uv;
-    };
-    int c = c0;
-    for (; c + 1 < c1; c += 2) {   // (the next step's weights while this one is multiplied)
-      load(c + 1, 1);
-      step(c, 0);
-      if (c + 2 < c1) load(c + 2, 0);
-      step(c + 1, 1);
+    for (int q = 0; q < 4; q++) {
+      const int e = 4 * threadIdx.x + q;
+      c4[q] = e < a.E ? (__popc(mask[e]) + MT - 1) / MT : 0;
+      t += c4[q];
     }
-    if (c < c1) step(c, 0);
-    s = (int64_t)ent * steps + c1;
+    int inc = t;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(inc, off, 64);
+      if (lane >= off) inc += o;
+    }
+    if (lane == 63) wsum[wv] = inc;
+    __syncthreads();
+    int off = inc - t;
+    chunks = 0;
+    for (int q = 0; q < nw; q++) {
+      off += q < wv ? wsum[q] : 0;
+      chunks += wsum[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int e = 4 * threadIdx.x + q;
+      if (e < a.E) first[e] = off;
+      off += c4[q];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e = ids[i], rank = __popc(mask[e] & ((1u << (i / a.top_k)) - 1));
+      member[(first[e] + rank / MT) * MT + rank % MT] = i;
+    }
+    __syncthreads();
+  }
+  const int RP = 64 >> a.log2l;
+  const UnpackK kc = f16_unpack_consts();
+  // steps of a chunk: groups of RP columns
+  const int steps = (a.I + RP - 1) / RP;
+  const int64_t total = (int64_t)chunks * steps;
+  int64_t s = total * blockIdx.x / gridDim.x;
+  const int64_t s_end = total * (blockIdx.x + 1) / gridDim.x;
+  bool again = false;
+  while (s < s_end) {   // (uniform over the workgroup)
+    const int ch = (int)(s / steps), c0 = (int)(s - (int64_t)ch * steps);
+    const int64_t left = s_end - (int64_t)ch * steps;
+    const int c1 = (int)(left < steps ? left : steps);
+    int ent[MT], cnt = 1;
+    if constexpr (MT > 1) {
+      cnt = 0;
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        ent[m] = __builtin_amdgcn_readfirstlane(member[ch * MT + m]);
+        cnt += ent[m] >= 0 ? 1 : 0;
+      }
+    } else {
+      ent[0] = ch;
+    }
+    const int e = __builtin_amdgcn_readfirstlane(ids[ent[0]]);
+    FewCols<SCH, NPL, 2, MT> f;
+    f.base = a.bank + (int64_t)e * 2 * a.I * a.rb;
+    f.sbase = SCH == SCH_MXFP4 ? a.scales + (int64_t)e * 2 * a.I * nb : nullptr;
+    f.rb = a.rb;
+    f.up = a.I;
+    f.nbs = nb;
+    f.U = nb / Unit<SCH>::BLOCKS;
+    f.log2l = a.log2l;
+    f.c_first = (c0 + wv) * RP;
+    f.c_step = nw * RP;
+    f.c_end = c1 * RP < a.I ? c1 * RP : a.I;
+    f.begin();
+    if (a.rows > 1) {
+      if (again) __syncthreads();   // (the rows before are no longer read)
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+        if (m < cnt) stage(m, ent[m] / a.top_k);
+      __syncthreads();
+    }
+    f.run(few_lds, xld, cnt, kc, [&](int m, int col, const float (&v)[2]) {
+      int en = ent[0];
+#pragma unroll
+      for (int q = 1; q < MT; q++) en = m == q ? ent[q] : en;
+      a.act[(int64_t)en * a.I + col] = v[0] / (1.f + expf(-v[0])) * v[1];   // silu(g) * u
+    });
+    again = true;
+    s = (int64_t)ch * steps + c1;
   }
 }
 
 // down and the weighted sum, a workgroup per (row, tile of columns): the row's
-// top_k activation vectors become planes in LDS, the waves share the slots
-// (waves / top_k of them per slot, each a part of the tile), and the slots are
-// added in slot order.  slots at once: top_k up to the waves, else all in turns.
-template <int SCH, int NU>
+// top_k activation vectors become records in LDS, the waves share the slots
+// (waves / top_k of them per slot, each a part of the tile; more slots than
+// waves in turns), and the slots are added in slot order.  Workgroups of one
+// column tile are dealt to one XCD (workgroup b runs on XCD b % 8), whose L2
+// then holds the rows of an expert that several tokens take.
+template <int SCH>
 RLXQ_DEV void moe_few_down(const rlxq_moe_few_args& a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-  const int r = blockIdx.x / a.tiles, c_beg = (blockIdx.x % a.tiles) * a.tile;
-  const int c_end = c_beg + a.tile < a.H ? c_beg + a.tile : a.H;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+  const int x8 = blockIdx.x & 7, q8 = blockIdx.x >> 3;
+  const int r = q8 % a.rows, tn = q8 / a.rows * 8 + x8;
+  if (tn >= a.tiles) return;
+  const int c_beg = tn * a.tile, c_end = c_beg + a.tile < a.H ? c_beg + a.tile : a.H;
   const int K = a.I, nb = K / 32;
-  uint16_t* hi = reinterpret_cast<uint16_t*>(few_lds);            // [top_k][K]
-  uint16_t* lo = hi + a.top_k * K;
-  float* meta = reinterpret_cast<float*>(lo + a.top_k * K);       // [top_k][nb][4]
-  float* vals = meta + a.top_k * nb * 4;                          // [top_k][tile]
-
-  const int L = 1 << a.log2l, RP = 64 >> a.log2l;
-  const int g = lane >> a.log2l, li = lane & (L - 1);
-  const int U = nb / Unit<SCH>::BLOCKS;
-  int uc[NU];
-  bool uok[NU];
-#pragma unroll
-  for (int c = 0; c < NU; c++) {
-    const int u = li + L * c;
-    uok[c] = u < U;
-    uc[c] = uok[c] ? u : U - 1;
-  }
+  constexpr int REC = RLXQ_FEW_REC(2);
+  float* vals = reinterpret_cast<float*>(few_lds + (size_t)a.top_k * nb * REC);   // [top_k][tile]
+  const int RP = 64 >> a.log2l;
   const UnpackK kc = f16_unpack_consts();
-  // wave -> slot and part of the tile
   const int parts = nw / a.top_k > 1 ? nw / a.top_k : 1;
-  const int j0 = wv / parts, part = wv - j0 * parts, jstep = nw / parts;
-  const int psize = ((a.tile + parts - 1) / parts + RP - 1) / RP * RP;   // whole steps
-  const int p_beg = c_beg + part * psize, p_end = p_beg + psize < c_end ? p_beg + psize : c_end;
+  const int part = wv % parts, jstep = nw / parts;
 
-  FewW<SCH, NU> w[2];
-  auto load = [&](int e, int col, int slot) {
-    col += g;
-    col = col < a.H ? col : a.H - 1;
-    w[slot].load(a.bank + ((int64_t)e * a.H + col) * a.rb,
-                 SCH == SCH_MXFP4 ? a.scales + ((int64_t)e * a.H + col) * nb : nullptr, uc);
+  FewCols<SCH, 2, 1, 1> f;
+  f.rb = a.rb;
+  f.up = 0;
+  f.nbs = nb;
+  f.U = nb / Unit<SCH>::BLOCKS;
+  f.log2l = a.log2l;
+  f.c_first = c_beg + part * RP;
+  f.c_step = parts * RP;
+  f.c_end = c_end;
+  auto begin = [&](int j) {
+    const int e = __builtin_amdgcn_readfirstlane(a.ids[r * a.top_k + j]);
+    f.base = a.bank + (int64_t)e * a.H * a.rb;
+    f.sbase = SCH == SCH_MXFP4 ? a.scales + (int64_t)e * a.H * nb : nullptr;
+    f.begin();
   };
-  int j = j0;
-  int e = j < a.top_k ? __builtin_amdgcn_readfirstlane(a.ids[r * a.top_k + j]) : 0;
-  if (j < a.top_k && p_beg < p_end) load(e, p_beg, 0);
-  // the row's activation vectors as planes
+  const int j0 = wv / parts;
+  if (j0 < a.top_k) begin(j0);
   const float* act = a.act + (int64_t)r * a.top_k * K;
   const int n4 = a.top_k * K / 4;
   for (int i0 = 0; i0 < n4; i0 += blockDim.x) {
@@ -512,33 +717,12 @@ RLXQ_DEV void moe_few_down(const rlxq_moe_few_args& a) {
       const float4 u = reinterpret_cast<const float4*>(act)[i];
       v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
     }
-    const PlaneQuad p = plane_quad(v, true);
-    if (i < n4) {
-      reinterpret_cast<uint2*>(hi)[i] = p.hi;
-      reinterpret_cast<uint2*>(lo)[i] = p.lo;
-      if ((i & 7) == 0) reinterpret_cast<float4*>(meta)[i >> 3] = make_float4(p.inv, p.sum, p.sum16, 0.f);
-    }
+    put_record(few_lds + (i >> 3) * REC, v, 2, few_order<SCH>(), i < n4);
   }
   __syncthreads();
-  for (; j < a.top_k; j += jstep) {
-    if (j != j0) {
-      e = __builtin_amdgcn_readfirstlane(a.ids[r * a.top_k + j]);
-      if (p_beg < p_end) load(e, p_beg, 0);
-    }
-    FewX<SCH, NU, 2> x;
-    x.load(hi + j * K, lo + j * K, meta + j * nb * 4, uc, uok);
-    auto step = [&](int col, int slot) {
-      const float v = few_sum(few_dot<SCH, NU, 2>(w[slot], x, uc, kc), a.log2l);
-      if (li == 0 && col + g < p_end) vals[j * a.tile + col + g - c_beg] = v;
-    };
-    int c = p_beg;
-    for (; c + RP < p_end; c += 2 * RP) {
-      load(e, c + RP, 1);
-      step(c, 0);
-      if (c + 2 * RP < p_end) load(e, c + 2 * RP, 0);
-      step(c + RP, 1);
-    }
-    if (c < p_end) step(c, 0);
+  for (int j = j0; j < a.top_k; j += jstep) {
+    if (j != j0) begin(j);
+    f.run(few_lds + (size_t)j * nb * REC, 0, 1, kc, [&](int, int col, const float (&v)[1]) { vals[j * a.tile + col - c_beg] = v[0]; });
   }
   __syncthreads();
   for (int c = threadIdx.x; c < c_end - c_beg; c += blockDim.x) {
@@ -561,7 +745,7 @@ RLXQ_DEV void moe_few_down(const rlxq_moe_few_args& a) {
   extern "C" __global__ __launch_bounds__(64) void rlxq_moe_logits_##XN##_##RN##_e4r8(rlxq_moe_logits_args a) {     \
     rlxq::moe_logits_body<XBF, RBF, 4, 8>(a, blockIdx.x, blockIdx.y);                                               \
   }                                                                                                                 \
-  extern "C" __global__ __launch_bounds__(64) void rlxq_moe_prep_##XN##_##RN(rlxq_moe_prep_args a) {                \
+  extern "C" __global__ __launch_bounds__(256) void rlxq_moe_prep_##XN##_##RN(rlxq_moe_prep_args a) {                \
     rlxq::moe_prep_body<XBF, RBF>(a);                                                                               \
   }
 RLXQ_LOGITS(f32, false, f32, false)
@@ -579,44 +763,38 @@ RLXQ_PICK(4)
 RLXQ_PICK(16)
 #endif
 
-// rlxq_moefew_gu_<scheme>_u<NU>_p<planes>, rlxq_moefew_dn_<scheme>_u<NU>
-#define RLXQ_FEW_U(SNAME, SCH, NU)                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void rlxq_moefew_gu_##SNAME##_u##NU##_p1(rlxq_moe_few_args a) { \
-    rlxq::moe_few_gate_up<SCH, NU, 1>(a);                                                                \
-  }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(512) void rlxq_moefew_gu_##SNAME##_u##NU##_p2(rlxq_moe_few_args a) { \
-    rlxq::moe_few_gate_up<SCH, NU, 2>(a);                                                                \
-  }                                                                                                      \
-  extern "C" __global__ __launch_bounds__(512) void rlxq_moefew_dn_##SNAME##_u##NU(rlxq_moe_few_args a) { \
-    rlxq::moe_few_down<SCH, NU>(a);                                                                      \
+// rlxq_moefew_gu_<scheme>_p<planes>_m<entries a pass>, rlxq_moefew_dn_<scheme>
+#define RLXQ_FEW_GU(SNAME, SCH, P, M)                                                                          \
+  extern "C" __global__ __launch_bounds__(512) void rlxq_moefew_gu_##SNAME##_p##P##_m##M(rlxq_moe_few_args a) { \
+    rlxq::moe_few_gate_up<SCH, P, M>(a);                                                                       \
   }
-// (units of two blocks: at most two per lane, which covers K = 8192 as four of
-// one do)
-#define RLXQ_FEW1(SNAME, SCH) \
-  RLXQ_FEW_U(SNAME, SCH, 1)   \
-  RLXQ_FEW_U(SNAME, SCH, 2)   \
-  RLXQ_FEW_U(SNAME, SCH, 3)   \
-  RLXQ_FEW_U(SNAME, SCH, 4)
-#define RLXQ_FEW2(SNAME, SCH) \
-  RLXQ_FEW_U(SNAME, SCH, 1)   \
-  RLXQ_FEW_U(SNAME, SCH, 2)
+#define RLXQ_FEW(SNAME, SCH)                                                                      \
+  RLXQ_FEW_GU(SNAME, SCH, 1, 1)                                                                   \
+  RLXQ_FEW_GU(SNAME, SCH, 2, 1)                                                                   \
+  RLXQ_FEW_GU(SNAME, SCH, 1, 2)                                                                   \
+  RLXQ_FEW_GU(SNAME, SCH, 2, 2)                                                                   \
+  RLXQ_FEW_GU(SNAME, SCH, 1, 4)                                                                   \
+  RLXQ_FEW_GU(SNAME, SCH, 2, 4)                                                                   \
+  extern "C" __global__ __launch_bounds__(512) void rlxq_moefew_dn_##SNAME(rlxq_moe_few_args a) { \
+    rlxq::moe_few_down<SCH>(a);                                                                   \
+  }
 #if RLXQ_PART_IS(1)
-RLXQ_FEW1(mxfp4, SCH_MXFP4)
-RLXQ_FEW1(q4_1, SCH_Q4_1)
+RLXQ_FEW(mxfp4, SCH_MXFP4)
+RLXQ_FEW(q4_1, SCH_Q4_1)
 #endif
 #if RLXQ_PART_IS(2)
-RLXQ_FEW2(q4_k, SCH_Q4_K)
-RLXQ_FEW2(q4_0, SCH_Q4_0)
-RLXQ_FEW2(q8_0, SCH_Q8_0)
+RLXQ_FEW(q4_k, SCH_Q4_K)
+RLXQ_FEW(q4_0, SCH_Q4_0)
 #endif
 #if RLXQ_PART_IS(3)
-RLXQ_FEW1(q6_k, SCH_Q6_K)
-RLXQ_FEW2(q5_k, SCH_Q5_K)
+RLXQ_FEW(q6_k, SCH_Q6_K)
+RLXQ_FEW(q8_0, SCH_Q8_0)
 #endif
 #if RLXQ_PART_IS(4)
-RLXQ_FEW1(q3_k, SCH_Q3_K)
+RLXQ_FEW(q3_k, SCH_Q3_K)
+RLXQ_FEW(q5_k, SCH_Q5_K)
 #endif
 #if RLXQ_PART_IS(5)
-RLXQ_FEW1(q2_k, SCH_Q2_K)
-RLXQ_FEW1(q8_k, SCH_Q8_K)
+RLXQ_FEW(q2_k, SCH_Q2_K)
+RLXQ_FEW(q8_k, SCH_Q8_K)
 #endif

@@ -555,24 +555,16 @@ int layer_pick(rlxq_ctx* ctx, const LayerCall& c, const float* logits, int32_t* 
   return launch(ctx, fn, dim3((unsigned)c.rows), dim3(64), 0, stream, args, name);
 }
 
-// Lanes (2^log2l) a weight row of K elements is spread over.  Fewer lanes a row
-// take more rows at once, which share the reduction and the stores and read an
-// activation record together; the waves still want `cols` columns' worth of
-// steps each.  Of the widths that give it, the one with the fewest idle lanes.
-int few_log2l(int scheme, int64_t k, double cols) {
+// Lanes (2^log2l) a weight row of K elements is spread over: 16, or 8 where
+// there is a group of eight columns for every wave or fewer lanes stay idle.
+// Fewer lanes a row take more rows at once, which share the reduction and the
+// stores and read an activation record together (16 rows of MXFP4, us for the
+// layer: 8 lanes 67, 16 lanes 69, 32 lanes 83, 64 lanes 90).
+int few_log2l(int scheme, int64_t k, double cols_per_wave) {
   const int blocks = scheme == RLXQ_GGUF_Q4_0 || scheme == RLXQ_GGUF_Q8_0 || scheme == RLXQ_GGUF_Q4_K ||
                      scheme == RLXQ_GGUF_Q5_K ? 2 : 1;
   const int64_t units = k / 32 / blocks;
-  int lo = 6;   // 64 / 2^lo rows at once
-  while (lo > 3 && (double)(64 >> (lo - 1)) <= cols) lo--;
-  if (const char* e = std::getenv("RLXQ_FEW_L")) lo = std::atoi(e);
-  int best = lo;
-  int64_t cap = ((units + (1 << lo) - 1) >> lo) << lo;
-  for (int l = lo - 1; l >= 3 && l >= lo - 1; l--) {
-    const int64_t c = ((units + (1 << l) - 1) >> l) << l;
-    if (c < cap) cap = c, best = l;
-  }
-  return best;
+  return cols_per_wave >= 8. || (units + 7) / 8 * 8 < (units + 15) / 16 * 16 ? 3 : 4;
 }
 int few_order(int scheme) {   // of a block's codes (moe_args.h)
   return scheme == RLXQ_MLX_MXFP4 ? 0 : scheme == RLXQ_GGUF_Q4_0 || scheme == RLXQ_GGUF_Q4_1 ? 1 : 2;
@@ -582,20 +574,29 @@ size_t few_down_lds(const LayerCall& c, int64_t tile) {
 }
 constexpr int64_t kFewTile = 256;   // most columns of a down workgroup
 
-// Entries of one expert that share a pass over its weights, by the entries per
-// fired expert to expect of even routing (one row: every expert once).
-int few_mt(const LayerCall& c) {
-  if (c.rows == 1) return 1;
+// Entries per fired expert to expect of even routing.
+double few_avg(const LayerCall& c) {
+  if (c.rows <= 1) return 1.;
   const double e = (double)c.experts, k = (double)c.top_k, r = (double)c.rows;
-  const double avg = r * k / (e * (1.0 - std::pow(1.0 - k / e, r)));
-  return avg < 1.1 ? 1 : avg < 2.2 ? 2 : 4;
+  return r * k / (e * (1.0 - std::pow(1.0 - k / e, r)));
 }
 
-// Whether the few-token kernels hold the call: entries fit a workgroup's tables,
-// the activation rows its LDS.
-bool few_holds(const rlxq_ctx* ctx, const LayerCall& c) {
-  const size_t lds = std::min<size_t>(ctx->max_lds, 160 * 1024) - 8192;   // (less the routing's tables)
-  return c.rows <= 32 && c.rows * c.top_k <= 256 &&
+// Entries of one expert that share a pass over its weights.  us for the layer at
+// 1 / 4 (2048 -> 768, 8 of 128): MXFP4 bf16 8 rows (1.24 entries) 38.8 / 43.7,
+// 16 (1.55) 61.3 / 60.1, 24 (1.9) 94.2 / 86.5, 32 (2.3) 113.6 / 95.8; Q4_K f32
+// 56.5 / 63.6, 97.0 / 97.1, 156.7 / 152.7, 180.5 / 165.9.  Two at once lay
+// between the two.
+int few_mt(const LayerCall& c) { return few_avg(c) < 1.75 ? 1 : 4; }
+
+// Whether the few-token kernels take the call: entries fit a workgroup's tables,
+// the activation rows its LDS, and fewer than eight entries come to a fired
+// expert: from there the grouped products run on the matrix instructions.  us
+// for the layer, few-token kernels / grouped (2 of 8 experts): Q4_1 5632 f32 24
+// rows (6 entries) 154 / 343, 32 rows (8 entries) 186 / 102; MXFP4 2816 bf16 67 /
+// 134 and 79 / 61; Q8_0 1024 bf16 43 / 98 and 54 / 50.
+bool few_takes(const rlxq_ctx* ctx, const LayerCall& c) {
+  const size_t lds = std::min<size_t>(ctx->max_lds, 160 * 1024) - 16384;   // (less the routing's tables)
+  return c.rows <= 32 && c.rows * c.top_k <= 256 && few_avg(c) < 8. &&
          (size_t)few_mt(c) * (size_t)(c.hidden / 32 * RLXQ_FEW_REC(c.x_dtype == RLXQ_BF16 ? 1 : 2)) <= lds &&
          few_down_lds(c, kFewTile) <= lds;
 }
@@ -659,11 +660,10 @@ int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   std::snprintf(name, sizeof name, "rlxq_moefew_gu_%s_p%d_m%d", scheme_name(c.gu_scheme), planes, mt);
   if ((rc = get_fn(ctx, name, &fn))) return rc;
   void* args[] = {&a};
-  // one round of workgroups: of four waves for up to four rows to route, else
-  // of eight
+  // one round of workgroups
   const size_t lds = (size_t)mt * xrow;
-  const int waves = c.rows <= 4 ? 4 : 8;
-  const int64_t wgs = cus * std::min(16 / waves, blocks_per_cu(ctx, name, fn, 64 * waves, lds));
+  const int waves = 8;
+  const int64_t wgs = cus * std::min(2, blocks_per_cu(ctx, name, fn, 64 * waves, lds));
   a.log2l = few_log2l(c.gu_scheme, c.hidden, (double)n * (double)c.inter / (double)(wgs * waves));
   const int64_t steps = (int64_t)n * ((c.inter + (64 >> a.log2l) - 1) / (64 >> a.log2l));
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(wgs, (steps + waves - 1) / waves));
@@ -673,15 +673,20 @@ int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   a.bank = static_cast<const uint8_t*>(c.d);
   a.scales = static_cast<const uint8_t*>(c.d_s);
   if ((rc = check_weights(ctx, "moe_layer down", c.d_scheme, 32, c.d, c.d_s, nullptr, RLXQ_U8, c.inter, &a.rb))) return rc;
-  // column tiles: two workgroups a CU, whole steps of the waves of a slot
-  const int64_t unit = (64 >> a.log2l) * std::max<int64_t>(1, 8 / c.top_k);
-  int64_t tile = (c.rows * c.hidden + 2 * cus - 1) / (2 * cus);
-  tile = std::min<int64_t>(kFewTile, std::max<int64_t>(unit, (tile + unit - 1) / unit * unit));
-  a.tile = (int32_t)tile;
-  a.tiles = (int32_t)((c.hidden + tile - 1) / tile);
   std::snprintf(name, sizeof name, "rlxq_moefew_dn_%s", scheme_name(c.d_scheme));
   if ((rc = get_fn(ctx, name, &fn))) return rc;
-  return launch(ctx, fn, dim3((unsigned)(c.rows * ((a.tiles + 7) / 8 * 8))), dim3(512), few_down_lds(c, tile), stream, args, name);
+  // column tiles: whole steps of the waves of a slot, so that the rounds of
+  // workgroups are short; a workgroup's records cost it some 24 columns' time
+  const int64_t unit = (64 >> a.log2l) * std::max<int64_t>(1, 8 / c.top_k);
+  const int64_t slots = cus * std::min(2, blocks_per_cu(ctx, name, fn, 512, few_down_lds(c, kFewTile)));
+  auto wgs_of = [&](int64_t tile) { return c.rows * (((c.hidden + tile - 1) / tile + 7) / 8 * 8); };
+  auto cost = [&](int64_t tile) { return (wgs_of(tile) + slots - 1) / slots * (tile + 24); };
+  int64_t tile = unit;
+  for (int64_t t = 2 * unit; t <= kFewTile; t += unit)
+    if (cost(t) < cost(tile)) tile = t;
+  a.tile = (int32_t)tile;
+  a.tiles = (int32_t)((c.hidden + tile - 1) / tile);
+  return launch(ctx, fn, dim3((unsigned)wgs_of(tile)), dim3(512), few_down_lds(c, tile), stream, args, name);
 }
 
 // The layer from the library's own calls: router product, top-k, grouped
@@ -804,7 +809,7 @@ int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype, const void* router
   if (!g.ok()) return fail(ctx, RLXQ_E_HIP, "moe_layer: hipSetDevice");
   const LayerCall c{x,        x_dtype, router, router_dtype, logits, gate_up_scheme, gate_up, gate_up_scales, down_scheme,
                     down,     down_scales, rows, hidden, inter, num_experts, top_k, renorm, ids, probs, y, y_dtype};
-  bool few = few_holds(ctx, c);
+  bool few = few_takes(ctx, c);
   if (const char* e = std::getenv("RLXQ_MOE_LAYER")) few = few && std::strcmp(e, "grouped") != 0;
   return few ? layer_few(ctx, c, stream) : layer_grouped(ctx, c, stream);
 }

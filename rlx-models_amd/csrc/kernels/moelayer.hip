@@ -106,6 +106,17 @@ RLXQ_DEV float wave_fmax(float v) {
   return fmaxf(fmaxf(at(0), at(16)), fmaxf(at(32), at(48)));
 }
 
+// Inclusive sum over a wave's lanes: within rows of 16, then across them.
+RLXQ_DEV int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // a row's last lane to the next row; to the upper half
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
 // Floats in their order as unsigned keys, all above 0 (-0 as 0).
 RLXQ_DEV uint32_t order_key(float f) {
   const uint32_t u = __float_as_uint(f + 0.f);
@@ -137,9 +148,8 @@ RLXQ_DEV void pick_row(const float* __restrict__ l, int E, int top_k, bool renor
     prob = __uint_as_float(0x7fc00000u);
     return;
   }
-  float kept = 0.f;
   id = 0;
-  prob = 0.f;
+  uint32_t mine = 0;   // lane j: the j-th key
   for (int j = 0; j < top_k; j++) {
     uint32_t best = 0;
 #pragma unroll
@@ -151,18 +161,17 @@ RLXQ_DEV void pick_row(const float* __restrict__ l, int E, int top_k, bool renor
       const uint64_t b = __ballot(key[i] == best);
       if (b) pick = 64 * i + __builtin_ctzll(b);
     }
-    const uint32_t u = best & 0x80000000u ? best & 0x7fffffffu : ~best;
-    const float p = expf(__uint_as_float(u) - mx) / s;
-    kept += p;
     if (lane == j) {
       id = pick;
-      prob = p;
+      mine = best;
     }
 #pragma unroll
     for (int i = 0; i < NPER; i++)
       if (lane + 64 * i == pick) key[i] = 0u;
   }
-  if (renorm) prob /= kept;
+  const float f = __uint_as_float(mine & 0x80000000u ? mine & 0x7fffffffu : ~mine);
+  prob = lane < top_k ? expf(f - mx) / s : 0.f;
+  if (renorm) prob /= lane_group_sum<64>(prob);
 }
 
 template <int NPER>
@@ -318,26 +327,6 @@ struct FewW {
   }
 };
 
-// One block's record in registers.
-template <int NPL>
-struct FewRec {
-  uint32_t h[16], l[NPL == 2 ? 16 : 1];
-  float4 me;
-  RLXQ_DEV void load(const uint8_t* rec, bool uok) {
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const uint4 v = reinterpret_cast<const uint4*>(rec)[q];
-      h[4 * q] = v.x; h[4 * q + 1] = v.y; h[4 * q + 2] = v.z; h[4 * q + 3] = v.w;
-      if constexpr (NPL == 2) {
-        const uint4 z = reinterpret_cast<const uint4*>(rec)[4 + q];
-        l[4 * q] = z.x; l[4 * q + 1] = z.y; l[4 * q + 2] = z.z; l[4 * q + 3] = z.w;
-      }
-    }
-    // (a unit past the row's end repeats the last one, times zero)
-    me = uok ? reinterpret_cast<const float4*>(rec)[4 * NPL] : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-};
-
 // A block of a weight row: exact f16 codes, multipliers of its code sum (of its
 // halves') and of its activations' sum (halves').
 template <int SCH>
@@ -352,90 +341,84 @@ struct FewBlk {
     else if constexpr (half_scales<SCH>()) block_scales_half<SCH>(w.dw, d, d2, mn, m2);
     else block_scales<SCH>(w.dw, bl, d, mn, u);
   }
-  template <int NPL>
-  RLXQ_DEV void add(const FewRec<NPL>& x, float& s) const {
-    float c0 = 0.f, c1 = 0.f;   // (two chains: the halves, hi and lo, or even and odd pairs)
+  // the codes times 32 f16 activations (a plane of a record), added to c
+  // (two chains: the block's halves, or even and odd pairs)
+  RLXQ_DEV void dots(const uint32_t (&h)[16], float (&c)[2]) const {
 #pragma unroll
     for (int t = 0; t < 16; t++) {
-      if constexpr (half_scales<SCH>()) {
-        float& c = t < 8 ? c0 : c1;
-        c = dot2_f16(pw[t], x.h[t], c);
-        if constexpr (NPL == 2) c = dot2_f16(pw[t], x.l[t], c);
-      } else if constexpr (NPL == 2) {
-        c0 = dot2_f16(pw[t], x.h[t], c0);
-        c1 = dot2_f16(pw[t], x.l[t], c1);
-      } else {
-        float& c = t & 1 ? c1 : c0;
-        c = dot2_f16(pw[t], x.h[t], c);
-      }
+      float& q = c[half_scales<SCH>() ? t / 8 : t % 2];
+      q = dot2_f16(pw[t], h[t], q);
     }
+  }
+  // the block's sum of products from its code sums and the record's factors
+  RLXQ_DEV float finish(const float (&c)[2], const float4& me, float s) const {
     if constexpr (half_scales<SCH>()) {
-      s = fmaf(d * x.me.x, c0, s);
-      s = fmaf(d2 * x.me.x, c1, s);
+      s = fmaf(d * me.x, c[0], s);
+      s = fmaf(d2 * me.x, c[1], s);
       if constexpr (SCH == SCH_Q2_K) {
-        s = fmaf(mn, x.me.z, s);
-        s = fmaf(m2, x.me.y - x.me.z, s);
+        s = fmaf(mn, me.z, s);
+        s = fmaf(m2, me.y - me.z, s);
       }
     } else {
-      s = fmaf(d * x.me.x, c0 + c1, s);
-      if constexpr (SCH == SCH_Q4_1 || SCH == SCH_Q4_K || SCH == SCH_Q5_K) s = fmaf(mn, x.me.y, s);
+      s = fmaf(d * me.x, c[0] + c[1], s);
+      if constexpr (SCH == SCH_Q4_1 || SCH == SCH_Q4_K || SCH == SCH_Q5_K) s = fmaf(mn, me.y, s);
     }
+    return s;
   }
 };
 
 // A unit's part of R weight rows (w[0 .. R - 1], unit u) times MT activation
-// rows (records of the unit's first block at x + m * xld).  One activation row:
-// its record stays in registers and the weight rows are decoded in turn; more:
-// the weight rows are decoded once and the records pass.  (The empty statements
+// rows (records of the unit's first block at x + m * xld): the weight rows are
+// decoded once, and the records pass a plane at a time.  (The empty statements
 // keep the products where they stand: the compiler would gather them behind the
-// reads of all records, in as many registers, and run them for absent rows.)
+// reads of all planes, in as many registers, and run them for absent rows.)  A
+// lane past the row's end repeats the last unit and leaves its sum alone: times
+// zero, an infinity would stay.
 template <int SCH, int NPL, int R, int MT>
 RLXQ_DEV void few_unit(const FewW<SCH> (&w)[R], const uint8_t* x, int xld, int cnt, int u, bool uok, const UnpackK& kc,
                        float (&acc)[R][MT]) {
 #pragma unroll
   for (int bl = 0; bl < Unit<SCH>::BLOCKS; bl++) {
-    if constexpr (MT == 1) {
-      FewRec<NPL> rec;
-      rec.load(x + bl * RLXQ_FEW_REC(NPL), uok);
+    FewBlk<SCH> b[R];
 #pragma unroll
-      for (int r = 0; r < R; r++) {
-        FewBlk<SCH> b;
-        b.decode(w[r], bl, u, kc);
-        b.add(rec, acc[r][0]);
-        asm volatile("" : "+v"(acc[r][0]));
-      }
-    } else {
-      FewBlk<SCH> b[R];
+    for (int r = 0; r < R; r++) b[r].decode(w[r], bl, u, kc);
 #pragma unroll
-      for (int r = 0; r < R; r++) b[r].decode(w[r], bl, u, kc);
+    for (int m = 0; m < MT; m++) {
+      if (m > 0 && m >= cnt) break;   // (uniform)
+      const uint4* rec = reinterpret_cast<const uint4*>(x + m * xld + bl * RLXQ_FEW_REC(NPL));
+      float c[R][2];
 #pragma unroll
-      for (int m = 0; m < MT; m++) {
-        if (m > 0 && m >= cnt) break;   // (uniform)
-        FewRec<NPL> rec;
-        rec.load(x + m * xld + bl * RLXQ_FEW_REC(NPL), uok);
+      for (int r = 0; r < R; r++) c[r][0] = c[r][1] = 0.f;
+#pragma unroll
+      for (int pl = 0; pl < NPL; pl++) {
+        uint32_t h[16];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const uint4 v = rec[4 * pl + q];
+          h[4 * q] = v.x; h[4 * q + 1] = v.y; h[4 * q + 2] = v.z; h[4 * q + 3] = v.w;
+        }
 #pragma unroll
         for (int r = 0; r < R; r++) {
-          b[r].add(rec, acc[r][m]);
-          asm volatile("" : "+v"(acc[r][m]));
+          b[r].dots(h, c[r]);
+          asm volatile("" : "+v"(c[r][0]), "+v"(c[r][1]));
         }
+      }
+      const float4 me = reinterpret_cast<const float4*>(rec)[4 * NPL];
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float s = b[r].finish(c[r], me, acc[r][m]);
+        acc[r][m] = uok ? s : acc[r][m];
       }
     }
   }
 }
 
-// Sum over aligned groups of L = 2^log2l lanes (4 .. 64), in every lane of the
-// group; the branches are uniform.
+// Sum over aligned groups of 2^log2l lanes (8 or 16), in every lane of the
+// group; the branch is uniform.
 RLXQ_DEV float few_sum(float v, int log2l) {
-  v = group4_sum(v);
-  if (log2l == 2) return v;
-  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xF, 0xF, false));
-  if (log2l == 3) return v;
-  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xF, 0xF, false));
-  if (log2l == 4) return v;
-  auto at = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
-  const float r0 = at(0), r1 = at(16), r2 = at(32), r3 = at(48);
-  if (log2l == 5) return (threadIdx.x & 32) ? r2 + r3 : r0 + r1;
-  return (r0 + r1) + (r2 + r3);
+  v = group8_sum(v);
+  if (log2l == 4) v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xF, 0xF, false));
+  return v;
 }
 
 RLXQ_DEV UnpackK f16_unpack_consts() {
@@ -453,7 +436,9 @@ RLXQ_DEV UnpackK f16_unpack_consts() {
 // needs the records in LDS.
 template <int SCH, int NPL, int R, int MT>
 struct FewCols {
-  static constexpr int D0 = 48 / (R * Unit<SCH>::DW), D = D0 < 1 ? 1 : D0 > 4 ? 4 : D0;   // (48 registers of weights)
+  // steps in 48 registers of weights (one step ahead of the wide units, which
+  // exceed them, cost more in waves than it hid: Q6_K, 8 rows, 48 -> 50 us)
+  static constexpr int D0 = 48 / (R * Unit<SCH>::DW), D = D0 < 1 ? 1 : D0 > 4 ? 4 : D0;
   FewW<SCH> ring[D][R];
   const uint8_t* base;
   const uint8_t* sbase;
@@ -542,7 +527,7 @@ RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
   __shared__ __attribute__((aligned(16))) int32_t ids[FEW_ENTRIES];
   // (MT > 1; a chunk holds at least one entry)
   __shared__ uint32_t mask[MT > 1 ? 1024 : 1];
-  __shared__ int32_t first[MT > 1 ? 1024 : 1], member[MT > 1 ? FEW_ENTRIES * MT : 1], wsum[8];
+  __shared__ int32_t first[MT > 1 ? 1024 : 1], member[MT > 1 ? FEW_ENTRIES * MT : 1], wsum[4], cut[4];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int n = a.rows * a.top_k, nb = a.H / 32, xld = nb * RLXQ_FEW_REC(NPL);
   auto stage = [&](int m, int r) {
@@ -574,59 +559,77 @@ RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
     }
   }
   __syncthreads();
-  int chunks = n;
-  if constexpr (MT > 1) {
+  // Entries in chunks of up to MT of one expert, and the workgroup's share of the
+  // (chunk, step) pairs in sequence: from step c_lo of chunk ch_lo up to step c_hi
+  // of chunk ch_hi.  A step, a group of RP columns, of a chunk of m entries counts
+  // 1 + m (counted alike, 16 rows at MT 4 took 75 us instead of 68).
+  const int RP = 64 >> a.log2l, steps = (a.I + RP - 1) / RP;
+  int ch_lo, c_lo, ch_hi, c_hi;
+  if constexpr (MT == 1) {
+    const int total = n * steps, share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int s0 = min(share * (int)blockIdx.x, total), s1 = min(s0 + share, total);
+    ch_lo = s0 / steps, c_lo = s0 - ch_lo * steps;
+    ch_hi = s1 / steps, c_hi = s1 - ch_hi * steps;
+  } else {
     // a row takes an expert once: an expert's entries are the bits of a mask of
     // rows, an entry's rank among them the bits below its row's
-    for (int i = threadIdx.x; i < n; i += blockDim.x) atomicOr(&mask[ids[i]], 1u << (i / a.top_k));
+    const float inv_k = 1.f / (float)a.top_k;
+    auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * inv_k); };   // (i < 256, top_k <= 64: exact)
+    for (int i = threadIdx.x; i < n; i += blockDim.x) atomicOr(&mask[ids[i]], 1u << row_of(i));
     __syncthreads();
-    // chunk offsets: exclusive sum over the experts, four a thread
-    int c4[4], t = 0;
+    // before each expert, in one sum over them (four a thread): chunks << 16 | entries
+    int at[4], t = 0, cnt[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int q = 0; q < 4; q++) {
       const int e = 4 * threadIdx.x + q;
-      c4[q] = e < a.E ? (__popc(mask[e]) + MT - 1) / MT : 0;
-      t += c4[q];
+      if (e < a.E) cnt[q] = __popc(mask[e]);
+      at[q] = t;
+      t += ((cnt[q] + MT - 1) / MT) << 16 | cnt[q];
     }
-    int inc = t;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(inc, off, 64);
-      if (lane >= off) inc += o;
-    }
-    if (lane == 63) wsum[wv] = inc;
+    const int inc = wave_scan(t);
+    if (lane == 63 && wv < 4) wsum[wv] = inc;
     __syncthreads();
-    int off = inc - t;
-    chunks = 0;
-    for (int q = 0; q < nw; q++) {
-      off += q < wv ? wsum[q] : 0;
-      chunks += wsum[q];
-    }
+    int before = inc - t, all = 0;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      const int e = 4 * threadIdx.x + q;
-      if (e < a.E) first[e] = off;
-      off += c4[q];
+      before += q < wv ? wsum[q] : 0;
+      all += wsum[q];
+    }
+    all = __builtin_amdgcn_readfirstlane(all);
+    const int total = ((all >> 16) + (all & 0xFFFF)) * steps, share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int s0 = min(share * (int)blockIdx.x, total), s1 = min(s0 + share, total);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      if (cnt[q] == 0) continue;
+      const int p = before + at[q], chunks = (cnt[q] + MT - 1) / MT;
+      first[4 * threadIdx.x + q] = p >> 16;
+      const int lo = ((p >> 16) + (p & 0xFFFF)) * steps, span = (chunks + cnt[q]) * steps;
+#pragma unroll
+      for (int side = 0; side < 2; side++) {
+        const int rel = (side ? s1 : s0) - lo;
+        if (rel < 0 || rel >= span) continue;
+        const int k = rel / ((MT + 1) * steps);   // (the chunks before an expert's last are full)
+        cut[2 * side] = (p >> 16) + k;
+        cut[2 * side + 1] = (rel - k * (MT + 1) * steps) / (min(MT, cnt[q] - k * MT) + 1);
+      }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int e = ids[i], rank = __popc(mask[e] & ((1u << (i / a.top_k)) - 1));
+      const int e = ids[i], rank = __popc(mask[e] & ((1u << row_of(i)) - 1));
       member[(first[e] + rank / MT) * MT + rank % MT] = i;
     }
     __syncthreads();
+    // (no expert holds the end of the sequence)
+    ch_lo = s0 < total ? __builtin_amdgcn_readfirstlane(cut[0]) : all >> 16;
+    c_lo = s0 < total ? __builtin_amdgcn_readfirstlane(cut[1]) : 0;
+    ch_hi = s1 < total ? __builtin_amdgcn_readfirstlane(cut[2]) : all >> 16;
+    c_hi = s1 < total ? __builtin_amdgcn_readfirstlane(cut[3]) : 0;
   }
-  const int RP = 64 >> a.log2l;
   const UnpackK kc = f16_unpack_consts();
-  // steps of a chunk: groups of RP columns
-  const int steps = (a.I + RP - 1) / RP;
-  const int64_t total = (int64_t)chunks * steps;
-  int64_t s = total * blockIdx.x / gridDim.x;
-  const int64_t s_end = total * (blockIdx.x + 1) / gridDim.x;
   bool again = false;
-  while (s < s_end) {   // (uniform over the workgroup)
-    const int ch = (int)(s / steps), c0 = (int)(s - (int64_t)ch * steps);
-    const int64_t left = s_end - (int64_t)ch * steps;
-    const int c1 = (int)(left < steps ? left : steps);
+  for (int ch = ch_lo; ch <= ch_hi; ch++) {   // (uniform over the workgroup)
+    const int c0 = ch == ch_lo ? c_lo : 0, c1 = ch == ch_hi ? c_hi : steps;
+    if (c0 >= c1) continue;
     int ent[MT], cnt = 1;
     if constexpr (MT > 1) {
       cnt = 0;
@@ -665,7 +668,6 @@ RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
       a.act[(int64_t)en * a.I + col] = v[0] / (1.f + expf(-v[0])) * v[1];   // silu(g) * u
     });
     again = true;
-    s = (int64_t)ch * steps + c1;
   }
 }
 
@@ -771,8 +773,6 @@ RLXQ_PICK(16)
 #define RLXQ_FEW(SNAME, SCH)                                                                      \
   RLXQ_FEW_GU(SNAME, SCH, 1, 1)                                                                   \
   RLXQ_FEW_GU(SNAME, SCH, 2, 1)                                                                   \
-  RLXQ_FEW_GU(SNAME, SCH, 1, 2)                                                                   \
-  RLXQ_FEW_GU(SNAME, SCH, 2, 2)                                                                   \
   RLXQ_FEW_GU(SNAME, SCH, 1, 4)                                                                   \
   RLXQ_FEW_GU(SNAME, SCH, 2, 4)                                                                   \
   extern "C" __global__ __launch_bounds__(512) void rlxq_moefew_dn_##SNAME(rlxq_moe_few_args a) { \

@@ -530,7 +530,8 @@ int layer_logits(rlxq_ctx* ctx, const LayerCall& c, float* logits, void* stream)
   hipFunction_t fn;
   int rc = get_fn(ctx, name, &fn);
   if (rc) return rc;
-  const int64_t gx = big ? (c.experts + 3) / 4 : c.experts, gy = big ? (c.rows + 7) / 8 : (c.rows + 3) / 4;
+  // (rows along x: the y dimension ends at 65536)
+  const int64_t gx = big ? (c.rows + 7) / 8 : (c.rows + 3) / 4, gy = big ? (c.experts + 3) / 4 : c.experts;
   void* args[] = {&a};
   return launch(ctx, fn, dim3((unsigned)gx, (unsigned)gy), dim3(64), 0, stream, args, name);
 }
@@ -585,20 +586,26 @@ double few_avg(const LayerCall& c) {
 // 1 / 4 (2048 -> 768, 8 of 128): MXFP4 bf16 8 rows (1.24 entries) 38.8 / 43.7,
 // 16 (1.55) 61.3 / 60.1, 24 (1.9) 94.2 / 86.5, 32 (2.3) 113.6 / 95.8; Q4_K f32
 // 56.5 / 63.6, 97.0 / 97.1, 156.7 / 152.7, 180.5 / 165.9.  Two at once lay
-// between the two.
-int few_mt(const LayerCall& c) { return few_avg(c) < 1.75 ? 1 : 4; }
+// between the two.  (One at once too where LDS does not hold four rows.)
+size_t few_row_bytes(const LayerCall& c) {
+  return (size_t)(c.hidden / 32 * RLXQ_FEW_REC(c.x_dtype == RLXQ_BF16 ? 1 : 2));
+}
+size_t few_lds(const rlxq_ctx* ctx) {   // (less the routing's tables)
+  return std::min<size_t>(ctx->max_lds, 160 * 1024) - 16384;
+}
+int few_mt(const rlxq_ctx* ctx, const LayerCall& c) {
+  return few_avg(c) < 1.75 || 4 * few_row_bytes(c) > few_lds(ctx) ? 1 : 4;
+}
 
 // Whether the few-token kernels take the call: entries fit a workgroup's tables,
-// the activation rows its LDS, and fewer than eight entries come to a fired
+// an activation row its LDS, and fewer than eight entries come to a fired
 // expert: from there the grouped products run on the matrix instructions.  us
 // for the layer, few-token kernels / grouped (2 of 8 experts): Q4_1 5632 f32 24
 // rows (6 entries) 154 / 343, 32 rows (8 entries) 186 / 102; MXFP4 2816 bf16 67 /
 // 134 and 79 / 61; Q8_0 1024 bf16 43 / 98 and 54 / 50.
 bool few_takes(const rlxq_ctx* ctx, const LayerCall& c) {
-  const size_t lds = std::min<size_t>(ctx->max_lds, 160 * 1024) - 16384;   // (less the routing's tables)
-  return c.rows <= 32 && c.rows * c.top_k <= 256 && few_avg(c) < 8. &&
-         (size_t)few_mt(c) * (size_t)(c.hidden / 32 * RLXQ_FEW_REC(c.x_dtype == RLXQ_BF16 ? 1 : 2)) <= lds &&
-         few_down_lds(c, kFewTile) <= lds;
+  return c.rows <= 32 && c.rows * c.top_k <= 256 && few_avg(c) < 8. && few_row_bytes(c) <= few_lds(ctx) &&
+         few_down_lds(c, kFewTile) <= few_lds(ctx);
 }
 
 // Three launches: router product and prepared rows; routing, gate|up and
@@ -607,7 +614,7 @@ int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   auto r256 = [](size_t b) { return (b + 255) & ~size_t(255); };
   const size_t n = (size_t)(c.rows * c.top_k);
   const int planes = c.x_dtype == RLXQ_BF16 ? 1 : 2;
-  const size_t xrow = (size_t)(c.hidden / 32 * RLXQ_FEW_REC(planes));
+  const size_t xrow = few_row_bytes(c);
   const size_t b_log = c.logits ? 0 : r256((size_t)(c.rows * c.experts) * 4), b_ids = r256(n * 4), b_pr = r256(n * 4);
   const size_t b_rec = r256((size_t)c.rows * xrow), b_act = r256(n * (size_t)c.inter * 4);
   void* ws = nullptr;
@@ -656,7 +663,7 @@ int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   a.bank = static_cast<const uint8_t*>(c.gu);
   a.scales = static_cast<const uint8_t*>(c.gu_s);
   if ((rc = check_weights(ctx, "moe_layer gate_up", c.gu_scheme, 32, c.gu, c.gu_s, nullptr, RLXQ_U8, c.hidden, &a.rb))) return rc;
-  const int mt = few_mt(c);
+  const int mt = few_mt(ctx, c);
   std::snprintf(name, sizeof name, "rlxq_moefew_gu_%s_p%d_m%d", scheme_name(c.gu_scheme), planes, mt);
   if ((rc = get_fn(ctx, name, &fn))) return rc;
   void* args[] = {&a};

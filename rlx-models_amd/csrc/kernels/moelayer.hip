@@ -742,10 +742,10 @@ RLXQ_DEV void moe_few_down(const rlxq_moe_few_args& a) {
 // rlxq_moe_logits_<x>_<router>_e<EB>r<RB>; rlxq_moe_prep_<x>_<router>
 #define RLXQ_LOGITS(XN, XBF, RN, RBF)                                                                               \
   extern "C" __global__ __launch_bounds__(64) void rlxq_moe_logits_##XN##_##RN##_e1r4(rlxq_moe_logits_args a) {     \
-    rlxq::moe_logits_body<XBF, RBF, 1, 4>(a, blockIdx.x, blockIdx.y);                                               \
+    rlxq::moe_logits_body<XBF, RBF, 1, 4>(a, blockIdx.y, blockIdx.x);                                               \
   }                                                                                                                 \
   extern "C" __global__ __launch_bounds__(64) void rlxq_moe_logits_##XN##_##RN##_e4r8(rlxq_moe_logits_args a) {     \
-    rlxq::moe_logits_body<XBF, RBF, 4, 8>(a, blockIdx.x, blockIdx.y);                                               \
+    rlxq::moe_logits_body<XBF, RBF, 4, 8>(a, blockIdx.y, blockIdx.x);                                               \
   }                                                                                                                 \
   extern "C" __global__ __launch_bounds__(256) void rlxq_moe_prep_##XN##_##RN(rlxq_moe_prep_args a) {                \
     rlxq::moe_prep_body<XBF, RBF>(a);                                                                               \

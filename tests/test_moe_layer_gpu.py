@@ -303,6 +303,77 @@ def test_streams_and_graphs(ctx, orc, rows):
         np.testing.assert_array_equal(z.cpu().numpy(), eager[2])
     ctx.release_stream(stream=st.cuda_stream)
 
+# many slots, many experts, few and many rows an expert, LDS-filling rows
+FEW = [(1, 128, 192, 1024, 64, "q4_0", "q8_0"), (4, 256, 64, 65, 64, "q8_0", "q4_0"), (2, 512, 256, 700, 33, "q6_k", "q3_k"),
+       (32, 96, 64, 96, 8, "mxfp4", "q4_1"), (32, 256, 256, 20, 4, "q5_k", "q2_k"), (21, 512, 288, 7, 2, "q4_k", "q4_1"),
+       (17, 256, 512, 64, 15, "q2_k", "q5_k"), (24, 1056, 32, 12, 3, "q4_1", "mxfp4"), (13, 64, 2112, 5, 2, "q8_0", "q8_0")]
+
+
+@pytest.mark.parametrize("xdt", ["bf16", "f32"])
+@pytest.mark.parametrize("case", FEW, ids=lambda c: "x".join(map(str, c)))
+def test_few_tokens(ctx, orc, case, xdt):
+    """Both sides of the few-token kernels' own rules: one entry a pass and
+    four, column tiles that do not divide the row, idle lanes, 64 slots."""
+    import torch
+
+    announce(f"moe_layer few tokens {case} x={xdt}")
+    L = Layer(orc, np.random.default_rng(sum(case[:5])), *case[:5], *case[5:], xdt=xdt)
+    ids, p, gap, big = L.route()
+    assert gap > 1e-7
+    y = L.call(ctx)
+    torch.cuda.synchronize()
+    L.check(y, ids, p, big)
+
+
+def test_bank_beyond_32_bit_offsets(ctx):
+    """An expert behind the first 4 GiB of the bank gives the bits it gives as a
+    bank of its own (one row a pass, and several)."""
+    import rlxq
+    import torch
+
+    H, I, E = 16384, 8192, 36
+    for rows in (1, 5):
+        announce(f"moe_layer large bank rows={rows}")
+        gen = torch.Generator(device="cuda")
+        gen.manual_seed(rows)
+        g = torch.zeros(E * 2 * I * (H // 2), dtype=torch.uint8, device="cuda")
+        d = torch.zeros(E * H * (I // 2), dtype=torch.uint8, device="cuda")
+        gs = torch.full((E * 2 * I, H // 32), 110, dtype=torch.uint8, device="cuda")
+        ds = torch.full((E * H, I // 32), 110, dtype=torch.uint8, device="cuda")
+        assert g.numel() > 2 ** 32
+        ge, de = g.view(E, -1)[-1], d.view(E, -1)[-1]
+        for t in (ge, de):
+            t.copy_(torch.randint(0, 256, t.shape, device="cuda", dtype=torch.uint8, generator=gen))
+        x = torch.randn((rows, H), device="cuda", generator=gen)
+        logits = torch.zeros((rows, E), device="cuda")
+        logits[:, E - 1] = 50.0
+        a = ctx.moe_layer(x, None, g, d, rlxq.MLX_MXFP4, rlxq.MLX_MXFP4, 1, I, E, logits=logits, gate_up_scales=gs,
+                          down_scales=ds)
+        b = ctx.moe_layer(x, None, ge, de, rlxq.MLX_MXFP4, rlxq.MLX_MXFP4, 1, I, 1, logits=logits[:, :1].contiguous(),
+                          gate_up_scales=gs[-2 * I:], down_scales=ds[-H:])
+        torch.cuda.synchronize()
+        assert torch.isfinite(b).all() and b.abs().max() > 0
+        assert torch.equal(a, b)
+        del g, d, gs, ds
+
+
+def test_more_rows_than_a_grid_dimension(ctx, orc):
+    import torch
+
+    announce("moe_layer 600000 rows")
+    L = Layer(orc, np.random.default_rng(9), 40, 32, 32, 4, 1)
+    x = L.x.repeat(15000, 1)
+    i = torch.empty((600000, 1), dtype=torch.int32, device="cuda")
+    L.shape = (600000,) + L.shape[1:]
+    y = L.call(ctx, x=x, ids=i)
+    torch.cuda.synchronize()
+    L.shape = (40,) + L.shape[1:]
+    ids, p, gap, big = L.route()
+    assert gap > 1e-6
+    np.testing.assert_array_equal(i.view(15000, 40).cpu().numpy(), np.broadcast_to(ids[:, 0], (15000, 40)))
+    for at in (0, 262144 // 40, 7000, 14999):
+        L.check(y.view(15000, 40, 32)[at], ids, p, big)
+
 
 def test_quantised_experts_together(ctx, orc):
     """The set as it is used: float experts packed by quantize_mxfp4, a dense

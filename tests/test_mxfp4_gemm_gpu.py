@@ -352,6 +352,49 @@ def test_gemm_on_another_stream_and_in_a_graph(ctx, orc, m):
     ctx.release_stream(stream=st.cuda_stream)
 
 
+def test_beyond_32_bit_offsets(ctx):
+    """Rows behind the first 4 GiB: of the quantiser's input, of the codes, of
+    the product's weights and of its output."""
+    import rlxq
+    import torch
+
+    announce("mxfp4 beyond 4 GiB")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    K, N = 4096, 2113536
+
+    def values(t):
+        c, sc = ctx.quantize_mxfp4(t)
+        return ctx.dequantize(c, rlxq.MLX_MXFP4, *t.shape, scales=sc).view(t.shape).double()
+
+    tail = torch.randn((48, K), device="cuda", generator=gen)
+    x = torch.zeros((N, K), device="cuda")   # 35 GB
+    x[-48:] = tail
+    codes, scales = ctx.quantize_mxfp4(x)
+    c0, s0 = ctx.quantize_mxfp4(tail)
+    assert codes.numel() > 2 ** 32
+    assert torch.equal(codes[-48:], c0) and torch.equal(scales[-48:], s0)
+    back = ctx.dequantize(codes, rlxq.MLX_MXFP4, N, K, scales=scales, out=x)
+    assert torch.equal(back.view(N, K)[-48:].double(), values(tail))
+    del x, back
+    # f32 sums of K exact products, in the order of the kernel: K 2^-24 of their size
+    for m in (1, 20, 40):
+        v = torch.randn((m, K), device="cuda", generator=gen)
+        y = ctx.mxfp4_gemm(v, codes, scales, N)
+        torch.cuda.synchronize()
+        assert not y[:, :-48].any()
+        vv, wv = values(v).cpu(), values(tail).cpu()
+        assert ((y[:, -48:].cpu().double() - vv @ wv.T).abs() <= K * 2.0 ** -24 * (vv.abs() @ wv.abs().T)).all()
+    del codes, scales, y
+    v = torch.randn((33000, 64), device="cuda", generator=gen)   # an output of 33000 x 33024, 4.4 GB
+    t = torch.randn((33024, 64), device="cuda", generator=gen)
+    w, ws = ctx.quantize_mxfp4(t)
+    y = ctx.mxfp4_gemm(v, w, ws, 33024)
+    torch.cuda.synchronize()
+    vv, wv = values(v[-40:].contiguous()).cpu(), values(t).cpu()
+    assert ((y[-40:].cpu().double() - vv @ wv.T).abs() <= 64 * 2.0 ** -24 * (vv.abs() @ wv.abs().T)).all()
+
+
 def test_status_codes(ctx):
     import ctypes as C
 

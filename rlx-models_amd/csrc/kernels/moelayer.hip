@@ -233,7 +233,8 @@ RLXQ_DEV void put_record(uint8_t* rec, const float (&x)[4], int planes, int orde
 }
 
 // Router logits (the first lblocks workgroups: an expert and four rows, H over
-// the four waves) and, beside them, the prepared rows.
+// the four waves) and, beside them, the prepared rows.  Latency: 3.6 us for a
+// row, 5.5 for 16 (2048 elements, 128 experts).
 template <bool XBF, bool RBF>
 RLXQ_DEV void moe_prep_body(const rlxq_moe_prep_args& a) {
   constexpr int RB = 4;
@@ -518,9 +519,13 @@ constexpr int FEW_ENTRIES = 256;   // most (row, slot) pairs of a call (of at mo
 // gate|up and SwiGLU.  Every workgroup routes all rows itself (a wave a row:
 // the grid is one round of workgroups, so the layer pays for it once, where a
 // launch of its own would cost more).  The entries of one expert are cut into
-// chunks of MT, and the workgroups share the (chunk, columns) evenly; a chunk's
+// chunks of MT, and the workgroups share the (chunk, columns) by cost; a chunk's
 // rows are copied to LDS and its weights read once for all of them.  Workgroup
 // 0 leaves the routing for the down launch.
+// Bound by decoding and dot products beside the weight stream, once it runs
+// (2048 -> 2 x 768, 8 of 128 experts): MXFP4, 1 row 8.6 us, of which some 6 to the
+// first product; 16 rows 39 us for 191 MB past L2, VALU busy half of the time;
+// Q4_K, 4 rows 18 us for 53 MB.
 template <int SCH, int NPL, int MT>
 RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];   // MT rows of records
@@ -676,7 +681,9 @@ RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
 // (waves / top_k of them per slot, each a part of the tile; more slots than
 // waves in turns), and the slots are added in slot order.  Workgroups of one
 // column tile are dealt to one XCD (workgroup b runs on XCD b % 8), whose L2
-// then holds the rows of an expert that several tokens take.
+// then holds the rows of an expert that several tokens take.  Bound as gate|up
+// (768 -> 2048, 8 of 128): MXFP4 16 rows 25.7 us, 73 MB read past L2 of 114 MB in
+// all; Q6_K 4 rows 16.7 us for 40 MB.
 template <int SCH>
 RLXQ_DEV void moe_few_down(const rlxq_moe_few_args& a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];

@@ -375,6 +375,54 @@ def test_more_rows_than_a_grid_dimension(ctx, orc):
         L.check(y.view(15000, 40, 32)[at], ids, p, big)
 
 
+@pytest.mark.parametrize("rows", [4, 25, 60])
+@pytest.mark.parametrize("xdt", ["bf16", "f32"])
+def test_activations_not_finite_on_given_logits(ctx, orc, rows, xdt):
+    """Finite logits of the caller's: a row of x with an infinity or a NaN leaves
+    its y not finite, and the other rows are as without it.  (The infinity sits
+    in the last block of a row whose blocks do not fill the lanes.)"""
+    import torch
+
+    announce(f"moe_layer x not finite rows={rows} x={xdt}")
+    rng = np.random.default_rng(10)
+    L = Layer(orc, rng, rows, 288, 96, 9, 2, "q4_1", "mxfp4", xdt=xdt)
+    logits = rng.standard_normal((rows, 9)).astype(np.float32)
+    x = L.x.clone()
+    x[0, 287], x[2, 5], x[3, 100] = float("inf"), float("nan"), float("-inf")
+    y = L.call(ctx, x=x, router=None, logits=_t(logits))
+    torch.cuda.synchronize()
+    got = y.cpu().numpy()
+    ids, p, gap, big = L.route(True, logits)
+    want, tol = L.exact(ids, p, big, act_eps=2.0 ** -8 if xdt == "bf16" else 0.0)
+    assert gap > 1e-6 and not np.any(np.isfinite(got[[0, 2, 3]]))
+    ok = [i for i in range(rows) if i not in (0, 2, 3)]
+    assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
+
+
+def test_two_streams_at_once(ctx, orc):
+    """Calls of one context under way on two streams, each with its scratch."""
+    import torch
+
+    announce("moe_layer and mxfp4_gemm on two streams")
+    rng = np.random.default_rng(11)
+    L = Layer(orc, rng, 12, 1024, 256, 32, 8, "mxfp4", "mxfp4", xdt="bf16")
+    xs = [_as(rng.standard_normal((12, 1024)).astype(np.float32), "bf16")[0] for _ in range(2)]
+    w, ws = ctx.quantize_mxfp4(_t(rng.standard_normal((512, 1024)).astype(np.float32)))
+    want = [(L.call(ctx, x=x).clone(), ctx.mxfp4_gemm(x, w, ws, 512).clone()) for x in xs]
+    torch.cuda.synchronize()
+    st = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(20):
+        for s, x, out in zip(st, xs, got):
+            with torch.cuda.stream(s):
+                out.append((L.call(ctx, x=x), ctx.mxfp4_gemm(x, w, ws, 512)))
+    torch.cuda.synchronize()
+    for out, (a, b) in zip(got, want):
+        assert all(torch.equal(y, a) and torch.equal(z, b) for y, z in out)
+    for s in st:
+        ctx.release_stream(stream=s.cuda_stream)
+
+
 def test_quantised_experts_together(ctx, orc):
     """The set as it is used: float experts packed by quantize_mxfp4, a dense
     MXFP4 product on 4-bit activations in front, and the expert layer on its

@@ -137,7 +137,7 @@ typedef struct rlxq_moe_few_args {
   void* y;                  /* [rows, H]                                     */
   int64_t rb;               /* bytes of a packed row                         */
   int32_t rows, H, I, E, top_k, renorm, y_bf16;
-  int32_t log2l;            /* lanes of a weight row: 4 .. 64                */
+  int32_t log2l;            /* lanes of a weight row: 8 or 16                */
   int32_t tile;             /* down: columns of a workgroup                  */
   int32_t tiles;            /* down: column tiles                            */
 } rlxq_moe_few_args;

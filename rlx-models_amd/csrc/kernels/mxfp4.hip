@@ -624,6 +624,10 @@ RLXQ_DEV void mx_gemm_tile(const rlxq_mx_gemm_args& a, int tm, int tn, uint8_t* 
   // (the loads past the last stage: none may land in another workgroup's LDS)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   mx_mfma_done();
+#pragma unroll
+  for (int j = 0; j < TN; j++)
+#pragma unroll
+    for (int i = 0; i < TM; i++) asm volatile("" : "+a"(acc[j][i]));   // (no use of them moves ahead of it)
 
   // A lane holds activation row (column of the MFMA's result) lane & 31 and
   // weight rows 8 q + 4 g .. + 3 of each tile: four consecutive outputs.  A

@@ -817,6 +817,7 @@ int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype, const void* router
   const LayerCall c{x,        x_dtype, router, router_dtype, logits, gate_up_scheme, gate_up, gate_up_scales, down_scheme,
                     down,     down_scales, rows, hidden, inter, num_experts, top_k, renorm, ids, probs, y, y_dtype};
   bool few = few_takes(ctx, c);
+  // RLXQ_MOE_LAYER=grouped: the grouped products for every call (sweeps, tests)
   if (const char* e = std::getenv("RLXQ_MOE_LAYER")) few = few && std::strcmp(e, "grouped") != 0;
   return few ? layer_few(ctx, c, stream) : layer_grouped(ctx, c, stream);
 }

@@ -423,6 +423,65 @@ def test_two_streams_at_once(ctx, orc):
         ctx.release_stream(stream=s.cuda_stream)
 
 
+@pytest.mark.parametrize("xdt", ["bf16", "f32"])
+@pytest.mark.parametrize("pair", [("mxfp4", "q4_1"), ("q6_k", "q8_0"), ("q4_k", "q4_k")], ids=lambda p: "-".join(p))
+def test_grouped_products_at_few_tokens(ctx, orc, pair, xdt, monkeypatch):
+    """The composition of the grouped products, which serves what the few-token
+    kernels do not take, within the same bounds on calls that they do."""
+    import torch
+
+    for rows in (1, 6, 30):
+        announce(f"moe_layer grouped {pair} x={xdt} rows={rows}")
+        L = Layer(orc, np.random.default_rng(20 + rows), rows, 512, 256, 12, 3, *pair, xdt=xdt)
+        ids, p, gap, big = L.route()
+        assert gap > 1e-6
+        few = L.call(ctx)
+        monkeypatch.setenv("RLXQ_MOE_LAYER", "grouped")
+        grouped = L.call(ctx)
+        monkeypatch.delenv("RLXQ_MOE_LAYER")
+        torch.cuda.synchronize()
+        L.check(few, ids, p, big)
+        L.check(grouped, ids, p, big)
+
+
+def test_two_graphs_on_one_scratch(ctx, orc):
+    """Two graphs captured on one stream share its scratch: replayed in turns,
+    with eager calls between, each gives the eager bits."""
+    import torch
+
+    announce("moe_layer and mxfp4_gemm graphs on one scratch")
+    rng = np.random.default_rng(12)
+    L = Layer(orc, rng, 9, 512, 256, 16, 4, "q4_1", "mxfp4", xdt="f32")
+    v = _t(rng.standard_normal((70, 512)).astype(np.float32))
+    w, ws = ctx.quantize_mxfp4(_t(rng.standard_normal((384, 512)).astype(np.float32)))
+    a, b = L.call(ctx).clone(), ctx.mxfp4_gemm(v, w, ws, 384).clone()
+    ya, yb = torch.empty_like(a), torch.empty_like(b)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):   # sizes the stream's scratch
+        L.call(ctx, y=ya)
+        ctx.mxfp4_gemm(v, w, ws, 384, y=yb)
+    st.synchronize()
+    ga, gb = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(ga, stream=st):
+        L.call(ctx, y=ya)
+    with torch.cuda.graph(gb, stream=st):
+        ctx.mxfp4_gemm(v, w, ws, 384, y=yb)
+    for _ in range(4):
+        ya.zero_()
+        yb.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            ga.replay()
+            gb.replay()
+            z = L.call(ctx)
+            ga.replay()
+        st.synchronize()
+        assert torch.equal(ya, a) and torch.equal(yb, b) and torch.equal(z, a)
+    del ga, gb
+    ctx.release_stream(stream=st.cuda_stream)
+
+
 def test_quantised_experts_together(ctx, orc):
     """The set as it is used: float experts packed by quantize_mxfp4, a dense
     MXFP4 product on 4-bit activations in front, and the expert layer on its

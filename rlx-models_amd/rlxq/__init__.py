@@ -158,11 +158,12 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
-def _stream(stream) -> int | None:
+def _stream(stream, device: int | None = None) -> int | None:
     if stream is None:
         import torch
 
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or None
+        # (of the context's device where the caller names it, else of the current one)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device) or None
     return int(stream)
 
 
@@ -594,7 +595,7 @@ class Context:
         rc = lib().rlxq_moe_layer(self.h, _ptr(x), _dt(x), _ptr(router), _dt(router) if router is not None else F32,
                                   _ptr(logits), gate_up_scheme, _ptr(gate_up), _ptr(gate_up_scales), down_scheme,
                                   _ptr(down), _ptr(down_scales), rows, hidden, inter, num_experts, top_k, int(renorm),
-                                  _ptr(ids), _ptr(probs), _ptr(y), _dt(y), _stream(stream))
+                                  _ptr(ids), _ptr(probs), _ptr(y), _dt(y), _stream(stream, self.device))
         self._check(rc, "moe_layer")
         return y
 
@@ -647,7 +648,7 @@ class Context:
             codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
         if scales is None:
             scales = torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
-        rc = lib().rlxq_quantize_mxfp4(self.h, _ptr(x), _dt(x), m, k, _ptr(codes), _ptr(scales), _stream(stream))
+        rc = lib().rlxq_quantize_mxfp4(self.h, _ptr(x), _dt(x), m, k, _ptr(codes), _ptr(scales), _stream(stream, self.device))
         self._check(rc, "quantize_mxfp4")
         return codes, scales
 
@@ -661,7 +662,7 @@ class Context:
         if y is None:
             y = torch.empty((m, n), dtype=y_dtype or torch.float32, device=x.device)
         rc = lib().rlxq_mxfp4_gemm(self.h, _ptr(x), _dt(x), _ptr(w), _ptr(w_scales), m, k, n, _ptr(y), _dt(y),
-                                   _stream(stream))
+                                   _stream(stream, self.device))
         self._check(rc, "mxfp4_gemm")
         return y
 

@@ -390,19 +390,22 @@ RLXQ_DEV void mx_mfma32(mx_f32x16_t& c, const uint4& a, const uint4& b, uint32_t
 }
 RLXQ_DEV void mx_mfma_done() { asm volatile("s_nop 15\n\ts_nop 15"); }
 
-// 64 lanes x 16 (or 4) bytes from base + off + I into LDS at M0 + I (base and
-// M0 wave-uniform).  Written as the instruction itself: the compiler cannot
+// 64 lanes x 16 (or 4) bytes from base + off + I into LDS at dst + I (base and
+// dst wave-uniform).  Written as the instruction itself: the compiler cannot
 // tell the buffer that is being filled from the one being read and would wait
 // for the fill ahead of every LDS read.  mx_loads_wait() waits for all but the
 // wave's last N loads; nothing else does.
-RLXQ_DEV void mx_lds_dst(uint32_t dst) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" : : "s"(dst) : "memory"); }
+// The instruction takes dst from M0, which the compiler may use for its own
+// between any two statements: each load sets it itself, one wait state ahead.
 template <int I>
-RLXQ_DEV void mx_to_lds16(const uint8_t* base, uint32_t off) {
-  asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" : : "v"(off), "s"(base), "n"(I) : "memory");
+RLXQ_DEV void mx_to_lds16(uint32_t dst, const uint8_t* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%2"
+               : : "v"(off), "s"(base), "n"(I), "s"(dst) : "memory", "m0");
 }
 template <int I>
-RLXQ_DEV void mx_to_lds4(const uint8_t* base, uint32_t off) {
-  asm volatile("global_load_lds_dword %0, %1 offset:%2" : : "v"(off), "s"(base), "n"(I) : "memory");
+RLXQ_DEV void mx_to_lds4(uint32_t dst, const uint8_t* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1 offset:%2"
+               : : "v"(off), "s"(base), "n"(I), "s"(dst) : "memory", "m0");
 }
 template <int N>
 RLXQ_DEV void mx_loads_wait() {
@@ -450,8 +453,8 @@ RLXQ_DEV void mx_gemm_tile(const rlxq_mx_gemm_args& a, int tm, int tn, uint8_t* 
   const int s1 = __builtin_amdgcn_readfirstlane(s0 + per < a.spans ? s0 + per : a.spans);
 
   // ---- loads.  A wave fills LX KB of the activations' part of a ring slot
-  // and LW KB of the weights', each one run of LDS: one M0 and immediate
-  // offsets, which move the source too (the lanes' offsets undo that).
+  // and LW KB of the weights', each one run of LDS at immediate offsets,
+  // which move the source too (the lanes' offsets undo that).
   // Its LX KB are whole halves of row blocks' fragments: 2 KB each.
   static_assert(LX % 2 == 0, "whole row blocks per wave");
   constexpr int XP = LX / 2;
@@ -506,11 +509,9 @@ RLXQ_DEV void mx_gemm_tile(const rlxq_mx_gemm_args& a, int tm, int tn, uint8_t* 
   auto load_codes = [&](auto ii, int slot) {
     constexpr int i = decltype(ii)::value;
     if constexpr (i < LX) {
-      if constexpr (i == 0) mx_lds_dst(x_dst + slot * STAGE);
-      mx_to_lds16<1024 * i>(xp[i / 2], l16);
+      mx_to_lds16<1024 * i>(x_dst + slot * STAGE, xp[i / 2], l16);
     } else {
-      if constexpr (i == LX) mx_lds_dst(w_dst + slot * STAGE);
-      mx_to_lds16<1024 * (i - LX)>(wp, wo[i - LX] - (w_end ? back : 0));
+      mx_to_lds16<1024 * (i - LX)>(w_dst + slot * STAGE, wp, wo[i - LX] - (w_end ? back : 0));
     }
   };
   // the activations' pointers from a stage (half h of a span) to the next;
@@ -522,8 +523,7 @@ RLXQ_DEV void mx_gemm_tile(const rlxq_mx_gemm_args& a, int tm, int tn, uint8_t* 
   };
   auto load_scales = [&](auto ii, int sp) {   // run i of span sp's scales
     constexpr int i = decltype(ii)::value;
-    if constexpr (i == 0) mx_lds_dst(s_dst + (sp & 1) * SCALES);
-    mx_to_lds4<256 * i>(sp_[i] + (int64_t)(sp < s1 ? sp : s1 - 1) * sstep[i], l4);
+    mx_to_lds4<256 * i>(s_dst + (sp & 1) * SCALES, sp_[i] + (int64_t)(sp < s1 ? sp : s1 - 1) * sstep[i], l4);
   };
   mx_f32x16_t acc[TN][TM];
 #pragma unroll

@@ -24,6 +24,10 @@ namespace {
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// Most entries (rows x top_k) of a call.  Callers compare rows with
+// kMaxPairs / top_k: the product of a large rows does not fit 64 bits.
+constexpr int64_t kMaxPairs = (int64_t)1 << 28;
+
 // Table + grouped GEMV (+ combine).  `ids` (int32) or `idx` (f32) give the
 // expert of each of the n entries; entry i reads activation row i / x_div.
 // The call's scratch starts ws_base bytes into the workspace (a caller that
@@ -38,7 +42,7 @@ int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const vo
   if (k <= 0 || n < 0 || n_entries < 0 || x_rows < 0) return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": bad sizes");
   if (num_experts <= 0 || num_experts > 1024)
     return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": need 0 < num_experts <= 1024");
-  if (n_entries > ((int64_t)1 << 28)) return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": too many rows");
+  if (n_entries > kMaxPairs) return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": too many rows");
   if (x_dtype != RLXQ_F32 && x_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, std::string(what) + ": x_dtype");
   if (y_dtype != RLXQ_F32 && y_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, std::string(what) + ": y_dtype");
   int64_t rb = 0;
@@ -764,6 +768,7 @@ int rlxq_moe_grouped(rlxq_ctx* ctx, int scheme, int mode, const void* x, int x_d
   if (!is_gguf(scheme) && kquant_bytes(scheme) < 0)
     return fail(ctx, RLXQ_E_SCHEME, "moe_grouped: GGUF schemes only");
   if (rows < 0 || top_k <= 0 || top_k > 64) return fail(ctx, RLXQ_E_SHAPE, "moe_grouped: need 0 < top_k <= 64");
+  if (rows > kMaxPairs / top_k) return fail(ctx, RLXQ_E_SHAPE, "moe_grouped: more than 2^28 rows x top_k");
   if (mode == RLXQ_MOE_EXPAND || mode == RLXQ_MOE_EXPAND_SWIGLU) {
     const bool sw = mode == RLXQ_MOE_EXPAND_SWIGLU;
     if (sw && n % 2) return fail(ctx, RLXQ_E_SHAPE, "moe_grouped: EXPAND_SWIGLU needs an even N (gate | up)");
@@ -797,7 +802,7 @@ int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype, const void* router
     return fail(ctx, RLXQ_E_SHAPE, "moe_layer: need rows >= 0, 0 < hidden, inter <= 2^24");
   if (num_experts <= 0 || num_experts > 1024 || top_k <= 0 || top_k > num_experts || top_k > 64)
     return fail(ctx, RLXQ_E_SHAPE, "moe_layer: need 0 < top_k <= min(num_experts, 64), num_experts <= 1024");
-  if (rows * top_k > ((int64_t)1 << 28)) return fail(ctx, RLXQ_E_SHAPE, "moe_layer: too many rows");
+  if (rows > kMaxPairs / top_k) return fail(ctx, RLXQ_E_SHAPE, "moe_layer: more than 2^28 rows x top_k");
   if (x_dtype != RLXQ_F32 && x_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, "moe_layer: x_dtype");
   if (y_dtype != RLXQ_F32 && y_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, "moe_layer: y_dtype");
   if (router && router_dtype != RLXQ_F32 && router_dtype != RLXQ_BF16)

@@ -50,11 +50,11 @@ int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const vo
   if (rc) return rc;
   if (!aligned(x, 16)) return fail(ctx, RLXQ_E_ALIGN, std::string(what) + ": x must be 16-byte aligned");
   if (n_entries == 0 || n == 0) return RLXQ_OK;
+  const bool combine = probs != nullptr;
+  const int64_t width = swiglu ? n / 2 : n;   // output columns
   DeviceGuard g(ctx->device);
   if (!g.ok()) return fail(ctx, RLXQ_E_HIP, std::string(what) + ": hipSetDevice");
 
-  const bool combine = probs != nullptr;
-  const int64_t width = swiglu ? n / 2 : n;   // output columns
   // Routing inside the grouped GEMV's workgroups for decode-sized calls (no
   // table launch; the entries of each expert cut into chunks of MT, one
   // workgroup per chunk and tile); the device table for larger ones.
@@ -221,6 +221,14 @@ int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const vo
     void* xargs[] = {&ga};
     return launch(ctx, fx, dim3((unsigned)grid), dim3(64 * top_k), (size_t)top_k * tc * 4, stream, xargs, name);
   }
+  // what the launches below cannot take, ahead of the first of them (and of a
+  // caller's own, which asks for its sizes first)
+  const size_t rec_lds = xr || sk ? 0 : (size_t)2 * (k / 32) * (xbf ? 20 : 36) * 4;   // two rows as records
+  if (rec_lds > ctx->max_lds)
+    return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": K = " + std::to_string(k) + " needs " + std::to_string(rec_lds) +
+                                       " B of LDS, device has " + std::to_string(ctx->max_lds));
+  if (combine && (width > 0xffffffffll / rows || !grid_fits((rows * width + 255) / 256, 256)))
+    return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": rows x columns need a launch of 2^32 work-items or more");
   const size_t table_bytes = fused || sk ? 0 : ((size_t)(2 + 2 * num_experts + n_entries) * 4 + 255) & ~size_t(255);
   const size_t tmp_bytes = combine ? (((size_t)n_entries * width * 4 + 255) & ~size_t(255)) : 0;
   // grouped MFMA path: chunks of RPC gathered rows, each expert's entries
@@ -473,9 +481,8 @@ int grouped_run(rlxq_ctx* ctx, const char* what, int scheme, int group, const vo
     ga.top_k = top_k;
     ga.out_bf16 = y_dtype == RLXQ_BF16 ? 1 : 0;
   }
-  const size_t lds = xr ? 0 : (size_t)2 * (k / 32) * (xbf ? 20 : 36) * 4;
   void* gargs[] = {&ga};
-  if ((rc = launch(ctx, fg, dim3((unsigned)grid), dim3(256), lds, stream, gargs, name))) return rc;
+  if ((rc = launch(ctx, fg, dim3((unsigned)grid), dim3(256), rec_lds, stream, gargs, name))) return rc;
   }
 
   // 3. probability-weighted sum over the top-k slots (in the GEMV launch
@@ -803,6 +810,8 @@ int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype, const void* router
   if (num_experts <= 0 || num_experts > 1024 || top_k <= 0 || top_k > num_experts || top_k > 64)
     return fail(ctx, RLXQ_E_SHAPE, "moe_layer: need 0 < top_k <= min(num_experts, 64), num_experts <= 1024");
   if (rows > kMaxPairs / top_k) return fail(ctx, RLXQ_E_SHAPE, "moe_layer: more than 2^28 rows x top_k");
+  // (the top-k launch: a wave a row)
+  if (!grid_fits(rows, 64)) return fail(ctx, RLXQ_E_SHAPE, "moe_layer: 2^26 rows or more");
   if (x_dtype != RLXQ_F32 && x_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, "moe_layer: x_dtype");
   if (y_dtype != RLXQ_F32 && y_dtype != RLXQ_BF16) return fail(ctx, RLXQ_E_DTYPE, "moe_layer: y_dtype");
   if (router && router_dtype != RLXQ_F32 && router_dtype != RLXQ_BF16)

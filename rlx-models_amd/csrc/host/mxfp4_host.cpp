@@ -24,6 +24,10 @@ size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 // 16 workgroups a CU (mx_quant_rows' figures).
 int rows_ilp(int64_t groups) { return groups >= (int64_t)4096 * 1024 ? 4 : 1; }
 
+// Workgroups of the preparation launch: a chunk of fragments each, and
+// `wblocks` for the weights' scales.
+int64_t frag_grid(const rlxq_mx_gemm_args& g, int rows, int64_t wblocks) { return (g.M + rows - 1) / rows * g.spans + wblocks; }
+
 // The activations as fragments of `rows` rows (mxfp4_args.h); wblocks > 0:
 // the weights' scales in the lane order of 32-row fragments beside them.
 int quant_frag(rlxq_ctx* ctx, const rlxq_mx_gemm_args& g, const void* x, int x_dtype, int rows, uint8_t* xf,
@@ -45,10 +49,8 @@ int quant_frag(rlxq_ctx* ctx, const rlxq_mx_gemm_args& g, const void* x, int x_d
   hipFunction_t fn;
   int rc = get_fn(ctx, name, &fn);
   if (rc) return rc;
-  const int64_t grid = (g.M + rows - 1) / rows * g.spans + wblocks;
-  if (grid > 0x7fffffff) return fail(ctx, RLXQ_E_SHAPE, "mxfp4_gemm: x too large");
   void* args[] = {&a};
-  return launch(ctx, fn, dim3((unsigned)grid), dim3(256), 0, stream, args, name);
+  return launch(ctx, fn, dim3((unsigned)frag_grid(g, rows, wblocks)), dim3(256), 0, stream, args, name);
 }
 
 // Compiled tilings (kernel rlxq_mx_gemm_<name>), and what they cost: `span` us
@@ -99,8 +101,10 @@ int gemm_tiled(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, c
   a.spans = (int)((a.K + 255) / 256);
   a.splits = span_splits(a.spans, splits);
   const int64_t tiles_m = (a.M + c.BM - 1) / c.BM, tiles_n = (a.N + c.BN - 1) / c.BN;
-  if (tiles_m * tiles_n > 0x7ffffff0) return fail(ctx, RLXQ_E_SHAPE, "mxfp4_gemm: too many tiles");
   const int64_t xb = (a.M + 31) / 32, wb = (a.N + 31) / 32;
+  const int64_t grid = 8 * ((tiles_m * tiles_n + 7) / 8), reduce = a.splits > 1 ? (a.M * a.N + 1023) / 1024 : 0;
+  if (!grid_fits(frag_grid(a, 32, wb), 256) || !grid_fits(grid, 64 * c.waves) || !grid_fits(reduce, 256))
+    return fail(ctx, RLXQ_E_SHAPE, "mxfp4_gemm: M, K and N need a launch of 2^32 work-items or more");
   const size_t b_xf = round256((size_t)xb * a.spans * RLXQ_MX_CHUNK), b_ws = (size_t)wb * a.spans * 256;
   const size_t b_z = round256((size_t)wb), b_part = a.splits > 1 ? (size_t)a.splits * a.M * a.N * 4 : 0;
   void* ws = nullptr;
@@ -119,15 +123,12 @@ int gemm_tiled(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, c
   hipFunction_t fn;
   if ((rc = get_fn(ctx, name, &fn))) return rc;
   void* args[] = {&a};
-  const int64_t grid = 8 * ((tiles_m * tiles_n + 7) / 8);
   if ((rc = launch(ctx, fn, dim3((unsigned)grid, (unsigned)a.splits), dim3(64 * c.waves), (size_t)(c.BM + c.BN) * (256 + 16), stream,
                    args, name)))
     return rc;
   if (a.splits > 1) {
     if ((rc = get_fn(ctx, "rlxq_mx_reduce", &fn))) return rc;
-    const int64_t blocks = (a.M * a.N + 1023) / 1024;
-    if (blocks > 0x7fffffff) return fail(ctx, RLXQ_E_SHAPE, "mxfp4_gemm: output too large");
-    if ((rc = launch(ctx, fn, dim3((unsigned)blocks), dim3(256), 0, stream, args, "rlxq_mx_reduce"))) return rc;
+    if ((rc = launch(ctx, fn, dim3((unsigned)reduce), dim3(256), 0, stream, args, "rlxq_mx_reduce"))) return rc;
     ctx->last_kernel = name;
   }
   return RLXQ_OK;
@@ -150,6 +151,9 @@ int gemm_decode(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, 
   const bool fused = mt == 1 && a.M * a.K <= 24576;
   int waves = nt == 2 && mt == 2 ? 4 : 8;
   if (nt == 1 && (a.N + 15) / 16 <= cus && (fused || a.spans >= 16)) waves = 16;
+  const int64_t grid = (a.N + 16 * nt - 1) / (16 * nt);
+  if (!grid_fits(grid, 64 * waves) || (!fused && !grid_fits(frag_grid(a, 16, 0), 256)))
+    return fail(ctx, RLXQ_E_SHAPE, "mxfp4_gemm: M, K and N need a launch of 2^32 work-items or more");
   char name[48];
   if (fused) {
     std::snprintf(name, sizeof name, "rlxq_mx_dec_n%d_f%s", nt, x_dtype == RLXQ_BF16 ? "bf16" : "f32");
@@ -167,7 +171,7 @@ int gemm_decode(rlxq_ctx* ctx, rlxq_mx_gemm_args a, const void* x, int x_dtype, 
   if (rc) return rc;
   const size_t lds = (size_t)waves * nt * mt * 1024 + (fused ? (size_t)((a.spans * a.M * 272 + 15) & ~15) : 0);
   void* args[] = {&a};
-  return launch(ctx, fn, dim3((unsigned)((a.N + 16 * nt - 1) / (16 * nt))), dim3(64 * waves), lds, stream, args, name);
+  return launch(ctx, fn, dim3((unsigned)grid), dim3(64 * waves), lds, stream, args, name);
 }
 
 }  // namespace
@@ -185,7 +189,7 @@ int mx_dequantize(rlxq_ctx* ctx, const void* codes, const void* scales, int64_t 
   int rc = get_fn(ctx, u == 1 ? "rlxq_mx_dequant_u1" : "rlxq_mx_dequant_u4", &fn);
   if (rc) return rc;
   const int64_t grid = (rows * (k / 4) + 256 * u - 1) / (256 * u);
-  if (grid > 0x7fffffff) return fail(ctx, RLXQ_E_SHAPE, "dequantize: too many weights");
+  if (!grid_fits(grid, 256)) return fail(ctx, RLXQ_E_SHAPE, "dequantize: 2^36 weights or more");
   void* args[] = {&a, &out};
   return launch(ctx, fn, dim3((unsigned)grid), dim3(256), 0, stream, args, "dequantize");
 }
@@ -225,7 +229,7 @@ int rlxq_quantize_mxfp4(rlxq_ctx* ctx, const void* x, int x_dtype, int64_t m, in
   int rc = get_fn(ctx, name, &fn);
   if (rc) return rc;
   const int64_t grid = (m * (k / 8) + 256 * u - 1) / (256 * u);
-  if (grid > 0x7fffffff) return fail(ctx, RLXQ_E_SHAPE, "quantize_mxfp4: more than 2^43 elements");
+  if (!grid_fits(grid, 256)) return fail(ctx, RLXQ_E_SHAPE, "quantize_mxfp4: 2^37 elements or more");
   void* args[] = {&a};
   return launch(ctx, fn, dim3((unsigned)grid), dim3(256), 0, stream, args, name);
 }

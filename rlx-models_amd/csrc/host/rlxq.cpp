@@ -158,6 +158,8 @@ int launch(rlxq_ctx* ctx, hipFunction_t fn, dim3 grid, dim3 block, size_t lds, v
            void** args, const char* what) {
   ctx->last_kernel = what;
   if (grid.x == 0 || grid.y == 0 || grid.z == 0) return RLXQ_OK;
+  if (!grid_fits(grid.x, block.x) || !grid_fits(grid.y, block.y) || !grid_fits(grid.z, block.z))
+    return fail(ctx, RLXQ_E_SHAPE, std::string(what) + ": a launch of 2^32 work-items or more");
   if (lds > ctx->max_lds)
     return fail(ctx, RLXQ_E_SHAPE,
                 std::string(what) + ": needs " + std::to_string(lds) + " B of LDS, device has " +

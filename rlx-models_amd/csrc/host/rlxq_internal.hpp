@@ -84,6 +84,11 @@ void noalloc_setup(rlxq_ctx* ctx);
 // at once (cached per kernel and LDS size; at least 1).
 int blocks_per_cu(rlxq_ctx* ctx, const std::string& name, hipFunction_t fn, int threads, size_t lds);
 
+// Whether a launch takes `blocks` workgroups of `threads` along a dimension
+// (fewer than 2^32 work-items).  Entries that queue several launches ask for
+// all of them ahead of the first.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= (int64_t)0xffffffff / threads; }
+
 // Launches `fn` with the kernelParams array `args`.
 int launch(rlxq_ctx* ctx, hipFunction_t fn, dim3 grid, dim3 block, size_t lds, void* stream,
            void** args, const char* what);

@@ -113,8 +113,9 @@ typedef struct rlxq_moe_pick_args {
  * largest magnitude into [2^14, 2^15), rounded to f16 (64 bytes), for f32 rows
  * their rounded remainders (64 bytes), both in the order in which the weight
  * scheme's codes unpack (order: 0 element by element, 1 the GGUF nibbles', 2
- * pairs two apart), and four floats: the factor that undoes the scaling, the
- * sum of the block's elements, that of its first 16, 0.                      */
+ * pairs two apart), and four floats: the factor that undoes the scaling (order
+ * 0, MXFP4: its exponent as an integer), the sum of the block's elements, that
+ * of its first 16, 0.                                                        */
 #define RLXQ_FEW_REC(planes) (64 * (planes) + 16)
 typedef struct rlxq_moe_prep_args {
   rlxq_moe_logits_args r;   /* the router's part (lblocks > 0)               */

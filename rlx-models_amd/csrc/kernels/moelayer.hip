@@ -225,7 +225,7 @@ RLXQ_DEV void put_record(uint8_t* rec, const float (&x)[4], int planes, int orde
   }
   if (q == 0) {
     float* m = reinterpret_cast<float*>(rec + 64 * planes);
-    m[0] = __uint_as_float((uint32_t)(127 + e) << 23);
+    m[0] = order == 0 ? __int_as_float(e) : __uint_as_float((uint32_t)(127 + e) << 23);
     m[1] = sum;
     m[2] = sum16;
     m[3] = 0.f;
@@ -330,14 +330,20 @@ struct FewW {
 
 // A block of a weight row: exact f16 codes, multipliers of its code sum (of its
 // halves') and of its activations' sum (halves').
+// MXFP4: the scale stays an exponent that is added to the record factor's: the
+// two powers of two need not have an f32 product (2^127 of zero codes on rows
+// beyond 2^15 made NaN of a zero).  Byte 0, a scale of zero, is an exponent that
+// leaves nothing of any finite sum; 255 reads as 254 (e8m0_to_f32).
 template <int SCH>
 struct FewBlk {
   uint32_t pw[16];
   float d, d2, mn, m2;
+  int e;
   RLXQ_DEV void decode(const FewW<SCH>& w, int bl, int u, const UnpackK& kc) {
     block_f16<SCH>(w.dw, bl, pw, kc);
-    d2 = mn = m2 = 0.f;
-    if constexpr (SCH == SCH_MXFP4) d = e8m0_to_f32(w.sc);
+    d = d2 = mn = m2 = 0.f;
+    e = 0;
+    if constexpr (SCH == SCH_MXFP4) e = w.sc == 0u ? -1024 : (int)(w.sc < 254u ? w.sc : 254u) - 127;
     else if constexpr (SCH == SCH_Q6_K) block_scales<SCH>(w.dw, bl, d, d2, u);
     else if constexpr (half_scales<SCH>()) block_scales_half<SCH>(w.dw, d, d2, mn, m2);
     else block_scales<SCH>(w.dw, bl, d, mn, u);
@@ -353,7 +359,9 @@ struct FewBlk {
   }
   // the block's sum of products from its code sums and the record's factors
   RLXQ_DEV float finish(const float (&c)[2], const float4& me, float s) const {
-    if constexpr (half_scales<SCH>()) {
+    if constexpr (SCH == SCH_MXFP4) {
+      s += __builtin_amdgcn_ldexpf(c[0] + c[1], e + __float_as_int(me.x));
+    } else if constexpr (half_scales<SCH>()) {
       s = fmaf(d * me.x, c[0], s);
       s = fmaf(d2 * me.x, c[1], s);
       if constexpr (SCH == SCH_Q2_K) {

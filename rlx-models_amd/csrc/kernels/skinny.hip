@@ -8,8 +8,9 @@
 //
 //  * rlxq_x16_prep: each activation row to f16, scaled by a power of two so
 //    its largest element lies in [2^9, 2^10) (exact; undone in the
-//    epilogue), and permuted within each 32-element block to the order in
-//    which a lane unpacks the codes: for the GGUF nibble formats position
+//    epilogue; MXFP4's bf16 rows are only scaled up), and permuted within
+//    each 32-element block to the order in which a lane unpacks the codes:
+//    for the GGUF nibble formats position
 //    8g + e holds element 4g + e (e < 4) or 16 + 4g + e - 4, for MLX's
 //    element 8g + 2e (e < 4) or 8g + 2(e - 4) + 1.  f32 rows become a hi and
 //    a lo row (split).  The block sums of the prepared values go beside them
@@ -796,6 +797,9 @@ RLXQ_DEV void x16_prep_body(const rlxq_x16_args& a) {
   if (amax > 0.f && amax <= 3.4e38f) {
     int sh = 9 - ilogbf(amax);
     sh = sh < -126 ? -126 : (sh > 126 ? 126 : sh);
+    // bf16 rows, of f32's range, are only scaled up: scaled down beside a large
+    // element, a small one would be lost
+    if (a.out_bf16 && sh < 0) sh = 0;
     s = ldexpf(1.f, sh);
     inv = ldexpf(ldexpf(1.f, -sh), a.post_exp);
   }

@@ -15,7 +15,7 @@ def _values(orc, codes, scales):
 
 
 @pytest.mark.parametrize("xdt", ["bf16", "f32"])
-@pytest.mark.parametrize("rows", [1, 3, 14])
+@pytest.mark.parametrize("rows", [1, 3, 14, 40])
 def test_far_scales(ctx, orc, rows, xdt):
     """gate|up: block 1 has byte 254 or 255 over zero codes, on rows of 2^20;
     block 2 2^105 on rows of 2^-104; block 3 byte 0 on rows of 2^30; block 4

@@ -158,12 +158,16 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
-def _stream(stream, device: int | None = None) -> int | None:
+def _stream(stream, device: int) -> int | None:
+    """The caller's stream, or torch's current one of `device` (the context's or
+    the tensor's, whichever device is current)."""
     if stream is None:
         import torch
 
-        # (of the context's device where the caller names it, else of the current one)
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device) or None
+        # (the handle alone where torch gives it: 0.1 us a call, the Stream object
+        # around it, which sets torch's GPU side up at the first call, 1.1)
+        raw = torch.cuda.is_initialized() and getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return (raw(device) if raw else torch.cuda.current_stream(device).cuda_stream) or None
     return int(stream)
 
 
@@ -454,27 +458,28 @@ class Context:
     def reserve_workspace(self, nbytes: int, *, stream=None) -> None:
         """Sizes the context scratch of `stream` to at least nbytes (before a
         graph capture)."""
-        self._check(lib().rlxq_reserve_workspace(self.h, _stream(stream), nbytes), "reserve_workspace")
+        rc = lib().rlxq_reserve_workspace(self.h, _stream(stream, self.device), nbytes)
+        self._check(rc, "reserve_workspace")
 
     def workspace_bytes(self, *, stream=None) -> int:
-        return int(lib().rlxq_workspace_bytes(self.h, _stream(stream)))
+        return int(lib().rlxq_workspace_bytes(self.h, _stream(stream, self.device)))
 
     def peak_probe(self, kind: int, work: int, *, buf=None, sink, stream=None) -> int:
         """rlxq_peak_probe: launches the probe on `stream`, returns the flops
         (PROBE_MFMA) or bytes (PROBE_READ, PROBE_READ4, PROBE_TILE20) it
         issues."""
         cnt = C.c_int64(0)
-        rc = lib().rlxq_peak_probe(self.h, kind, _ptr(buf), work, _ptr(sink), C.byref(cnt), _stream(stream))
+        rc = lib().rlxq_peak_probe(self.h, kind, _ptr(buf), work, _ptr(sink), C.byref(cnt), _stream(stream, self.device))
         self._check(rc, "peak_probe")
         return int(cnt.value)
 
     def workspace_retired_bytes(self, *, stream=None) -> int:
         """Bytes of replaced scratch buffers `stream` still holds."""
-        return int(lib().rlxq_workspace_retired_bytes(self.h, _stream(stream)))
+        return int(lib().rlxq_workspace_retired_bytes(self.h, _stream(stream, self.device)))
 
     def release_stream(self, *, stream=None) -> None:
         """Frees the scratch buffers of `stream` after waiting for it."""
-        self._check(lib().rlxq_release_stream(self.h, _stream(stream)), "release_stream")
+        self._check(lib().rlxq_release_stream(self.h, _stream(stream, self.device)), "release_stream")
 
     def bind_dequant_matmul(self, x, w, scheme: int, n: int, *, y, stream, group: int = 32, scales=None,
                             biases=None):
@@ -490,7 +495,7 @@ class Context:
         fn = lib().rlxq_dequant_matmul
         args = (self.h, C.c_int(scheme), C.c_int(group), C.c_void_p(_ptr(x)), C.c_int(_dt(x)), C.c_void_p(_ptr(w)),
                 C.c_void_p(_ptr(scales)), C.c_void_p(_ptr(biases)), C.c_int(sb), C.c_int64(m), C.c_int64(k),
-                C.c_int64(n), C.c_void_p(_ptr(y)), C.c_int(_dt(y)), C.c_void_p(_stream(stream)))
+                C.c_int64(n), C.c_void_p(_ptr(y)), C.c_int(_dt(y)), C.c_void_p(_stream(stream, self.device)))
 
         def call():
             rc = fn(*args)
@@ -510,7 +515,7 @@ class Context:
             y = torch.empty((m, n), dtype=y_dtype or torch.float32, device=x.device)
         sb = _dt(scales) if scales is not None else F32
         rc = lib().rlxq_dequant_matmul(self.h, scheme, group, _ptr(x), _dt(x), _ptr(w), _ptr(scales), _ptr(biases),
-                                       sb, m, k, n, _ptr(y), _dt(y), _stream(stream))
+                                       sb, m, k, n, _ptr(y), _dt(y), _stream(stream, self.device))
         self._check(rc, "dequant_matmul")
         return y
 
@@ -522,7 +527,7 @@ class Context:
         m, k = x.shape
         sb = _dt(scales) if scales is not None else F32
         rc = lib().rlxq_dequant_matmul_noalloc(self.h, scheme, group, _ptr(x), _dt(x), _ptr(w), _ptr(scales),
-                                               _ptr(biases), sb, m, k, n, _ptr(y), _dt(y), _stream(stream))
+                                               _ptr(biases), sb, m, k, n, _ptr(y), _dt(y), _stream(stream, self.device))
         self._check(rc, "dequant_matmul_noalloc")
         return y
 
@@ -541,7 +546,7 @@ class Context:
         _on_device(self.device, w=w, scales=scales, biases=biases, out=out)
         sb = _dt(scales) if scales is not None else F32
         rc = lib().rlxq_dequantize(self.h, scheme, group, _ptr(w), _ptr(scales), _ptr(biases), sb, rows, k,
-                                   _ptr(out), _stream(stream))
+                                   _ptr(out), _stream(stream, self.device))
         self._check(rc, "dequantize")
         return out
 
@@ -557,7 +562,7 @@ class Context:
         sb = _dt(scales) if scales is not None else F32
         rc = lib().rlxq_dequant_grouped_matmul(self.h, scheme, group, _ptr(x), _dt(x), _ptr(bank), _ptr(scales),
                                                _ptr(biases), sb, _ptr(expert_idx), rows, k, n, num_experts,
-                                               _ptr(y), _dt(y), _stream(stream))
+                                               _ptr(y), _dt(y), _stream(stream, self.device))
         self._check(rc, "dequant_grouped_matmul")
         return y
 
@@ -573,7 +578,7 @@ class Context:
         if y is None:
             y = torch.empty((out_rows, width), dtype=y_dtype or torch.float32, device=x.device)
         rc = lib().rlxq_moe_grouped(self.h, scheme, mode, _ptr(x), _dt(x), _ptr(bank), _ptr(ids), _ptr(probs),
-                                    rows, top_k, k, n, num_experts, _ptr(y), _dt(y), _stream(stream))
+                                    rows, top_k, k, n, num_experts, _ptr(y), _dt(y), _stream(stream, self.device))
         self._check(rc, "moe_grouped")
         return y
 
@@ -608,7 +613,7 @@ class Context:
         ids = torch.empty((rows, top_k), dtype=torch.int32, device=logits.device)
         probs = torch.empty((rows, top_k), dtype=torch.float32, device=logits.device)
         rc = lib().rlxq_moe_route(self.h, _ptr(logits), rows, e, top_k, int(renorm), _ptr(ids), _ptr(probs),
-                                  _stream(stream))
+                                  _stream(stream, self.device))
         self._check(rc, "moe_route")
         return ids, probs
 
@@ -622,7 +627,7 @@ class Context:
             out = torch.empty((rows, inter), dtype=out_dtype or gu.dtype, device=gu.device)
         _check_out(out, (rows, inter), "swiglu")
         _on_device(self.device, gu=gu, out=out)
-        rc = lib().rlxq_swiglu(self.h, _ptr(gu), _dt(gu), rows, inter, _ptr(out), _dt(out), _stream(stream))
+        rc = lib().rlxq_swiglu(self.h, _ptr(gu), _dt(gu), rows, inter, _ptr(out), _dt(out), _stream(stream, self.device))
         self._check(rc, "swiglu")
         return out
 
@@ -634,7 +639,7 @@ class Context:
         m, k = x.shape
         q = torch.empty((m, k), dtype=torch.int8, device=x.device)
         s = torch.empty((m,), dtype=torch.float32, device=x.device)
-        rc = lib().rlxq_quantize_act_int8(self.h, _ptr(x), _dt(x), m, k, _ptr(q), _ptr(s), _stream(stream))
+        rc = lib().rlxq_quantize_act_int8(self.h, _ptr(x), _dt(x), m, k, _ptr(q), _ptr(s), _stream(stream, self.device))
         self._check(rc, "quantize_act_int8")
         return q, s
 
@@ -648,7 +653,8 @@ class Context:
             codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
         if scales is None:
             scales = torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
-        rc = lib().rlxq_quantize_mxfp4(self.h, _ptr(x), _dt(x), m, k, _ptr(codes), _ptr(scales), _stream(stream, self.device))
+        rc = lib().rlxq_quantize_mxfp4(self.h, _ptr(x), _dt(x), m, k, _ptr(codes), _ptr(scales),
+                                       _stream(stream, self.device))
         self._check(rc, "quantize_mxfp4")
         return codes, scales
 
@@ -674,7 +680,7 @@ class Context:
         if y is None:
             y = torch.empty((m, n), dtype=y_dtype or torch.float32, device=x.device)
         rc = lib().rlxq_w8a8_gemm(self.h, _ptr(x), _dt(x), _ptr(wq), _ptr(w_scale), m, k, n, _ptr(y), _dt(y),
-                                  _stream(stream))
+                                  _stream(stream, self.device))
         self._check(rc, "w8a8_gemm")
         return y
 
@@ -856,7 +862,7 @@ class GgufFile:
     def upload(self, name: str, dst, *, stream=None):
         """The tensor's bytes into the device tensor `dst` (pread + pinned staging)."""
         nbytes = dst.numel() * dst.element_size()
-        self._check(lib().rlxq_gguf_upload(self.h, name.encode(), _ptr(dst), nbytes, _stream(stream)))
+        self._check(lib().rlxq_gguf_upload(self.h, name.encode(), _ptr(dst), nbytes, _stream(stream, dst.get_device())))
         return dst
 
 
@@ -931,5 +937,5 @@ class MlxFile:
 
     def upload(self, name: str, dst, *, stream=None):
         nbytes = dst.numel() * dst.element_size()
-        self._check(lib().rlxq_mlx_upload(self.h, name.encode(), _ptr(dst), nbytes, _stream(stream)))
+        self._check(lib().rlxq_mlx_upload(self.h, name.encode(), _ptr(dst), nbytes, _stream(stream, dst.get_device())))
         return dst

@@ -289,6 +289,10 @@ int rlxq_moe_route(rlxq_ctx* ctx, const float* logits, int64_t rows,
  * [rows, top_k] receive the routing, or are NULL.
  * A row whose logits hold a NaN or +inf, or nothing but -inf, has no softmax:
  * its y is NaN (ids 0 .. top_k - 1, probs NaN); -inf alone masks an expert.
+ * The gated activations silu * up stay f32, except that more rows, or wider
+ * experts, than the few-token kernels take (32 rows; 256 pairs; about 32000
+ * inter x top_k) have them rounded to bf16 where x and y are both bf16, or x is
+ * and inter is above 18176.
  * A row of x that is not finite, on the caller's finite logits, leaves its own
  * row of y not finite and the others alone.
  * num_experts <= 1024, top_k <= min(num_experts, 64); hidden and inter as the

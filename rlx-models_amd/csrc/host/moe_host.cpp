@@ -709,30 +709,48 @@ int layer_few(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
 
 // The layer from the library's own calls: router product, top-k, grouped
 // gate|up + SwiGLU, grouped down + weighted sum.  The activations between the
-// two grouped products have x's type (bf16 ones are what the grouped register
-// and MFMA kernels take; the layer's few-token kernels keep them in f32).
+// two grouped products are f32, as in the few-token kernels, but for two cases.
+//   - x and y both bf16: bf16 ones.  Each is off by at most 2^-8 of itself, as y
+//     is by its own rounding (over random layers 1.6e-3 of y's RMS, what y's
+//     rounding costs again).  f32 ones cost more where experts hold few entries:
+//     us for the layer in bf16 / f32, 8 of 128 experts, 2048 -> 768, 40 and 96
+//     tokens: MXFP4 137 / 176 and 226 / 298, Q4_1 138 / 168 and 238 / 295, Q4_K
+//     186 / 210 and 328 / 362.
+//   - bf16 x with f32 y, where down's f32 rows do not fit LDS (inter above 18176
+//     and fewer than eight entries a fired expert): the call is served in bf16.
 int layer_grouped(rlxq_ctx* ctx, const LayerCall& c, void* stream) {
   auto r256 = [](size_t b) { return (b + 255) & ~size_t(255); };
-  const size_t n = (size_t)(c.rows * c.top_k), xs = c.x_dtype == RLXQ_BF16 ? 2 : 4;
+  const size_t n = (size_t)(c.rows * c.top_k);
   const size_t b_log = c.logits ? 0 : r256((size_t)(c.rows * c.experts) * 4), b_ids = r256(n * 4), b_pr = r256(n * 4);
-  const size_t b_act = r256(n * (size_t)c.inter * xs), base = b_log + b_ids + b_pr + b_act;
+  int act_dtype = c.x_dtype == RLXQ_BF16 && c.y_dtype == RLXQ_BF16 ? RLXQ_BF16 : RLXQ_F32;
+  size_t base = 0;   // the layer's own scratch
+  auto sizes = [&] { base = b_log + b_ids + b_pr + r256(n * (size_t)c.inter * (act_dtype == RLXQ_BF16 ? 2 : 4)); };
+  sizes();
   const char* what = "moe_layer";
   auto gate_up = [&](void* act, const int32_t* ids, size_t* need) {
     return grouped_run(ctx, what, c.gu_scheme, 32, c.x, c.x_dtype, c.gu, c.gu_s, nullptr, RLXQ_U8, ids, nullptr,
-                       (int64_t)n, c.rows, (int32_t)c.top_k, c.hidden, 2 * c.inter, c.experts, act, c.x_dtype, nullptr,
+                       (int64_t)n, c.rows, (int32_t)c.top_k, c.hidden, 2 * c.inter, c.experts, act, act_dtype, nullptr,
                        c.rows, (int32_t)c.top_k, true, stream, base, need);
   };
   auto down = [&](const void* act, const int32_t* ids, const float* probs, size_t* need) {
-    return grouped_run(ctx, what, c.d_scheme, 32, act, c.x_dtype, c.d, c.d_s, nullptr, RLXQ_U8, ids, nullptr, (int64_t)n,
+    return grouped_run(ctx, what, c.d_scheme, 32, act, act_dtype, c.d, c.d_s, nullptr, RLXQ_U8, ids, nullptr, (int64_t)n,
                        (int64_t)n, 1, c.inter, c.hidden, c.experts, c.y, c.y_dtype, probs, c.rows, (int32_t)c.top_k,
                        false, stream, base, need);
   };
   // (any non-null pointers: sizes only)
   alignas(16) static const char dummy[16] = {};
   size_t n1 = 0, n2 = 0;
-  int rc;
-  if ((rc = gate_up(const_cast<char*>(dummy), reinterpret_cast<const int32_t*>(dummy), &n1))) return rc;
-  if ((rc = down(dummy, reinterpret_cast<const int32_t*>(dummy), reinterpret_cast<const float*>(dummy), &n2))) return rc;
+  auto need = [&] {
+    const int rg = gate_up(const_cast<char*>(dummy), reinterpret_cast<const int32_t*>(dummy), &n1);
+    return rg ? rg : down(dummy, reinterpret_cast<const int32_t*>(dummy), reinterpret_cast<const float*>(dummy), &n2);
+  };
+  int rc = need();
+  if (rc == RLXQ_E_SHAPE && c.x_dtype == RLXQ_BF16 && act_dtype == RLXQ_F32) {
+    act_dtype = RLXQ_BF16;
+    sizes();
+    rc = need();
+  }
+  if (rc) return rc;
   void* ws = nullptr;
   if ((rc = workspace(ctx, base + std::max(n1, n2), &ws, stream))) return rc;
   char* p = static_cast<char*>(ws);

@@ -1,0 +1,116 @@
+"""Accuracy of the whole expert layer beside its worst-case bounds: the RMS error
+over the RMS of y against float64, which a rounding or an element too many
+cannot hide in.
+
+Bound of the grouped products (f32 between them): a factor held as a high and a
+low part is off by at most 2^-16 of itself, evenly spread and of either sign, so
+a dot product by 2^-16 / sqrt(3) = 8.8e-6 of its RMS; f32 sums of some 100
+additions add 1e-6.  silu(g) u holds two such errors (a slope of 1.1 at most),
+down one more: sqrt(1 + 1.1^2 + 1) 8.8e-6 = 1.6e-5.  GROUPED takes 2^-15, twice
+that.  Activations rounded to bf16 (at most 2^-8, 2^-8 / sqrt(3) / 1.4 RMS over
+a binade) are 1.6e-3 off."""
+import numpy as np
+import pytest
+
+from conftest import announce
+from test_moe_layer_gpu import GGUF, Layer, _bank, _t
+
+GROUPED = 2.0 ** -15
+
+
+def _bf16(v):
+    import torch
+
+    return torch.from_numpy(np.ascontiguousarray(v, np.float32)).to(torch.bfloat16).float().numpy().astype(np.float64)
+
+
+class Values:
+    """A layer's inputs as float64 (and packed), with logits of the caller's that
+    give every slot weight."""
+
+    def __init__(self, orc, rows, hidden, inter, experts, top_k, gu, down, xdt, seed=0):
+        rng = np.random.default_rng(seed + rows + hidden + inter)
+        self.shape, self.names, self.xdt = (rows, hidden, inter, experts, top_k), (gu, down), xdt
+        self.g, self.gs, gv = _bank(orc, gu, rng, experts * 2 * inter, hidden)
+        self.d, self.ds, dv = _bank(orc, down, rng, experts * hidden, inter)
+        self.gv, self.dv = gv.reshape(experts, 2 * inter, hidden), dv.reshape(experts, hidden, inter)
+        x = rng.standard_normal((rows, hidden)) / max(1.0, float(np.std(self.gv)) * hidden ** 0.5 / 2)
+        self.x = _bf16(x) if xdt == "bf16" else x.astype(np.float32).astype(np.float64)
+        self.logits = (rng.standard_normal((rows, experts)) * 0.1).astype(np.float32)
+        l = self.logits.astype(np.float64)
+        self.ids = np.argsort(-l, axis=1, kind="stable")[:, :top_k]
+        p = np.exp(np.take_along_axis(l, self.ids, 1))
+        self.p = p / p.sum(1, keepdims=True)
+
+    def forward(self, x=lambda v: v, a=lambda v: v, slots=None):
+        """y in float64, with x and the gated activations passed through the
+        functions given, over the first `slots` slots."""
+        rows, hidden, inter, _, top_k = self.shape
+        y = np.zeros((rows, hidden))
+        for r in range(rows):
+            v = x(self.x[r])
+            for j in range(slots or top_k):
+                e = self.ids[r, j]
+                gu = self.gv[e] @ v
+                y[r] += self.p[r, j] * (self.dv[e] @ a(gu[:inter] / (1 + np.exp(-gu[:inter])) * gu[inter:]))
+        return y
+
+    def call(self, ctx, y_dtype):
+        import rlxq
+        import torch
+
+        rows, hidden, inter, experts, top_k = self.shape
+        x = torch.from_numpy(self.x.astype(np.float32)).to(torch.bfloat16 if self.xdt == "bf16" else torch.float32).cuda()
+        sch = [rlxq.MLX_MXFP4 if n == "mxfp4" else GGUF[n] for n in self.names]
+        gs, ds = (None if s is None else _t(s) for s in (self.gs, self.ds))
+        y = ctx.moe_layer(x, None, _t(self.g), _t(self.d), sch[0], sch[1], top_k, inter, experts, logits=_t(self.logits),
+                          gate_up_scales=gs, down_scales=ds, y_dtype=y_dtype)
+        torch.cuda.synchronize()
+        return y.double().cpu().numpy()
+
+
+def _rms(v):
+    return float(np.sqrt(np.mean(v * v)))
+
+
+# (rows, hidden, inter, experts, top_k): experts too wide for the few-token
+# kernels, few and many entries an expert
+GROUPED_SHAPES = [(1, 256, 5632, 8, 7), (40, 512, 256, 24, 4), (70, 256, 256, 9, 3), (200, 512, 256, 4, 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xdt", ["bf16", "f32"])
+@pytest.mark.parametrize("name", ["mxfp4", "q4_1", "q8_0", "q4_k"])
+@pytest.mark.parametrize("shape", GROUPED_SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_grouped_products_keep_f32_between_them(ctx, orc, shape, name, xdt):
+    import torch
+
+    announce(f"moe_layer accuracy {shape} {name} x={xdt}")
+    v = Values(orc, *shape, name, name, xdt)
+    want = v.forward()
+    err = _rms(v.call(ctx, torch.float32) - want) / _rms(want)
+    assert "moefew" not in ctx.last_kernel
+    assert err <= GROUPED, f"{err:.2e}"
+
+
+@pytest.mark.gpu
+def test_wide_down_rows_are_served(ctx, orc):
+    """inter past what LDS holds of an f32 row: bf16 x still gives f32 y, each
+    activation off by at most 2^-8 of itself.  How far that moves y depends on how
+    its terms cancel: the bound is the element-wise one of test_moe_layer_gpu.py,
+    with 2^-8 |a| among the errors of an activation."""
+    import torch
+
+    announce("moe_layer inter 20480")
+    v = Values(orc, 2, 32, 20480, 3, 2, "q4_1", "q4_1", "bf16")
+    L = Layer.__new__(Layer)
+    L.shape, L.xdt, L.xv, L.gv, L.dv = v.shape, v.xdt, v.x, v.gv, v.dv
+    L.check(torch.from_numpy(v.call(ctx, torch.float32)), v.ids, v.p, float(np.abs(v.logits).max()), act_eps=2.0 ** -8)
+
+
+def test_the_bound_sees_bf16_activations(orc):
+    """On the CPU: a forward that rounds the activations between the products to
+    bf16 is far outside the bound."""
+    v = Values(orc, 3, 512, 256, 6, 2, "q4_1", "q4_1", "bf16")
+    want = v.forward()
+    assert _rms(v.forward(a=_bf16) - want) > 16 * GROUPED * _rms(want)

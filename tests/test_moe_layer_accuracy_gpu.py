@@ -8,14 +8,22 @@ a dot product by 2^-16 / sqrt(3) = 8.8e-6 of its RMS; f32 sums of some 100
 additions add 1e-6.  silu(g) u holds two such errors (a slope of 1.1 at most),
 down one more: sqrt(1 + 1.1^2 + 1) 8.8e-6 = 1.6e-5.  GROUPED takes 2^-15, twice
 that.  Activations rounded to bf16 (at most 2^-8, 2^-8 / sqrt(3) / 1.4 RMS over
-a binade) are 1.6e-3 off."""
+a binade) are 1.6e-3 off.
+
+Bound of the few-token kernels: f32 rows and the gated activations as two f16
+planes (off by at most 2^-22), codes exact, so what is left is f32 sums: at most
+64 additions of a block's products, K / 32 / 8 of its lane's blocks and 4 across
+lanes, each off by 2^-24 / sqrt(3) RMS of a partial sum that stays below 4 times
+the RMS of the dot product (unsigned codes ahead of their minimum): sqrt(64 + 16
++ 4) 4 2^-24 / sqrt(3) = 1.3e-6 for K up to 4096, over the products as above
+sqrt(1 + 1.1^2 + 1) 1.3e-6 = 2.3e-6.  FEW takes 2^-18 = 3.8e-6."""
 import numpy as np
 import pytest
 
 from conftest import announce
 from test_moe_layer_gpu import GGUF, Layer, _bank, _t
 
-GROUPED = 2.0 ** -15
+GROUPED, FEW = 2.0 ** -15, 2.0 ** -18
 
 
 def _bf16(v):
@@ -114,3 +122,62 @@ def test_the_bound_sees_bf16_activations(orc):
     v = Values(orc, 3, 512, 256, 6, 2, "q4_1", "q4_1", "bf16")
     want = v.forward()
     assert _rms(v.forward(a=_bf16) - want) > 16 * GROUPED * _rms(want)
+
+
+# every format, wide and narrow layers, up to 64 slots of nearly even weight, one
+# and four entries a pass
+FEW_CASES = [((3, 512, 256, 6, 2), n, n) for n in ("mxfp4", *GGUF)] + [
+    ((1, 4096, 1536, 4, 3), "mxfp4", "q4_k"), ((7, 2048, 768, 9, 8), "mxfp4", "mxfp4"), ((7, 2048, 768, 9, 8), "q4_1", "q4_1"),
+    ((16, 1024, 512, 12, 4), "q4_k", "q6_k"), ((32, 512, 256, 40, 8), "q8_0", "mxfp4"), ((4, 256, 64, 65, 64), "q8_0", "q4_0"),
+    ((1, 128, 96, 70, 64), "mxfp4", "q4_1"), ((24, 1056, 160, 12, 3), "q4_1", "mxfp4")]
+
+
+def _few_id(c):
+    return "-".join(["x".join(map(str, c[0])), *c[1:]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xdt", ["bf16", "f32"])
+@pytest.mark.parametrize("case", FEW_CASES, ids=_few_id)
+def test_few_tokens(ctx, orc, case, xdt):
+    import torch
+
+    announce(f"moe_layer accuracy {case} x={xdt}")
+    v = Values(orc, *case[0], *case[1:], xdt)
+    want = v.forward()
+    err = _rms(v.call(ctx, torch.float32) - want) / _rms(want)
+    assert "moefew" in ctx.last_kernel
+    assert err <= FEW, f"{err:.2e}"
+
+
+def _f16(v):
+    """One f16 plane per 32 elements, the remainder plane lost."""
+    b = v.reshape(-1, 32)
+    s = 2.0 ** (14 - np.floor(np.log2(np.abs(b).max(1, keepdims=True))))
+    return ((b * s).astype(np.float16).astype(np.float64) / s).reshape(v.shape)
+
+
+def _without(i):
+    def f(v):
+        v = v.copy()
+        v[i] = 0.0
+        return v
+
+    return f
+
+
+@pytest.mark.parametrize("case", [c for c in FEW_CASES if c[0][0] * c[0][4] <= 64] + [((4, 256, 64, 65, 64), "q8_0", "q4_0")],
+                         ids=_few_id)
+def test_the_bound_sees_what_is_lost(orc, case):
+    """On the CPU: forwards that lose the remainder plane of the rows or of the
+    activations, the last element of either, or the last slot, are far outside
+    the few-token bound."""
+    v = Values(orc, *case[0], *case[1:], "f32")
+    want = v.forward()
+    far = 4 * FEW * _rms(want)
+    assert _rms(v.forward(x=_f16) - want) > far
+    assert _rms(v.forward(a=_f16) - want) > far
+    assert _rms(v.forward(x=_without(-1)) - want) > far
+    assert _rms(v.forward(a=_without(-1)) - want) > far
+    if case[0][4] > 1:
+        assert _rms(v.forward(slots=case[0][4] - 1) - want) > far

@@ -273,7 +273,7 @@ int rlxq_moe_route(rlxq_ctx* ctx, const float* logits, int64_t rows,
                    int32_t* ids, float* probs, void* stream);
 
 /* The whole routed-expert layer in one call, from the rows to the weighted
- * sum (the layer of rlxq_moe_route and two rlxq_moe_grouped calls, with the
+ * sum (what rlxq_moe_route and two rlxq_moe_grouped calls compute, with the
  * router's own product in front):
  *   l[r, e] = sum_h x[r, h] * router[e, h], summed in f64 and rounded to f32;
  *   the top_k largest logits of a row (ties to the lower expert) with their
@@ -288,7 +288,12 @@ int rlxq_moe_route(rlxq_ctx* ctx, const float* logits, int64_t rows,
  * [num_experts, rows of a slab, K/32].  y [rows, hidden].  ids / probs
  * [rows, top_k] receive the routing, or are NULL.
  * A row whose logits hold a NaN or +inf, or nothing but -inf, has no softmax:
- * its y is NaN (ids 0 .. top_k - 1, probs NaN); -inf alone masks an expert.
+ * its y is NaN (ids 0 .. top_k - 1, probs NaN); -inf alone masks an expert.  A
+ * row with fewer than top_k others takes masked ones at weight 0 (a product that
+ * is not finite is NaN then).
+ * The choice is by logit.  rlxq_moe_route chooses by the rounded probability:
+ * logits closer than expf tells apart are a tie there, for the lower expert, and
+ * rows without a softmax have no defined routing.
  * The gated activations silu * up stay f32, except that more rows, or wider
  * experts, than the few-token kernels take (32 rows; 256 pairs; about 32000
  * inter x top_k) have them rounded to bf16 where x and y are both bf16, or x is

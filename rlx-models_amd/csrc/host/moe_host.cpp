@@ -608,12 +608,14 @@ int few_mt(const rlxq_ctx* ctx, const LayerCall& c) {
   return few_avg(c) < 1.75 || 4 * few_row_bytes(c) > few_lds(ctx) ? 1 : 4;
 }
 
-// Whether the few-token kernels take the call: entries fit a workgroup's tables,
-// an activation row its LDS, and fewer than eight entries come to a fired
-// expert: from there the grouped products run on the matrix instructions.  us
-// for the layer, few-token kernels / grouped (2 of 8 experts): Q4_1 5632 f32 24
-// rows (6 entries) 154 / 343, 32 rows (8 entries) 186 / 102; MXFP4 2816 bf16 67 /
-// 134 and 79 / 61; Q8_0 1024 bf16 43 / 98 and 54 / 50.
+// Whether the few-token kernels take the call: entries fit a workgroup's tables
+// (a mask of 32 rows, 256 entries: layers of many experts end there with the
+// grouped products still the slower ones), an activation row its LDS, and fewer
+// than eight entries come to a fired expert: from there the grouped products run
+// on the matrix instructions.  us for the layer, few-token kernels / grouped (2 of
+// 8 experts, hidden 2048, f32 y): Q4_1 5632 f32 24 rows (6 entries) 165 / 346, 32
+// rows (8 entries) 188 / 117; MXFP4 2816 bf16 69 / 197 and 81 / 61; Q8_0 1024 bf16
+// 44 / 101 and 55 / 53.
 bool few_takes(const rlxq_ctx* ctx, const LayerCall& c) {
   return c.rows <= 32 && c.rows * c.top_k <= 256 && few_avg(c) < 8. && few_row_bytes(c) <= few_lds(ctx) &&
          few_down_lds(c, kFewTile) <= few_lds(ctx);

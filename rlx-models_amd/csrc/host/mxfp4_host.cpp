@@ -75,9 +75,10 @@ int span_splits(int spans, int splits) {   // K splits that all have spans
 
 // Tiling and K splits by the model above, the CUs filled evenly round by
 // round, plus 3.3 us and 8 bytes per partial sum at 8.8 TB/s where K is split.
-// Fitted to 1404 calls (33 to 4096 rows, K 1056 to 12288, N 2048 to 24576); its
-// choices are 1.4% behind the fastest of all tilings on average, 18% at worst
-// (384 x 4096 x 24576: 256 x 256 tiles 52 us, 128 x 128 ones 45).
+// Fitted to calls of 33 to 4096 rows, K 1056 to 12288 and N 2048 to 24576 on every
+// tiling (RLXQ_MX_CFG).  It is not always the fastest: 384 x 4096 -> 24576 takes
+// 51 us on the 256 x 256 tiles it picks and 42 on 128 x 128 ones, 197 x 4096 ->
+// 6144 17.5 on 128 x 64 and 16.2 on 64 x 64.
 const MxCfg& pick_tiling(int64_t m, int64_t k, int64_t n, int cus, int* splits) {
   const MxCfg* best = &kMx[0];
   double best_t = 1e300;

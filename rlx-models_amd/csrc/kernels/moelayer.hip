@@ -530,10 +530,12 @@ constexpr int FEW_ENTRIES = 256;   // most (row, slot) pairs of a call (of at mo
 // chunks of MT, and the workgroups share the (chunk, columns) by cost; a chunk's
 // rows are copied to LDS and its weights read once for all of them.  Workgroup
 // 0 leaves the routing for the down launch.
-// Bound by decoding and dot products beside the weight stream, once it runs
-// (2048 -> 2 x 768, 8 of 128 experts): MXFP4, 1 row 8.6 us, of which some 6 to the
-// first product; 16 rows 39 us for 191 MB past L2, VALU busy half of the time;
-// Q4_K, 4 rows 18 us for 53 MB.
+// (2048 -> 2 x 768, 8 of 128 experts) MXFP4, 1 row: 8.4 us, of which some 6 to the
+// first product.  16 rows: 39 us for 191 MB past L2, 53 of them rows of experts
+// that a second entry reads again; Q4_K, 4 rows: 18 us for 53 MB.  VALU busy half
+// of the time, LDS a tenth; three quarters of decoding and dot products left out
+// (both launches, a timing experiment) were worth 8 of the layer's 67 us at 16
+// rows, so most of what separates it from its bytes is elsewhere.
 template <int SCH, int NPL, int MT>
 RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];   // MT rows of records
@@ -689,9 +691,10 @@ RLXQ_DEV void moe_few_gate_up(const rlxq_moe_few_args& a) {
 // (waves / top_k of them per slot, each a part of the tile; more slots than
 // waves in turns), and the slots are added in slot order.  Workgroups of one
 // column tile are dealt to one XCD (workgroup b runs on XCD b % 8), whose L2
-// then holds the rows of an expert that several tokens take.  Bound as gate|up
-// (768 -> 2048, 8 of 128): MXFP4 16 rows 25.7 us, 73 MB read past L2 of 114 MB in
-// all; Q6_K 4 rows 16.7 us for 40 MB.
+// then holds the rows of an expert that several tokens take.  (768 -> 2048, 8 of
+// 128) MXFP4, 16 rows: 25.9 us, 73 MB read past L2 of 114 MB in all, VALU busy half
+// of the time, LDS a quarter (a lane reads a record of 144 bytes for each block of
+// one weight row); Q6_K, 4 rows: 16.6 us for 40 MB.
 template <int SCH>
 RLXQ_DEV void moe_few_down(const rlxq_moe_few_args& a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];

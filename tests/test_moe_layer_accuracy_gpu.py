@@ -107,6 +107,7 @@ def test_wide_down_rows_are_served(ctx, orc):
     activation off by at most 2^-8 of itself.  How far that moves y depends on how
     its terms cancel: the bound is the element-wise one of test_moe_layer_gpu.py,
     with 2^-8 |a| among the errors of an activation."""
+    import rlxq
     import torch
 
     announce("moe_layer inter 20480")
@@ -114,6 +115,25 @@ def test_wide_down_rows_are_served(ctx, orc):
     L = Layer.__new__(Layer)
     L.shape, L.xdt, L.xv, L.gv, L.dv = v.shape, v.xdt, v.x, v.gv, v.dv
     L.check(torch.from_numpy(v.call(ctx, torch.float32)), v.ids, v.p, float(np.abs(v.logits).max()), act_eps=2.0 ** -8)
+    assert rlxq.lib().rlxq_last_error(ctx.h) == b""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["mxfp4", "q4_1"])
+def test_more_f32_activations_than_the_matrix_kernels_hold(ctx, orc, name):
+    """bf16 x, f32 y and more than 1 GiB of gathered f32 activations: down runs in
+    pieces of rows (the last one shorter), each row as in a call of its own size."""
+    import torch
+
+    rows, times = 37, 541   # 20017 rows of 14336 activations
+    announce(f"moe_layer {rows * times} rows of inter 14336 {name}")
+    v = Values(orc, rows, 32, 14336, 2, 1, name, name, "bf16")
+    want = v.forward()
+    v.x, v.logits = np.tile(v.x, (times, 1)), np.tile(v.logits, (times, 1))
+    v.shape = (rows * times,) + v.shape[1:]
+    y = v.call(ctx, torch.float32).reshape(times, rows, 32)
+    assert _rms(y - want) <= GROUPED * _rms(want)
+    assert max(_rms(t - want) for t in y) <= GROUPED * _rms(want)
 
 
 def test_the_bound_sees_bf16_activations(orc):

@@ -3,11 +3,15 @@ over the RMS of y against float64, which a rounding or an element too many
 cannot hide in.
 
 Bound of the grouped products (f32 between them): a factor held as a high and a
-low part is off by at most 2^-16 of itself, evenly spread and of either sign, so
-a dot product by 2^-16 / sqrt(3) = 8.8e-6 of its RMS; f32 sums of some 100
-additions add 1e-6.  silu(g) u holds two such errors (a slope of 1.1 at most),
-down one more: sqrt(1 + 1.1^2 + 1) 8.8e-6 = 1.6e-5.  GROUPED takes 2^-15, twice
-that.  Activations rounded to bf16 (at most 2^-8, 2^-8 / sqrt(3) / 1.4 RMS over
+low part is off by at most 2^-16 of itself, evenly spread and of either sign: 2^-16
+/ sqrt(3) / 1.4 = 6.3e-6 RMS over a binade.  Unsigned 4-bit codes carry it ahead of
+their minimum: their RMS is sqrt(77.5) = 8.8 where the centred weight's is 4.6, so
+1.9 times of it reaches a dot product, 1.2e-5 of its RMS; f32 sums of some 100
+additions add 1e-6.  silu(g) u holds two such errors (a slope of 1.1 at most), down
+one more: sqrt(1 + 1.1^2 + 1) 1.2e-5 = 2.1e-5.  GROUPED takes 2^-15 = 3.1e-5, for
+the formats tested here (the minima of the generated Q5_K and Q2_K banks are
+further from their codes' mean).
+Activations rounded to bf16 (at most 2^-8, 2^-8 / sqrt(3) / 1.4 RMS over
 a binade) are 1.6e-3 off.
 
 Bound of the few-token kernels: f32 rows and the gated activations as two f16

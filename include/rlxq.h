@@ -294,10 +294,10 @@ int rlxq_moe_route(rlxq_ctx* ctx, const float* logits, int64_t rows,
  * The choice is by logit.  rlxq_moe_route chooses by the rounded probability:
  * logits closer than expf tells apart are a tie there, for the lower expert, and
  * rows without a softmax have no defined routing.
- * The gated activations silu * up stay f32, except that more rows, or wider
- * experts, than the few-token kernels take (32 rows; 256 pairs; about 32000
- * inter x top_k) have them rounded to bf16 where x and y are both bf16, or x is
- * and inter is above 18176.
+ * The gated activations silu * up stay f32, except in calls past the few-token
+ * kernels (32 rows, 256 pairs, eight pairs an expert, about 32000 inter x
+ * top_k): those may round them to bf16 where x and y are both bf16, or where x
+ * is and inter is above 18176.
  * A row of x that is not finite, on the caller's finite logits, leaves its own
  * row of y not finite and the others alone.
  * num_experts <= 1024, top_k <= min(num_experts, 64); hidden and inter as the

@@ -589,8 +589,8 @@ class Context:
         caller's logits, router=None), top-k, gate|up + SwiGLU, down and the
         weighted sum; returns y [rows, hidden].  ids / probs [rows, top_k]
         receive the routing if given.  The activations between the products are
-        f32; with bf16 x and y and more than 32 rows (or very wide experts) they
-        may be bf16."""
+        f32; with bf16 x and y, calls past the few-token kernels (include/rlxq.h)
+        may round them to bf16."""
         import torch
 
         check_moe_layer(x, router, gate_up, down, gate_up_scheme, down_scheme, top_k, inter, num_experts, logits=logits,

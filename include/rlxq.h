@@ -318,6 +318,74 @@ int rlxq_moe_layer(rlxq_ctx* ctx, const void* x, int x_dtype,
 int rlxq_swiglu(rlxq_ctx* ctx, const void* gu, int gu_dtype, int64_t rows,
                 int64_t inter, void* out, int out_dtype, void* stream);
 
+/* ---- around the packed products of a served batch --------------------------
+ * (no counterpart on the reference's hot path; crates/rlx-tune holds its
+ * adapters, which it folds into float weights) */
+
+/* Low-rank adapters of many requests beside a shared projection, each row its own:
+ *   y[i, c] = base[i, c] + scales[e] * sum_{r < ranks[e]} b[e, c, r] * v[i, g, r],
+ *   v[i, g, r] = sum_h a[e, g * rank + r, h] * x[i, h],   e = ids[i],
+ * where g is the segment of column c: the columns of a fused projection (q|k|v,
+ * gate|up) have adapters of their own.  base is usually the output of the
+ * projection (rlxq_dequant_matmul) and may be y itself; NULL is zero.
+ * x [m, k]; ids [m] int32 in any order, a row whose id is outside
+ * [0, num_adapters) has no adapter (y = base, bit for bit); a
+ * [num_adapters, segs * rank, k], b [num_adapters, n, rank] of ab_dtype; ranks
+ * [num_adapters] int32 (clamped to [0, rank]; what a and b hold past them is
+ * not used) or NULL: rank; scales [num_adapters] f32 or NULL: 1; base and y
+ * [m, n] of y_dtype.  seg_ends: host array of segs (1 to 4) column ends, rising
+ * to n; NULL with segs = 1.  v and the sums are f32; y is rounded once.
+ * k % 8 == 0, rank % 8 == 0 and at most 256; m, k, n up to 2^24;
+ * num_adapters up to 2^20; x, a, b 16-byte aligned.  With m = 0 or n = 0
+ * nothing is read or written. */
+int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype,
+                     const int32_t* ids, const void* a, const void* b,
+                     int ab_dtype, const int32_t* ranks, const float* scales,
+                     const int64_t* seg_ends, int64_t segs, int64_t m,
+                     int64_t k, int64_t n, int64_t rank, int64_t num_adapters,
+                     const void* base, void* y, int y_dtype, void* stream);
+
+/* The norms after one block and before the next, with the gate and the residual
+ * sum between them:
+ *   t = block;  t *= (weight_offset + post_weight) / sqrt(mean(t^2) + eps)
+ *   h = resid + scale * gate * t;                                sum = h
+ *   y = h * (weight_offset + pre_weight) / sqrt(mean(h^2) + eps)
+ * block [rows, hidden] or NULL (zero); resid [rows, hidden] or NULL (zero), at
+ * least one of the two; gate [gate_rows, hidden] or NULL (one), gate_rows a
+ * divisor of rows: consecutive rows / gate_rows rows share a gate row;
+ * post_weight [hidden] or NULL: block is not normalised; pre_weight [hidden] and
+ * y [rows, hidden] both given or both NULL; both weights of weight_dtype; sum
+ * [rows, hidden] of resid_dtype, or NULL.  sum may be resid, and y or sum may be
+ * block where the types agree.  f32 arithmetic; y is of the sum before it is
+ * rounded.  With rows = 0 nothing is read or written. */
+int rlxq_residual_norm(rlxq_ctx* ctx, const void* block, int block_dtype,
+                       const void* resid, int resid_dtype, const void* gate,
+                       int gate_dtype, int64_t gate_rows,
+                       const void* post_weight, const void* pre_weight,
+                       int weight_dtype, float weight_offset, float scale,
+                       float eps, int64_t rows, int64_t hidden, void* sum,
+                       void* y, int y_dtype, void* stream);
+
+/* A token per row of logits [rows, vocab] (f32 or bf16), drawn with the caller's
+ * uniform number u[row] in [0, 1).  With T = temperature[row], w_j = exp((l_j -
+ * max l) / T) and the tokens ordered by falling logit (equal ones by rising
+ * index), the kept ones are: the first top_k; of these the shortest prefix whose
+ * mass is at least top_p times theirs, one token at least; of these the ones
+ * with w >= min_p (the likeliest always).  tokens[row] is the lowest index whose
+ * sum of kept w over it and all lower indices exceeds u times the kept sum;
+ * probs[row] its share of that sum.  T <= 0: the likeliest token (the lowest index
+ * of equal ones), probability 1.  temperature, top_k, top_p, min_p [rows] each,
+ * or NULL: 1, off, off, off; top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0
+ * (or NaN) are off.  u below 0 counts as 0, from 1 up as just below 1.  A logit of
+ * -inf masks its token.  A row with a NaN or +inf logit, nothing but -inf, or a
+ * NaN temperature or u gets token -1 and probability NaN.  probs may be NULL.
+ * The weights and sums are f64: the same call gives the same tokens.  vocab up to
+ * 2^20.  With rows = 0 nothing is read or written. */
+int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype,
+                int64_t rows, int64_t vocab, const float* temperature,
+                const int32_t* top_k, const float* top_p, const float* min_p,
+                const float* u, int32_t* tokens, float* probs, void* stream);
+
 /* W8A8 GEMM: per-row int8 activation quantisation computed on the fly
  * (crates/rlx-quant-calib/src/bitnet.rs:76-93) times per-channel int8
  * weights (crates/rlx-kimi-k3/src/common.rs:466-482, wq [K, N], w_scale [N])

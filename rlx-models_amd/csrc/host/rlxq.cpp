@@ -58,6 +58,9 @@ RLXQ_EMBED(rlxq_co_moelayer2, "moelayer2.co")
 RLXQ_EMBED(rlxq_co_moelayer3, "moelayer3.co")
 RLXQ_EMBED(rlxq_co_moelayer4, "moelayer4.co")
 RLXQ_EMBED(rlxq_co_moelayer5, "moelayer5.co")
+RLXQ_EMBED(rlxq_co_lora, "lora.co")
+RLXQ_EMBED(rlxq_co_resnorm, "resnorm.co")
+RLXQ_EMBED(rlxq_co_sample, "sample.co")
 
 namespace {
 
@@ -94,6 +97,9 @@ const Image kImages[] = {
     {rlxq_co_moelayer3_begin, rlxq_co_moelayer3_end, "moelayer3"},
     {rlxq_co_moelayer4_begin, rlxq_co_moelayer4_end, "moelayer4"},
     {rlxq_co_moelayer5_begin, rlxq_co_moelayer5_end, "moelayer5"},
+    {rlxq_co_lora_begin, rlxq_co_lora_end, "lora"},
+    {rlxq_co_resnorm_begin, rlxq_co_resnorm_end, "resnorm"},
+    {rlxq_co_sample_begin, rlxq_co_sample_end, "sample"},
 };
 
 std::string hip_msg(hipError_t e) { return std::string(hipGetErrorName(e)) + ": " + hipGetErrorString(e); }

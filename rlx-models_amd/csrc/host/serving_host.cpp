@@ -1,0 +1,185 @@
+// Host side of the operators around a served batch's packed products: low-rank
+// adapters, the residual norm, sampling.
+#include <hip/hip_runtime_api.h>
+
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+#include <string>
+
+#include "lora_args.h"
+#include "resnorm_args.h"
+#include "rlxq.h"
+#include "rlxq_internal.hpp"
+#include "sample_args.h"
+
+using namespace rlxq;
+
+namespace {
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool act_dtype(int d) { return d == RLXQ_F32 || d == RLXQ_BF16; }
+// Whether p holds whole elements of dtype d.
+bool element_aligned(const void* p, int d) { return aligned(p, d == RLXQ_BF16 ? 2 : 4); }
+
+int run_kernel(rlxq_ctx* ctx, const char* name, int64_t grid, int threads, size_t lds, void* args, void* stream) {
+  hipFunction_t fn;
+  int rc = get_fn(ctx, name, &fn);
+  if (rc) return rc;
+  void* kargs[] = {args};
+  return launch(ctx, fn, dim3((unsigned)grid), dim3(threads), lds, stream, kargs, name);
+}
+
+}  // namespace
+
+extern "C" {
+
+int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* ids, const void* a, const void* b,
+                     int ab_dtype, const int32_t* ranks, const float* scales, const int64_t* seg_ends, int64_t segs,
+                     int64_t m, int64_t k, int64_t n, int64_t rank, int64_t num_adapters, const void* base, void* y,
+                     int y_dtype, void* stream) {
+  if (!ctx) return RLXQ_E_NULL;
+  ctx->last_error.clear();
+  if (m < 0 || n < 0 || k <= 0) return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: need m >= 0, n >= 0, k > 0");
+  if (m > (1 << 24) || n > (1 << 24) || k > (1 << 24))
+    return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: m, k and n up to 2^24");
+  if (rank <= 0 || rank > 256 || rank % 8) return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: rank is a multiple of 8 up to 256");
+  if (num_adapters <= 0 || num_adapters > (1 << 20))
+    return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: 1 to 2^20 adapters");
+  if (k % 8) return fail(ctx, RLXQ_E_ALIGN, "lora_matmul: K must be a multiple of 8");
+  if (!act_dtype(x_dtype)) return fail(ctx, RLXQ_E_DTYPE, "lora_matmul: x_dtype");
+  if (!act_dtype(ab_dtype)) return fail(ctx, RLXQ_E_DTYPE, "lora_matmul: ab_dtype");
+  if (!act_dtype(y_dtype)) return fail(ctx, RLXQ_E_DTYPE, "lora_matmul: y_dtype");
+  rlxq_lora_args g;
+  std::memset(&g, 0, sizeof g);
+  if (seg_ends) {
+    if (segs < 1 || segs > RLXQ_LORA_SEGS) return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: 1 to 4 segments");
+    for (int64_t i = 0; i < segs; i++) {
+      if (seg_ends[i] < (i ? seg_ends[i - 1] : 0) || seg_ends[i] > n)
+        return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: segment ends must rise from 0 to n");
+      g.ends[i] = seg_ends[i];
+    }
+    if (g.ends[segs - 1] != n) return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: the last segment must end at n");
+  } else {
+    if (segs != 1) return fail(ctx, RLXQ_E_NULL, "lora_matmul: seg_ends of several segments");
+    g.ends[0] = n;
+  }
+  if (m == 0 || n == 0) return RLXQ_OK;   // nothing is read or written
+  if (!x || !ids || !a || !b || !y) return fail(ctx, RLXQ_E_NULL, "lora_matmul: null pointer");
+  if (!aligned(x, 16) || !aligned(a, 16) || !aligned(b, 16))
+    return fail(ctx, RLXQ_E_ALIGN, "lora_matmul: x, a and b must be 16-byte aligned");
+  if (!element_aligned(y, y_dtype) || !element_aligned(base, y_dtype) || !aligned(ids, 4) || !aligned(ranks, 4) ||
+      !aligned(scales, 4))
+    return fail(ctx, RLXQ_E_ALIGN, "lora_matmul: base, y, ids, ranks and scales must be element aligned");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok()) return fail(ctx, RLXQ_E_HIP, "lora_matmul: hipSetDevice");
+  g.x = x;
+  g.ids = ids;
+  g.a = a;
+  g.b = b;
+  g.ranks = ranks;
+  g.scales = scales;
+  g.base = base;
+  g.y = y;
+  g.M = m;
+  g.K = k;
+  g.N = n;
+  g.R = (int32_t)rank;
+  g.E = (int32_t)num_adapters;
+  g.S = (int32_t)segs;
+  g.x_bf16 = x_dtype == RLXQ_BF16;
+  g.ab_bf16 = ab_dtype == RLXQ_BF16;
+  g.y_bf16 = y_dtype == RLXQ_BF16;
+  const int64_t shrink = (m * segs * rank + 3) / 4, expand = (m * n + 255) / 256;
+  if (!grid_fits(shrink, 256) || !grid_fits(expand, 256))
+    return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: m, n and rank need a launch of 2^32 work-items or more");
+  void* ws = nullptr;
+  int rc = workspace(ctx, (size_t)(m * segs * rank) * 4, &ws, stream);
+  if (rc) return rc;
+  g.v = static_cast<float*>(ws);
+  if ((rc = run_kernel(ctx, "rlxq_lora_shrink", shrink, 256, 0, &g, stream))) return rc;
+  return run_kernel(ctx, "rlxq_lora_expand", expand, 256, 0, &g, stream);
+}
+
+int rlxq_residual_norm(rlxq_ctx* ctx, const void* block, int block_dtype, const void* resid, int resid_dtype,
+                       const void* gate, int gate_dtype, int64_t gate_rows, const void* post_weight,
+                       const void* pre_weight, int weight_dtype, float weight_offset, float scale, float eps,
+                       int64_t rows, int64_t hidden, void* sum, void* y, int y_dtype, void* stream) {
+  if (!ctx) return RLXQ_E_NULL;
+  ctx->last_error.clear();
+  if (rows < 0 || hidden <= 0) return fail(ctx, RLXQ_E_SHAPE, "residual_norm: need rows >= 0, hidden > 0");
+  if (hidden > (1 << 24)) return fail(ctx, RLXQ_E_SHAPE, "residual_norm: hidden up to 2^24");
+  if (!grid_fits(rows, 1024)) return fail(ctx, RLXQ_E_SHAPE, "residual_norm: rows need a launch of 2^32 work-items or more");
+  if ((block && !act_dtype(block_dtype)) || !act_dtype(resid_dtype) || (gate && !act_dtype(gate_dtype)) ||
+      ((post_weight || pre_weight) && !act_dtype(weight_dtype)) || (y && !act_dtype(y_dtype)))
+    return fail(ctx, RLXQ_E_DTYPE, "residual_norm: dtypes are f32 or bf16");
+  if (!(eps >= 0.0f)) return fail(ctx, RLXQ_E_SHAPE, "residual_norm: eps must be >= 0");
+  if (gate && (gate_rows <= 0 || (rows > 0 && (gate_rows > rows || rows % gate_rows))))
+    return fail(ctx, RLXQ_E_SHAPE, "residual_norm: gate_rows must divide rows");
+  if (rows == 0) return RLXQ_OK;   // nothing is read or written
+  if (!block && !resid) return fail(ctx, RLXQ_E_NULL, "residual_norm: neither block nor resid");
+  if (!block && (gate || post_weight)) return fail(ctx, RLXQ_E_NULL, "residual_norm: gate and post_weight need block");
+  if (!sum && !y) return fail(ctx, RLXQ_E_NULL, "residual_norm: neither sum nor y");
+  if ((y == nullptr) != (pre_weight == nullptr)) return fail(ctx, RLXQ_E_NULL, "residual_norm: y and pre_weight go together");
+  if (!element_aligned(block, block_dtype) || !element_aligned(resid, resid_dtype) || !element_aligned(gate, gate_dtype) ||
+      !element_aligned(post_weight, weight_dtype) || !element_aligned(pre_weight, weight_dtype) ||
+      !element_aligned(sum, resid_dtype) || !element_aligned(y, y_dtype))
+    return fail(ctx, RLXQ_E_ALIGN, "residual_norm: pointers must be element aligned");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok()) return fail(ctx, RLXQ_E_HIP, "residual_norm: hipSetDevice");
+  rlxq_resnorm_args g;
+  std::memset(&g, 0, sizeof g);
+  g.block = block;
+  g.resid = resid;
+  g.gate = gate;
+  g.post_w = post_weight;
+  g.pre_w = pre_weight;
+  g.sum = sum;
+  g.y = y;
+  g.M = rows;
+  g.H = hidden;
+  g.gate_span = gate ? rows / gate_rows : 1;
+  g.alpha = scale;
+  g.eps = eps;
+  g.w_off = weight_offset;
+  g.block_bf16 = block_dtype == RLXQ_BF16;
+  g.resid_bf16 = resid_dtype == RLXQ_BF16;
+  g.gate_bf16 = gate_dtype == RLXQ_BF16;
+  g.w_bf16 = weight_dtype == RLXQ_BF16;
+  g.y_bf16 = y_dtype == RLXQ_BF16;
+  return run_kernel(ctx, "rlxq_resnorm_any", rows, 256, 0, &g, stream);
+}
+
+int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t rows, int64_t vocab,
+                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
+                int32_t* tokens, float* probs, void* stream) {
+  if (!ctx) return RLXQ_E_NULL;
+  ctx->last_error.clear();
+  if (rows < 0 || vocab <= 0) return fail(ctx, RLXQ_E_SHAPE, "sample: need rows >= 0, vocab > 0");
+  if (vocab > RLXQ_SAMPLE_MAX_VOCAB) return fail(ctx, RLXQ_E_SHAPE, "sample: vocab up to 2^20");
+  if (!grid_fits(rows, 1024)) return fail(ctx, RLXQ_E_SHAPE, "sample: rows need a launch of 2^32 work-items or more");
+  if (!act_dtype(logits_dtype)) return fail(ctx, RLXQ_E_DTYPE, "sample: logits_dtype");
+  if (rows == 0) return RLXQ_OK;   // nothing is read or written
+  if (!logits || !u || !tokens) return fail(ctx, RLXQ_E_NULL, "sample: null pointer");
+  if (!element_aligned(logits, logits_dtype) || !aligned(temperature, 4) || !aligned(top_k, 4) || !aligned(top_p, 4) ||
+      !aligned(min_p, 4) || !aligned(u, 4) || !aligned(tokens, 4) || !aligned(probs, 4))
+    return fail(ctx, RLXQ_E_ALIGN, "sample: pointers must be element aligned");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok()) return fail(ctx, RLXQ_E_HIP, "sample: hipSetDevice");
+  rlxq_sample_args g;
+  std::memset(&g, 0, sizeof g);
+  g.logits = logits;
+  g.temperature = temperature;
+  g.top_k = top_k;
+  g.top_p = top_p;
+  g.min_p = min_p;
+  g.u = u;
+  g.tokens = tokens;
+  g.probs = probs;
+  g.M = rows;
+  g.V = (int32_t)vocab;
+  g.bf16 = logits_dtype == RLXQ_BF16;
+  return run_kernel(ctx, "rlxq_sample_scan", rows, 1024, 0, &g, stream);
+}
+
+}  // extern "C"

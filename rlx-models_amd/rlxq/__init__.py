@@ -92,6 +92,10 @@ def lib() -> C.CDLL:
         "rlxq_quantize_act_int8": (I, [P, P, I, I64, I64, P, P, P]),
         "rlxq_quantize_mxfp4": (I, [P, P, I, I64, I64, P, P, P]),
         "rlxq_mxfp4_gemm": (I, [P, P, I, P, P, I64, I64, I64, P, I, P]),
+        "rlxq_lora_matmul": (I, [P, P, I, P, P, P, I, P, P, C.POINTER(I64), I64, I64, I64, I64, I64, I64, P, P, I, P]),
+        "rlxq_residual_norm": (I, [P, P, I, P, I, P, I, I64, P, P, I, C.c_float, C.c_float, C.c_float, I64, I64, P, P,
+                                   I, P]),
+        "rlxq_sample": (I, [P, P, I, I64, I64, P, P, P, P, P, P, P, P]),
         "rlxq_dequantize": (I, [P, I, I, P, P, P, I, I64, I64, P, P]),
         "rlxq_dm_try_new": (I, [I, C.POINTER(P)]),
         "rlxq_dm_free": (None, [P]),
@@ -425,6 +429,86 @@ def check_mxfp4_gemm(x, w, w_scales, n: int, *, y=None, device=None) -> None:
         _on_device(device, x=x, w=w, w_scales=w_scales, y=y)
 
 
+def check_lora_matmul(x, ids, a, b, *, ranks=None, scales=None, segments=None, base=None, y=None, device=None) -> None:
+    import torch
+
+    _tensor(x, "lora_matmul: x", _act_dtypes(), 2)
+    m, k = x.shape
+    _tensor(ids, "lora_matmul: ids", (torch.int32,), 1)
+    if ids.shape[0] != m:
+        raise ValueError(f"lora_matmul: ids has {ids.shape[0]} entries, x has {m} rows")
+    _tensor(a, "lora_matmul: a", _act_dtypes(), 3)
+    _tensor(b, "lora_matmul: b", (a.dtype,), 3)
+    e, n, rank = b.shape
+    segs = 1 if segments is None else len(segments)
+    if tuple(a.shape) != (e, segs * rank, k):
+        raise ValueError(f"lora_matmul: a has shape {tuple(a.shape)}, expected {(e, segs * rank, k)}")
+    if segments is not None and (min(segments, default=-1) < 0 or sum(segments) != n):
+        raise ValueError(f"lora_matmul: segments {list(segments)} do not add up to {n} columns")
+    for nm, t, dt in (("ranks", ranks, torch.int32), ("scales", scales, torch.float32)):
+        if t is not None:
+            _tensor(t, "lora_matmul: " + nm, (dt,), 1)
+            if t.shape[0] != e:
+                raise ValueError(f"lora_matmul: {nm} has {t.shape[0]} entries, there are {e} adapters")
+    for nm, t in (("base", base), ("y", y)):
+        if t is not None:
+            _tensor(t, "lora_matmul: " + nm, _act_dtypes(), 2)
+            if tuple(t.shape) != (m, n):
+                raise ValueError(f"lora_matmul: {nm} has shape {tuple(t.shape)}, expected {(m, n)}")
+    if base is not None and y is not None and base.dtype != y.dtype:
+        raise ValueError(f"lora_matmul: base is {base.dtype}, y {y.dtype}")
+    if device is not None:
+        _on_device(device, x=x, ids=ids, a=a, b=b, ranks=ranks, scales=scales, base=base, y=y)
+
+
+def check_residual_norm(block, resid, *, pre_weight=None, post_weight=None, gate=None, sum=None, y=None,
+                        device=None) -> None:
+    _need(block is not None or resid is not None, "residual_norm: neither block nor resid")
+    _need(block is not None or (gate is None and post_weight is None), "residual_norm: gate and post_weight need block")
+    _need(y is None or pre_weight is not None, "residual_norm: y needs pre_weight")
+    rows = hidden = None
+    for nm, t in (("block", block), ("resid", resid), ("sum", sum), ("y", y)):
+        if t is not None:
+            _tensor(t, "residual_norm: " + nm, _act_dtypes(), 2)
+            if rows is None:
+                rows, hidden = t.shape
+            if tuple(t.shape) != (rows, hidden):
+                raise ValueError(f"residual_norm: {nm} has shape {tuple(t.shape)}, expected {(rows, hidden)}")
+    for nm, t in (("pre_weight", pre_weight), ("post_weight", post_weight)):
+        if t is not None:
+            _tensor(t, "residual_norm: " + nm, _act_dtypes(), 1)
+            if t.shape[0] != hidden:
+                raise ValueError(f"residual_norm: {nm} has {t.shape[0]} elements, hidden = {hidden}")
+    if pre_weight is not None and post_weight is not None and pre_weight.dtype != post_weight.dtype:
+        raise ValueError("residual_norm: pre_weight and post_weight must share a dtype")
+    if resid is not None and sum is not None and sum.dtype != resid.dtype:
+        raise ValueError(f"residual_norm: sum is {sum.dtype}, resid {resid.dtype}")
+    if gate is not None:
+        _tensor(gate, "residual_norm: gate", _act_dtypes(), 2)
+        if gate.shape[1] != hidden or gate.shape[0] == 0 or rows % gate.shape[0] or gate.shape[0] > max(rows, 1):
+            raise ValueError(f"residual_norm: gate has shape {tuple(gate.shape)}, expected [a divisor of {rows}, {hidden}]")
+    if device is not None:
+        _on_device(device, block=block, resid=resid, pre_weight=pre_weight, post_weight=post_weight, gate=gate, sum=sum, y=y)
+
+
+def check_sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None,
+                 device=None) -> None:
+    import torch
+
+    _tensor(logits, "sample: logits", _act_dtypes(), 2)
+    _tensor(u, "sample: u", (torch.float32,), 1)
+    for nm, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                      ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int32),
+                      ("probs", probs, torch.float32)):
+        if t is not None:
+            _tensor(t, "sample: " + nm, (dt,), 1)
+            if t.shape[0] != logits.shape[0]:
+                raise ValueError(f"sample: {nm} has {t.shape[0]} entries, logits have {logits.shape[0]} rows")
+    if device is not None:
+        _on_device(device, logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                   tokens=tokens, probs=probs)
+
+
 class Context:
     """Owns an rlxq_ctx on one device (rlxq_init / rlxq_destroy)."""
 
@@ -685,6 +769,89 @@ class Context:
                                   _stream(stream, self.device))
         self._check(rc, "w8a8_gemm")
         return y
+
+
+class Serving:
+    """The operators around the packed products of a served batch, on a Context
+    (its device, its scratch, its errors): low-rank adapters, the residual norm
+    and sampling."""
+
+    def __init__(self, ctx: Context):
+        self.ctx = ctx
+
+    def lora_matmul(self, x, ids, a, b, *, ranks=None, scales=None, segments=None, base=None, y=None, y_dtype=None,
+                    stream=None):
+        """y[i] = base[i] + scales[e] * b[e] . (a[e] . x[i]), e = ids[i]: x [m, k],
+        a [adapters, segments * rank, k], b [adapters, n, rank]; segments: the
+        widths of the column ranges of a fused projection, each with its own
+        rank rows of a.  A row whose id is outside [0, adapters) is base's.
+        Returns y (allocated if not given, of base's dtype, else f32); y may be base."""
+        import torch
+
+        c = self.ctx
+        check_lora_matmul(x, ids, a, b, ranks=ranks, scales=scales, segments=segments, base=base, y=y, device=c.device)
+        m, k = x.shape
+        e, n, rank = b.shape
+        if y is None:
+            y = torch.empty((m, n), dtype=base.dtype if base is not None else y_dtype or torch.float32, device=x.device)
+        ends, segs = None, 1
+        if segments is not None:
+            segs, at = len(segments), 0
+            ends = (C.c_int64 * segs)()
+            for i, w in enumerate(segments):
+                at += w
+                ends[i] = at
+        rc = lib().rlxq_lora_matmul(c.h, _ptr(x), _dt(x), _ptr(ids), _ptr(a), _ptr(b), _dt(a), _ptr(ranks), _ptr(scales),
+                                    ends, segs, m, k, n, rank, e, _ptr(base), _ptr(y), _dt(y), _stream(stream, c.device))
+        c._check(rc, "lora_matmul")
+        return y
+
+    def residual_norm(self, block, resid, *, pre_weight=None, post_weight=None, gate=None, scale: float = 1.0,
+                      eps: float = 1e-6, weight_offset: float = 0.0, sum=None, y=None, y_dtype=None, stream=None):
+        """h = resid + scale * gate * norm(block, post_weight), y = norm(h,
+        pre_weight); returns (h, y).  block or resid None: zero; gate [groups, h]
+        or None; post_weight None: block as it is; pre_weight None: no y.  h has
+        resid's dtype (f32 without resid) and may be written over resid
+        (sum=resid); y has y_dtype, or h's dtype."""
+        import torch
+
+        c = self.ctx
+        check_residual_norm(block, resid, pre_weight=pre_weight, post_weight=post_weight, gate=gate, sum=sum, y=y,
+                            device=c.device)
+        first = block if block is not None else resid
+        rows, hidden = first.shape
+        if sum is None:
+            sum = torch.empty((rows, hidden), dtype=resid.dtype if resid is not None else torch.float32, device=first.device)
+        if y is None and pre_weight is not None:
+            y = torch.empty((rows, hidden), dtype=y_dtype or sum.dtype, device=first.device)
+        w = pre_weight if pre_weight is not None else post_weight
+        rc = lib().rlxq_residual_norm(c.h, _ptr(block), _dt(block) if block is not None else F32, _ptr(resid), _dt(sum),
+                                      _ptr(gate), _dt(gate) if gate is not None else F32,
+                                      gate.shape[0] if gate is not None else 1, _ptr(post_weight), _ptr(pre_weight),
+                                      _dt(w) if w is not None else F32, weight_offset, scale, eps, rows, hidden,
+                                      _ptr(sum), _ptr(y), _dt(y) if y is not None else F32, _stream(stream, c.device))
+        c._check(rc, "residual_norm")
+        return sum, y
+
+    def sample(self, logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None,
+               stream=None):
+        """A token per row of logits, from the uniform numbers u [rows]: returns
+        (tokens int32, probs f32).  The settings are [rows] tensors, or None
+        (temperature 1, the others off); temperature 0 is the likeliest token."""
+        import torch
+
+        c = self.ctx
+        check_sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, tokens=tokens, probs=probs,
+                     device=c.device)
+        rows, vocab = logits.shape
+        if tokens is None:
+            tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+        if probs is None:
+            probs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+        rc = lib().rlxq_sample(c.h, _ptr(logits), _dt(logits), rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                               _ptr(min_p), _ptr(u), _ptr(tokens), _ptr(probs), _stream(stream, c.device))
+        c._check(rc, "sample")
+        return tokens, probs
 
 
 class DeviceMatmul:

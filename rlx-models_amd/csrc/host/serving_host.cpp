@@ -2,6 +2,7 @@
 // adapters, the residual norm, sampling.
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -147,7 +148,19 @@ int rlxq_residual_norm(rlxq_ctx* ctx, const void* block, int block_dtype, const 
   g.gate_bf16 = gate_dtype == RLXQ_BF16;
   g.w_bf16 = weight_dtype == RLXQ_BF16;
   g.y_bf16 = y_dtype == RLXQ_BF16;
-  return run_kernel(ctx, "rlxq_resnorm_any", rows, 256, 0, &g, stream);
+  bool vec = hidden % 8 == 0 && hidden <= 16384;
+  for (const void* p : {block, resid, gate, post_weight, pre_weight, static_cast<const void*>(sum), static_cast<const void*>(y)})
+    vec = vec && aligned(p, 16);
+  if (!vec) return run_kernel(ctx, "rlxq_resnorm_any", rows, 256, 0, &g, stream);
+  // pieces of eight a thread
+  const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
+  const int64_t pieces = hidden / 8;
+  const int ch = pieces > 1024 ? 4 : (pieces <= 64 || rows <= 2 * cus ? 1 : 2);
+  const int threads = (int)(((pieces + ch - 1) / ch + 63) / 64 * 64);
+  static const char* const kDt[2] = {"f32", "bf16"};
+  char name[40];
+  std::snprintf(name, sizeof name, "rlxq_resnorm_%s_%s_c%d", kDt[block ? g.block_bf16 : 0], kDt[g.resid_bf16], ch);
+  return run_kernel(ctx, name, rows, threads, 0, &g, stream);
 }
 
 int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t rows, int64_t vocab,
@@ -179,7 +192,33 @@ int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t row
   g.M = rows;
   g.V = (int32_t)vocab;
   g.bf16 = logits_dtype == RLXQ_BF16;
-  return run_kernel(ctx, "rlxq_sample_scan", rows, 1024, 0, &g, stream);
+  const bool bf = logits_dtype == RLXQ_BF16;
+  const int lead = bf ? 7 : 3;   // elements ahead of the row in its first 16 bytes, at most
+  g.chunks = (int32_t)((vocab + lead + RLXQ_SAMPLE_CHUNK - 1) / RLXQ_SAMPLE_CHUNK);
+  // rows in batches whose chunks take up to 128 MB of scratch
+  const int64_t row_bytes = g.chunks * (int64_t)(sizeof(rlxq_sample_chunk) + RLXQ_SAMPLE_BINS * (8 + 2));
+  const int64_t batch = std::min<int64_t>(rows, std::max<int64_t>(1, (128 << 20) / row_bytes));
+  void* ws = nullptr;
+  int rc = workspace(ctx, (size_t)(batch * row_bytes), &ws, stream);
+  if (rc) return rc;
+  g.heads = static_cast<rlxq_sample_chunk*>(ws);
+  g.masses = reinterpret_cast<uint64_t*>(g.heads + batch * g.chunks);
+  g.counts = reinterpret_cast<uint16_t*>(g.masses + batch * g.chunks * RLXQ_SAMPLE_BINS);
+  for (int64_t at = 0; at < rows; at += batch) {
+    g.M = std::min(batch, rows - at);
+    g.logits = static_cast<const char*>(logits) + at * vocab * (bf ? 2 : 4);
+    if (temperature) g.temperature = temperature + at;
+    if (top_k) g.top_k = top_k + at;
+    if (top_p) g.top_p = top_p + at;
+    if (min_p) g.min_p = min_p + at;
+    g.u = u + at;
+    g.tokens = tokens + at;
+    if (probs) g.probs = probs + at;
+    if ((rc = run_kernel(ctx, bf ? "rlxq_sample_hist_bf16" : "rlxq_sample_hist_f32", g.M * g.chunks, 256, 0, &g, stream)) ||
+        (rc = run_kernel(ctx, bf ? "rlxq_sample_pick_bf16" : "rlxq_sample_pick_f32", g.M, 512, 0, &g, stream)))
+      return rc;
+  }
+  return RLXQ_OK;
 }
 
 }  // extern "C"

@@ -336,7 +336,7 @@ int rlxq_swiglu(rlxq_ctx* ctx, const void* gu, int gu_dtype, int64_t rows,
  * [m, n] of y_dtype.  seg_ends: host array of segs (1 to 4) column ends, rising
  * to n; NULL with segs = 1.  v and the sums are f32; y is rounded once.
  * k % 8 == 0, rank % 8 == 0 and at most 256; m, k, n up to 2^24;
- * num_adapters up to 2^20; x, a, b 16-byte aligned.  With m = 0 or n = 0
+ * num_adapters up to 16384; x, a, b 16-byte aligned.  With m = 0 or n = 0
  * nothing is read or written. */
 int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype,
                      const int32_t* ids, const void* a, const void* b,

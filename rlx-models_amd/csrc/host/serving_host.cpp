@@ -44,9 +44,9 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   if (m < 0 || n < 0 || k <= 0) return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: need m >= 0, n >= 0, k > 0");
   if (m > (1 << 24) || n > (1 << 24) || k > (1 << 24))
     return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: m, k and n up to 2^24");
-  if (rank <= 0 || rank > 256 || rank % 8) return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: rank is a multiple of 8 up to 256");
-  if (num_adapters <= 0 || num_adapters > (1 << 20))
-    return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: 1 to 2^20 adapters");
+  if (rank <= 0 || rank > RLXQ_LORA_MAX_RANK || rank % 8) return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: rank is a multiple of 8 up to 256");
+  if (num_adapters <= 0 || num_adapters > RLXQ_LORA_MAX_ADAPTERS)
+    return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: 1 to 16384 adapters");
   if (k % 8) return fail(ctx, RLXQ_E_ALIGN, "lora_matmul: K must be a multiple of 8");
   if (!act_dtype(x_dtype)) return fail(ctx, RLXQ_E_DTYPE, "lora_matmul: x_dtype");
   if (!act_dtype(ab_dtype)) return fail(ctx, RLXQ_E_DTYPE, "lora_matmul: ab_dtype");
@@ -88,18 +88,55 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   g.R = (int32_t)rank;
   g.E = (int32_t)num_adapters;
   g.S = (int32_t)segs;
-  g.x_bf16 = x_dtype == RLXQ_BF16;
-  g.ab_bf16 = ab_dtype == RLXQ_BF16;
-  g.y_bf16 = y_dtype == RLXQ_BF16;
-  const int64_t shrink = (m * segs * rank + 3) / 4, expand = (m * n + 255) / 256;
+  const bool xb = x_dtype == RLXQ_BF16, ab = ab_dtype == RLXQ_BF16, yb = y_dtype == RLXQ_BF16;
+  const bool many = m > RLXQ_LORA_FEW;
+  const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
+  const int64_t per = yb ? 8 : 4;   // elements of 16 bytes
+  g.vec = n % per == 0 && aligned(base, 16) && aligned(y, 16);
+  for (int64_t i = 0; i < segs; i++) g.vec = g.vec && g.ends[i] % per == 0;
+  g.copy = base != y;
+  // tiles: a row each may lead one of 16, or whole tiles of 64 and one more for
+  // each adapter (and for the rows without one)
+  const int64_t used = std::min<int64_t>(num_adapters, m);
+  const int64_t tiles = many ? m / 64 + std::min<int64_t>(num_adapters + 1, m) : m;
+  g.max_tiles = (int32_t)tiles;
+  // v: slices of K until there are two workgroups a CU, of 512 elements at least
+  const int64_t sr = segs * rank;
+  g.jblocks = (int32_t)((sr + (many ? 63 : 15)) / (many ? 64 : 16));
+  const int64_t likely = (many ? (m + 31) / 32 : used) * g.jblocks;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * cus / likely, k / 512));
+  g.kslice = (int32_t)(((k + want - 1) / want + 127) / 128 * 128);
+  g.splits = (int32_t)((k + g.kslice - 1) / g.kslice);
+  // y: 256 columns a workgroup, or up to 1024 while there are four workgroups a CU
+  const int64_t rows_wgs = many ? (m + 63) / 64 : used;
+  g.cols = 256;
+  while (g.cols < 1024 && rows_wgs * (n / (2 * g.cols)) >= 4 * cus) g.cols *= 2;
+  int64_t cb = 0;
+  for (int64_t i = 0; i < segs; i++) {
+    g.cfirst[i] = (int32_t)cb;
+    cb += (g.ends[i] - (i ? g.ends[i - 1] : 0) + g.cols - 1) / g.cols;
+  }
+  g.cblocks = (int32_t)cb;
+  const int64_t shrink = tiles * (many ? 2 : 1) * g.jblocks * g.splits, expand = tiles * cb;
   if (!grid_fits(shrink, 256) || !grid_fits(expand, 256))
     return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: m, n and rank need a launch of 2^32 work-items or more");
+  const size_t b_v = ((size_t)(g.splits * m * sr) * 4 + 255) & ~(size_t)255;
+  const size_t b_tiles = many ? (size_t)tiles * sizeof(rlxq_lora_tile) : 0;
   void* ws = nullptr;
-  int rc = workspace(ctx, (size_t)(m * segs * rank) * 4, &ws, stream);
+  int rc = workspace(ctx, b_v + b_tiles + (many ? (size_t)m * 4 : 0), &ws, stream);
   if (rc) return rc;
   g.v = static_cast<float*>(ws);
-  if ((rc = run_kernel(ctx, "rlxq_lora_shrink", shrink, 256, 0, &g, stream))) return rc;
-  return run_kernel(ctx, "rlxq_lora_expand", expand, 256, 0, &g, stream);
+  g.tiles = reinterpret_cast<rlxq_lora_tile*>(static_cast<char*>(ws) + b_v);
+  g.order = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + b_v + b_tiles);
+  static const char* const kDt[2] = {"f32", "bf16"};
+  const char* size = many ? "many" : "few";
+  char name[48];
+  if (many && (rc = run_kernel(ctx, "rlxq_lora_sort", 1, 1024, (size_t)(num_adapters + 1) * 4, &g, stream))) return rc;
+  std::snprintf(name, sizeof name, "rlxq_lora_shrink_%s_%s_%s", kDt[xb], kDt[ab], size);
+  if ((rc = run_kernel(ctx, name, shrink, 256, 0, &g, stream))) return rc;
+  const size_t pieces = ab && !yb ? 3 : 2;   // of v, a lane (lr_expand)
+  std::snprintf(name, sizeof name, "rlxq_lora_expand_%s_%s_%s", kDt[ab], kDt[yb], size);
+  return run_kernel(ctx, name, expand, 256, (size_t)((rank + 31) / 32) * (many ? 4 : 1) * pieces * 1024, &g, stream);
 }
 
 int rlxq_residual_norm(rlxq_ctx* ctx, const void* block, int block_dtype, const void* resid, int resid_dtype,

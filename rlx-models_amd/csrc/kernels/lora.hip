@@ -1,15 +1,29 @@
 // Low-rank adapters of many requests beside a shared projection:
 //   y[i, n] = base[i, n] + s[e] sum_{r < rank[e]} B[e, n, r] v[i, g(n), r],
 //   v[i, g, r] = sum_k A[e, g R + r, k] x[i, k],   e = ids[i],
-// g(n) the segment of column n.  v stays f32.
+// g(n) the segment of column n.
+//
+// Rows of one adapter are taken together, in tiles: up to RLXQ_LORA_FEW rows
+// every workgroup finds its tile of 16 among the ids itself (a launch less), for
+// more a launch of one workgroup sorts the rows and cuts them into tiles of 64.
+// Two launches then: v (K over the waves of a workgroup and, where the
+// workgroups would be few, over workgroups), then y.  Both put the adapter's rows
+// on the long side of a 16x16 MFMA tile and the activation rows on the other, so
+// the results of one activation row lie on one lane: v leaves as 16-byte pieces,
+// y's columns are dealt to the tiles so that a lane holds 16 neighbouring ones.
+//
+// Types: x and A both bf16 use the bf16 MFMA; otherwise the f32 one, on the
+// values as they are.  v stays f32; against bf16 B it takes part as bf16 terms,
+// three (all of its bits) for f32 y, two (2^-17 of it at most left out) for bf16
+// y, whose own rounding is 2^-9.  Sums are f32, y is rounded once.
 #include "common.hip.h"
 #include "lora_args.h"
 
 namespace rlxq {
 
-RLXQ_DEV float lr_ld(const void* p, int bf16, int64_t i) {
-  return bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[i]) : reinterpret_cast<const float*>(p)[i];
-}
+typedef float lr_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 lr_bf8 __attribute__((ext_vector_type(8)));
+
 // Rank of adapter e: what lies past it in A and B is never multiplied.
 RLXQ_DEV int lr_rank(const rlxq_lora_args& a, int e) {
   if (!a.ranks) return a.R;
@@ -17,45 +31,425 @@ RLXQ_DEV int lr_rank(const rlxq_lora_args& a, int e) {
   return r < 0 ? 0 : (r > a.R ? a.R : r);
 }
 
+// Eight neighbouring elements: as loaded (bf16), or as floats.
+template <bool BF>
+struct LrFrag {
+  uint4 q[BF ? 1 : 2];
+};
+template <bool BF>
+RLXQ_DEV LrFrag<BF> lr_zero() {
+  LrFrag<BF> f;
+  f.q[0] = make_uint4(0, 0, 0, 0);
+  if constexpr (!BF) f.q[1] = f.q[0];
+  return f;
+}
+// From element i of p, of type bf16 (MEM) or f32, as BF.
+template <bool BF, bool MEM>
+RLXQ_DEV LrFrag<BF> lr_load(const void* p, int64_t i) {
+  static_assert(MEM || !BF, "no rounding here");
+  LrFrag<BF> f;
+  const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + i * (MEM ? 2 : 4));
+  f.q[0] = s[0];
+  if constexpr (!MEM) {
+    f.q[1] = s[1];
+  } else if constexpr (!BF) {
+    const uint4 w = f.q[0];
+    f.q[0] = make_uint4(w.x << 16, w.x & 0xffff0000u, w.y << 16, w.y & 0xffff0000u);
+    f.q[1] = make_uint4(w.z << 16, w.z & 0xffff0000u, w.w << 16, w.w & 0xffff0000u);
+  }
+  return f;
+}
+// The first n of the eight, the others zero.
+template <bool BF>
+RLXQ_DEV void lr_keep(LrFrag<BF>& f, int n) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(f.q);
+#pragma unroll
+  for (int j = 0; j < (BF ? 4 : 8); j++) {
+    if (BF) w[j] = n >= 2 * j + 2 ? w[j] : (n == 2 * j + 1 ? w[j] & 0xffffu : 0u);
+    else w[j] = n > j ? w[j] : 0u;
+  }
+}
+// acc += the products of 32 k: lane l holds row (a) or column (b) l % 16, k 8 (l /
+// 16) .. + 7 of them.  The f32 MFMA takes four k at a time; which four is the same
+// on both sides.
+template <bool BF>
+RLXQ_DEV lr_f4 lr_mfma(const LrFrag<BF>& a, const LrFrag<BF>& b, lr_f4 acc) {
+  if constexpr (BF) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lr_bf8, a.q[0]), __builtin_bit_cast(lr_bf8, b.q[0]), acc,
+                                                   0, 0, 0);
+  } else {
+    const float* x = reinterpret_cast<const float*>(a.q);
+    const float* y = reinterpret_cast<const float*>(b.q);
+#pragma unroll
+    for (int j = 0; j < 8; j++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], acc, 0, 0, 0);
+    return acc;
+  }
+}
+
+constexpr int kLrThreads = 256;
+
+// Tile `index`: its rows into LDS, its adapter (-1: none) and number.  False:
+// there is no such tile.  Every thread of the workgroup calls it.
+template <bool LIST>
+RLXQ_DEV bool lr_tile(const rlxq_lora_args& a, int index, int* rows, uint64_t* masks, int& e, int& count) {
+  const int t = threadIdx.x;
+  if constexpr (LIST) {
+    const rlxq_lora_tile tile = a.tiles[index];
+    e = tile.e, count = tile.count;
+    if (count <= 0) return false;
+    if (t < count) rows[t] = a.order[tile.start + t];
+  } else {
+    // row `index` leads a tile if the rows of its adapter ahead of it fill whole ones
+    e = a.ids[index];
+    e = e >= 0 && e < a.E ? e : -1;
+    int mine = t < a.M ? a.ids[t] : -2;
+    if (t < a.M) mine = mine >= 0 && mine < a.E ? mine : -1;
+    const uint64_t m = __ballot(mine == e);
+    if ((t & 63) == 0) masks[t >> 6] = m;
+    __syncthreads();
+    int lead = 0, ahead = 0, all = 0;
+    for (int w = 0; w < kLrThreads / 64; w++) {
+      const uint64_t q = masks[w];
+      const int n = __popcll(q);
+      lead += w < index >> 6 ? n : (w == index >> 6 ? __popcll(q & ((1ull << (index & 63)) - 1)) : 0);
+      ahead += w < t >> 6 ? n : (w == t >> 6 ? __popcll(q & ((1ull << (t & 63)) - 1)) : 0);
+      all += n;
+    }
+    if (lead & 15) return false;
+    count = all - lead < 16 ? all - lead : 16;
+    if (mine == e && ahead >= lead && ahead < lead + 16) rows[ahead - lead] = t;
+  }
+  __syncthreads();
+  return true;
+}
+
+// v of 16 FR rows and 16 RT rows of A, one slice of K: the waves take a quarter
+// of it each and join their sums in LDS.
+template <bool XB, bool AB, bool LIST, int FR, int RT>
+RLXQ_DEV void lr_shrink(const rlxq_lora_args& a) {
+  constexpr bool BF = XB && AB;
+  __shared__ int rows[64];
+  __shared__ uint64_t masks[4];
+  __shared__ lr_f4 part[4][RT * FR][64];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int sub = LIST ? 64 / (16 * FR) : 1;   // workgroups over a tile's rows
+  int b = blockIdx.x;
+  const int split = b % a.splits;
+  b /= a.splits;
+  const int jb = b % a.jblocks;
+  b /= a.jblocks;
+  int e, count;
+  if (!lr_tile<LIST>(a, b / sub, rows, masks, e, count) || e < 0) return;
+  const int r0 = (b % sub) * 16 * FR, sr = a.S * a.R, j0 = jb * 16 * RT;
+  if (r0 >= count) return;
+  const int rank = lr_rank(a, e), col = lane & 15, kk = 8 * (lane >> 4);
+  int64_t xrow[FR], arow[RT];
+  bool xon[FR], aon[RT];
+#pragma unroll
+  for (int f = 0; f < FR; f++) {
+    xon[f] = r0 + 16 * f + col < count;
+    xrow[f] = xon[f] ? (int64_t)rows[r0 + 16 * f + col] * a.K : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < RT; j++) {
+    const int row = j0 + 16 * j + col;
+    aon[j] = row < sr && row % a.R < rank;
+    arow[j] = ((int64_t)e * sr + (aon[j] ? row : 0)) * a.K;
+  }
+  const int64_t k0 = (int64_t)split * a.kslice, k_end = k0 + a.kslice < a.K ? k0 + a.kslice : a.K;
+  const int64_t quarter = (a.kslice / 4 + 31) / 32 * 32;
+  const int64_t w0 = k0 + wave * quarter, w1 = w0 + quarter < k_end ? w0 + quarter : k_end;
+  lr_f4 acc[RT][FR];
+#pragma unroll
+  for (int j = 0; j < RT; j++)
+#pragma unroll
+    for (int f = 0; f < FR; f++) acc[j][f] = (lr_f4){0.f, 0.f, 0.f, 0.f};
+  constexpr int U = FR * RT == 1 ? 4 : 2;   // steps of 32 whose loads are on their way together
+  for (int64_t k = w0; k < w1; k += 32 * U) {
+    LrFrag<BF> xf[U][FR], af[U][RT];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int64_t at = k + 32 * u + kk;
+      const bool in = at < w1;   // (K is whole eights)
+#pragma unroll
+      for (int f = 0; f < FR; f++) xf[u][f] = in && xon[f] ? lr_load<BF, XB>(a.x, xrow[f] + at) : lr_zero<BF>();
+#pragma unroll
+      for (int j = 0; j < RT; j++) af[u][j] = in && aon[j] ? lr_load<BF, AB>(a.a, arow[j] + at) : lr_zero<BF>();
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int j = 0; j < RT; j++)
+#pragma unroll
+        for (int f = 0; f < FR; f++) acc[j][f] = lr_mfma<BF>(af[u][j], xf[u][f], acc[j][f]);
+  }
+#pragma unroll
+  for (int j = 0; j < RT; j++)
+#pragma unroll
+    for (int f = 0; f < FR; f++) part[wave][j * FR + f][lane] = acc[j][f];
+  __syncthreads();
+  // (lane: row 16 f + lane % 16 of the tile, rows 16 j + 4 (lane / 16) .. + 3 of A)
+  for (int i = wave; i < RT * FR; i += 4) {
+    const int row = r0 + 16 * (i % FR) + col, j = j0 + 16 * (i / FR) + 4 * (lane >> 4);
+    if (row >= count || j >= sr) continue;
+    const lr_f4 s = (part[0][i][lane] + part[1][i][lane]) + (part[2][i][lane] + part[3][i][lane]);
+    *reinterpret_cast<lr_f4*>(a.v + ((int64_t)split * a.M + rows[row]) * sr + j) = s;
+  }
+}
+
+// bf16 terms of eight floats: what the terms before it leave, rounded.
+RLXQ_DEV uint4 lr_term(float* v) {
+  uint4 q;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+    v[2 * j] -= __uint_as_float(w[j] << 16);
+    v[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
+  }
+  return q;
+}
+
+// y of 16 FR rows and a.cols columns of one segment.  A wave takes 64 columns at a
+// time as four tiles: tile q's row p is column 16 (p / 4) + 4 q + p % 4 of them,
+// so a lane has 16 neighbouring columns of its activation row.  v lies in LDS as
+// the MFMA takes it, made once for the workgroup.
+template <bool BB, bool YB, bool LIST, int FR>
+RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
+  constexpr int NT = BB ? (YB ? 2 : 3) : 2;   // 16-byte pieces of v a lane and 32 k (f32: the eight floats)
+  extern __shared__ uint4 lds[];              // [steps][FR][NT][64]
+  __shared__ int rows[64];
+  __shared__ uint64_t masks[4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int cb = blockIdx.x % a.cblocks;
+  int e, count;
+  if (!lr_tile<LIST>(a, blockIdx.x / a.cblocks, rows, masks, e, count)) return;
+  int seg = 0;
+  while (seg + 1 < a.S && cb >= a.cfirst[seg + 1]) seg++;
+  const int64_t c0 = (seg ? a.ends[seg - 1] : 0) + (int64_t)(cb - a.cfirst[seg]) * a.cols;
+  const int64_t c1 = c0 + a.cols < a.ends[seg] ? c0 + a.cols : a.ends[seg];
+  if (e < 0) {   // base's bits
+    if (!a.copy) return;
+    const int es = YB ? 2 : 4, per = a.vec ? 16 / es : 1, n = (int)(c1 - c0) / per;
+    for (int i = t; i < count * n; i += kLrThreads) {
+      const int64_t o = (int64_t)rows[i / n] * a.N + c0 + (int64_t)(i % n) * per;
+      if (a.vec)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + o * es) =
+            a.base ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.base) + o * es) : make_uint4(0, 0, 0, 0);
+      else if (YB)
+        reinterpret_cast<uint16_t*>(a.y)[o] = a.base ? reinterpret_cast<const uint16_t*>(a.base)[o] : 0;
+      else
+        reinterpret_cast<uint32_t*>(a.y)[o] = a.base ? reinterpret_cast<const uint32_t*>(a.base)[o] : 0;
+    }
+    return;
+  }
+  const int rank = lr_rank(a, e), steps = (rank + 31) / 32, sr = a.S * a.R;
+  const float scale = a.scales ? a.scales[e] : 1.0f;
+  for (int i = t; i < steps * FR * 64; i += kLrThreads) {
+    const int l = i & 63, f = (i >> 6) % FR, s = (i >> 6) / FR, r = 32 * s + 8 * (l >> 4), row = 16 * f + (l & 15);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = 0.f;
+    if (row < count && r < rank) {
+      const float* p = a.v + (int64_t)rows[row] * sr + seg * a.R + r;
+      for (int q = 0; q < a.splits; q++, p += a.M * sr) {
+        const float4 lo = reinterpret_cast<const float4*>(p)[0], hi = reinterpret_cast<const float4*>(p)[1];
+        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+        v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = r + j < rank ? v[j] * scale : 0.f;
+    }
+    uint4* d = lds + (int64_t)(s * FR + f) * NT * 64 + l;
+    if constexpr (BB) {
+#pragma unroll
+      for (int q = 0; q < NT; q++) d[q * 64] = lr_term(v);
+    } else {
+      d[0] = __builtin_bit_cast(uint4, make_float4(v[0], v[1], v[2], v[3]));
+      d[64] = __builtin_bit_cast(uint4, make_float4(v[4], v[5], v[6], v[7]));
+    }
+  }
+  __syncthreads();
+  const int col = lane & 15, kk = 8 * (lane >> 4), frags = (count + 15) / 16;
+  int64_t yrow[FR];
+  bool on[FR];
+#pragma unroll
+  for (int f = 0; f < FR; f++) {
+    on[f] = 16 * f + col < count;
+    yrow[f] = on[f] ? (int64_t)rows[16 * f + col] * a.N : 0;
+  }
+  for (int64_t c = c0 + 64 * wave; c < c1; c += 64 * (kLrThreads / 64)) {
+    const int64_t mine = c + 16 * (lane >> 4);   // this lane's 16 columns
+    const int width = mine < c1 ? (int)(c1 - mine < 16 ? c1 - mine : 16) : 0;
+    lr_f4 acc[4][FR];
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+      for (int f = 0; f < FR; f++) acc[q][f] = (lr_f4){0.f, 0.f, 0.f, 0.f};
+    // base, ahead of the products
+    constexpr int P = YB ? 2 : 4;   // 16-byte pieces of 16 columns
+    uint4 bq[FR][P];
+    const bool whole = a.vec && width == 16;
+#pragma unroll
+    for (int f = 0; f < FR; f++)
+#pragma unroll
+      for (int p = 0; p < P; p++) {
+        bq[f][p] = make_uint4(0, 0, 0, 0);
+        if (a.base && whole && on[f])
+          bq[f][p] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.base) + (yrow[f] + mine) * (YB ? 2 : 4))[p];
+      }
+    int64_t brow[4];
+    bool bon[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int64_t n = c + 16 * (col >> 2) + 4 * q + (col & 3);
+      bon[q] = n < c1;
+      brow[q] = ((int64_t)e * a.N + (bon[q] ? n : c0)) * a.R;
+    }
+    for (int s = 0; s < steps; s++) {
+      const int r = 32 * s + kk;
+      LrFrag<BB> bf[4];
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        bf[q] = bon[q] && r < rank ? lr_load<BB, BB>(a.b, brow[q] + r) : lr_zero<BB>();
+        if (rank - r < 8) lr_keep<BB>(bf[q], rank - r);
+      }
+#pragma unroll
+      for (int f = 0; f < FR; f++) {
+        if (f >= frags) break;
+        const uint4* d = lds + (int64_t)(s * FR + f) * NT * 64 + lane;
+        if constexpr (BB) {
+#pragma unroll
+          for (int w = 0; w < NT; w++) {
+            LrFrag<BB> vf;
+            vf.q[0] = d[w * 64];
+#pragma unroll
+            for (int q = 0; q < 4; q++) acc[q][f] = lr_mfma<BB>(bf[q], vf, acc[q][f]);
+          }
+        } else {
+          LrFrag<BB> vf;
+          vf.q[0] = d[0];
+          vf.q[1] = d[64];
+#pragma unroll
+          for (int q = 0; q < 4; q++) acc[q][f] = lr_mfma<BB>(bf[q], vf, acc[q][f]);
+        }
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < FR; f++) {
+      if (!on[f] || width == 0) continue;
+      if (whole) {
+        uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + (yrow[f] + mine) * (YB ? 2 : 4));
+        if constexpr (YB) {
+#pragma unroll
+          for (int p = 0; p < 2; p++) {
+            const uint32_t w[4] = {bq[f][p].x, bq[f][p].y, bq[f][p].z, bq[f][p].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const int at = 8 * p + 2 * j;   // column of the lane's 16: tile at / 4, its row at % 4
+              o[j] = pack_bf16x2(__uint_as_float(w[j] << 16) + acc[at >> 2][f][at & 3],
+                                 __uint_as_float(w[j] & 0xffff0000u) + acc[at >> 2][f][(at & 3) + 1]);
+            }
+            d[p] = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < 4; p++) {
+            const float4 w = __builtin_bit_cast(float4, bq[f][p]);
+            d[p] = __builtin_bit_cast(uint4, make_float4(w.x + acc[p][f][0], w.y + acc[p][f][1], w.z + acc[p][f][2],
+                                                         w.w + acc[p][f][3]));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          if (j >= width) continue;
+          const int64_t o = yrow[f] + mine + j;
+          const float s = acc[j >> 2][f][j & 3];
+          if constexpr (YB) {
+            const float w = a.base ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.base)[o]) : 0.f;
+            reinterpret_cast<uint16_t*>(a.y)[o] = (uint16_t)f32_to_bf16_bits(w + s);
+          } else {
+            const float w = a.base ? reinterpret_cast<const float*>(a.base)[o] : 0.f;
+            reinterpret_cast<float*>(a.y)[o] = w + s;
+          }
+        }
+      }
+    }
+  }
+}
+
 }  // namespace rlxq
 
 using namespace rlxq;
 
-// v: a wave per row and row of A.
-extern "C" __global__ __launch_bounds__(256) void rlxq_lora_shrink(rlxq_lora_args a) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), sr = (int64_t)a.S * a.R;
-  if (w >= a.M * sr) return;
-  const int64_t i = w / sr, j = w - i * sr;
-  const int e = a.ids[i];
-  if (e < 0 || e >= a.E || (int)(j % a.R) >= lr_rank(a, e)) return;
-  float s = 0.f;
-  for (int64_t k = threadIdx.x & 63; k < a.K; k += 64)
-    s = __fmaf_rn(lr_ld(a.x, a.x_bf16, i * a.K + k), lr_ld(a.a, a.ab_bf16, (e * sr + j) * a.K + k), s);
-  s = group_sum<64>(s);
-  if ((threadIdx.x & 63) == 0) a.v[w] = a.scales ? s * a.scales[e] : s;
+// The rows by adapter (those without one last), cut into tiles of up to 64: one
+// workgroup; LDS holds a counter for each adapter.  The order of an adapter's
+// rows is that of the counters' atomics; no result depends on it.
+extern "C" __global__ __launch_bounds__(1024) void rlxq_lora_sort(rlxq_lora_args a) {
+  extern __shared__ int count[];   // [E + 1]: rows, then where the next one goes
+  __shared__ int red[2][16];
+  const int t = threadIdx.x, n = a.E + 1;
+  for (int e = t; e < n; e += 1024) count[e] = 0;
+  __syncthreads();
+  for (int64_t i = t; i < a.M; i += 1024) {
+    const int e = a.ids[i];
+    atomicAdd(&count[e >= 0 && e < a.E ? e : a.E], 1);
+  }
+  __syncthreads();
+  // a run of adapters a thread: rows and tiles ahead of it
+  const int per = (n + 1023) / 1024, lo = t * per, hi = lo + per < n ? lo + per : n;
+  int rows = 0, tiles = 0;
+  for (int e = lo; e < hi; e++) rows += count[e], tiles += (count[e] + 63) / 64;
+  int ri = rows, ti = tiles;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int ro = __shfl_up(ri, off, 64), to = __shfl_up(ti, off, 64);
+    if ((t & 63) >= off) ri += ro, ti += to;
+  }
+  if ((t & 63) == 63) red[0][t >> 6] = ri, red[1][t >> 6] = ti;
+  __syncthreads();
+  int all = 0;
+  for (int w = 0; w < 16; w++) {
+    if (w < t >> 6) ri += red[0][w], ti += red[1][w];
+    all += red[1][w];
+  }
+  int start = ri - rows, tile = ti - tiles;
+  for (int e = lo; e < hi; e++) {
+    const int c = count[e];
+    for (int at = 0; at < c; at += 64) a.tiles[tile++] = {e < a.E ? e : -1, start + at, c - at < 64 ? c - at : 64, 0};
+    count[e] = start;
+    start += c;
+  }
+  for (int i = all + t; i < a.max_tiles; i += 1024) a.tiles[i] = {-1, 0, 0, 0};
+  __syncthreads();
+  for (int64_t i = t; i < a.M; i += 1024) {
+    const int e = a.ids[i];
+    a.order[atomicAdd(&count[e >= 0 && e < a.E ? e : a.E], 1)] = (int)i;
+  }
 }
 
-// y: a thread per output.
-extern "C" __global__ __launch_bounds__(256) void rlxq_lora_expand(rlxq_lora_args a) {
-  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (o >= a.M * a.N) return;
-  const int64_t i = o / a.N, n = o - i * a.N;
-  const int e = a.ids[i];
-  float s = a.base ? lr_ld(a.base, a.y_bf16, o) : 0.f;
-  if (e < 0 || e >= a.E) {   // base's bits
-    if (a.y_bf16) reinterpret_cast<uint16_t*>(a.y)[o] = a.base ? reinterpret_cast<const uint16_t*>(a.base)[o] : 0;
-    else reinterpret_cast<float*>(a.y)[o] = s;
-    return;
+// _few: tiles of 16 rows that every workgroup finds; _many: of 64 from the list
+#define RLXQ_LORA_SHRINK(X, A, xn, an)                                                                                  \
+  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_shrink_##xn##_##an##_few(rlxq_lora_args a) {                \
+    lr_shrink<X, A, false, 1, 1>(a);                                                                                    \
+  }                                                                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_shrink_##xn##_##an##_many(rlxq_lora_args a) {               \
+    lr_shrink<X, A, true, 2, 4>(a);                                                                                     \
   }
-  {
-    int g = 0;
-    while (n >= a.ends[g]) g++;
-    const float* v = a.v + (i * a.S + g) * a.R;
-    const int rank = lr_rank(a, e);
-    float d = 0.f;
-    for (int r = 0; r < rank; r++) d = __fmaf_rn(v[r], lr_ld(a.b, a.ab_bf16, ((int64_t)e * a.N + n) * a.R + r), d);
-    s += d;
+RLXQ_LORA_SHRINK(true, true, bf16, bf16)
+RLXQ_LORA_SHRINK(true, false, bf16, f32)
+RLXQ_LORA_SHRINK(false, true, f32, bf16)
+RLXQ_LORA_SHRINK(false, false, f32, f32)
+#define RLXQ_LORA_EXPAND(B, Y, bn, yn)                                                                                  \
+  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_expand_##bn##_##yn##_few(rlxq_lora_args a) {                \
+    lr_expand<B, Y, false, 1>(a);                                                                                       \
+  }                                                                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_expand_##bn##_##yn##_many(rlxq_lora_args a) {               \
+    lr_expand<B, Y, true, 4>(a);                                                                                        \
   }
-  if (a.y_bf16) reinterpret_cast<uint16_t*>(a.y)[o] = (uint16_t)f32_to_bf16_bits(s);
-  else reinterpret_cast<float*>(a.y)[o] = s;
-}
+RLXQ_LORA_EXPAND(true, true, bf16, bf16)
+RLXQ_LORA_EXPAND(true, false, bf16, f32)
+RLXQ_LORA_EXPAND(false, true, f32, bf16)
+RLXQ_LORA_EXPAND(false, false, f32, f32)

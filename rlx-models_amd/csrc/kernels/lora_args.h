@@ -4,7 +4,17 @@
 #define RLXQ_LORA_ARGS_H
 #include <stdint.h>
 
-#define RLXQ_LORA_SEGS 4   /* most column segments of a call */
+#define RLXQ_LORA_SEGS 4           /* most column segments of a call            */
+#define RLXQ_LORA_MAX_RANK 256
+#define RLXQ_LORA_MAX_ADAPTERS 16384
+#define RLXQ_LORA_FEW 256          /* rows whose tiles every workgroup finds    */
+
+/* Rows of one adapter that a workgroup takes together (prompts). */
+typedef struct rlxq_lora_tile {
+  int32_t e;               /* adapter, or -1: rows without one                */
+  int32_t start, count;    /* order[start .. start + count)                   */
+  int32_t pad;
+} rlxq_lora_tile;
 
 typedef struct rlxq_lora_args {
   const void* x;           /* [M, K]                                          */
@@ -15,11 +25,19 @@ typedef struct rlxq_lora_args {
   const float* scales;     /* [E], or NULL (1)                                */
   const void* base;        /* [M, N], or NULL (zero)                          */
   void* y;                 /* [M, N]                                          */
-  float* v;                /* [M, S * R]: scale * (A x)                       */
+  float* v;                /* [splits, M, S * R]: A x, by slice of K          */
+  int32_t* order;          /* [M]: rows by adapter (M > RLXQ_LORA_FEW)        */
+  rlxq_lora_tile* tiles;   /* [max_tiles], unused ones with count 0           */
   int64_t M, K, N;
   int32_t R, E, S;
-  int32_t x_bf16, ab_bf16, y_bf16;
-  int64_t ends[RLXQ_LORA_SEGS];   /* column ends of the segments (the last N) */
+  int32_t splits, kslice;  /* slices of K, a multiple of 32 each              */
+  int32_t jblocks;         /* shrink: workgroups over S * R                   */
+  int32_t cols, cblocks;   /* expand: columns a workgroup, workgroups over N  */
+  int32_t max_tiles;
+  int32_t vec;             /* base, y and the segments allow 16-byte accesses */
+  int32_t copy;            /* rows without an adapter are base's: copied      */
+  int64_t ends[RLXQ_LORA_SEGS];    /* column ends of the segments (the last N) */
+  int32_t cfirst[RLXQ_LORA_SEGS];  /* expand: first workgroup of a segment    */
 } rlxq_lora_args;
 
 #endif

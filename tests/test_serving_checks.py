@@ -140,7 +140,7 @@ REFUSED = [
     (_lora, dict(m=2 ** 62), "E_SHAPE"), (_lora, dict(n=2 ** 62), "E_SHAPE"), (_lora, dict(k=2 ** 62), "E_SHAPE"),
     (_lora, dict(m=2 ** 24, n=2 ** 24), "E_SHAPE"),
     (_lora, dict(rank=0), "E_SHAPE"), (_lora, dict(rank=12), "E_SHAPE"), (_lora, dict(rank=264), "E_SHAPE"), (_lora, dict(e=0), "E_SHAPE"),
-    (_lora, dict(e=2 ** 20 + 1), "E_SHAPE"), (_lora, dict(k=60), "E_ALIGN"), (_lora, dict(x_dtype=2), "E_DTYPE"),
+    (_lora, dict(e=2 ** 14 + 1), "E_SHAPE"), (_lora, dict(k=60), "E_ALIGN"), (_lora, dict(x_dtype=2), "E_DTYPE"),
     (_lora, dict(ab=2), "E_DTYPE"), (_lora, dict(y_dtype=7), "E_DTYPE"), (_lora, dict(segs=2), "E_NULL"), (_lora, dict(segs=0), "E_NULL"),
     (_lora, dict(ends=[32], segs=0), "E_SHAPE"), (_lora, dict(ends=[8, 16, 20, 24, 32], segs=5), "E_SHAPE"),
     (_lora, dict(ends=[31], segs=1), "E_SHAPE"), (_lora, dict(ends=[33], segs=1), "E_SHAPE"), (_lora, dict(ends=[-1, 32], segs=2), "E_SHAPE"),

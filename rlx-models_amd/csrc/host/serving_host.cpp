@@ -95,20 +95,20 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   g.vec = n % per == 0 && aligned(base, 16) && aligned(y, 16);
   for (int64_t i = 0; i < segs; i++) g.vec = g.vec && g.ends[i] % per == 0;
   g.copy = base != y;
-  // tiles: a row each may lead one of 16, or whole tiles of 64 and one more for
+  // tiles: a row each may lead one of 16, or whole tiles from the list and one more for
   // each adapter (and for the rows without one)
   const int64_t used = std::min<int64_t>(num_adapters, m);
-  const int64_t tiles = many ? m / 64 + std::min<int64_t>(num_adapters + 1, m) : m;
+  const int64_t tiles = many ? m / RLXQ_LORA_ROWS + std::min<int64_t>(num_adapters + 1, m) : m;
   g.max_tiles = (int32_t)tiles;
   // v: slices of K until there are two workgroups a CU, of 512 elements at least
   const int64_t sr = segs * rank;
   g.jblocks = (int32_t)((sr + (many ? 63 : 15)) / (many ? 64 : 16));
-  const int64_t likely = (many ? (m + 31) / 32 : used) * g.jblocks;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * cus / likely, k / 512));
+  const int64_t rows_wgs = many ? (m + RLXQ_LORA_ROWS - 1) / RLXQ_LORA_ROWS : used;
+  const int64_t likely = rows_wgs * g.jblocks;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((many ? 2 : 6) * cus / likely, k / 512));
   g.kslice = (int32_t)(((k + want - 1) / want + 127) / 128 * 128);
   g.splits = (int32_t)((k + g.kslice - 1) / g.kslice);
   // y: 256 columns a workgroup, or up to 1024 while there are four workgroups a CU
-  const int64_t rows_wgs = many ? (m + 63) / 64 : used;
   g.cols = 256;
   while (g.cols < 1024 && rows_wgs * (n / (2 * g.cols)) >= 4 * cus) g.cols *= 2;
   int64_t cb = 0;
@@ -117,7 +117,7 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
     cb += (g.ends[i] - (i ? g.ends[i - 1] : 0) + g.cols - 1) / g.cols;
   }
   g.cblocks = (int32_t)cb;
-  const int64_t shrink = tiles * (many ? 2 : 1) * g.jblocks * g.splits, expand = tiles * cb;
+  const int64_t shrink = tiles * g.jblocks * g.splits, expand = tiles * cb;
   if (!grid_fits(shrink, 256) || !grid_fits(expand, 256))
     return fail(ctx, RLXQ_E_SHAPE, "lora_matmul: m, n and rank need a launch of 2^32 work-items or more");
   const size_t b_v = ((size_t)(g.splits * m * sr) * 4 + 255) & ~(size_t)255;
@@ -135,8 +135,9 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   std::snprintf(name, sizeof name, "rlxq_lora_shrink_%s_%s_%s", kDt[xb], kDt[ab], size);
   if ((rc = run_kernel(ctx, name, shrink, 256, 0, &g, stream))) return rc;
   const size_t pieces = ab && !yb ? 3 : 2;   // of v, a lane (lr_expand)
-  std::snprintf(name, sizeof name, "rlxq_lora_expand_%s_%s_%s", kDt[ab], kDt[yb], size);
-  return run_kernel(ctx, name, expand, 256, (size_t)((rank + 31) / 32) * (many ? 4 : 1) * pieces * 1024, &g, stream);
+  const int steps = rank <= 32 ? 1 : (rank <= 64 ? 2 : (rank <= 128 ? 4 : 8));
+  std::snprintf(name, sizeof name, "rlxq_lora_expand_%s_%s_%s_s%d", kDt[ab], kDt[yb], size, steps);
+  return run_kernel(ctx, name, expand, 256, (size_t)((rank + 31) / 32) * (many ? RLXQ_LORA_ROWS / 16 : 1) * pieces * 1024, &g, stream);
 }
 
 int rlxq_residual_norm(rlxq_ctx* ctx, const void* block, int block_dtype, const void* resid, int resid_dtype,

@@ -87,6 +87,7 @@ RLXQ_DEV lr_f4 lr_mfma(const LrFrag<BF>& a, const LrFrag<BF>& b, lr_f4 acc) {
 }
 
 constexpr int kLrThreads = 256;
+constexpr int kLrFrags = RLXQ_LORA_ROWS / 16;   // of a tile from the list
 
 // Tile `index`: its rows into LDS, its adapter (-1: none) and number.  False:
 // there is no such tile.  Every thread of the workgroup calls it.
@@ -128,27 +129,22 @@ RLXQ_DEV bool lr_tile(const rlxq_lora_args& a, int index, int* rows, uint64_t* m
 template <bool XB, bool AB, bool LIST, int FR, int RT>
 RLXQ_DEV void lr_shrink(const rlxq_lora_args& a) {
   constexpr bool BF = XB && AB;
-  __shared__ int rows[64];
+  __shared__ int rows[RLXQ_LORA_ROWS];
   __shared__ uint64_t masks[4];
   __shared__ lr_f4 part[4][RT * FR][64];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int sub = LIST ? 64 / (16 * FR) : 1;   // workgroups over a tile's rows
-  int b = blockIdx.x;
-  const int split = b % a.splits;
-  b /= a.splits;
-  const int jb = b % a.jblocks;
-  b /= a.jblocks;
+  static_assert(FR == (LIST ? kLrFrags : 1), "a workgroup takes a whole tile");
   int e, count;
-  if (!lr_tile<LIST>(a, b / sub, rows, masks, e, count) || e < 0) return;
-  const int r0 = (b % sub) * 16 * FR, sr = a.S * a.R, j0 = jb * 16 * RT;
-  if (r0 >= count) return;
+  if (!lr_tile<LIST>(a, blockIdx.x / (a.jblocks * a.splits), rows, masks, e, count) || e < 0) return;
+  const int other = blockIdx.x % (a.jblocks * a.splits);
+  const int split = other % a.splits, sr = a.S * a.R, j0 = other / a.splits * 16 * RT;
   const int rank = lr_rank(a, e), col = lane & 15, kk = 8 * (lane >> 4);
   int64_t xrow[FR], arow[RT];
   bool xon[FR], aon[RT];
 #pragma unroll
   for (int f = 0; f < FR; f++) {
-    xon[f] = r0 + 16 * f + col < count;
-    xrow[f] = xon[f] ? (int64_t)rows[r0 + 16 * f + col] * a.K : 0;
+    xon[f] = 16 * f + col < count;
+    xrow[f] = xon[f] ? (int64_t)rows[16 * f + col] * a.K : 0;
   }
 #pragma unroll
   for (int j = 0; j < RT; j++) {
@@ -190,7 +186,7 @@ RLXQ_DEV void lr_shrink(const rlxq_lora_args& a) {
   __syncthreads();
   // (lane: row 16 f + lane % 16 of the tile, rows 16 j + 4 (lane / 16) .. + 3 of A)
   for (int i = wave; i < RT * FR; i += 4) {
-    const int row = r0 + 16 * (i % FR) + col, j = j0 + 16 * (i / FR) + 4 * (lane >> 4);
+    const int row = 16 * (i % FR) + col, j = j0 + 16 * (i / FR) + 4 * (lane >> 4);
     if (row >= count || j >= sr) continue;
     const lr_f4 s = (part[0][i][lane] + part[1][i][lane]) + (part[2][i][lane] + part[3][i][lane]);
     *reinterpret_cast<lr_f4*>(a.v + ((int64_t)split * a.M + rows[row]) * sr + j) = s;
@@ -210,15 +206,32 @@ RLXQ_DEV uint4 lr_term(float* v) {
   return q;
 }
 
-// y of 16 FR rows and a.cols columns of one segment.  A wave takes 64 columns at a
-// time as four tiles: tile q's row p is column 16 (p / 4) + 4 q + p % 4 of them,
-// so a lane has 16 neighbouring columns of its activation row.  v lies in LDS as
-// the MFMA takes it, made once for the workgroup.
-template <bool BB, bool YB, bool LIST, int FR>
+// The column that row p of tile q of a wave's 64 columns stands for: chosen so that
+// a lane's results (rows 4 g .. 4 g + 3 of every tile, g = lane / 16) make 16-byte
+// pieces, neighbouring ones in neighbouring g.  Piece u of a lane starts at column
+// lr_piece and is tile u (f32), or tiles 2 u and 2 u + 1 (bf16).
+template <bool YB>
+RLXQ_DEV int lr_column(int q, int p) {
+  return YB ? 32 * (q >> 1) + 8 * (p >> 2) + 4 * (q & 1) + (p & 3) : 16 * q + p;
+}
+template <bool YB>
+RLXQ_DEV int lr_piece(int u, int g) {
+  return YB ? 32 * u + 8 * g : 16 * u + 4 * g;
+}
+
+// y of a tile's rows and a.cols columns of one segment, ranks up to 32 STEPS.  A
+// wave takes 64 columns at a time, their rows of B in registers (the next ones on
+// their way where two sets fit), and goes through the tile's rows 16 at a time
+// against them.  v lies in LDS as the MFMA takes it, made once for the workgroup
+// while the first of B and base are on their way.
+template <bool BB, bool YB, bool LIST, int STEPS>
 RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
+  constexpr int FR = LIST ? kLrFrags : 1;
   constexpr int NT = BB ? (YB ? 2 : 3) : 2;   // 16-byte pieces of v a lane and 32 k (f32: the eight floats)
+  constexpr bool AHEAD = STEPS <= 2;
+  constexpr int P = YB ? 2 : 4, ES = YB ? 2 : 4;   // pieces of a lane's 16 columns
   extern __shared__ uint4 lds[];              // [steps][FR][NT][64]
-  __shared__ int rows[64];
+  __shared__ int rows[RLXQ_LORA_ROWS];
   __shared__ uint64_t masks[4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int cb = blockIdx.x % a.cblocks;
@@ -230,12 +243,12 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
   const int64_t c1 = c0 + a.cols < a.ends[seg] ? c0 + a.cols : a.ends[seg];
   if (e < 0) {   // base's bits
     if (!a.copy) return;
-    const int es = YB ? 2 : 4, per = a.vec ? 16 / es : 1, n = (int)(c1 - c0) / per;
+    const int per = a.vec ? 16 / ES : 1, n = (int)(c1 - c0) / per;
     for (int i = t; i < count * n; i += kLrThreads) {
       const int64_t o = (int64_t)rows[i / n] * a.N + c0 + (int64_t)(i % n) * per;
       if (a.vec)
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + o * es) =
-            a.base ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.base) + o * es) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + o * ES) =
+            a.base ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.base) + o * ES) : make_uint4(0, 0, 0, 0);
       else if (YB)
         reinterpret_cast<uint16_t*>(a.y)[o] = a.base ? reinterpret_cast<const uint16_t*>(a.base)[o] : 0;
       else
@@ -243,24 +256,58 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
     }
     return;
   }
-  const int rank = lr_rank(a, e), steps = (rank + 31) / 32, sr = a.S * a.R;
+  const int rank = lr_rank(a, e), sr = a.S * a.R, col = lane & 15, g = lane >> 4, kk = 8 * g;
+  LrFrag<BB> bf[STEPS][4], bn[AHEAD ? STEPS : 1][4];
+  auto fetch = [&](LrFrag<BB>(&dst)[STEPS][4], int64_t c) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int64_t n = c + lr_column<YB>(q, col);
+      const bool on = n < c1;
+      const int64_t row = ((int64_t)e * a.N + (on ? n : c0)) * a.R;
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        const int r = 32 * s + kk;
+        dst[s][q] = on && r < rank ? lr_load<BB, BB>(a.b, row + r) : lr_zero<BB>();
+      }
+    }
+  };
+  fetch(bf, c0 + 64 * wave);
+  int64_t yrow[FR];
+  bool on[FR];
+#pragma unroll
+  for (int f = 0; f < FR; f++) {
+    on[f] = 16 * f + col < count;
+    yrow[f] = on[f] ? (int64_t)rows[16 * f + col] * a.N : 0;
+  }
   const float scale = a.scales ? a.scales[e] : 1.0f;
-  for (int i = t; i < steps * FR * 64; i += kLrThreads) {
-    const int l = i & 63, f = (i >> 6) % FR, s = (i >> 6) / FR, r = 32 * s + 8 * (l >> 4), row = 16 * f + (l & 15);
+  const int steps = (rank + 31) / 32, frags = (count + 15) / 16;
+  for (int i = t; i < steps * frags * 64; i += kLrThreads) {
+    const int l = i & 63, f = (i >> 6) % frags, s = (i >> 6) / frags, r = 32 * s + 8 * (l >> 4), row = 16 * f + (l & 15);
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = 0.f;
     if (row < count && r < rank) {
       const float* p = a.v + (int64_t)rows[row] * sr + seg * a.R + r;
-      for (int q = 0; q < a.splits; q++, p += a.M * sr) {
-        const float4 lo = reinterpret_cast<const float4*>(p)[0], hi = reinterpret_cast<const float4*>(p)[1];
-        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-        v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+      const int64_t step = a.M * sr;
+      // (slices in order, four of them on their way; past the last: the last, not added)
+      for (int q0 = 0; q0 < a.splits; q0 += 4) {
+        float4 lo[4], hi[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const float* at = p + (q0 + q < a.splits ? q0 + q : a.splits - 1) * step;
+          lo[q] = reinterpret_cast<const float4*>(at)[0], hi[q] = reinterpret_cast<const float4*>(at)[1];
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          if (q0 + q >= a.splits) break;
+          v[0] += lo[q].x, v[1] += lo[q].y, v[2] += lo[q].z, v[3] += lo[q].w;
+          v[4] += hi[q].x, v[5] += hi[q].y, v[6] += hi[q].z, v[7] += hi[q].w;
+        }
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] = r + j < rank ? v[j] * scale : 0.f;
     }
-    uint4* d = lds + (int64_t)(s * FR + f) * NT * 64 + l;
+    uint4* d = lds + (s * FR + f) * NT * 64 + l;
     if constexpr (BB) {
 #pragma unroll
       for (int q = 0; q < NT; q++) d[q * 64] = lr_term(v);
@@ -270,112 +317,98 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
     }
   }
   __syncthreads();
-  const int col = lane & 15, kk = 8 * (lane >> 4), frags = (count + 15) / 16;
-  int64_t yrow[FR];
-  bool on[FR];
-#pragma unroll
-  for (int f = 0; f < FR; f++) {
-    on[f] = 16 * f + col < count;
-    yrow[f] = on[f] ? (int64_t)rows[16 * f + col] * a.N : 0;
-  }
-  for (int64_t c = c0 + 64 * wave; c < c1; c += 64 * (kLrThreads / 64)) {
-    const int64_t mine = c + 16 * (lane >> 4);   // this lane's 16 columns
-    const int width = mine < c1 ? (int)(c1 - mine < 16 ? c1 - mine : 16) : 0;
-    lr_f4 acc[4][FR];
-#pragma unroll
-    for (int q = 0; q < 4; q++)
-#pragma unroll
-      for (int f = 0; f < FR; f++) acc[q][f] = (lr_f4){0.f, 0.f, 0.f, 0.f};
-    // base, ahead of the products
-    constexpr int P = YB ? 2 : 4;   // 16-byte pieces of 16 columns
-    uint4 bq[FR][P];
-    const bool whole = a.vec && width == 16;
-#pragma unroll
-    for (int f = 0; f < FR; f++)
-#pragma unroll
-      for (int p = 0; p < P; p++) {
-        bq[f][p] = make_uint4(0, 0, 0, 0);
-        if (a.base && whole && on[f])
-          bq[f][p] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.base) + (yrow[f] + mine) * (YB ? 2 : 4))[p];
-      }
-    int64_t brow[4];
-    bool bon[4];
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const int64_t n = c + 16 * (col >> 2) + 4 * q + (col & 3);
-      bon[q] = n < c1;
-      brow[q] = ((int64_t)e * a.N + (bon[q] ? n : c0)) * a.R;
+  constexpr int kStep = 64 * (kLrThreads / 64);
+  for (int64_t c = c0 + 64 * wave; c < c1; c += kStep) {
+    if constexpr (!AHEAD) {
+      if (c != c0 + 64 * wave) fetch(bf, c);
+    } else if (c + kStep < c1) {
+      fetch(bn, c + kStep);
     }
-    for (int s = 0; s < steps; s++) {
-      const int r = 32 * s + kk;
-      LrFrag<BB> bf[4];
+    uint4 bq[FR][P];
+    bool whole[P];
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        bf[q] = bon[q] && r < rank ? lr_load<BB, BB>(a.b, brow[q] + r) : lr_zero<BB>();
-        if (rank - r < 8) lr_keep<BB>(bf[q], rank - r);
-      }
+    for (int u = 0; u < P; u++) {
+      whole[u] = a.vec && c + lr_piece<YB>(u, g) < c1;   // (with vec, segments are whole pieces)
 #pragma unroll
       for (int f = 0; f < FR; f++) {
-        if (f >= frags) break;
-        const uint4* d = lds + (int64_t)(s * FR + f) * NT * 64 + lane;
+        bq[f][u] = make_uint4(0, 0, 0, 0);
+        if (a.base && whole[u] && on[f])
+          bq[f][u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.base) +
+                                                     (yrow[f] + c + lr_piece<YB>(u, g)) * ES);
+      }
+    }
+    if (rank & 7) {   // what lies past the rank in its eight
+#pragma unroll
+      for (int s = 0; s < STEPS; s++)
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+          if (rank - 32 * s - kk < 8) lr_keep<BB>(bf[s][q], rank - 32 * s - kk);
+    }
+#pragma unroll
+    for (int f = 0; f < FR; f++) {
+      if (f >= frags) break;
+      lr_f4 acc[4];
+#pragma unroll
+      for (int q = 0; q < 4; q++) acc[q] = (lr_f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        if (s >= steps) break;
+        const uint4* d = lds + (s * FR + f) * NT * 64 + lane;
         if constexpr (BB) {
 #pragma unroll
           for (int w = 0; w < NT; w++) {
             LrFrag<BB> vf;
             vf.q[0] = d[w * 64];
 #pragma unroll
-            for (int q = 0; q < 4; q++) acc[q][f] = lr_mfma<BB>(bf[q], vf, acc[q][f]);
+            for (int q = 0; q < 4; q++) acc[q] = lr_mfma<BB>(bf[s][q], vf, acc[q]);
           }
         } else {
           LrFrag<BB> vf;
           vf.q[0] = d[0];
           vf.q[1] = d[64];
 #pragma unroll
-          for (int q = 0; q < 4; q++) acc[q][f] = lr_mfma<BB>(bf[q], vf, acc[q][f]);
+          for (int q = 0; q < 4; q++) acc[q] = lr_mfma<BB>(bf[s][q], vf, acc[q]);
+        }
+      }
+      if (!on[f]) continue;
+#pragma unroll
+      for (int u = 0; u < P; u++) {
+        const int64_t n = c + lr_piece<YB>(u, g);
+        if (whole[u]) {
+          uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + (yrow[f] + n) * ES);
+          if constexpr (YB) {
+            const uint32_t w[4] = {bq[f][u].x, bq[f][u].y, bq[f][u].z, bq[f][u].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              o[j] = pack_bf16x2(__uint_as_float(w[j] << 16) + acc[2 * u + (j >> 1)][2 * j & 3],
+                                 __uint_as_float(w[j] & 0xffff0000u) + acc[2 * u + (j >> 1)][(2 * j & 3) + 1]);
+            *d = make_uint4(o[0], o[1], o[2], o[3]);
+          } else {
+            const float4 w = __builtin_bit_cast(float4, bq[f][u]);
+            *d = __builtin_bit_cast(uint4, make_float4(w.x + acc[u][0], w.y + acc[u][1], w.z + acc[u][2], w.w + acc[u][3]));
+          }
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 16 / P; j++) {
+          if (n + j >= c1) break;
+          const int64_t o = yrow[f] + n + j;
+          if constexpr (YB) {
+            const float w = a.base ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.base)[o]) : 0.f;
+            reinterpret_cast<uint16_t*>(a.y)[o] = (uint16_t)f32_to_bf16_bits(w + acc[2 * u + (j >> 2)][j & 3]);
+          } else {
+            const float w = a.base ? reinterpret_cast<const float*>(a.base)[o] : 0.f;
+            reinterpret_cast<float*>(a.y)[o] = w + acc[u][j & 3];
+          }
         }
       }
     }
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int f = 0; f < FR; f++) {
-      if (!on[f] || width == 0) continue;
-      if (whole) {
-        uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + (yrow[f] + mine) * (YB ? 2 : 4));
-        if constexpr (YB) {
+      for (int s = 0; s < STEPS; s++)
 #pragma unroll
-          for (int p = 0; p < 2; p++) {
-            const uint32_t w[4] = {bq[f][p].x, bq[f][p].y, bq[f][p].z, bq[f][p].w};
-            uint32_t o[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const int at = 8 * p + 2 * j;   // column of the lane's 16: tile at / 4, its row at % 4
-              o[j] = pack_bf16x2(__uint_as_float(w[j] << 16) + acc[at >> 2][f][at & 3],
-                                 __uint_as_float(w[j] & 0xffff0000u) + acc[at >> 2][f][(at & 3) + 1]);
-            }
-            d[p] = make_uint4(o[0], o[1], o[2], o[3]);
-          }
-        } else {
-#pragma unroll
-          for (int p = 0; p < 4; p++) {
-            const float4 w = __builtin_bit_cast(float4, bq[f][p]);
-            d[p] = __builtin_bit_cast(uint4, make_float4(w.x + acc[p][f][0], w.y + acc[p][f][1], w.z + acc[p][f][2],
-                                                         w.w + acc[p][f][3]));
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-          if (j >= width) continue;
-          const int64_t o = yrow[f] + mine + j;
-          const float s = acc[j >> 2][f][j & 3];
-          if constexpr (YB) {
-            const float w = a.base ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.base)[o]) : 0.f;
-            reinterpret_cast<uint16_t*>(a.y)[o] = (uint16_t)f32_to_bf16_bits(w + s);
-          } else {
-            const float w = a.base ? reinterpret_cast<const float*>(a.base)[o] : 0.f;
-            reinterpret_cast<float*>(a.y)[o] = w + s;
-          }
-        }
-      }
+        for (int q = 0; q < 4; q++) bf[s][q] = bn[s][q];
     }
   }
 }
@@ -384,24 +417,43 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
 
 using namespace rlxq;
 
+namespace rlxq {
+// count[e]++ by every active lane, and the number it had: prompts are runs of
+// one adapter, so the first lanes' adapters are counted a wave at a time.
+RLXQ_DEV int lr_take(int* count, int e) {
+  for (int turn = 0; turn < 2; turn++) {
+    const int first = __builtin_amdgcn_readfirstlane(e);
+    const uint64_t same = __ballot(e == first);
+    if (e == first) {
+      const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+      int base = 0;
+      if (at == 0) base = atomicAdd(&count[first], __popcll(same));
+      return __builtin_amdgcn_readfirstlane(base) + at;
+    }
+  }
+  return atomicAdd(&count[e], 1);
+}
+}  // namespace rlxq
+
 // The rows by adapter (those without one last), cut into tiles of up to 64: one
 // workgroup; LDS holds a counter for each adapter.  The order of an adapter's
 // rows is that of the counters' atomics; no result depends on it.
 extern "C" __global__ __launch_bounds__(1024) void rlxq_lora_sort(rlxq_lora_args a) {
   extern __shared__ int count[];   // [E + 1]: rows, then where the next one goes
   __shared__ int red[2][16];
+  constexpr int kRows = RLXQ_LORA_ROWS;
   const int t = threadIdx.x, n = a.E + 1;
   for (int e = t; e < n; e += 1024) count[e] = 0;
   __syncthreads();
   for (int64_t i = t; i < a.M; i += 1024) {
     const int e = a.ids[i];
-    atomicAdd(&count[e >= 0 && e < a.E ? e : a.E], 1);
+    (void)lr_take(count, e >= 0 && e < a.E ? e : a.E);
   }
   __syncthreads();
   // a run of adapters a thread: rows and tiles ahead of it
   const int per = (n + 1023) / 1024, lo = t * per, hi = lo + per < n ? lo + per : n;
   int rows = 0, tiles = 0;
-  for (int e = lo; e < hi; e++) rows += count[e], tiles += (count[e] + 63) / 64;
+  for (int e = lo; e < hi; e++) rows += count[e], tiles += (count[e] + kRows - 1) / kRows;
   int ri = rows, ti = tiles;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -418,7 +470,7 @@ extern "C" __global__ __launch_bounds__(1024) void rlxq_lora_sort(rlxq_lora_args
   int start = ri - rows, tile = ti - tiles;
   for (int e = lo; e < hi; e++) {
     const int c = count[e];
-    for (int at = 0; at < c; at += 64) a.tiles[tile++] = {e < a.E ? e : -1, start + at, c - at < 64 ? c - at : 64, 0};
+    for (int at = 0; at < c; at += kRows) a.tiles[tile++] = {e < a.E ? e : -1, start + at, c - at < kRows ? c - at : kRows, 0};
     count[e] = start;
     start += c;
   }
@@ -426,7 +478,7 @@ extern "C" __global__ __launch_bounds__(1024) void rlxq_lora_sort(rlxq_lora_args
   __syncthreads();
   for (int64_t i = t; i < a.M; i += 1024) {
     const int e = a.ids[i];
-    a.order[atomicAdd(&count[e >= 0 && e < a.E ? e : a.E], 1)] = (int)i;
+    a.order[lr_take(count, e >= 0 && e < a.E ? e : a.E)] = (int)i;
   }
 }
 
@@ -436,19 +488,21 @@ extern "C" __global__ __launch_bounds__(1024) void rlxq_lora_sort(rlxq_lora_args
     lr_shrink<X, A, false, 1, 1>(a);                                                                                    \
   }                                                                                                                     \
   extern "C" __global__ __launch_bounds__(256) void rlxq_lora_shrink_##xn##_##an##_many(rlxq_lora_args a) {               \
-    lr_shrink<X, A, true, 2, 4>(a);                                                                                     \
+    lr_shrink<X, A, true, kLrFrags, 4>(a);                                                                                     \
   }
 RLXQ_LORA_SHRINK(true, true, bf16, bf16)
 RLXQ_LORA_SHRINK(true, false, bf16, f32)
 RLXQ_LORA_SHRINK(false, true, f32, bf16)
 RLXQ_LORA_SHRINK(false, false, f32, f32)
-#define RLXQ_LORA_EXPAND(B, Y, bn, yn)                                                                                  \
-  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_expand_##bn##_##yn##_few(rlxq_lora_args a) {                \
-    lr_expand<B, Y, false, 1>(a);                                                                                       \
+#define RLXQ_LORA_EXPAND1(B, Y, bn, yn, st)                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_expand_##bn##_##yn##_few_s##st(rlxq_lora_args a) {          \
+    lr_expand<B, Y, false, st>(a);                                                                                      \
   }                                                                                                                     \
-  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_expand_##bn##_##yn##_many(rlxq_lora_args a) {               \
-    lr_expand<B, Y, true, 4>(a);                                                                                        \
+  extern "C" __global__ __launch_bounds__(256) void rlxq_lora_expand_##bn##_##yn##_many_s##st(rlxq_lora_args a) {         \
+    lr_expand<B, Y, true, st>(a);                                                                                       \
   }
+#define RLXQ_LORA_EXPAND(B, Y, bn, yn) \
+  RLXQ_LORA_EXPAND1(B, Y, bn, yn, 1) RLXQ_LORA_EXPAND1(B, Y, bn, yn, 2) RLXQ_LORA_EXPAND1(B, Y, bn, yn, 4) RLXQ_LORA_EXPAND1(B, Y, bn, yn, 8)
 RLXQ_LORA_EXPAND(true, true, bf16, bf16)
 RLXQ_LORA_EXPAND(true, false, bf16, f32)
 RLXQ_LORA_EXPAND(false, true, f32, bf16)

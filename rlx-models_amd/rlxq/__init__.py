@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from itertools import accumulate
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent.parent
@@ -771,13 +772,23 @@ class Context:
         return y
 
 
+def _fits(t, dtype, shape, device: int) -> bool:
+    """Whether t (or None) is what a call wants: the short form of the checks
+    above, which say what is wrong where it is not."""
+    return t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous())
+
+
 class Serving:
     """The operators around the packed products of a served batch, on a Context
     (its device, its scratch, its errors): low-rank adapters, the residual norm
     and sampling."""
 
     def __init__(self, ctx: Context):
+        import torch
+
         self.ctx = ctx
+        self._f32, self._i32 = torch.float32, torch.int32
+        self._acts = {torch.float32: F32, torch.bfloat16: BF16}
 
     def lora_matmul(self, x, ids, a, b, *, ranks=None, scales=None, segments=None, base=None, y=None, y_dtype=None,
                     stream=None):
@@ -786,24 +797,33 @@ class Serving:
         widths of the column ranges of a fused projection, each with its own
         rank rows of a.  A row whose id is outside [0, adapters) is base's.
         Returns y (allocated if not given, of base's dtype, else f32); y may be base."""
-        import torch
-
-        c = self.ctx
-        check_lora_matmul(x, ids, a, b, ranks=ranks, scales=scales, segments=segments, base=base, y=y, device=c.device)
-        m, k = x.shape
-        e, n, rank = b.shape
+        c, acts = self.ctx, self._acts
+        dev = c.device
+        try:
+            (m, k), (e, n, rank) = x.shape, b.shape
+            segs = 1 if segments is None else len(segments)
+            yt = y.dtype if y is not None else base.dtype if base is not None else y_dtype or self._f32
+            fit = (x.dtype in acts and a.dtype in acts and yt in acts and (segments is None or (segs and min(segments) >= 0
+                   and sum(segments) == n)) and _fits(x, x.dtype, (m, k), dev) and _fits(ids, self._i32, (m,), dev)
+                   and _fits(a, a.dtype, (e, segs * rank, k), dev) and _fits(b, a.dtype, (e, n, rank), dev)
+                   and _fits(ranks, self._i32, (e,), dev) and _fits(scales, self._f32, (e,), dev)
+                   and _fits(base, yt, (m, n), dev) and _fits(y, yt, (m, n), dev) and ids is not None)
+        except (AttributeError, TypeError, ValueError):
+            fit = False
+        if not fit:
+            check_lora_matmul(x, ids, a, b, ranks=ranks, scales=scales, segments=segments, base=base, y=y, device=dev)
+            if yt not in acts:
+                raise ValueError(f"lora_matmul: y_dtype {yt} is not one of {[str(d) for d in acts]}")
         if y is None:
-            y = torch.empty((m, n), dtype=base.dtype if base is not None else y_dtype or torch.float32, device=x.device)
-        ends, segs = None, 1
-        if segments is not None:
-            segs, at = len(segments), 0
-            ends = (C.c_int64 * segs)()
-            for i, w in enumerate(segments):
-                at += w
-                ends[i] = at
-        rc = lib().rlxq_lora_matmul(c.h, _ptr(x), _dt(x), _ptr(ids), _ptr(a), _ptr(b), _dt(a), _ptr(ranks), _ptr(scales),
-                                    ends, segs, m, k, n, rank, e, _ptr(base), _ptr(y), _dt(y), _stream(stream, c.device))
-        c._check(rc, "lora_matmul")
+            import torch
+
+            y = torch.empty((m, n), dtype=yt, device=x.device)
+        ends = (C.c_int64 * segs)(*accumulate(segments)) if segments is not None else None
+        rc = lib().rlxq_lora_matmul(c.h, x.data_ptr(), acts[x.dtype], ids.data_ptr(), a.data_ptr(), b.data_ptr(),
+                                    acts[a.dtype], _ptr(ranks), _ptr(scales), ends, segs, m, k, n, rank, e, _ptr(base),
+                                    y.data_ptr(), acts[yt], _stream(stream, dev))
+        if rc != OK:
+            c._check(rc, "lora_matmul")
         return y
 
     def residual_norm(self, block, resid, *, pre_weight=None, post_weight=None, gate=None, scale: float = 1.0,
@@ -813,24 +833,43 @@ class Serving:
         or None; post_weight None: block as it is; pre_weight None: no y.  h has
         resid's dtype (f32 without resid) and may be written over resid
         (sum=resid); y has y_dtype, or h's dtype."""
-        import torch
-
-        c = self.ctx
-        check_residual_norm(block, resid, pre_weight=pre_weight, post_weight=post_weight, gate=gate, sum=sum, y=y,
-                            device=c.device)
+        c, acts = self.ctx, self._acts
+        dev = c.device
         first = block if block is not None else resid
-        rows, hidden = first.shape
-        if sum is None:
-            sum = torch.empty((rows, hidden), dtype=resid.dtype if resid is not None else torch.float32, device=first.device)
-        if y is None and pre_weight is not None:
-            y = torch.empty((rows, hidden), dtype=y_dtype or sum.dtype, device=first.device)
-        w = pre_weight if pre_weight is not None else post_weight
-        rc = lib().rlxq_residual_norm(c.h, _ptr(block), _dt(block) if block is not None else F32, _ptr(resid), _dt(sum),
-                                      _ptr(gate), _dt(gate) if gate is not None else F32,
-                                      gate.shape[0] if gate is not None else 1, _ptr(post_weight), _ptr(pre_weight),
-                                      _dt(w) if w is not None else F32, weight_offset, scale, eps, rows, hidden,
-                                      _ptr(sum), _ptr(y), _dt(y) if y is not None else F32, _stream(stream, c.device))
-        c._check(rc, "residual_norm")
+        try:
+            rows, hidden = first.shape
+            st = resid.dtype if resid is not None else sum.dtype if sum is not None else self._f32
+            yt = y.dtype if y is not None else y_dtype or st
+            w = pre_weight if pre_weight is not None else post_weight
+            wt = w.dtype if w is not None else self._f32
+            fit = (st in acts and yt in acts and wt in acts and first.dtype in acts
+                   and (block is not None or (gate is None and post_weight is None)) and (y is None or pre_weight is not None)
+                   and _fits(block, first.dtype, (rows, hidden), dev) and _fits(resid, st, (rows, hidden), dev)
+                   and _fits(pre_weight, wt, (hidden,), dev) and _fits(post_weight, wt, (hidden,), dev)
+                   and _fits(sum, st, (rows, hidden), dev) and _fits(y, yt, (rows, hidden), dev)
+                   and (gate is None or (gate.dtype in acts and _fits(gate, gate.dtype, (len(gate), hidden), dev)
+                                         and 0 < len(gate) <= rows and rows % len(gate) == 0)))
+        except (AttributeError, TypeError, ValueError):
+            fit = False
+        if not fit:
+            check_residual_norm(block, resid, pre_weight=pre_weight, post_weight=post_weight, gate=gate, sum=sum, y=y,
+                                device=dev)
+            if pre_weight is not None and yt not in acts:
+                raise ValueError(f"residual_norm: y_dtype {yt} is not one of {[str(d) for d in acts]}")
+        if sum is None or (y is None and pre_weight is not None):
+            import torch
+
+            if sum is None:
+                sum = torch.empty((rows, hidden), dtype=st, device=first.device)
+            if y is None and pre_weight is not None:
+                y = torch.empty((rows, hidden), dtype=yt, device=first.device)
+        rc = lib().rlxq_residual_norm(c.h, _ptr(block), acts[first.dtype], _ptr(resid), acts[st], _ptr(gate),
+                                      acts[gate.dtype] if gate is not None else F32,
+                                      gate.shape[0] if gate is not None else 1, _ptr(post_weight), _ptr(pre_weight), acts[wt],
+                                      weight_offset, scale, eps, rows, hidden, sum.data_ptr(), _ptr(y),
+                                      acts[yt] if y is not None else F32, _stream(stream, dev))
+        if rc != OK:
+            c._check(rc, "residual_norm")
         return sum, y
 
     def sample(self, logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None,
@@ -838,19 +877,30 @@ class Serving:
         """A token per row of logits, from the uniform numbers u [rows]: returns
         (tokens int32, probs f32).  The settings are [rows] tensors, or None
         (temperature 1, the others off); temperature 0 is the likeliest token."""
-        import torch
+        c, acts, f32, i32 = self.ctx, self._acts, self._f32, self._i32
+        dev = c.device
+        try:
+            rows, vocab = logits.shape
+            one = (rows,)
+            fit = (logits.dtype in acts and u is not None and _fits(logits, logits.dtype, (rows, vocab), dev) and _fits(u, f32, one, dev)
+                   and _fits(temperature, f32, one, dev) and _fits(top_k, i32, one, dev) and _fits(top_p, f32, one, dev)
+                   and _fits(min_p, f32, one, dev) and _fits(tokens, i32, one, dev) and _fits(probs, f32, one, dev))
+        except (AttributeError, TypeError, ValueError):
+            fit = False
+        if not fit:
+            check_sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, tokens=tokens,
+                         probs=probs, device=dev)
+        if tokens is None or probs is None:
+            import torch
 
-        c = self.ctx
-        check_sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, tokens=tokens, probs=probs,
-                     device=c.device)
-        rows, vocab = logits.shape
-        if tokens is None:
-            tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-        if probs is None:
-            probs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
-        rc = lib().rlxq_sample(c.h, _ptr(logits), _dt(logits), rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                               _ptr(min_p), _ptr(u), _ptr(tokens), _ptr(probs), _stream(stream, c.device))
-        c._check(rc, "sample")
+            if tokens is None:
+                tokens = torch.empty((rows,), dtype=i32, device=logits.device)
+            if probs is None:
+                probs = torch.empty((rows,), dtype=f32, device=logits.device)
+        rc = lib().rlxq_sample(c.h, logits.data_ptr(), acts[logits.dtype], rows, vocab, _ptr(temperature), _ptr(top_k),
+                               _ptr(top_p), _ptr(min_p), u.data_ptr(), tokens.data_ptr(), probs.data_ptr(), _stream(stream, dev))
+        if rc != OK:
+            c._check(rc, "sample")
         return tokens, probs
 
 

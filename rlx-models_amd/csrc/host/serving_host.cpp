@@ -235,6 +235,7 @@ int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t row
   g.chunks = (int32_t)((vocab + lead + RLXQ_SAMPLE_CHUNK - 1) / RLXQ_SAMPLE_CHUNK);
   // rows in batches whose chunks take up to 128 MB of scratch
   const int64_t row_bytes = g.chunks * (int64_t)(sizeof(rlxq_sample_chunk) + RLXQ_SAMPLE_BINS * (8 + 2));
+  const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
   const int64_t batch = std::min<int64_t>(rows, std::max<int64_t>(1, (128 << 20) / row_bytes));
   void* ws = nullptr;
   int rc = workspace(ctx, (size_t)(batch * row_bytes), &ws, stream);
@@ -244,6 +245,8 @@ int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t row
   g.counts = reinterpret_cast<uint16_t*>(g.masses + batch * g.chunks * RLXQ_SAMPLE_BINS);
   for (int64_t at = 0; at < rows; at += batch) {
     g.M = std::min(batch, rows - at);
+    // (a chunk each, or up to four while there are six workgroups a CU)
+    g.per = (int32_t)std::max<int64_t>(1, std::min<int64_t>(4, g.M * g.chunks / (6 * cus)));
     g.logits = static_cast<const char*>(logits) + at * vocab * (bf ? 2 : 4);
     if (temperature) g.temperature = temperature + at;
     if (top_k) g.top_k = top_k + at;
@@ -252,7 +255,7 @@ int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t row
     g.u = u + at;
     g.tokens = tokens + at;
     if (probs) g.probs = probs + at;
-    if ((rc = run_kernel(ctx, bf ? "rlxq_sample_hist_bf16" : "rlxq_sample_hist_f32", g.M * g.chunks, 256, 0, &g, stream)) ||
+    if ((rc = run_kernel(ctx, bf ? "rlxq_sample_hist_bf16" : "rlxq_sample_hist_f32", g.M * ((g.chunks + g.per - 1) / g.per), RLXQ_SAMPLE_CHUNK / 16, 0, &g, stream)) ||
         (rc = run_kernel(ctx, bf ? "rlxq_sample_pick_bf16" : "rlxq_sample_pick_f32", g.M, 512, 0, &g, stream)))
       return rc;
   }

@@ -53,7 +53,7 @@ constexpr int kSmpThreads = 512;
 struct SmpRow {
   double inv_t, min_w;
   float top;             // the largest logit
-  float p, u;
+  float temperature, p, q, u;
   int k;                 // 0: off
 };
 
@@ -96,7 +96,7 @@ struct SmpShared {
   uint32_t r32[16];
   uint32_t pick, pick_count;
   uint64_t pick_mass;
-  int found, last;
+  int found, last, first_past[8], last_some[8];
 };
 
 // Border among the elements at or ahead of `within`: the one of rank `k` (BY =
@@ -201,16 +201,29 @@ RLXQ_DEV void smp_choose(const rlxq_sample_args& a, const SmpRow& r, int64_t row
   const double incl = before + smp_scan<double>(m, s.rd, &all);
   if (total < 0.0) total = all;
   const double target = (double)r.u * total;
-  if (threadIdx.x == 0) s.found = 0x7fffffff, s.last = -1;
+  // the first thread whose sum exceeds the target, else (rounding, or u = 1) the
+  // last that keeps anything
+  const int t = threadIdx.x, wave = t >> 6;
+  const uint64_t some = __ballot(last >= 0), past = __ballot(m > 0.0 && incl > target);
+  if ((t & 63) == 0) {
+    s.first_past[wave] = past ? t + __builtin_ctzll(past) : -1;
+    s.last_some[wave] = some ? t + 63 - __builtin_clzll(some) : -1;
+  }
   __syncthreads();
-  // (no sum above the target: rounding, or u = 1: the last that is kept)
-  if (last >= 0) atomicMax(&s.last, last);
-  if (m > 0.0 && incl > target) atomicMin(&s.found, at(incl - m, target));
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int tok = s.found == 0x7fffffff ? s.last : s.found;   // (-1: nothing kept, which no row comes to)
+  int who = -1, end = -1;
+  for (int w = kSmpThreads / 64 - 1; w >= 0; w--) {
+    if (s.first_past[w] >= 0) who = s.first_past[w];
+    if (end < 0) end = s.last_some[w];
+  }
+  if (who < 0 && end < 0) {   // (nothing kept, which no row comes to)
+    if (t == 0) {
+      a.tokens[row] = -1;
+      if (a.probs) a.probs[row] = __builtin_nanf("");
+    }
+  } else if (t == (who >= 0 ? who : end)) {
+    const int tok = who >= 0 ? at(incl - m, target) : last;
     a.tokens[row] = tok;
-    if (a.probs) a.probs[row] = tok < 0 ? __builtin_nanf("") : (float)(smp_w(r, smp_ld(a, row, tok)) / total);
+    if (a.probs) a.probs[row] = (float)(smp_w(r, smp_ld(a, row, tok)) / total);
   }
 }
 
@@ -233,13 +246,19 @@ RLXQ_DEV void smp_best(uint64_t& best, uint32_t& bad, uint64_t* r64, uint32_t* r
   __syncthreads();
 }
 
-// The row's settings.  False: its token is already written (no distribution,
-// or the likeliest was asked for).
-RLXQ_DEV bool smp_row(const rlxq_sample_args& a, int64_t row, uint64_t best, uint32_t bad, SmpRow& r) {
-  const float T = a.temperature ? a.temperature[row] : 1.0f;
+// The row's settings; temperature is not positive where the likeliest is asked for.
+RLXQ_DEV void smp_settings(const rlxq_sample_args& a, int64_t row, SmpRow& r) {
+  r.temperature = a.temperature ? a.temperature[row] : 1.0f;
   r.u = a.u[row];
-  const bool none = bad || !best || T != T || r.u != r.u;
-  if (none || !(T > 0.0f)) {
+  r.k = a.top_k ? a.top_k[row] : 0;
+  r.p = a.top_p ? a.top_p[row] : 1.0f;
+  r.q = a.min_p ? a.min_p[row] : 0.0f;
+}
+// The row's largest logit is known.  False: its token is already written (no
+// distribution, or the likeliest was asked for).
+RLXQ_DEV bool smp_row(const rlxq_sample_args& a, int64_t row, uint64_t best, uint32_t bad, SmpRow& r) {
+  const bool none = bad || !best || r.temperature != r.temperature || r.u != r.u;
+  if (none || !(r.temperature > 0.0f)) {
     if (threadIdx.x == 0) {
       a.tokens[row] = none ? -1 : (int32_t)~(uint32_t)best;
       if (a.probs) a.probs[row] = none ? __builtin_nanf("") : 1.0f;
@@ -247,11 +266,8 @@ RLXQ_DEV bool smp_row(const rlxq_sample_args& a, int64_t row, uint64_t best, uin
     return false;
   }
   r.top = of_key((uint32_t)(best >> 32));
-  r.inv_t = 1.0 / (double)T;
-  r.k = a.top_k ? a.top_k[row] : 0;
-  r.p = a.top_p ? a.top_p[row] : 1.0f;
-  const float q = a.min_p ? a.min_p[row] : 0.0f;
-  r.min_w = q > 0.0f ? (q < 1.0f ? (double)q : 1.0) : 0.0;
+  r.inv_t = 1.0 / (double)r.temperature;
+  r.min_w = r.q > 0.0f ? (r.q < 1.0f ? (double)r.q : 1.0) : 0.0;
   return true;
 }
 
@@ -315,8 +331,9 @@ RLXQ_DEV void smp_scan_row(const rlxq_sample_args& a, const SmpRow& r, int64_t r
 // noise): smp_scan_row.
 
 constexpr int kBins = RLXQ_SAMPLE_BINS, kGroups = RLXQ_SAMPLE_GROUPS, kGroup = kBins / kGroups;
-constexpr int kHistThreads = RLXQ_SAMPLE_CHUNK / 16;
+constexpr int kHistThreads = RLXQ_SAMPLE_CHUNK / 16, kHistWaves = kHistThreads / 64;
 constexpr int kSmpList = 4096;
+constexpr int kSmpSort = 512;   // kept elements that are sorted as a whole
 constexpr int kSmpChunks = RLXQ_SAMPLE_MAX_VOCAB / RLXQ_SAMPLE_CHUNK + 1;   // (a row may start inside 16 bytes)
 
 // Bin number of v on the row's grid, a whole number that does not fall as v
@@ -327,6 +344,17 @@ RLXQ_DEV float smp_bin(float v, float scale) { return floorf(v * scale); }
 RLXQ_DEV float smp_anchor(float bin) { return ceilf(bin * (1.0f / kGroup)) * kGroup; }
 RLXQ_DEV int smp_below(float anchor, float bin) { return (int)fminf(anchor - bin, (float)(kBins - 1)); }
 
+// The elements of 16 bytes.
+template <int BF>
+RLXQ_DEV void smp_unpack(const uint4& q, float* v) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if (BF) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    else v[j] = __uint_as_float(w[j]);
+  }
+}
+
 // The elements of one aligned 16-byte vector of a row: i0 is the index of the
 // first, which may lie ahead of the row (its start need not be aligned), unless
 // all of it is known to be inside.
@@ -334,14 +362,8 @@ template <int BF>
 RLXQ_DEV void smp_ld16(const rlxq_sample_args& a, int64_t row, int i0, float* v, bool inside) {
   constexpr int N = BF ? 8 : 4;
   if (inside || (i0 >= 0 && i0 + N <= a.V)) {
-    const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.logits) +
-                                                    (row * a.V + i0) * (BF ? 2 : 4));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if (BF) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      else v[j] = __uint_as_float(w[j]);
-    }
+    smp_unpack<BF>(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.logits) + (row * a.V + i0) * (BF ? 2 : 4)),
+                   v);
     return;
   }
 #pragma unroll
@@ -367,28 +389,15 @@ RLXQ_DEV int smp_lead(const rlxq_sample_args& a, int64_t row) {
   return (int)((p & 15) / (BF ? 2 : 4));
 }
 
+// One chunk of smp_hist, its elements in v.
 template <int BF>
-RLXQ_DEV void smp_hist(const rlxq_sample_args& a) {
-  constexpr int N = BF ? 8 : 4, TH = kHistThreads;
-  __shared__ unsigned long long mass[kBins];
-  __shared__ uint32_t count[kBins];
-  __shared__ double pow2[32];
-  __shared__ uint64_t r64[TH / 64];
-  __shared__ uint32_t r32[TH / 64];
-  __shared__ float rf[TH / 64];
-  __shared__ int at;
-  const int64_t row = blockIdx.x / a.chunks;
-  const int c = (int)(blockIdx.x - row * a.chunks), t = threadIdx.x;
-  const int first = c * RLXQ_SAMPLE_CHUNK - smp_lead<BF>(a, row);
-  float v[16];
-  smp_ld_chunk<BF, 16 / N>(a, row, first, t, TH, v);
-  const float T = a.temperature ? a.temperature[row] : 1.0f;
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.0f, q = a.min_p ? a.min_p[row] : 0.0f;
-  const bool by_k = k > 0 && k < a.V, bins = by_k || p < 1.0f || q > 0.0f;
+RLXQ_DEV void smp_hist_chunk(const rlxq_sample_args& a, int64_t row, int c, int first, const float* v, float T, bool by_k,
+                             bool bins, unsigned long long* mass, uint32_t* count, const double* pow2, uint64_t* r64,
+                             uint32_t* r32, float* rf, int* at) {
+  constexpr int N = BF ? 8 : 4, TH = kHistThreads, kPiece = RLXQ_SAMPLE_CHUNK / kHistWaves;
+  const int t = threadIdx.x;
   for (int i = t; i < kBins; i += TH) mass[i] = 0, count[i] = 0;
-  if (t < 32) pow2[t] = 2.0 * exp_neg((t - 32) * (0.6931471805599453 / 32));
-  if (t == 0) at = 0x7fffffff;
+  if (t == 0) *at = 0x7fffffff;
   float top = -__builtin_inff();
   bool odd = false;
 #pragma unroll
@@ -399,78 +408,84 @@ RLXQ_DEV void smp_hist(const rlxq_sample_args& a) {
 #pragma unroll
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   uint32_t bad = __ballot(odd) != 0;
-  if ((t & 63) == 0) rf[t >> 6] = top, r32[t >> 6] = bad;
+  rlxq_sample_chunk* head = a.heads + row * a.chunks + c;
+  if ((t & 63) == 0) rf[t >> 6] = head->tops[t >> 6] = top, r32[t >> 6] = bad;
   __syncthreads();
   for (int w = 0; w < TH / 64; w++) top = fmaxf(top, rf[w]), bad |= r32[w];
-  // the lowest index of the largest
-  int mine = 0x7fffffff;
+  if (rf[t >> 6] == top) {   // the lowest index of the largest
+    int mine = 0x7fffffff;
 #pragma unroll
-  for (int j = 15; j >= 0; j--)
-    if (v[j] == top) mine = first + ((j / N) * TH + t) * N + j % N;
-  if (mine != 0x7fffffff) atomicMin(&at, mine);
+    for (int j = 15; j >= 0; j--)
+      if (v[j] == top) mine = first + (t >> 6) * kPiece + ((j / N) * 64 + (t & 63)) * N + j % N;
+    if (mine != 0x7fffffff) atomicMin(at, mine);
+  }
   __syncthreads();
-  rlxq_sample_chunk* head = a.heads + row * a.chunks + c;
   uint64_t* masses = a.masses + (row * a.chunks + c) * kBins;
   uint16_t* counts = a.counts + (row * a.chunks + c) * kBins;
-  const uint64_t best = key_of(top) ? smp_comp(key_of(top), at) : 0;
+  const uint64_t best = key_of(top) ? smp_comp(key_of(top), *at) : 0;
   if (!(T > 0.0f) || bad || !best) {   // (no weights; no bins are read but those of a chunk that is all masked)
     if (t == 0) head->best = best, head->mass = 0, head->bad = bad, head->count = 0;
     return;
   }
   const float scale = smp_bin_scale(T), anchor = smp_anchor(smp_bin(top, scale));
   // w 2^48 = 2^(n / 32 + 48) 2^(f / 32), n the integer nearest x = 32 (l - top) / (T
-  // ln 2), f = x - n: a table by n mod 32, and the Taylor series of the second
-  // about 0, whose first term left out is below (ln 2 / 64)^6 / 720 = 3e-15.  n is
-  // read off the sum 1.5 2^52 + x.  What is 2^-70 of the top or less, masked
-  // tokens among it, counts as that, which rounds to 0.
+  // ln 2), f = x - n: a table by n mod 32 (its entries times 2^48), and the Taylor
+  // series of the second about 0, whose first term left out is below (ln 2 / 64)^6 /
+  // 720 = 3e-15.  n is read off the sum 1.5 2^52 + x.  What is 2^-69 of the top or
+  // less, masked tokens among it, counts as that, which rounds to 0.
   constexpr double L = 0.6931471805599453 / 32, kRound = 0x1.8p52;
   const double top64 = (double)top, c32 = 32.0 / (0.6931471805599453 * (double)T);
   const double least = -48.0 * (double)T;
-  uint64_t sum = 0;
+  const bool wide = !(T < 1e36f);   // (nothing is that far below the top then: masked tokens by name)
+  double sum = 0x1p52;              // 2^52 + whole numbers: each addition rounds the weight to one
 #pragma unroll
   for (int half = 0; half < 2; half++) {
-    uint64_t w[8];
+    double e[8], f2[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const double d = __builtin_fmax((double)v[8 * half + j] - top64, least);
       const double y = __builtin_fma(d, c32, kRound);
       const uint32_t n = (uint32_t)__double_as_longlong(y);
       const double f = __builtin_fma(d, c32, kRound - y);
-      double e = __builtin_fma(f, L * L * L * L * L / 120, L * L * L * L / 24);
-      e = __builtin_fma(e, f, L * L * L / 6);
-      e = __builtin_fma(e, f, L * L / 2);
-      e = __builtin_fma(e, f, L);
-      e = __builtin_fma(e, f, 1.0);
-      const uint64_t b = (uint64_t)__double_as_longlong(pow2[n & 31]);
-      const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(((int32_t)n >> 5) + 48) << 20);
-      // the integer it rounds to: 2^52 + it, whose low bits it is
-      w[j] = (uint64_t)__double_as_longlong(__builtin_fma(e, __hiloint2double((int)hi, (int)(uint32_t)b), 0x1p52)) -
-             0x4330000000000000ull;
-      sum += w[j];
+      e[j] = __builtin_fma(f, L * L * L * L * L / 120, L * L * L * L / 24);
+      e[j] = __builtin_fma(e[j], f, L * L * L / 6);
+      e[j] = __builtin_fma(e[j], f, L * L / 2);
+      e[j] = __builtin_fma(e[j], f, L);
+      e[j] = __builtin_fma(e[j], f, 1.0);
+      const uint2 b = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pow2) + (n << 3 & 0xf8));
+      f2[j] = __hiloint2double((int)(b.y + ((n & ~31u) << 15)), (int)b.x);
     }
-    if (!(T < 1e36f)) {   // (nothing is that far below the top then: masked tokens by name)
+    if (wide) {
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (v[8 * half + j] == -__builtin_inff()) sum -= w[j], w[j] = 0;
+        if (v[8 * half + j] == -__builtin_inff()) e[j] = f2[j] = 0.0;
     }
     if (bins) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
+        const uint64_t w = (uint64_t)__double_as_longlong(__builtin_fma(e[j], f2[j], 0x1p52)) & 0xfffffffffffffull;
         const int d = smp_below(anchor, smp_bin(v[8 * half + j], scale));
-        atomicAdd(&mass[d], (unsigned long long)w[j]);
+        atomicAdd(&mass[d], (unsigned long long)w);
         if (by_k && v[8 * half + j] > -__builtin_inff()) atomicAdd(&count[d], 1u);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum = __builtin_fma(e[j], f2[j], sum);
     }
   }
+  if (!bins) {
+    uint64_t all = (uint64_t)(sum - 0x1p52);
 #pragma unroll
-  for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if ((t & 63) == 0) r64[t >> 6] = sum;
-  __syncthreads();
-  if (t == 0) {
-    for (int w = 1; w < TH / 64; w++) sum += r64[w];
-    head->best = best, head->mass = sum, head->bad = 0;
+    for (int off = 32; off; off >>= 1) all += __shfl_xor(all, off, 64);
+    if ((t & 63) == 0) r64[t >> 6] = all;
+    __syncthreads();
+    if (t == 0) {
+      for (int w = 1; w < TH / 64; w++) all += r64[w];
+      head->best = best, head->mass = all, head->bad = 0;
+    }
+    return;
   }
-  if (!bins) return;
+  __syncthreads();
   static_assert(kBins == 2 * TH && kGroup == 32, "a thread takes two bins, 16 threads a group");
   const uint64_t m0 = mass[2 * t], m1 = mass[2 * t + 1];
   const uint32_t n0 = count[2 * t], n1 = count[2 * t + 1];
@@ -481,24 +496,73 @@ RLXQ_DEV void smp_hist(const rlxq_sample_args& a) {
 #pragma unroll
   for (int off = 8; off; off >>= 1) gm += __shfl_xor(gm, off, 64), gn += __shfl_xor(gn, off, 64);
   if ((t & 15) == 0) head->group_mass[t >> 4] = gm, head->group_count[t >> 4] = gn;
-  if (!by_k) return;
-  __syncthreads();
 #pragma unroll
-  for (int off = 32; off >= 16; off >>= 1) gn += __shfl_xor(gn, off, 64);
-  if ((t & 63) == 0) r32[t >> 6] = gn;
+  for (int off = 32; off >= 16; off >>= 1) gm += __shfl_xor(gm, off, 64), gn += __shfl_xor(gn, off, 64);
+  if ((t & 63) == 0) r64[t >> 6] = gm, r32[t >> 6] = gn;
   __syncthreads();
   if (t == 0) {
-    for (int w = 1; w < TH / 64; w++) gn += r32[w];
-    head->count = gn;
+    for (int w = 1; w < TH / 64; w++) gm += r64[w], gn += r32[w];
+    head->best = best, head->mass = gm, head->bad = 0, head->count = gn;
+  }
+}
+
+template <int BF>
+RLXQ_DEV void smp_hist(const rlxq_sample_args& a) {
+  constexpr int N = BF ? 8 : 4, TH = kHistThreads;
+  __shared__ unsigned long long mass[kBins];
+  __shared__ uint32_t count[kBins];
+  __shared__ double pow2[32];
+  __shared__ uint64_t r64[TH / 64];
+  __shared__ uint32_t r32[TH / 64];
+  __shared__ float rf[TH / 64];
+  __shared__ int at;
+  // a.per chunks of one row, one after the other
+  const int runs = (a.chunks + a.per - 1) / a.per, t = threadIdx.x;
+  const int64_t row = blockIdx.x / runs;
+  const int c0 = (int)(blockIdx.x - row * runs) * a.per, c1 = c0 + a.per < a.chunks ? c0 + a.per : a.chunks;
+  const int lead = smp_lead<BF>(a, row);
+  // (a wave's elements: kPiece neighbouring ones)
+  constexpr int kPiece = RLXQ_SAMPLE_CHUNK / kHistWaves;
+  uint4 raw[16 / N];   // a chunk that lies in the row as a whole, on its way
+  auto inside = [&](int first) { return first >= 0 && first + RLXQ_SAMPLE_CHUNK <= a.V; };
+  auto fetch = [&](int first) {
+#pragma unroll
+    for (int j = 0; j < 16 / N; j++)
+      raw[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.logits) +
+                                               (row * a.V + first + (t >> 6) * kPiece + (j * 64 + (t & 63)) * N) * (BF ? 2 : 4));
+  };
+  if (inside(c0 * RLXQ_SAMPLE_CHUNK - lead)) fetch(c0 * RLXQ_SAMPLE_CHUNK - lead);
+  const float T = a.temperature ? a.temperature[row] : 1.0f;
+  const int k = a.top_k ? a.top_k[row] : 0;
+  const float p = a.top_p ? a.top_p[row] : 1.0f, q = a.min_p ? a.min_p[row] : 0.0f;
+  const bool by_k = k > 0 && k < a.V, bins = by_k || p < 1.0f || q > 0.0f;
+  if (t < 32) pow2[t] = 0x1p49 * exp_neg((t - 32) * (0.6931471805599453 / 32));
+#pragma unroll 1
+  for (int c = c0; c < c1; c++) {
+    const int first = c * RLXQ_SAMPLE_CHUNK - lead;
+    float v[16];
+    if (inside(first)) {
+#pragma unroll
+      for (int j = 0; j < 16 / N; j++) smp_unpack<BF>(raw[j], v + j * N);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16 / N; j++) smp_ld16<BF>(a, row, first + (t >> 6) * kPiece + (j * 64 + (t & 63)) * N, v + j * N, false);
+    }
+    if (c + 1 < c1 && inside(first + RLXQ_SAMPLE_CHUNK)) fetch(first + RLXQ_SAMPLE_CHUNK);
+    if (c > c0) __syncthreads();   // (the last one's LDS is read)
+    smp_hist_chunk<BF>(a, row, c, first, v, T, by_k, bins, mass, count, pow2, r64, r32, rf, &at);
   }
 }
 
 struct SmpPick {
   double scale[kSmpChunks], kept[kSmpChunks];   // chunks: their weights' scale in the row; their kept mass
   unsigned long long add[kSmpChunks];           // kept weights of listed elements, in 2^-50
+  uint64_t gmass[kSmpChunks][kGroups];          // the chunks' groups, as the first launch left them
+  uint32_t gnum[kSmpChunks][kGroups];
   int shift[kSmpChunks];                        // groups from the row's top to the chunk's
   uint32_t some[kSmpChunks];                    // which bins of the group that smp_fine took hold something
-  uint16_t flagged[kSmpChunks];
+  uint16_t flagged[kSmpChunks * kHistWaves];    // pieces to read again
+  float tops[kSmpChunks][kHistWaves];           // their largest logits
   uint8_t flag[kSmpChunks];
   double part[16][32];
   uint32_t part_n[16][32];
@@ -506,11 +570,11 @@ struct SmpPick {
   uint32_t gcnt[kGroups], fcnt[kGroup];         // elements
   uint64_t list[kSmpList];
   uint64_t few[64], lo, hi;
-  double few_w[64];
-  uint32_t n, n_few, n_flag;
+  double few_w[64], sorted_w[kSmpSort];
+  uint32_t n, n_few, n_flag, kept_n;
   int bin;
-  double before, base;
-  uint32_t base_n;
+  double before, base, total;
+  uint32_t base_n, bin_n;
 };
 
 // The mass and number of elements down to each bin of the row's group j, and
@@ -564,40 +628,45 @@ RLXQ_DEV void smp_fine(const rlxq_sample_args& a, int64_t row, int j, bool by_k,
   __syncthreads();
 }
 
-// The border among the n listed elements within [lo, hi] (as smp_comp): the one
-// of rank `need` (BY 0), or the last whose sum of the elements ahead is below
-// `target` (BY 1); base and base_n are what lies ahead of all of them.  *incl:
-// the sum down to the border.
-template <int BY>
-RLXQ_DEV uint64_t smp_select(const SmpRow& r, SmpPick& g, SmpShared& s, int n, uint64_t lo, uint64_t hi, double base,
-                             uint32_t base_n, uint32_t need, double target, double* incl) {
-  const int t = threadIdx.x;
+// The border among the listed elements of bins b_lo .. b_hi that are not smaller
+// than `lo` (as smp_comp): by_rank the one of rank `need`, else the last whose sum
+// of the elements ahead is below `target`; base and base_n are what lies
+// ahead of all of them.  *incl: the sum down to the border.  Bins over the range
+// of what is left narrow it until a wave can sort it.
+template <class B>
+RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShared& s, int n, B&& bin_at, int b_lo, int b_hi, uint64_t lo,
+                             uint64_t hi, double base, uint32_t base_n, uint32_t need, double target, double* incl) {
+  const int t = threadIdx.x, lane = t & 63;
   auto w_of = [&](uint64_t e) { return smp_w(r, of_key((uint32_t)(e >> 32))); };
-  for (;;) {
+  auto within = [&](uint64_t e) {
+    if (e < lo || e > hi) return false;
+    const int d = bin_at(of_key((uint32_t)(e >> 32)));
+    return d >= b_lo && d <= b_hi;
+  };
+  uint32_t left = (uint32_t)n;   // at most so many
+  for (bool first = true;; first = false) {
     __syncthreads();
-    if (t == 0) g.n_few = 0, g.lo = ~0ull, g.hi = 0;
+    if (t == 0) g.n_few = 0, g.lo = ~0ull, g.hi = 0, g.bin = 0;
+    s.mass[t] = 0;
+    s.count[t] = 0;
     __syncthreads();
-    for (int i = t; i < n; i += kSmpThreads) {
-      const uint64_t e = g.list[i];
-      if (e < lo || e > hi) continue;
-      const uint32_t at = atomicAdd(&g.n_few, 1u);
-      if (at < 64) g.few[at] = e;
-    }
-    __syncthreads();
-    const uint32_t m = g.n_few;
-    if (m <= 64) {   // a wave: every lane's rank, then the sums in order
-      if (t < 64) {
-        const uint64_t e = t < (int)m ? g.few[t] : 0;
-        if (t >= (int)m) g.few[t] = 0;
+    if (left <= 64) {
+      for (int i = t; i < n; i += kSmpThreads)
+        if (within(g.list[i])) g.few[atomicAdd(&g.n_few, 1u)] = g.list[i];
+      __syncthreads();
+      const int m = (int)g.n_few;
+      if (t < 64) {   // a wave: every lane's rank, then the sums in order
+        const uint64_t e = t < m ? g.few[t] : 0;
+        if (t >= m) g.few[t] = 0;
         __threadfence_block();
         int rank = 0;
-#pragma unroll
+#pragma unroll 8
         for (int i = 0; i < 64; i++) rank += g.few[i] > e;
-        const double w = t < (int)m ? w_of(e) : 0.0;
+        const double w = t < m ? w_of(e) : 0.0;
         // (to the lane of its rank: the wave's lanes have all read by now)
-        if (t < (int)m) g.few[rank] = e, g.few_w[rank] = w;
+        if (t < m) g.few[rank] = e, g.few_w[rank] = w;
         __threadfence_block();
-        double c = t < (int)m ? g.few_w[t] : 0.0;
+        double c = t < m ? g.few_w[t] : 0.0;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
           const double o = __shfl_up(c, off, 64);
@@ -605,7 +674,7 @@ RLXQ_DEV uint64_t smp_select(const SmpRow& r, SmpPick& g, SmpShared& s, int n, u
         }
         double ahead = __shfl_up(c, 1, 64);
         if (t == 0) ahead = 0.0;
-        const bool in = t < (int)m && (BY == 0 ? base_n + t < need : t == 0 || base + ahead < target);
+        const bool in = t < m && (by_rank ? base_n + t < need : t == 0 || base + ahead < target);
         const uint64_t which = __ballot(in);
         const int last = 63 - __builtin_clzll(which | 1);
         // (nothing listed: as where nothing is kept behind what lies ahead)
@@ -617,24 +686,31 @@ RLXQ_DEV uint64_t smp_select(const SmpRow& r, SmpPick& g, SmpShared& s, int n, u
       __syncthreads();
       return border;
     }
-    // 512 bins over the elements' own range
-    uint64_t e_lo = ~0ull, e_hi = 0;
-    for (int i = t; i < n; i += kSmpThreads) {
-      const uint64_t e = g.list[i];
-      if (e < lo || e > hi) continue;
-      e_lo = e < e_lo ? e : e_lo;
-      e_hi = e > e_hi ? e : e_hi;
+    if (!first) {   // the elements' own range
+      uint64_t e_lo = ~0ull, e_hi = 0;
+      for (int i = t; i < n; i += kSmpThreads) {
+        const uint64_t e = g.list[i];
+        if (!within(e)) continue;
+        e_lo = e < e_lo ? e : e_lo;
+        e_hi = e > e_hi ? e : e_hi;
+      }
+#pragma unroll
+      for (int off = 32; off; off >>= 1) {
+        const uint64_t ol = __shfl_xor(e_lo, off, 64), oh = __shfl_xor(e_hi, off, 64);
+        e_lo = ol < e_lo ? ol : e_lo;
+        e_hi = oh > e_hi ? oh : e_hi;
+      }
+      if (lane == 0) {
+        atomicMin((unsigned long long*)&g.lo, (unsigned long long)e_lo);
+        atomicMax((unsigned long long*)&g.hi, (unsigned long long)e_hi);
+      }
+      __syncthreads();
+      lo = g.lo, hi = g.hi;
     }
-    atomicMin((unsigned long long*)&g.lo, (unsigned long long)e_lo);
-    atomicMax((unsigned long long*)&g.hi, (unsigned long long)e_hi);
-    s.mass[t] = 0;
-    s.count[t] = 0;
-    __syncthreads();
-    lo = g.lo, hi = g.hi;
-    const int bits = 64 - __builtin_clzll(hi - lo), shift = bits > 9 ? bits - 9 : 0;
+    const int bits = hi > lo ? 64 - __builtin_clzll(hi - lo) : 1, shift = bits > 9 ? bits - 9 : 0;
     for (int i = t; i < n; i += kSmpThreads) {
       const uint64_t e = g.list[i];
-      if (e < lo || e > hi) continue;
+      if (!within(e)) continue;
       const uint32_t d = (uint32_t)((hi - e) >> shift);
       atomicAdd((unsigned long long*)&s.mass[d], (unsigned long long)(w_of(e) * 0x1p50 + 0.5));
       atomicAdd(&s.count[d], 1u);
@@ -646,19 +722,69 @@ RLXQ_DEV uint64_t smp_select(const SmpRow& r, SmpPick& g, SmpShared& s, int n, u
     uint32_t ct;
     const double ahead = base + smp_scan<double>(w, s.rd, &wt) - w;
     const uint32_t ahead_n = smp_scan<uint32_t>(c, s.r32, &ct) - c;
-    const bool in = c && (BY == 0 ? base_n + ahead_n < need : ahead_n == 0 || ahead < target);
-    if (t == 0) g.bin = 0;
+    const bool in = c && (by_rank ? base_n + ahead_n < need : ahead_n == 0 || ahead < target);
+    // the last bin that starts ahead of the border
+    const uint64_t which = __ballot(in);
+    if (lane == 0 && which) atomicMax(&g.bin, t + 63 - __builtin_clzll(which));
     __syncthreads();
-    if (in) atomicMax(&g.bin, t);   // the last bin that starts ahead of the border
-    __syncthreads();
-    if (t == g.bin) g.base = ahead, g.base_n = base_n + ahead_n;
+    if (t == g.bin) g.base = ahead, g.base_n = base_n + ahead_n, g.bin_n = c;
     __syncthreads();
     const uint64_t d = (uint64_t)g.bin;
-    base = g.base, base_n = g.base_n;
+    base = g.base, base_n = g.base_n, left = g.bin_n;
     const uint64_t top = hi - (d << shift), width = (1ull << shift) - 1;
     lo = top - lo > width ? top - width : lo;
     hi = top;
   }
+}
+
+// A row whose n listed elements (at most kSmpSort) are everything down to a bin
+// behind K's border: sorted as a whole, the borders follow from prefix sums, and
+// the token from the kept ones sorted by index.
+RLXQ_DEV void smp_small(const rlxq_sample_args& a, const SmpRow& r, int64_t row, int n, SmpPick& g, SmpShared& s) {
+  static_assert(kSmpSort == kSmpThreads, "an element a thread");
+  const int t = threadIdx.x;
+  const uint64_t e = t < n ? g.list[t] : 0;
+  const double w = t < n ? smp_w(r, of_key((uint32_t)(e >> 32))) : 0.0;
+  if (t >= n) g.list[t] = 0;   // (up to a multiple of 8)
+  __syncthreads();
+  auto rank_of = [&](const uint64_t* v, uint64_t x, int count) {   // elements of v that are larger
+    int rank = 0;
+    for (int i = 0; i < count; i += 8) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) rank += v[i + j] > x;
+    }
+    return rank;
+  };
+  const int rank = rank_of(g.list, e, n);
+  if (t < n) g.sorted_w[rank] = w;
+  __syncthreads();
+  const int k = r.k < n ? r.k : n;
+  const double mine = t < k ? g.sorted_w[t] : 0.0;
+  double mass_k;
+  const double incl = smp_scan<double>(mine, s.rd, &mass_k);
+  const double target = r.p < 1.0f ? (r.p > 0.0f ? (double)r.p * mass_k : 0.0) : __builtin_inf();
+  // of K's in order: what starts ahead of P's border and is not below min-p
+  const bool keep = t < k && (t == 0 || (incl - mine < target && mine >= r.min_w));
+  const uint64_t which = __ballot(keep);
+  if ((t & 63) == 0) s.r32[t >> 6] = (uint32_t)__popcll(which);
+  __syncthreads();
+  int m = 0;
+  for (int i = 0; i < kSmpThreads / 64; i++) m += (int)s.r32[i];
+  // by index: the kept ones' places
+  const bool mine_kept = t < n && rank < m;
+  const uint32_t idx = ~(uint32_t)e;
+  uint64_t* by_index = s.mass;   // (falling, as rank_of counts)
+  if (mine_kept) by_index[rank] = (uint64_t)(uint32_t)~idx + 1;
+  if (t >= m && t < m + 8) by_index[t] = 0;
+  __syncthreads();
+  if (mine_kept) {
+    const int at = rank_of(by_index, (uint64_t)(uint32_t)~idx + 1, m);
+    g.sorted_w[at] = w;
+    g.list[at] = (uint64_t)idx;
+  }
+  __syncthreads();
+  const double kw = t < m ? g.sorted_w[t] : 0.0;
+  smp_choose(a, r, row, kw, kw > 0.0 ? (int)g.list[t] : -1, 0.0, -1.0, s, [&](double, double) { return (int)g.list[t]; });
 }
 
 template <int BF>
@@ -667,16 +793,26 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   __shared__ SmpShared s;
   __shared__ SmpPick g;
   const int64_t row = blockIdx.x;
-  const int t = threadIdx.x, C = a.chunks;
+  const int t = threadIdx.x, C = a.chunks, lane = t & 63, wave = t >> 6;
   const rlxq_sample_chunk* heads = a.heads + row * C;
   uint64_t best = 0, my_best = 0, my_mass = 0;
   uint32_t bad = 0;
   if (t < C) my_best = heads[t].best, my_mass = heads[t].mass, bad = heads[t].bad;
+  SmpRow r;
+  smp_settings(a, row, r);
+  const bool by_p = r.p < 1.0f, by_q = r.q > 0.0f;
+  bool by_k = r.k > 0 && r.k < a.V;
+  const bool borders = by_k || by_p || by_q;
+  if (borders)   // (not written for the likeliest, nor read)
+    for (int i = t; i < C * kGroups; i += kSmpThreads) {
+      g.gmass[i / kGroups][i % kGroups] = heads[i / kGroups].group_mass[i % kGroups];
+      g.gnum[i / kGroups][i % kGroups] = heads[i / kGroups].group_count[i % kGroups];
+      if (i % kGroups < kHistWaves) g.tops[i / kGroups][i % kGroups] = heads[i / kGroups].tops[i % kGroups];
+    }
   best = my_best;
   smp_best(best, bad, s.r64, s.r32);
-  SmpRow r;
   if (!smp_row(a, row, best, bad, r)) return;
-  const float scale = smp_bin_scale(a.temperature ? a.temperature[row] : 1.0f), anchor = smp_anchor(smp_bin(r.top, scale));
+  const float scale = smp_bin_scale(r.temperature), anchor = smp_anchor(smp_bin(r.top, scale));
   if (t < C) {
     const float top = of_key((uint32_t)(my_best >> 32));
     g.scale[t] = my_best ? exp_neg(((double)top - (double)r.top) * r.inv_t) : 0.0;
@@ -685,21 +821,19 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
     g.add[t] = 0;
     g.flag[t] = 0;
   }
-  const bool by_p = r.p < 1.0f, by_q = r.min_w > 0.0;
-  bool by_k = r.k > 0 && r.k < a.V;
+  if (t == 0) g.n = 0, g.n_flag = 0;
   uint64_t border = 1;
   const int lead = smp_lead<BF>(a, row);
   __syncthreads();
-  if (by_k || by_p || by_q) {
+  if (borders) {
     // the row's groups: a wave each, a lane a chunk.  (The last is the rest.)
-    const int lane = t & 63, wave = t >> 6;
     for (int j = wave; j < kGroups; j += kSmpThreads / 64) {
       double m = 0.0;
       uint32_t n = 0;
       for (int c = lane; c < C; c += 64) {
         const int jj = j - g.shift[c];
-        if (j == kGroups - 1) m += g.kept[c], n += heads[c].count;
-        else if (jj >= 0) m += (double)heads[c].group_mass[jj] * 0x1p-48 * g.scale[c], n += by_k ? heads[c].group_count[jj] : 0;
+        if (j == kGroups - 1) m += g.kept[c], n += by_k ? heads[c].count : 0;
+        else if (jj >= 0) m += (double)g.gmass[c][jj] * 0x1p-48 * g.scale[c], n += g.gnum[c][jj];
       }
 #pragma unroll
       for (int off = 32; off; off >>= 1) m += __shfl_xor(m, off, 64), n += __shfl_xor(n, off, 64);
@@ -708,6 +842,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
     __syncthreads();
     const double all = g.gcum[kGroups - 1];
     const uint32_t all_n = g.gcnt[kGroups - 1];
+    __syncthreads();
     if (t < 16) {
       double m = t < kGroups - 1 ? g.gcum[t] : 0.0;
       uint32_t n = t < kGroups - 1 ? g.gcnt[t] : 0;
@@ -721,7 +856,6 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
       g.gcum[t] = m;
       g.gcnt[t] = n;
     }
-    if (t == 0) g.n = 0, g.n_flag = 0;
     __syncthreads();
     by_k = by_k && (uint32_t)r.k < all_n;   // (fewer than k that are not masked: all of them)
     // the first group, and the first bin of fcum's, whose mass or number reaches x
@@ -732,13 +866,8 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
     const int bl = lane & (kGroup - 1), gl = lane & (kGroups - 1);
     auto group_of = [&](double x) { return first_of(g.gcum[gl] >= x, kGroups); };
     auto bin_of_mass = [&](double x) { return first_of(g.fcum[bl] >= x, kGroup); };
-    auto flag = [&](int lo, int hi) {   // the chunks that hold something in bins lo .. hi of the group
-      for (int c = t; c < C; c += kSmpThreads)
-        if (g.some[c] & ((2u << (hi - lo)) - 1) << lo) g.flag[c] = 1;
-    };
     // bins to look into: K's border's, P's, and about min-p's
-    int kg = kGroups;
-    if (by_k) kg = first_of(g.gcnt[gl] >= (uint32_t)r.k, kGroups);
+    const int kg = by_k ? first_of(g.gcnt[gl] >= (uint32_t)r.k, kGroups) : kGroups;
     const double p = r.p > 1e-30f ? (double)r.p : 1e-30, under = 1.0 - 1e-12, over = 1.0 + 1e-12;
     int kb = kBins, p_lo = kBins, p_hi = -1, q_lo = kBins, q_hi = -1;
     const int pg = by_p ? group_of(p * (by_k ? (kg ? g.gcum[kg - 1] : 0.0) : all) * under) : kGroups;
@@ -752,83 +881,148 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
     double k_lo = all, k_hi = all;   // the least and the most that K can weigh
     double k_ahead = 0.0, p_ahead = 0.0;
     uint32_t k_ahead_n = 0;
-    if (!q_only) {
-      if (by_k) {
-        smp_fine(a, row, kg, true, all, all_n, g);
+    bool small = false;   // K is little enough to be listed and sorted as a whole
+    int kind = 0, j = kg, j0 = kg, j1 = by_k && !q_only ? kg : -1;   // K's group; P's groups; min-p's
+#pragma unroll 1
+    for (;;) {
+      double lo = 0.0, hi = 0.0;
+      if (kind == 0 && j > j1) {
+        kind = 1, j = 0, j1 = -1;
+        if (by_p && !q_only && !small) {
+          lo = p * k_lo * under, hi = p * k_hi * over;
+          j = j0 = group_of(lo), j1 = group_of(hi);
+        }
+      }
+      if (kind == 1 && j > j1) {
+        kind = 2, j = 0, j1 = -1;
+        if (small || (!q_only && q_lo > (by_p ? p_hi : kb))) q_lo = kBins, q_hi = -1;   // min-p ends behind them
+        if (q_hi >= 0) j = j0 = q_lo / kGroup, j1 = q_hi / kGroup;
+      }
+      if (j > j1) break;
+      smp_fine(a, row, j, by_k, all, all_n, g);
+      int from = 0, to = kGroup - 1;   // bins of the group whose chunks are read again
+      if (kind == 0) {
         const int b = first_of(g.fcnt[bl] >= (uint32_t)r.k, kGroup);
         kb = kg * kGroup + b;
         k_ahead = b ? g.fcum[b - 1] : (kg ? g.gcum[kg - 1] : 0.0);
         k_ahead_n = b ? g.fcnt[b - 1] : (kg ? g.gcnt[kg - 1] : 0);
         k_lo = k_ahead, k_hi = g.fcum[b];
-        flag(b, b);
-      }
-      if (by_p) {
-        const double lo = p * k_lo * under, hi = p * k_hi * over;
-        const int j0 = group_of(lo), j1 = group_of(hi);
-        smp_fine(a, row, j0, by_k, all, all_n, g);
-        const int b = bin_of_mass(lo);
-        p_lo = j0 * kGroup + b;
-        p_ahead = b ? g.fcum[b - 1] : (j0 ? g.gcum[j0 - 1] : 0.0);
-        int e = j1 > j0 ? kGroup - 1 : bin_of_mass(hi);
-        flag(b, e);
-        for (int j = j0 + 1; j <= j1; j++) {
-          smp_fine(a, row, j, by_k, all, all_n, g);
-          e = j < j1 ? kGroup - 1 : bin_of_mass(hi);
-          flag(0, e);
+        small = g.fcnt[b] <= kSmpSort;
+        from = small ? 0 : b, to = b;
+        // (everything ahead of K's group too)
+        if (small && t < C && g.shift[t] < kg) g.flag[t] = 1;
+      } else if (kind == 1) {
+        lo = p * k_lo * under, hi = p * k_hi * over;
+        if (j == j0) {
+          from = bin_of_mass(lo);
+          p_lo = j * kGroup + from;
+          p_ahead = from ? g.fcum[from - 1] : (j ? g.gcum[j - 1] : 0.0);
         }
-        p_hi = j1 * kGroup + e;
+        if (j == j1) to = bin_of_mass(hi);
+        p_hi = j * kGroup + to;
+      } else {
+        if (j == j0) from = q_lo % kGroup;
+        if (j == j1) to = q_hi % kGroup;
       }
+      for (int c = t; c < C; c += kSmpThreads)   // the chunks that hold something there
+        if (g.some[c] & ((2u << (to - from)) - 1) << from) g.flag[c] = 1;
+      j++;
     }
-    if (!q_only && q_lo > (by_p ? p_hi : kb)) q_lo = kBins, q_hi = -1;   // min-p ends behind them
-    if (q_hi >= 0)
-      for (int j = q_lo / kGroup; j <= q_hi / kGroup; j++) {
-        smp_fine(a, row, j, by_k, all, all_n, g);
-        flag(j == q_lo / kGroup ? q_lo % kGroup : 0, j == q_hi / kGroup ? q_hi % kGroup : kGroup - 1);
-      }
     const int kp = p_lo < kb ? p_lo : kb;
     const int d_lo = q_lo < kp ? q_lo : kp;   // bins ahead of it are kept whole
     auto bin_at = [&](float v) { return smp_below(anchor, smp_bin(v, scale)); };
-    auto wanted = [&](int d) { return d == kb || (d >= p_lo && d <= p_hi) || (d >= q_lo && d <= q_hi); };
-    // (an open bin of a chunk below the row's top may hold what falls into a later
-    // bin of the row: the row's own last one, for which every chunk is flagged)
-    __syncthreads();
-    if (t < C && g.flag[t]) g.flagged[atomicAdd(&g.n_flag, 1u)] = (uint16_t)t;
-    __syncthreads();
-    // (x = l scale of the bins d_first .. d_last, and some more: wanted() decides.  An
-    // x past the largest number is in the open bin, and `to` is past it too then.)
-    const int d_first = kp < q_lo ? kp : q_lo;
+    // pieces (what a wave of the first launch held) to read again: of a flagged
+    // chunk, and high enough for the last bin wanted
+    const int d_first = small ? 0 : d_lo;
     int d_last = p_hi > q_hi ? p_hi : q_hi;
     if (kb < kBins && kb > d_last) d_last = kb;
-    const float slack = 1.0f + fabsf(anchor) * 0x1p-22f;
-    const float from = d_last == kBins - 1 ? -__builtin_inff() : anchor - (float)d_last - slack;
-    const float to = anchor - (float)d_first + 1.0f + slack;
-    constexpr int kPerThread = RLXQ_SAMPLE_CHUNK / kSmpThreads, kAtOnce = 4;
+    __syncthreads();
+    for (int i = t; i < C * kHistWaves; i += kSmpThreads) {
+      const int c = i / kHistWaves;
+      const bool take = g.flag[c] && (d_last == kBins - 1 || bin_at(g.tops[c][i % kHistWaves]) <= d_last);
+      const uint64_t which = __ballot(take);
+      uint32_t at = 0;
+      if (which && (int)__builtin_ctzll(which) == lane) at = atomicAdd(&g.n_flag, (uint32_t)__popcll(which));
+      if (which) at = __shfl(at, __builtin_ctzll(which), 64);
+      if (take) g.flagged[at + __popcll(which & ((1ull << lane) - 1))] = (uint16_t)i;
+    }
+    __syncthreads();
+    // wanted: bins 0 .. kb, or kb, p_lo .. p_hi and q_lo .. q_hi.  One range of them is
+    // from <= l scale < to, exactly, where no rounding is in the way.
+    const float k0 = small ? 0.0f : (float)kb, k1 = (float)kb, p0 = (float)p_lo, p1 = (float)p_hi, q0 = (float)q_lo,
+                q1 = (float)q_hi;
+    const float from = anchor - (float)d_last, to = anchor - (float)d_first + 1.0f;
+    const bool exact = fabsf(anchor) < 0x1p20f && d_last < kBins - 1 && (small || (!by_k && !by_p) || q_only ||
+                                                                       ((kb == kBins || !by_p) && q_hi < 0));
+    constexpr int kPiece = RLXQ_SAMPLE_CHUNK / kHistWaves, kPieceLane = kPiece / 64;
     const int n_flag = (int)g.n_flag;
-    for (int f0 = 0; f0 < n_flag; f0 += kAtOnce) {
-      float v[kAtOnce][kPerThread];
-      int first[kAtOnce];
+    // (a wave's pieces are the same for its lanes; the next one that lies in the row
+    // as a whole is on its way, as it is in memory)
+    auto first_at = [&](int f) {
+      const int i = __builtin_amdgcn_readfirstlane((int)g.flagged[f]);
+      return i / kHistWaves * RLXQ_SAMPLE_CHUNK - lead + i % kHistWaves * kPiece;
+    };
+    auto inside = [&](int first) { return first >= 0 && first + kPiece <= a.V; };
+    const int w0 = __builtin_amdgcn_readfirstlane(wave);
+    constexpr int kVecs = kPieceLane / N;
+    uint4 raw[kVecs];
+    auto fetch = [&](int first) {
 #pragma unroll
-      for (int u = 0; u < kAtOnce; u++) {
-        // (past the last: the last again, whose elements are not taken)
-        first[u] = (int)g.flagged[f0 + u < n_flag ? f0 + u : n_flag - 1] * RLXQ_SAMPLE_CHUNK - lead;
-        smp_ld_chunk<BF, kPerThread / N>(a, row, first[u], t, kSmpThreads, v[u]);
+      for (int j = 0; j < kVecs; j++)
+        raw[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.logits) +
+                                                 (row * a.V + first + (j * 64 + lane) * N) * (BF ? 2 : 4));
+    };
+    int next = 0;
+    if (w0 < n_flag) {
+      next = first_at(w0);
+      if (inside(next)) fetch(next);
+    }
+#pragma unroll 1
+    for (int f = w0; f < n_flag; f += kSmpThreads / 64) {
+      const int here = next;
+      float v[kPieceLane];
+      if (inside(here)) {
+#pragma unroll
+        for (int j = 0; j < kVecs; j++) smp_unpack<BF>(raw[j], v + j * N);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVecs; j++) smp_ld16<BF>(a, row, here + (j * 64 + lane) * N, v + j * N, false);
       }
+      if (f + kSmpThreads / 64 < n_flag) {
+        next = first_at(f + kSmpThreads / 64);
+        if (inside(next)) fetch(next);
+      }
+      // (no short circuits: a branch an element costs more than the comparisons)
+      uint64_t hit[kPieceLane];
+      uint32_t hits = 0;
+      if (exact) {
 #pragma unroll
-      for (int u = 0; u < kAtOnce; u++) {
-        if (f0 + u >= n_flag) break;
-        uint32_t in = 0;
-#pragma unroll
-        for (int j = 0; j < kPerThread; j++) {
-          const float x = v[u][j] * scale;
-          in |= (!(x < from) && !(x > to)) ? 1u << j : 0u;
+        for (int i = 0; i < kPieceLane; i++) {
+          const float x = v[i] * scale;
+          hit[i] = __ballot(x >= from) & __ballot(x < to);
+          hits += (uint32_t)__popcll(hit[i]);
         }
-        if (!in) continue;
+      } else {
 #pragma unroll
-        for (int j = 0; j < kPerThread; j++) {
-          if (!(in >> j & 1) || v[u][j] == -__builtin_inff() || !wanted(bin_at(v[u][j]))) continue;
-          const uint32_t at = atomicAdd(&g.n, 1u);
-          if (at < kSmpList) g.list[at] = smp_comp(key_of(v[u][j]), first[u] + ((j / N) * kSmpThreads + t) * N + j % N);
+        for (int i = 0; i < kPieceLane; i++) {
+          const float d = fminf(anchor - smp_bin(v[i], scale), (float)(kBins - 1));
+          hit[i] = ((__ballot(d >= k0) & __ballot(d <= k1)) | (__ballot(d >= p0) & __ballot(d <= p1)) |
+                    (__ballot(d >= q0) & __ballot(d <= q1))) & __ballot(v[i] != -__builtin_inff());
+          hits += (uint32_t)__popcll(hit[i]);
         }
+      }
+      if (!hits) continue;
+      // a place in the list for all of the wave's at once
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&g.n, hits);
+      at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+#pragma unroll
+      for (int i = 0; i < kPieceLane; i++) {
+        if (!hit[i]) continue;
+        const uint32_t mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(hit[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[i], 0));
+        if ((bool)(hit[i] >> lane & 1) & (mine < kSmpList))
+          g.list[mine] = smp_comp(key_of(v[i]), here + ((i / N) * 64 + lane) * N + i % N);
+        at += (uint32_t)__popcll(hit[i]);
       }
     }
     __syncthreads();
@@ -837,39 +1031,34 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
       smp_scan_row(a, r, row, s);
       return;
     }
-    // the listed elements of bins lo .. hi, as a range of smp_comp
-    auto range = [&](int lo, int hi, uint64_t* from, uint64_t* to) {
-      __syncthreads();
-      if (t == 0) g.lo = ~0ull, g.hi = 0;
-      __syncthreads();
-      uint64_t f = ~0ull, l = 0;
-      for (int i = t; i < n; i += kSmpThreads) {
-        const uint64_t e = g.list[i];
-        const int d = bin_at(of_key((uint32_t)(e >> 32)));
-        if (d < lo || d > hi) continue;
-        f = e < f ? e : f;
-        l = e > l ? e : l;
-      }
-      if (l) {
-        atomicMin((unsigned long long*)&g.lo, (unsigned long long)f);
-        atomicMax((unsigned long long*)&g.hi, (unsigned long long)l);
-      }
-      __syncthreads();
-      *from = g.lo, *to = g.hi;
-    };
+    if (small) {
+      smp_small(a, r, row, n, g, s);
+      return;
+    }
     if (!q_only && (by_k || by_p)) {
+      // (the bins' range in smp_comp, or more: the bins' numbers decide)
+      constexpr float kMost = 3.402823466e38f;
+      auto lowest = [&](int d) {
+        float x = (anchor - (float)(d + 1)) / scale;
+        x -= fabsf(x) * 0x1p-20f;
+        return d >= kBins - 1 ? 1ull : smp_comp(key_of(x > -kMost ? x : -kMost), 0xffffffffu);
+      };
+      auto highest = [&](int d) {
+        float x = (anchor - (float)(d - 2)) / scale;
+        x += fabsf(x) * 0x1p-20f;
+        return smp_comp(key_of(x < kMost ? x : kMost), 0);
+      };
       double mass_k = all;
-      uint64_t lo, hi;
-      if (by_k) {
-        range(kb, kb, &lo, &hi);
-        border = smp_select<0>(r, g, s, n, lo, hi, k_ahead, k_ahead_n, (uint32_t)r.k, 0.0, &mass_k);
-      }
-      if (by_p) {
-        range(p_lo, p_hi, &lo, &hi);
-        if (lo < border) lo = border;
+#pragma unroll 1
+      for (int by = by_k ? 0 : 1; by < (by_p ? 2 : 1); by++) {   // K's border, then P's
         // (what is not in K is behind its border)
-        double ignored;
-        border = smp_select<1>(r, g, s, n, lo, hi, p_ahead, 0, 0, p * mass_k, &ignored);
+        const int b0 = by ? p_lo : kb, b1 = by ? p_hi : kb;
+        uint64_t lo = lowest(b1);
+        lo = lo > border ? lo : border;
+        double incl;
+        border = smp_select(by == 0, r, g, s, n, bin_at, b0, b1, lo, highest(b0), by ? p_ahead : k_ahead, by ? 0 : k_ahead_n,
+                            (uint32_t)r.k, p * mass_k, &incl);
+        mass_k = incl;
       }
     }
     // the chunks' kept mass: whole groups and bins, and what is listed (without any
@@ -880,7 +1069,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
         double m = 0.0;
         if (jj >= 0) {
           if (b < d_lo % kGroup) m = (double)a.masses[(row * C + c) * kBins + jj * kGroup + b];
-          if (b < jj) m += (double)heads[c].group_mass[b];
+          if (b < jj) m += (double)g.gmass[c][b];
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) m += __shfl_xor(m, off, 32);
@@ -888,9 +1077,9 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
       }
       for (int i = t; i < n; i += kSmpThreads) {
         const uint64_t e = g.list[i];
-        const float v = of_key((uint32_t)(e >> 32));
-        if (e < border || bin_at(v) < d_lo) continue;
-        const double w = smp_w(r, v);
+        const float x = of_key((uint32_t)(e >> 32));
+        if (e < border || bin_at(x) < d_lo) continue;
+        const double w = smp_w(r, x);
         if (w < r.min_w) continue;
         const int idx = (int)~(uint32_t)e;
         atomicAdd(&g.add[(idx + lead) / RLXQ_SAMPLE_CHUNK], (unsigned long long)(w * 0x1p50 + 0.5));
@@ -905,10 +1094,9 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   const double target = (double)r.u * total;
   if (t == 0) s.found = 0x7fffffff, s.last = -1;
   __syncthreads();
-  if (m > 0.0) {
-    atomicMax(&s.last, t);
-    if (incl > target) atomicMin(&s.found, t);
-  }
+  const uint64_t some = __ballot(m > 0.0), past = __ballot(m > 0.0 && incl > target);
+  if (lane == 0 && some) atomicMax(&s.last, t + 63 - __builtin_clzll(some));
+  if (lane == 0 && past) atomicMin(&s.found, t + __builtin_ctzll(past));
   __syncthreads();
   const int c = s.found != 0x7fffffff ? s.found : (s.last > 0 ? s.last : 0);
   if (t == c) g.before = incl - m;
@@ -916,25 +1104,27 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   constexpr int kPer = RLXQ_SAMPLE_CHUNK / kSmpThreads;
   const int first = c * RLXQ_SAMPLE_CHUNK - lead;
   float v[kPer];
-  double w[kPer], mine = 0.0;
-  int last = -1;
   smp_ld_chunk<BF, kPer / N>(a, row, first, t * (kPer / N), 1, v);
+  float* mine = reinterpret_cast<float*>(g.list) + t;   // (its elements, kSmpThreads apart; nothing listed is read any more)
 #pragma unroll
+  for (int j = 0; j < kPer; j++) mine[j * kSmpThreads] = v[j];
+  double kept = 0.0;
+  int last = -1;
+#pragma unroll 4
   for (int j = 0; j < kPer; j++) {
-    const int i = first + t * kPer + j;
-    w[j] = smp_kept(r, border, v[j], i);
-    mine += w[j];
-    if (w[j] > 0.0) last = i;
+    const double w = smp_kept(r, border, mine[j * kSmpThreads], first + t * kPer + j);
+    kept += w;
+    if (w > 0.0) last = first + t * kPer + j;
   }
-  smp_choose(a, r, row, mine, last, g.before, total, s, [&](double sum, double target) {
-    int tok = last;
-    bool past = false;
-#pragma unroll
+  smp_choose(a, r, row, kept, last, g.before, total, s, [&](double sum, double goal) {
     for (int j = 0; j < kPer; j++) {
-      sum += w[j];
-      if (!past && sum > target && w[j] > 0.0) tok = first + t * kPer + j, past = true;
+      const int i = first + t * kPer + j;
+      if (i == last) break;
+      const double w = smp_kept(r, border, mine[j * kSmpThreads], i);
+      sum += w;
+      if (sum > goal && w > 0.0) return i;
     }
-    return tok;
+    return last;
   });
 }
 
@@ -959,6 +1149,7 @@ extern "C" __global__ __launch_bounds__(kSmpThreads) void rlxq_sample_scan(rlxq_
   }
   smp_best(best, bad, s.r64, s.r32);
   SmpRow r;
+  smp_settings(a, row, r);
   if (smp_row(a, row, best, bad, r)) smp_scan_row(a, r, row, s);
 }
 

@@ -16,7 +16,8 @@ typedef struct rlxq_sample_chunk {
   uint64_t best;      /* largest (key, falling index) of the chunk; 0: all masked */
   uint64_t mass;      /* its weights over its own largest, in 2^-48            */
   uint32_t bad;       /* holds a NaN or +inf                                   */
-  uint32_t count;     /* elements that are not masked                          */
+  uint32_t count;     /* elements that are not masked (rows with top_k)        */
+  float tops[4];      /* the largest logit of each quarter                     */
   uint64_t group_mass[RLXQ_SAMPLE_GROUPS];    /* (rows with a border)          */
   uint32_t group_count[RLXQ_SAMPLE_GROUPS];   /* (rows with top_k)             */
 } rlxq_sample_chunk;
@@ -32,7 +33,7 @@ typedef struct rlxq_sample_args {
   float* probs;              /* [M], or NULL                                  */
   int64_t M;
   int32_t V, bf16;
-  int32_t chunks, pad;       /* of a row                                      */
+  int32_t chunks, per;       /* of a row; of a workgroup                      */
   rlxq_sample_chunk* heads;  /* [M, chunks]                                   */
   uint64_t* masses;          /* [M, chunks, BINS]                             */
   uint16_t* counts;          /* [M, chunks, BINS]                             */

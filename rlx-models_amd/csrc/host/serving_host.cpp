@@ -100,12 +100,14 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   const int64_t used = std::min<int64_t>(num_adapters, m);
   const int64_t tiles = many ? m / RLXQ_LORA_ROWS + std::min<int64_t>(num_adapters + 1, m) : m;
   g.max_tiles = (int32_t)tiles;
-  // v: slices of K until there are two workgroups a CU, of 512 elements at least
+  // v: slices of K until there are two workgroups a CU (few rows, whose workgroups
+  // are small: six), of 512 elements at least; no more than eight, which every
+  // workgroup of y adds up (33 rows 12288 -> 4096, 24 slices 19.6 us, 8 17.4)
   const int64_t sr = segs * rank;
   g.jblocks = (int32_t)((sr + (many ? 63 : 15)) / (many ? 64 : 16));
   const int64_t rows_wgs = many ? (m + RLXQ_LORA_ROWS - 1) / RLXQ_LORA_ROWS : used;
   const int64_t likely = rows_wgs * g.jblocks;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((many ? 2 : 6) * cus / likely, k / 512));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({(many ? 2 : 6) * cus / likely, k / 512, RLXQ_LORA_SPLITS}));
   g.kslice = (int32_t)(((k + want - 1) / want + 127) / 128 * 128);
   g.splits = (int32_t)((k + g.kslice - 1) / g.kslice);
   // y: 256 columns a workgroup, or up to 1024 while there are four workgroups a CU

@@ -12,8 +12,8 @@
 // the results of one activation row lie on one lane: v leaves as 16-byte pieces,
 // y's columns are dealt to the tiles so that a lane holds 16 neighbouring ones.
 //
-// Types: x and A both bf16 use the bf16 MFMA; otherwise the f32 one, on the
-// values as they are.  v stays f32; against bf16 B it takes part as bf16 terms,
+// Types: the bf16 MFMA, f32 x and A as three bf16 terms each (all of their bits).
+// v stays f32; against bf16 B it takes part as bf16 terms,
 // three (all of its bits) for f32 y, two (2^-17 of it at most left out) for bf16
 // y, whose own rounding is 2^-9.  Sums are f32, y is rounded once.
 #include "common.hip.h"
@@ -124,11 +124,53 @@ RLXQ_DEV bool lr_tile(const rlxq_lora_args& a, int index, int* rows, uint64_t* m
   return true;
 }
 
+// Eight f32 as three bf16 terms that add up to them: a float's 24 significant bits
+// cut into eights (cut, not rounded: no term can exceed the float).
+RLXQ_DEV void lr_cut(const LrFrag<false>& f, uint4* term) {
+  uint32_t v[8] = {f.q[0].x, f.q[0].y, f.q[0].z, f.q[0].w, f.q[1].x, f.q[1].y, f.q[1].z, f.q[1].w};
+#pragma unroll
+  for (int s = 0; s < 3; s++) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      w[j] = perm_b32(v[2 * j + 1], v[2 * j], 0x07060302u);   // the upper halves
+#pragma unroll
+      for (int i = 2 * j; i < 2 * j + 2; i++)
+        v[i] = __float_as_uint(__uint_as_float(v[i]) - __uint_as_float(v[i] & 0xffff0000u));
+    }
+    term[s] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+// The bf16 terms of a fragment: itself, or three.
+template <bool BF>
+struct LrTerms {
+  uint4 t[BF ? 1 : 3];
+};
+template <bool BF>
+RLXQ_DEV LrTerms<BF> lr_terms(const LrFrag<BF>& f) {
+  LrTerms<BF> r;
+  if constexpr (BF) r.t[0] = f.q[0];
+  else lr_cut(f, r.t);
+  return r;
+}
+// acc += the products of 32 k, term by term (of the last ones, 2^-30 of the first
+// at most, none).
+template <bool AB, bool XB>
+RLXQ_DEV lr_f4 lr_products(const LrTerms<AB>& a, const LrTerms<XB>& x, lr_f4 acc) {
+#pragma unroll
+  for (int i = 0; i < (AB ? 1 : 3); i++)
+#pragma unroll
+    for (int j = 0; j < (XB ? 1 : 3); j++)
+      if (i + j < 4)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lr_bf8, a.t[i]), __builtin_bit_cast(lr_bf8, x.t[j]), acc,
+                                                      0, 0, 0);
+  return acc;
+}
+
 // v of 16 FR rows and 16 RT rows of A, one slice of K: the waves take a quarter
 // of it each and join their sums in LDS.
 template <bool XB, bool AB, bool LIST, int FR, int RT>
 RLXQ_DEV void lr_shrink(const rlxq_lora_args& a) {
-  constexpr bool BF = XB && AB;
   __shared__ int rows[RLXQ_LORA_ROWS];
   __shared__ uint64_t masks[4];
   __shared__ lr_f4 part[4][RT * FR][64];
@@ -160,24 +202,34 @@ RLXQ_DEV void lr_shrink(const rlxq_lora_args& a) {
   for (int j = 0; j < RT; j++)
 #pragma unroll
     for (int f = 0; f < FR; f++) acc[j][f] = (lr_f4){0.f, 0.f, 0.f, 0.f};
-  constexpr int U = FR * RT == 1 ? 4 : 2;   // steps of 32 whose loads are on their way together
-  for (int64_t k = w0; k < w1; k += 32 * U) {
-    LrFrag<BF> xf[U][FR], af[U][RT];
+  constexpr int U = FR * RT == 1 ? 4 : (XB && AB ? 2 : 1);   // steps of 32 whose loads are on their way together
+  LrFrag<XB> xf[U][FR];
+  LrFrag<AB> af[U][RT];
+  auto fetch = [&](int64_t k) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int64_t at = k + 32 * u + kk;
       const bool in = at < w1;   // (K is whole eights)
 #pragma unroll
-      for (int f = 0; f < FR; f++) xf[u][f] = in && xon[f] ? lr_load<BF, XB>(a.x, xrow[f] + at) : lr_zero<BF>();
+      for (int f = 0; f < FR; f++) xf[u][f] = in && xon[f] ? lr_load<XB, XB>(a.x, xrow[f] + at) : lr_zero<XB>();
 #pragma unroll
-      for (int j = 0; j < RT; j++) af[u][j] = in && aon[j] ? lr_load<BF, AB>(a.a, arow[j] + at) : lr_zero<BF>();
+      for (int j = 0; j < RT; j++) af[u][j] = in && aon[j] ? lr_load<AB, AB>(a.a, arow[j] + at) : lr_zero<AB>();
     }
+  };
+  for (int64_t k = w0; k < w1; k += 32 * U) {
+    fetch(k);
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int u = 0; u < U; u++) {
+      LrTerms<XB> xt[FR];
 #pragma unroll
-      for (int j = 0; j < RT; j++)
+      for (int f = 0; f < FR; f++) xt[f] = lr_terms<XB>(xf[u][f]);
 #pragma unroll
-        for (int f = 0; f < FR; f++) acc[j][f] = lr_mfma<BF>(af[u][j], xf[u][f], acc[j][f]);
+      for (int j = 0; j < RT; j++) {
+        const LrTerms<AB> at = lr_terms<AB>(af[u][j]);
+#pragma unroll
+        for (int f = 0; f < FR; f++) acc[j][f] = lr_products<AB, XB>(at, xt[f], acc[j][f]);
+      }
+    }
   }
 #pragma unroll
   for (int j = 0; j < RT; j++)
@@ -289,20 +341,18 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
     if (row < count && r < rank) {
       const float* p = a.v + (int64_t)rows[row] * sr + seg * a.R + r;
       const int64_t step = a.M * sr;
-      // (slices in order, four of them on their way; past the last: the last, not added)
-      for (int q0 = 0; q0 < a.splits; q0 += 4) {
-        float4 lo[4], hi[4];
+      // (slices in order, all on their way at once; past the last: the last, not added)
+      float4 lo[RLXQ_LORA_SPLITS], hi[RLXQ_LORA_SPLITS];
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const float* at = p + (q0 + q < a.splits ? q0 + q : a.splits - 1) * step;
-          lo[q] = reinterpret_cast<const float4*>(at)[0], hi[q] = reinterpret_cast<const float4*>(at)[1];
-        }
+      for (int q = 0; q < RLXQ_LORA_SPLITS; q++) {
+        const float* at = p + (q < a.splits ? q : a.splits - 1) * step;
+        lo[q] = reinterpret_cast<const float4*>(at)[0], hi[q] = reinterpret_cast<const float4*>(at)[1];
+      }
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          if (q0 + q >= a.splits) break;
-          v[0] += lo[q].x, v[1] += lo[q].y, v[2] += lo[q].z, v[3] += lo[q].w;
-          v[4] += hi[q].x, v[5] += hi[q].y, v[6] += hi[q].z, v[7] += hi[q].w;
-        }
+      for (int q = 0; q < RLXQ_LORA_SPLITS; q++) {
+        if (q >= a.splits) break;
+        v[0] += lo[q].x, v[1] += lo[q].y, v[2] += lo[q].z, v[3] += lo[q].w;
+        v[4] += hi[q].x, v[5] += hi[q].y, v[6] += hi[q].z, v[7] += hi[q].w;
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] = r + j < rank ? v[j] * scale : 0.f;

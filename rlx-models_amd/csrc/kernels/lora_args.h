@@ -6,6 +6,7 @@
 
 #define RLXQ_LORA_SEGS 4           /* most column segments of a call            */
 #define RLXQ_LORA_MAX_RANK 256
+#define RLXQ_LORA_SPLITS 8         /* most slices of K                          */
 #define RLXQ_LORA_MAX_ADAPTERS 16384
 #define RLXQ_LORA_ROWS 64          /* rows of a tile past that                  */
 #define RLXQ_LORA_FEW 256          /* rows whose tiles every workgroup finds    */

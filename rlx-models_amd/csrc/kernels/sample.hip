@@ -1132,27 +1132,6 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
 
 using namespace rlxq;
 
-// A workgroup a row.
-extern "C" __global__ __launch_bounds__(kSmpThreads) void rlxq_sample_scan(rlxq_sample_args a) {
-  __shared__ SmpShared s;
-  const int64_t row = blockIdx.x;
-  const int t = threadIdx.x;
-  // the largest logit, the lowest index that has it; NaN and +inf
-  uint64_t best = 0;
-  uint32_t bad = 0;
-  for (int i = t; i < a.V; i += kSmpThreads) {
-    const float v = smp_ld(a, row, i);
-    if (!(v < __builtin_inff())) bad = 1;
-    const uint32_t key = key_of(v);
-    const uint64_t c = key ? smp_comp(key, i) : 0;
-    best = c > best ? c : best;
-  }
-  smp_best(best, bad, s.r64, s.r32);
-  SmpRow r;
-  smp_settings(a, row, r);
-  if (smp_row(a, row, best, bad, r)) smp_scan_row(a, r, row, s);
-}
-
 extern "C" __global__ __launch_bounds__(kHistThreads) void rlxq_sample_hist_f32(rlxq_sample_args a) { smp_hist<0>(a); }
 extern "C" __global__ __launch_bounds__(kHistThreads) void rlxq_sample_hist_bf16(rlxq_sample_args a) { smp_hist<1>(a); }
 extern "C" __global__ __launch_bounds__(kSmpThreads) void rlxq_sample_pick_f32(rlxq_sample_args a) { smp_pick<0>(a); }

@@ -258,6 +258,40 @@ def test_lora_offsets_past_32_bits(srv):
     assert float(base[m - 1, n - 1]) == 64.0 and not bool(base[:m - 1].any()) and not bool(base[m - 1, :n - 1].any())
 
 
+@pytest.mark.parametrize("m,e", [(300, 16384), (40, 16384), (257, 1), (700, 699)])
+def test_lora_many_adapters(srv, m, e):
+    """The most adapters a call takes, rows of nearly as many; and one for all."""
+    import torch
+
+    announce(f"lora many adapters m={m} e={e}")
+    d = _lora_case(m + e, m, 16, 24, 8, e, "bf16", "bf16", "f32", ints=True, ranks=True)
+    d["ids"][: m // 2] = e - 1
+    y = _run_lora(srv, d, None)
+    torch.cuda.synchronize()
+    assert torch.equal(y.cpu(), _lora_f64(d, None)[0].float())
+
+
+def test_lora_values_of_every_size(srv):
+    """f32 x and A take part in bf16 terms: tiny, large and mixed magnitudes, signed zeros."""
+    import torch
+
+    announce("lora f32 magnitudes")
+    for m in (5, 300):
+        for x, ab in (("f32", "f32"), ("f32", "bf16"), ("bf16", "f32")):
+            d = _lora_case(m, m, 256, 40, 16, 2, x, ab, "f32")
+            g = _gen(m + 1)
+            size = torch.exp2(torch.randint(-60, 61, (m, 1), generator=g).float())
+            d["x"] = (d["x"].float() * size).to(_dt(x))
+            d["x"][:, ::7] = -0.0
+            d["a"] = (d["a"].float() * torch.exp2(torch.randint(-20, 21, (2, 16, 1), generator=g).float())).to(_dt(ab))
+            d["base"].zero_()
+            y = _run_lora(srv, d, None)
+            torch.cuda.synchronize()
+            want, mag, _ = _lora_f64(d, None)
+            tol = (256 / 8 + 16 + 40) * U32 * mag + U32 * want.abs() + 1e-30
+            assert bool(((y.cpu().double() - want).abs() <= tol).all())
+
+
 # ---- residual norm ---------------------------------------------------------
 def _norm_case(seed, rows, h, bdt, rdt, gdt, wdt, gate_rows, post, pre, block=True, resid=True):
     import torch
@@ -556,6 +590,50 @@ def test_sample_unaligned_and_rows_behind(srv):
             t, p, q, u = (np.asarray(x, np.float32) for x in (t, p, q, u))
             want = [_sample_row(l[i].float().cpu().numpy(), t[i], k[i], p[i], q[i], u[i])[0] for i in range(5)]
             assert tok.tolist() == want + [99, 99] and pr[5:].tolist() == [99.0, 99.0]
+
+
+def test_sample_hot_rows_with_masked_tokens(srv):
+    """Temperatures past every difference of the logits: the tokens that are not
+    masked alike, the masked ones none."""
+    import torch
+
+    announce("sample hot rows")
+    rng = np.random.default_rng(21)
+    for v in (300, 9000):
+        l = np.where(rng.random((8, v)) < 0.5, -np.inf, 5 * rng.standard_normal((8, v))).astype(np.float32)
+        _check_sample(srv, torch.from_numpy(l), [np.inf, 1e37, 3e38, 1e36, np.inf, 1e30, np.inf, 1e38],
+                      [0, 0, 7, 0, v - 1, 0, 0, 100], [1, 0.5, 1, 1, 0.25, 0.75, 1, 0.5], [0, 0, 0, 0.5, 0, 0, 1, 0],
+                      rng.random(8))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_sample_largest_vocabulary(srv, dt):
+    """2^20 tokens, rows that start inside 16 bytes; flat ones among them."""
+    import torch
+
+    announce(f"sample 2^20 {dt}")
+    v, rng = 1 << 20, np.random.default_rng(31)
+    buf = torch.zeros(5 * v + 1, dtype=_dt(dt), device="cuda")
+    l = torch.from_numpy(rng.standard_normal((5, v)).astype(np.float32)).to(_dt(dt))
+    buf[1:] = l.view(-1).cuda()
+    t, k, p, q, u = [1.0, 0.7, 8.0, 1.0, 1.3], [0, 700000, 0, 300, 0], [1.0, 0.9, 0.8, 1.0, 0.97], [0, 0, 0, 0, 1e-3], rng.random(5)
+    f = lambda a, d: torch.tensor(a, dtype=d).cuda()   # noqa: E731
+    tok, _ = srv.sample(buf[1:].view(5, v), f(u, torch.float32), temperature=f(t, torch.float32), top_k=f(k, torch.int32),
+                        top_p=f(p, torch.float32), min_p=f(q, torch.float32))
+    torch.cuda.synchronize()
+    t, p, q, u = (np.asarray(x, np.float32) for x in (t, p, q, u))
+    assert tok.tolist() == [_sample_row(l[i].float().numpy(), t[i], k[i], p[i], q[i], u[i])[0] for i in range(5)]
+
+
+def test_sample_rows_past_a_batch(srv):
+    """More rows than one pair of launches takes."""
+    import torch
+
+    announce("sample rows past a batch")
+    rng = np.random.default_rng(41)
+    rows, v = 26000, 9   # (a row of one chunk takes 5.3 KB of the 128 MB)
+    logits = torch.from_numpy(rng.standard_normal((rows, v)).astype(np.float32))
+    _check_sample(srv, logits, *_settings(rng, rows, v))
 
 
 def test_sample_repeats_itself(srv):

@@ -239,16 +239,18 @@ int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t row
   const int64_t row_bytes = g.chunks * (int64_t)(sizeof(rlxq_sample_chunk) + RLXQ_SAMPLE_BINS * (8 + 2));
   const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
   const int64_t batch = std::min<int64_t>(rows, std::max<int64_t>(1, (128 << 20) / row_bytes));
+  const size_t b_heads = ((size_t)(batch * g.chunks) * sizeof(rlxq_sample_chunk) + 255) & ~(size_t)255;
   void* ws = nullptr;
-  int rc = workspace(ctx, (size_t)(batch * row_bytes), &ws, stream);
+  int rc = workspace(ctx, b_heads + (size_t)(batch * g.chunks) * RLXQ_SAMPLE_BINS * (8 + 2), &ws, stream);
   if (rc) return rc;
   g.heads = static_cast<rlxq_sample_chunk*>(ws);
-  g.masses = reinterpret_cast<uint64_t*>(g.heads + batch * g.chunks);
+  g.masses = reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + b_heads);
   g.counts = reinterpret_cast<uint16_t*>(g.masses + batch * g.chunks * RLXQ_SAMPLE_BINS);
   for (int64_t at = 0; at < rows; at += batch) {
     g.M = std::min(batch, rows - at);
-    // (a chunk each, or up to four while there are six workgroups a CU)
-    g.per = (int32_t)std::max<int64_t>(1, std::min<int64_t>(4, g.M * g.chunks / (6 * cus)));
+    // A chunk a workgroup, or up to three while there are six workgroups a CU (256
+    // rows of 128000: one 61 us, two 55, three 45, four 53, five 48).
+    g.per = (int32_t)std::max<int64_t>(1, std::min<int64_t>(3, g.M * g.chunks / (6 * cus)));
     g.logits = static_cast<const char*>(logits) + at * vocab * (bf ? 2 : 4);
     if (temperature) g.temperature = temperature + at;
     if (top_k) g.top_k = top_k + at;
@@ -257,7 +259,8 @@ int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t row
     g.u = u + at;
     g.tokens = tokens + at;
     if (probs) g.probs = probs + at;
-    if ((rc = run_kernel(ctx, bf ? "rlxq_sample_hist_bf16" : "rlxq_sample_hist_f32", g.M * ((g.chunks + g.per - 1) / g.per), RLXQ_SAMPLE_CHUNK / 16, 0, &g, stream)) ||
+    const int64_t hist = g.M * ((g.chunks + g.per - 1) / g.per);
+    if ((rc = run_kernel(ctx, bf ? "rlxq_sample_hist_bf16" : "rlxq_sample_hist_f32", hist, RLXQ_SAMPLE_CHUNK / 16, 0, &g, stream)) ||
         (rc = run_kernel(ctx, bf ? "rlxq_sample_pick_bf16" : "rlxq_sample_pick_f32", g.M, 512, 0, &g, stream)))
       return rc;
   }

@@ -1132,7 +1132,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
 
 using namespace rlxq;
 
-extern "C" __global__ __launch_bounds__(kHistThreads) void rlxq_sample_hist_f32(rlxq_sample_args a) { smp_hist<0>(a); }
-extern "C" __global__ __launch_bounds__(kHistThreads) void rlxq_sample_hist_bf16(rlxq_sample_args a) { smp_hist<1>(a); }
+extern "C" __global__ __launch_bounds__(kHistThreads, 4) void rlxq_sample_hist_f32(rlxq_sample_args a) { smp_hist<0>(a); }
+extern "C" __global__ __launch_bounds__(kHistThreads, 4) void rlxq_sample_hist_bf16(rlxq_sample_args a) { smp_hist<1>(a); }
 extern "C" __global__ __launch_bounds__(kSmpThreads) void rlxq_sample_pick_f32(rlxq_sample_args a) { smp_pick<0>(a); }
 extern "C" __global__ __launch_bounds__(kSmpThreads) void rlxq_sample_pick_bf16(rlxq_sample_args a) { smp_pick<1>(a); }

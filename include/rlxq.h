@@ -334,7 +334,10 @@ int rlxq_swiglu(rlxq_ctx* ctx, const void* gu, int gu_dtype, int64_t rows,
  * [num_adapters] int32 (clamped to [0, rank]; what a and b hold past them is
  * not used) or NULL: rank; scales [num_adapters] f32 or NULL: 1; base and y
  * [m, n] of y_dtype.  seg_ends: host array of segs (1 to 4) column ends, rising
- * to n; NULL with segs = 1.  v and the sums are f32; y is rounded once.
+ * to n; NULL with segs = 1.  v and the sums are f32; y is rounded once.  A row of
+ * x that is not finite, or its adapter's a, b or scale, or a v that overflows,
+ * leaves the row of y not finite (NaN also where the sum would be an infinity) and
+ * the others alone.
  * k % 8 == 0, rank % 8 == 0 and at most 256; m, k, n up to 2^24;
  * num_adapters up to 16384; x, a, b 16-byte aligned.  With m = 0 or n = 0
  * nothing is read or written. */

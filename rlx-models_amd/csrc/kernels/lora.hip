@@ -16,6 +16,16 @@
 // v stays f32; against bf16 B it takes part as bf16 terms,
 // three (all of its bits) for f32 y, two (2^-17 of it at most left out) for bf16
 // y, whose own rounding is 2^-9.  Sums are f32, y is rounded once.
+//
+// What bounds it: many adapters at few rows, their bytes (64 rows of 48 adapters of
+// rank 64, 4096 -> 24576: v 13.4 us for 50 MB, y 41.6 for 157, 3.7 TB/s); one
+// adapter at one row, the two launches (4.0 and 6.6 us); prompts, base and y (4096
+// rows of 8 adapters, 4096 -> 24576: sort 7.6 us, v 26, y 137 for 503 MB with the
+// half of B that L2 no longer holds).  Tried on the last: tiles of 32 and 128 rows
+// (a tenth slower and more), 256, 512 and 2048 columns a workgroup (198, 170 and
+// 185 us of the call against 164 at 1024), B's sharers on one XCD (145 us for y against
+// 136: fewer columns at a time reach fewer memory channels), B's next rows not ahead
+// of their use and accesses past the caches (within 3%).
 #include "common.hip.h"
 #include "lora_args.h"
 
@@ -43,20 +53,13 @@ RLXQ_DEV LrFrag<BF> lr_zero() {
   if constexpr (!BF) f.q[1] = f.q[0];
   return f;
 }
-// From element i of p, of type bf16 (MEM) or f32, as BF.
-template <bool BF, bool MEM>
+// From element i of p.
+template <bool BF>
 RLXQ_DEV LrFrag<BF> lr_load(const void* p, int64_t i) {
-  static_assert(MEM || !BF, "no rounding here");
   LrFrag<BF> f;
-  const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + i * (MEM ? 2 : 4));
+  const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + i * (BF ? 2 : 4));
   f.q[0] = s[0];
-  if constexpr (!MEM) {
-    f.q[1] = s[1];
-  } else if constexpr (!BF) {
-    const uint4 w = f.q[0];
-    f.q[0] = make_uint4(w.x << 16, w.x & 0xffff0000u, w.y << 16, w.y & 0xffff0000u);
-    f.q[1] = make_uint4(w.z << 16, w.z & 0xffff0000u, w.w << 16, w.w & 0xffff0000u);
-  }
+  if constexpr (!BF) f.q[1] = s[1];
   return f;
 }
 // The first n of the eight, the others zero.
@@ -211,9 +214,9 @@ RLXQ_DEV void lr_shrink(const rlxq_lora_args& a) {
       const int64_t at = k + 32 * u + kk;
       const bool in = at < w1;   // (K is whole eights)
 #pragma unroll
-      for (int f = 0; f < FR; f++) xf[u][f] = in && xon[f] ? lr_load<XB, XB>(a.x, xrow[f] + at) : lr_zero<XB>();
+      for (int f = 0; f < FR; f++) xf[u][f] = in && xon[f] ? lr_load<XB>(a.x, xrow[f] + at) : lr_zero<XB>();
 #pragma unroll
-      for (int j = 0; j < RT; j++) af[u][j] = in && aon[j] ? lr_load<AB, AB>(a.a, arow[j] + at) : lr_zero<AB>();
+      for (int j = 0; j < RT; j++) af[u][j] = in && aon[j] ? lr_load<AB>(a.a, arow[j] + at) : lr_zero<AB>();
     }
   };
   for (int64_t k = w0; k < w1; k += 32 * U) {
@@ -319,7 +322,7 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
 #pragma unroll
       for (int s = 0; s < STEPS; s++) {
         const int r = 32 * s + kk;
-        dst[s][q] = on && r < rank ? lr_load<BB, BB>(a.b, row + r) : lr_zero<BB>();
+        dst[s][q] = on && r < rank ? lr_load<BB>(a.b, row + r) : lr_zero<BB>();
       }
     }
   };

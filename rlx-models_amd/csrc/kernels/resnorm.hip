@@ -7,6 +7,9 @@
 //
 // f32 arithmetic and statistics; sum and y are each rounded once, from the f32
 // h (y's norm is that of the unrounded sum).
+//
+// Bound by memory: 16384 x 4096 bf16 in 107 us for 537 MB, the rate of a copy (with
+// its workgroups going on from row to row, the next row on its way, it took 134); 197 x 5120 in 6.0, one row in 2.6, by the latency of two sums.
 #include "common.hip.h"
 #include "resnorm_args.h"
 

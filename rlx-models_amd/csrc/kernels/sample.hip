@@ -329,6 +329,16 @@ RLXQ_DEV void smp_scan_row(const rlxq_sample_args& a, const SmpRow& r, int64_t r
 // only the chunks that hold anything in those bins; what it finds there is
 // listed and settles the borders.  More than the list holds (rows as flat as
 // noise): smp_scan_row.
+//
+// What bounds it: the first launch the vector unit and the loads' latency (256
+// rows of 128000 bf16, no borders: 45 us, 30 instructions an element, half of the
+// time issuing; 64 of 151936 f32, most of them with borders: 25, with the bins; 512
+// threads a chunk took a sixth more, and held to fewer registers it spilled); the
+// second a row's chain of dependent steps on one CU: 19 us for one row of 151936
+// with top-k 50; a row with min-p and 42 pieces 22 (settings and heads 3, groups and
+// bins 6, the pieces 6, their list, the border and the token 7); up to 50 where a
+// wide top-p reads the whole row again at a CU's 20 GB/s.  1024 threads were 8%
+// faster there and 10% slower for one row; more of its loads ahead changed nothing.
 
 constexpr int kBins = RLXQ_SAMPLE_BINS, kGroups = RLXQ_SAMPLE_GROUPS, kGroup = kBins / kGroups;
 constexpr int kHistThreads = RLXQ_SAMPLE_CHUNK / 16, kHistWaves = kHistThreads / 64;

@@ -89,97 +89,13 @@ RLXQ_DEV T smp_scan(T v, T* red, T* total) {
 }
 
 struct SmpShared {
-  uint64_t mass[2048];
-  uint32_t count[2048];
+  uint64_t mass[kSmpThreads + 8];
+  uint32_t count[kSmpThreads];
   uint64_t r64[16];
   double rd[16];
   uint32_t r32[16];
-  uint32_t pick, pick_count;
-  uint64_t pick_mass;
   int found, last, first_past[8], last_some[8];
 };
-
-// Border among the elements at or ahead of `within`: the one of rank `k` (BY =
-// 0, from 1), or the first at which the mass reaches `target` (BY = 1, in fixed
-// point).  Three passes over the row narrow its key digit by digit; equal keys
-// are told apart by their index.
-template <int BY>
-RLXQ_DEV uint64_t smp_radix(const rlxq_sample_args& a, const SmpRow& r, int64_t row, uint64_t within, double one,
-                            uint64_t need, SmpShared& s, uint64_t* above_mass) {
-  const int t = threadIdx.x;
-  uint32_t prefix = 0;
-  uint64_t above = 0, mass_above = 0;   // ranks or mass ahead of the digit's bin
-  int shift = 32;
-  for (int bits : {11, 11, 10}) {
-    shift -= bits;
-    const int bins = 1 << bits;
-    for (int i = t; i < bins; i += kSmpThreads) s.mass[i] = 0, s.count[i] = 0;
-    __syncthreads();
-    for (int i = t; i < a.V; i += kSmpThreads) {
-      const float v = smp_ld(a, row, i);
-      const uint32_t key = key_of(v);
-      if (!key || smp_comp(key, i) < within) continue;
-      if (shift + bits < 32 && (key >> (shift + bits)) != (prefix >> (shift + bits))) continue;
-      const uint32_t bin = (key >> shift) & (bins - 1);
-      atomicAdd(&s.count[bin], 1u);
-      atomicAdd((unsigned long long*)&s.mass[bin], (unsigned long long)(smp_w(r, v) * one + 0.5));
-    }
-    __syncthreads();
-    // bins from the top: thread t holds kPer of them, b0 the highest
-    constexpr int kPer = 2048 / kSmpThreads;
-    const int b0 = bins - 1 - kPer * t;
-    uint64_t m = 0, mt;
-    uint32_t c = 0, ct;
-    for (int j = 0; j < kPer; j++)
-      if (b0 - j >= 0) m += s.mass[b0 - j], c += s.count[b0 - j];
-    uint64_t mb = mass_above + smp_scan<uint64_t>(m, s.r64, &mt) - m;
-    uint64_t cb = above + smp_scan<uint32_t>(c, s.r32, &ct) - c;
-    const uint64_t all_c = above + ct;
-    for (int j = 0; j < kPer && b0 - j >= 0; j++) {
-      const uint64_t mj = s.mass[b0 - j], cj = s.count[b0 - j];
-      if (!cj) continue;
-      // (the last bin with anything in it ends the search where rounding left the
-      // target above the whole mass)
-      const bool here = BY == 0 ? cb < need && cb + cj >= need
-                                : (mb < need || cb == 0) && (mb + mj >= need || cb + cj == all_c);
-      if (here) s.pick = b0 - j, s.pick_mass = mb, s.pick_count = (uint32_t)cb;
-      mb += mj, cb += cj;
-    }
-    __syncthreads();
-    prefix |= s.pick << shift;
-    mass_above = s.pick_mass;
-    above = s.pick_count;
-    __syncthreads();
-  }
-  // equal keys: how many of them, then the index of the last
-  const uint64_t each = (uint64_t)(smp_w(r, of_key(prefix)) * one + 0.5);
-  uint64_t ties;
-  if (BY == 0) ties = need - above;
-  else ties = need <= mass_above || !each ? 1 : (need - mass_above + each - 1) / each;
-  if (ties < 1) ties = 1;
-  const int per = (a.V + kSmpThreads - 1) / kSmpThreads, lo = t * per, hi = lo + per < a.V ? lo + per : a.V;
-  uint32_t mine = 0, last = 0;
-  for (int i = lo; i < hi; i++) {
-    const uint32_t key = key_of(smp_ld(a, row, i));
-    if (key == prefix && smp_comp(key, i) >= within) mine++, last = i;
-  }
-  uint32_t all;
-  const uint32_t incl = smp_scan<uint32_t>(mine, s.r32, &all);
-  if (ties > all) ties = all;
-  if (mine && incl - mine < ties && incl >= ties) {
-    uint32_t n = incl - mine;
-    for (int i = lo; i < hi && n < ties; i++) {
-      const uint32_t key = key_of(smp_ld(a, row, i));
-      if (key == prefix && smp_comp(key, i) >= within) n++, last = i;
-    }
-    s.pick = last;
-  }
-  __syncthreads();
-  const uint32_t idx = s.pick;
-  __syncthreads();
-  *above_mass = mass_above + ties * each;
-  return smp_comp(prefix, idx);
-}
 
 // Whether a row with at least one token that is not masked keeps v at or ahead
 // of its border.
@@ -271,54 +187,6 @@ RLXQ_DEV bool smp_row(const rlxq_sample_args& a, int64_t row, uint64_t best, uin
   return true;
 }
 
-// A row by itself: the row read again for every digit of a border.
-RLXQ_DEV void smp_scan_row(const rlxq_sample_args& a, const SmpRow& r, int64_t row, SmpShared& s) {
-  const int t = threadIdx.x;
-  // fixed point: the whole row's mass below 2^62
-  const int lg = 32 - __builtin_clz((uint32_t)a.V);
-  const double one = (double)(1ull << (62 - lg));
-  uint64_t border = 1, mass = 0;   // every element that is not masked
-  if (r.k > 0 && r.k < a.V) {
-    // (fewer than k that are not masked: all of them)
-    uint32_t n = 0, all;
-    for (int i = t; i < a.V; i += kSmpThreads) n += key_of(smp_ld(a, row, i)) != 0;
-    (void)smp_scan<uint32_t>(n, s.r32, &all);
-    __syncthreads();
-    if ((uint32_t)r.k < all) border = smp_radix<0>(a, r, row, border, one, (uint64_t)r.k, s, &mass);
-  }
-  if (r.p < 1.0f) {
-    uint64_t m = 0;
-    for (int i = t; i < a.V; i += kSmpThreads) {
-      const float v = smp_ld(a, row, i);
-      const uint32_t key = key_of(v);
-      if (key && smp_comp(key, i) >= border) m += (uint64_t)(smp_w(r, v) * one + 0.5);
-    }
-    (void)smp_scan<uint64_t>(m, s.r64, &mass);
-    __syncthreads();
-    const double want = r.p > 0.0f ? (double)r.p * (double)mass : 0.0;
-    uint64_t need = (uint64_t)want;
-    need += (double)need < want;
-    border = smp_radix<1>(a, r, row, border, one, need, s, &mass);
-  }
-  // the kept mass in index order: every thread a run of the row
-  const int per = (a.V + kSmpThreads - 1) / kSmpThreads, lo = t * per, hi = lo + per < a.V ? lo + per : a.V;
-  double m = 0.0;
-  int last = -1;
-  for (int i = lo; i < hi; i++) {
-    const double w = smp_kept(r, border, smp_ld(a, row, i), i);
-    m += w;
-    if (w > 0.0) last = i;
-  }
-  smp_choose(a, r, row, m, last, 0.0, -1.0, s, [&](double c, double target) {
-    for (int i = lo; i < last; i++) {
-      c += smp_kept(r, border, smp_ld(a, row, i), i);
-      if (c > target) return i;
-    }
-    return last;
-  });
-}
-
-
 // ---- two launches: chunk histograms, then a workgroup a row ----------------
 //
 // The first reads the logits once: each workgroup a chunk of a row, in
@@ -327,8 +195,9 @@ RLXQ_DEV void smp_scan_row(const rlxq_sample_args& a, const SmpRow& r, int64_t r
 // lie on one grid, so the second launch adds them up (groups of 32 bins, then the
 // 32 of one group), finds the bin that each border falls into, and reads again
 // only the chunks that hold anything in those bins; what it finds there is
-// listed and settles the borders.  More than the list holds (rows as flat as
-// noise): smp_scan_row.
+// listed and settles the borders.  Where that is more than the list holds (rows as
+// flat as noise), the flagged chunks are gone through once more, which narrows the
+// border to what can be listed, and again for the kept mass.
 //
 // What bounds it: the first launch the vector unit and the loads' latency (256
 // rows of 128000 bf16, no borders: 45 us, 30 instructions an element, half of the
@@ -342,7 +211,7 @@ RLXQ_DEV void smp_scan_row(const rlxq_sample_args& a, const SmpRow& r, int64_t r
 
 constexpr int kBins = RLXQ_SAMPLE_BINS, kGroups = RLXQ_SAMPLE_GROUPS, kGroup = kBins / kGroups;
 constexpr int kHistThreads = RLXQ_SAMPLE_CHUNK / 16, kHistWaves = kHistThreads / 64;
-constexpr int kSmpList = 4096;
+constexpr int kSmpList = 8192;
 constexpr int kSmpSort = 512;   // kept elements that are sorted as a whole
 constexpr int kSmpChunks = RLXQ_SAMPLE_MAX_VOCAB / RLXQ_SAMPLE_CHUNK + 1;   // (a row may start inside 16 bytes)
 
@@ -638,13 +507,35 @@ RLXQ_DEV void smp_fine(const rlxq_sample_args& a, int64_t row, int j, bool by_k,
   __syncthreads();
 }
 
+// f of every element of the flagged chunks that is not masked, a thread's in
+// order of their index.
+template <int BF, class F>
+RLXQ_DEV void smp_each(const rlxq_sample_args& a, int64_t row, int lead, const SmpPick& g, F&& f) {
+  constexpr int N = BF ? 8 : 4, PER = RLXQ_SAMPLE_CHUNK / kSmpThreads;
+  const int x = threadIdx.x * (PER / N);
+  float v[PER], next[PER];   // (the next chunk is on its way)
+  smp_ld_chunk<BF, PER / N>(a, row, -lead, x, 1, next);
+#pragma unroll 1
+  for (int c = 0; c < a.chunks; c++) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] = next[j];
+    const int first = c * RLXQ_SAMPLE_CHUNK - lead;
+    if (c + 1 < a.chunks) smp_ld_chunk<BF, PER / N>(a, row, first + RLXQ_SAMPLE_CHUNK, x, 1, next);
+    if (!g.flag[c]) continue;
+#pragma unroll
+    for (int j = 0; j < PER; j++)
+      if (v[j] > -__builtin_inff()) f(smp_comp(key_of(v[j]), first + threadIdx.x * PER + j));
+  }
+}
+
 // The border among the listed elements of bins b_lo .. b_hi that are not smaller
-// than `lo` (as smp_comp): by_rank the one of rank `need`, else the last whose sum
+// than `lo` (as smp_comp), n of them, or (n above kSmpList) among those that
+// `each` goes through: by_rank the one of rank `need`, else the last whose sum
 // of the elements ahead is below `target`; base and base_n are what lies
 // ahead of all of them.  *incl: the sum down to the border.  Bins over the range
 // of what is left narrow it until a wave can sort it.
-template <class B>
-RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShared& s, int n, B&& bin_at, int b_lo, int b_hi, uint64_t lo,
+template <class B, class E>
+RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShared& s, int n, E&& each, B&& bin_at, int b_lo, int b_hi, uint64_t lo,
                              uint64_t hi, double base, uint32_t base_n, uint32_t need, double target, double* incl) {
   const int t = threadIdx.x, lane = t & 63;
   auto w_of = [&](uint64_t e) { return smp_w(r, of_key((uint32_t)(e >> 32))); };
@@ -654,12 +545,24 @@ RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShare
     return d >= b_lo && d <= b_hi;
   };
   uint32_t left = (uint32_t)n;   // at most so many
+  bool listed = n <= kSmpList;
   for (bool first = true;; first = false) {
     __syncthreads();
     if (t == 0) g.n_few = 0, g.lo = ~0ull, g.hi = 0, g.bin = 0;
     s.mass[t] = 0;
     s.count[t] = 0;
     __syncthreads();
+    if (!listed && left <= kSmpList) {
+      each([&](uint64_t e) {
+        if (within(e)) g.list[atomicAdd(&g.n_few, 1u)] = e;
+      });
+      __syncthreads();
+      n = (int)g.n_few;
+      listed = true;
+      __syncthreads();
+      if (t == 0) g.n_few = 0;
+      __syncthreads();
+    }
     if (left <= 64) {
       for (int i = t; i < n; i += kSmpThreads)
         if (within(g.list[i])) g.few[atomicAdd(&g.n_few, 1u)] = g.list[i];
@@ -698,12 +601,15 @@ RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShare
     }
     if (!first) {   // the elements' own range
       uint64_t e_lo = ~0ull, e_hi = 0;
-      for (int i = t; i < n; i += kSmpThreads) {
-        const uint64_t e = g.list[i];
-        if (!within(e)) continue;
+      auto range = [&](uint64_t e) {
+        if (!within(e)) return;
         e_lo = e < e_lo ? e : e_lo;
         e_hi = e > e_hi ? e : e_hi;
-      }
+      };
+      if (listed)
+        for (int i = t; i < n; i += kSmpThreads) range(g.list[i]);
+      else
+        each(range);
 #pragma unroll
       for (int off = 32; off; off >>= 1) {
         const uint64_t ol = __shfl_xor(e_lo, off, 64), oh = __shfl_xor(e_hi, off, 64);
@@ -718,16 +624,21 @@ RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShare
       lo = g.lo, hi = g.hi;
     }
     const int bits = hi > lo ? 64 - __builtin_clzll(hi - lo) : 1, shift = bits > 9 ? bits - 9 : 0;
-    for (int i = t; i < n; i += kSmpThreads) {
-      const uint64_t e = g.list[i];
-      if (!within(e)) continue;
+    // (fixed point: kSmpList, or a whole row, of weights up to 1 at most 2^63)
+    const double one = listed ? 0x1p50 : 0x1p42, unit = listed ? 0x1p-50 : 0x1p-42;
+    auto narrow = [&](uint64_t e) {
+      if (!within(e)) return;
       const uint32_t d = (uint32_t)((hi - e) >> shift);
-      atomicAdd((unsigned long long*)&s.mass[d], (unsigned long long)(w_of(e) * 0x1p50 + 0.5));
+      atomicAdd((unsigned long long*)&s.mass[d], (unsigned long long)(w_of(e) * one + 0.5));
       atomicAdd(&s.count[d], 1u);
-    }
+    };
+    if (listed)
+      for (int i = t; i < n; i += kSmpThreads) narrow(g.list[i]);
+    else
+      each(narrow);
     __syncthreads();
     const uint32_t c = s.count[t];
-    const double w = (double)s.mass[t] * 0x1p-50;
+    const double w = (double)s.mass[t] * unit;
     double wt;
     uint32_t ct;
     const double ahead = base + smp_scan<double>(w, s.rd, &wt) - w;
@@ -1037,10 +948,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
     }
     __syncthreads();
     const int n = (int)g.n;
-    if (n > kSmpList) {
-      smp_scan_row(a, r, row, s);
-      return;
-    }
+    auto each = [&](auto&& f) { smp_each<BF>(a, row, lead, g, f); };
     if (small) {
       smp_small(a, r, row, n, g, s);
       return;
@@ -1066,7 +974,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
         uint64_t lo = lowest(b1);
         lo = lo > border ? lo : border;
         double incl;
-        border = smp_select(by == 0, r, g, s, n, bin_at, b0, b1, lo, highest(b0), by ? p_ahead : k_ahead, by ? 0 : k_ahead_n,
+        border = smp_select(by == 0, r, g, s, n, each, bin_at, b0, b1, lo, highest(b0), by ? p_ahead : k_ahead, by ? 0 : k_ahead_n,
                             (uint32_t)r.k, p * mass_k, &incl);
         mass_k = incl;
       }
@@ -1085,15 +993,18 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
         for (int off = 16; off; off >>= 1) m += __shfl_xor(m, off, 32);
         if (c < C && b == 0) g.kept[c] = m * 0x1p-48 * g.scale[c];
       }
-      for (int i = t; i < n; i += kSmpThreads) {
-        const uint64_t e = g.list[i];
+      auto add = [&](uint64_t e) {
         const float x = of_key((uint32_t)(e >> 32));
-        if (e < border || bin_at(x) < d_lo) continue;
+        if (e < border || bin_at(x) < d_lo) return;
         const double w = smp_w(r, x);
-        if (w < r.min_w) continue;
+        if (w < r.min_w) return;
         const int idx = (int)~(uint32_t)e;
         atomicAdd(&g.add[(idx + lead) / RLXQ_SAMPLE_CHUNK], (unsigned long long)(w * 0x1p50 + 0.5));
-      }
+      };
+      if (n <= kSmpList)
+        for (int i = t; i < n; i += kSmpThreads) add(g.list[i]);
+      else
+        each(add);
     }
     __syncthreads();
   }

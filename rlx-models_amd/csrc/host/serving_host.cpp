@@ -89,7 +89,12 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   g.E = (int32_t)num_adapters;
   g.S = (int32_t)segs;
   const bool xb = x_dtype == RLXQ_BF16, ab = ab_dtype == RLXQ_BF16, yb = y_dtype == RLXQ_BF16;
-  const bool many = m > RLXQ_LORA_FEW;
+  // every workgroup finds its tile among up to 256 ids, a launch of the list less (bf16,
+  // rank 32, 64 rows of 16 adapters 4096 -> 6144 12.5 us against 16.9, 256 of 48 23.0
+  // against 24.2), unless columns are many and adapters few: a workgroup a row and 256
+  // columns then is mostly for nothing (192 rows -> 24576, 16 adapters 31.1 against
+  // 26.8, 48 34.6 against 53; 256 rows of 4 33.8 against 23.0)
+  const bool many = m > RLXQ_LORA_FEW || (m * n > (3 << 20) && 8 * num_adapters <= m);
   const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
   const int64_t per = yb ? 8 : 4;   // elements of 16 bytes
   g.vec = n % per == 0 && aligned(base, 16) && aligned(y, 16);
@@ -100,17 +105,19 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   const int64_t used = std::min<int64_t>(num_adapters, m);
   const int64_t tiles = many ? m / RLXQ_LORA_ROWS + std::min<int64_t>(num_adapters + 1, m) : m;
   g.max_tiles = (int32_t)tiles;
-  // v: slices of K until there are two workgroups a CU (few rows, whose workgroups
-  // are small: six), of 512 elements at least; no more than eight, which every
-  // workgroup of y adds up (33 rows 12288 -> 4096, 24 slices 19.6 us, 8 17.4)
+  // v: slices of K until there is a workgroup a CU (few rows, whose workgroups are
+  // small: six), of 512 elements at least (4096 rows 4096 -> 24576, rank 64, two slices
+  // 168 us, four 173; 1500 f32 rows of rank 256, one slice 259, two 227); no more than eight,
+  // which every workgroup of y adds up (33 rows 12288 -> 4096, 24 slices 19.6, 8 17.4)
   const int64_t sr = segs * rank;
   g.jblocks = (int32_t)((sr + (many ? 63 : 15)) / (many ? 64 : 16));
   const int64_t rows_wgs = many ? (m + RLXQ_LORA_ROWS - 1) / RLXQ_LORA_ROWS : used;
   const int64_t likely = rows_wgs * g.jblocks;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({(many ? 2 : 6) * cus / likely, k / 512, RLXQ_LORA_SPLITS}));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({many ? (cus + likely - 1) / likely : 6 * cus / likely, k / 512, RLXQ_LORA_SPLITS}));
   g.kslice = (int32_t)(((k + want - 1) / want + 127) / 128 * 128);
   g.splits = (int32_t)((k + g.kslice - 1) / g.kslice);
-  // y: 256 columns a workgroup, or up to 1024 while there are four workgroups a CU
+  // y: 256 columns a workgroup, or up to 1024 while there are four workgroups a CU (4096
+  // rows -> 24576 256 198 us of a call, 512 170, 1024 164, 2048 185; 777 rows -> 4096 48, 55, 67)
   g.cols = 256;
   while (g.cols < 1024 && rows_wgs * (n / (2 * g.cols)) >= 4 * cus) g.cols *= 2;
   int64_t cb = 0;
@@ -192,7 +199,8 @@ int rlxq_residual_norm(rlxq_ctx* ctx, const void* block, int block_dtype, const 
   for (const void* p : {block, resid, gate, post_weight, pre_weight, static_cast<const void*>(sum), static_cast<const void*>(y)})
     vec = vec && aligned(p, 16);
   if (!vec) return run_kernel(ctx, "rlxq_resnorm_any", rows, 256, 0, &g, stream);
-  // pieces of eight a thread
+  // pieces of eight a thread: two with many rows (512 of 5120 f32, a call with one piece
+  // 10.4 us, two 11.1; 2048 of 8192 bf16 31.1 against 28.7, four 30.6)
   const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
   const int64_t pieces = hidden / 8;
   const int ch = pieces > 1024 ? 4 : (pieces <= 64 || rows <= 2 * cus ? 1 : 2);

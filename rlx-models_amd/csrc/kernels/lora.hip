@@ -3,9 +3,9 @@
 //   v[i, g, r] = sum_k A[e, g R + r, k] x[i, k],   e = ids[i],
 // g(n) the segment of column n.
 //
-// Rows of one adapter are taken together, in tiles: up to RLXQ_LORA_FEW rows
+// Rows of one adapter are taken together, in tiles: of up to RLXQ_LORA_FEW rows
 // every workgroup finds its tile of 16 among the ids itself (a launch less), for
-// more a launch of one workgroup sorts the rows and cuts them into tiles of 64.
+// more a launch of one workgroup sorts the rows and cuts them into tiles of 32.
 // Two launches then: v (K over the waves of a workgroup and, where the
 // workgroups would be few, over workgroups), then y.  Both put the adapter's rows
 // on the long side of a 16x16 MFMA tile and the activation rows on the other, so
@@ -488,7 +488,7 @@ RLXQ_DEV int lr_take(int* count, int e) {
 }
 }  // namespace rlxq
 
-// The rows by adapter (those without one last), cut into tiles of up to 64: one
+// The rows by adapter (those without one last), cut into tiles of up to 32: one
 // workgroup; LDS holds a counter for each adapter.  The order of an adapter's
 // rows is that of the counters' atomics; no result depends on it.
 extern "C" __global__ __launch_bounds__(1024) void rlxq_lora_sort(rlxq_lora_args a) {
@@ -535,7 +535,7 @@ extern "C" __global__ __launch_bounds__(1024) void rlxq_lora_sort(rlxq_lora_args
   }
 }
 
-// _few: tiles of 16 rows that every workgroup finds; _many: of 64 from the list
+// _few: tiles of 16 rows that every workgroup finds; _many: of 32 from the list
 #define RLXQ_LORA_SHRINK(X, A, xn, an)                                                                                  \
   extern "C" __global__ __launch_bounds__(256) void rlxq_lora_shrink_##xn##_##an##_few(rlxq_lora_args a) {                \
     lr_shrink<X, A, false, 1, 1>(a);                                                                                    \

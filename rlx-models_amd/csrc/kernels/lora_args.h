@@ -8,8 +8,8 @@
 #define RLXQ_LORA_MAX_RANK 256
 #define RLXQ_LORA_SPLITS 8         /* most slices of K                          */
 #define RLXQ_LORA_MAX_ADAPTERS 16384
-#define RLXQ_LORA_ROWS 64          /* rows of a tile past that                  */
-#define RLXQ_LORA_FEW 256          /* rows whose tiles every workgroup finds    */
+#define RLXQ_LORA_ROWS 32          /* rows of a tile of the list                */
+#define RLXQ_LORA_FEW 256          /* most rows whose tiles every workgroup finds */
 
 /* Rows of one adapter that a workgroup takes together (prompts). */
 typedef struct rlxq_lora_tile {
@@ -28,7 +28,7 @@ typedef struct rlxq_lora_args {
   const void* base;        /* [M, N], or NULL (zero)                          */
   void* y;                 /* [M, N]                                          */
   float* v;                /* [splits, M, S * R]: A x, by slice of K          */
-  int32_t* order;          /* [M]: rows by adapter (M > RLXQ_LORA_FEW)        */
+  int32_t* order;          /* [M]: rows by adapter (with the list)            */
   rlxq_lora_tile* tiles;   /* [max_tiles], unused ones with count 0           */
   int64_t M, K, N;
   int32_t R, E, S;

@@ -773,3 +773,19 @@ def test_two_streams_at_once(srv, orc):
         torch.cuda.synchronize()
         for (_, out, _, _), w in zip(steps, want):
             assert all(torch.equal(out[k], w[k]) for k in out)
+
+
+@pytest.mark.parametrize("types", TYPES[:4], ids="_".join)
+@pytest.mark.parametrize("m", [30, 129, 256])
+def test_lora_few_rows_of_few_adapters_many_columns(srv, m, types):
+    """More than 3 2^20 outputs of at most 256 rows by few adapters, and fewer
+    outputs: integers, as in test_lora_integers_exact."""
+    import torch
+
+    announce(f"lora m={m} n=24600 {types}")
+    d = _lora_case(m, m, 136, 24600, 24, 3, *types, segs=[24000, 600], ints=True, ranks=True)
+    y = _run_lora(srv, d, [24000, 600])
+    torch.cuda.synchronize()
+    want, mag, _ = _lora_f64(d, [24000, 600])
+    assert float(mag.max()) < 2 ** 24
+    assert torch.equal(y.cpu(), want.to(_dt(types[2])))

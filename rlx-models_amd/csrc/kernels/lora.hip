@@ -20,12 +20,11 @@
 // What bounds it: many adapters at few rows, their bytes (64 rows of 48 adapters of
 // rank 64, 4096 -> 24576: v 13.4 us for 50 MB, y 41.6 for 157, 3.7 TB/s); one
 // adapter at one row, the two launches (4.0 and 6.6 us); prompts, base and y (4096
-// rows of 8 adapters, 4096 -> 24576: sort 7.6 us, v 26, y 137 for 503 MB with the
-// half of B that L2 no longer holds).  Tried on the last: tiles of 32 and 128 rows
-// (a tenth slower and more), 256, 512 and 2048 columns a workgroup (198, 170 and
-// 185 us of the call against 164 at 1024), B's sharers on one XCD (145 us for y against
-// 136: fewer columns at a time reach fewer memory channels), B's next rows not ahead
-// of their use and accesses past the caches (within 3%).
+// rows of 8 adapters, 4096 -> 24576: sort 8 us, v 31, y 134 for 458 MB, 3.4 TB/s).
+// Tried on y of the last: tiles of 16, 64 and 128 rows (217, 172 and 193 us of the call
+// against 173; 777 f32 rows of rank 128, 64 rows 41.8, 32 35.9), B's sharers on one XCD
+// (145 us against 136: fewer columns at a time reach fewer memory channels), B's
+// next rows not ahead of their use and accesses past the caches (within 3%).
 #include "common.hip.h"
 #include "lora_args.h"
 

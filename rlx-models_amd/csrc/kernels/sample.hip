@@ -533,7 +533,10 @@ RLXQ_DEV void smp_each(const rlxq_sample_args& a, int64_t row, int lead, const S
 // `each` goes through: by_rank the one of rank `need`, else the last whose sum
 // of the elements ahead is below `target`; base and base_n are what lies
 // ahead of all of them.  *incl: the sum down to the border.  Bins over the range
-// of what is left narrow it until a wave can sort it.
+// of what is left narrow it until a wave can sort it.  Their sums are fixed point,
+// in steps of 2^-42 (2^-50 of a list's) of the weight at the range's upper end: at
+// most 2^20 elements, so that they are off by 2^-23 of that weight at most,
+// however small it is beside the row's largest.
 template <class B, class E>
 RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShared& s, int n, E&& each, B&& bin_at, int b_lo, int b_hi, uint64_t lo,
                              uint64_t hi, double base, uint32_t base_n, uint32_t need, double target, double* incl) {
@@ -624,12 +627,14 @@ RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShare
       lo = g.lo, hi = g.hi;
     }
     const int bits = hi > lo ? 64 - __builtin_clzll(hi - lo) : 1, shift = bits > 9 ? bits - 9 : 0;
-    // (fixed point: kSmpList, or a whole row, of weights up to 1 at most 2^63)
-    const double one = listed ? 0x1p50 : 0x1p42, unit = listed ? 0x1p-50 : 0x1p-42;
+    // (kSmpList, or a whole row, of weights up to 1 at most 2^63)
+    const float end = of_key((uint32_t)(hi >> 32));
+    const double one = listed ? 0x1p50 : 0x1p42, unit = smp_w(r, end) / one;
     auto narrow = [&](uint64_t e) {
       if (!within(e)) return;
       const uint32_t d = (uint32_t)((hi - e) >> shift);
-      atomicAdd((unsigned long long*)&s.mass[d], (unsigned long long)(w_of(e) * one + 0.5));
+      const double w = exp_neg(((double)of_key((uint32_t)(e >> 32)) - (double)end) * r.inv_t);
+      atomicAdd((unsigned long long*)&s.mass[d], (unsigned long long)(w * one + 0.5));
       atomicAdd(&s.count[d], 1u);
     };
     if (listed)
@@ -964,7 +969,8 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
       auto highest = [&](int d) {
         float x = (anchor - (float)(d - 2)) / scale;
         x += fabsf(x) * 0x1p-20f;
-        return smp_comp(key_of(x < kMost ? x : kMost), 0);
+        x = x < kMost ? x : kMost;
+        return smp_comp(key_of(x < r.top ? x : r.top), 0);
       };
       double mass_k = all;
 #pragma unroll 1

@@ -1,0 +1,75 @@
+"""Sampling where a border or a token lies among weights far below the row's
+largest: rows of a few equal likely tokens over a floor of equal others, whose
+kept set follows from one division.
+
+With h likely tokens of weight 1 and a floor of weight w, top-p keeps the likely
+ones and the first r of the floor (by index), r the least whole number with h + r w
+>= p M, M the mass of what top-k leaves.  u = 1 takes the last kept token, so the
+token names the border itself.  A sum of f64 roundings moves (p M - h) / w by at
+most some 8 2^-53 M / w, so cases whose fraction lies within that (and 0.01) of a whole number
+are not taken."""
+import numpy as np
+import pytest
+
+from conftest import announce
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def srv(ctx):
+    import rlxq
+
+    return rlxq.Serving(ctx)
+
+
+def _row(v, heads, floor):
+    l = np.full(v, floor, np.float32)
+    l[heads] = 0.0
+    return l
+
+
+def _weight(floor, t=1.0):
+    return np.exp(np.longdouble(np.float32(floor)) / np.longdouble(np.float32(t)))
+
+
+def border(v, heads, floor, p, k=0, t=1.0):
+    """(the last kept token, the kept mass, the weight of a floor token)."""
+    h, w = len(heads), _weight(floor, t)
+    mass = h + ((k if 0 < k < v else v) - h) * w
+    x = (np.longdouble(np.float32(p)) * mass - h) / w
+    away = abs(x - np.rint(x))
+    assert x > 1 and away > 0.01 and away > 8 * 2.0 ** -53 * mass / w, (float(x), float(away))
+    r = int(np.ceil(x))
+    at = np.delete(np.arange(v), heads)[r - 1]   # the last one of the floor's
+    return max(int(at), max(heads)), h + r * w, w
+
+
+def _sample(srv, l, u, dt="f32", **kw):
+    import torch
+
+    rows = l.shape[0]
+    types = {"top_k": torch.int32}
+    l = torch.from_numpy(l).to({"f32": torch.float32, "bf16": torch.bfloat16}[dt]).cuda()
+    f = lambda x, d: torch.tensor(np.asarray(x), dtype=d).cuda().expand(rows).contiguous()   # noqa: E731
+    tok, pr = srv.sample(l, f(u, torch.float32), **{n: f(x, types.get(n, torch.float32)) for n, x in kw.items()})
+    torch.cuda.synchronize()
+    return tok.cpu().tolist(), pr.cpu().double().tolist()
+
+
+# (vocabulary, floor, top-p, top-k, temperature): more floor tokens than are listed
+FLOORS = [(151936, -23.0, 0.99999, 0, 1.0), (151936, -24.5, 1 - 2.0 ** -23, 0, 1.0),
+          (60001, -12.0, 0.999999, 0, 0.5), (151936, -23.0, 0.99999, 140001, 1.0),
+          (151936, -27.25, 1 - 2.0 ** -24, 150000, 1.0), (20003, -11.5, 0.999999, 0, 0.5)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("case", FLOORS, ids=lambda c: "_".join(map(str, c)))
+def test_border_in_a_floor_past_the_list(srv, case, dt):
+    v, floor, p, k, t = case
+    announce(f"sample floor {case} {dt}")
+    heads = [2]
+    want, mass, w = border(v, heads, floor, p, k, t)
+    tok, pr = _sample(srv, _row(v, heads, floor)[None], 1.0, dt, top_p=p, top_k=k, temperature=t)
+    assert tok == [want]
+    assert abs(pr[0] - float(w / mass)) <= 2.0 ** -23 * float(w / mass)

@@ -223,6 +223,15 @@ RLXQ_DEV float smp_bin(float v, float scale) { return floorf(v * scale); }
 RLXQ_DEV float smp_anchor(float bin) { return ceilf(bin * (1.0f / kGroup)) * kGroup; }
 RLXQ_DEV int smp_below(float anchor, float bin) { return (int)fminf(anchor - bin, (float)(kBins - 1)); }
 
+// Bin d of a chunk is summed in steps of 2^-(48 + s) of the chunk's largest weight,
+// s = d fine / 256 cut to a whole number: 23 / 256 is a little less than the 1 /
+// (16 ln 2) binary digits that weights fall by from bin to bin.  So each of a bin's
+// 4096 at most stays below 2^51 steps (up to 31 bins lie between the anchor and the
+// top, two more are rounding) and has 46 bits or more, in all bins but the last.
+// Where l / T is past 2^18 the bins' numbers round to more than that: 2^-48 in all.
+RLXQ_DEV int smp_fine_steps(float anchor) { return fabsf(anchor) < 0x1p22f ? 23 : 0; }
+RLXQ_DEV double smp_bin_mass(uint64_t m, int d, int fine) { return __builtin_ldexp((double)m, -(d * fine >> 8)); }
+
 // The elements of 16 bytes.
 template <int BF>
 RLXQ_DEV void smp_unpack(const uint4& q, float* v) {
@@ -271,7 +280,7 @@ RLXQ_DEV int smp_lead(const rlxq_sample_args& a, int64_t row) {
 // One chunk of smp_hist, its elements in v.
 template <int BF>
 RLXQ_DEV void smp_hist_chunk(const rlxq_sample_args& a, int64_t row, int c, int first, const float* v, float T, bool by_k,
-                             bool bins, unsigned long long* mass, uint32_t* count, const double* pow2, uint64_t* r64,
+                             bool bins, unsigned long long* mass, uint32_t* count, const double* pow2, double* rd,
                              uint32_t* r32, float* rf, int* at) {
   constexpr int N = BF ? 8 : 4, TH = kHistThreads, kPiece = RLXQ_SAMPLE_CHUNK / kHistWaves;
   const int t = threadIdx.x;
@@ -307,16 +316,18 @@ RLXQ_DEV void smp_hist_chunk(const rlxq_sample_args& a, int64_t row, int c, int 
     return;
   }
   const float scale = smp_bin_scale(T), anchor = smp_anchor(smp_bin(top, scale));
+  const int fine = smp_fine_steps(anchor);
   // w 2^48 = 2^(n / 32 + 48) 2^(f / 32), n the integer nearest x = 32 (l - top) / (T
   // ln 2), f = x - n: a table by n mod 32 (its entries times 2^48), and the Taylor
   // series of the second about 0, whose first term left out is below (ln 2 / 64)^6 /
-  // 720 = 3e-15.  n is read off the sum 1.5 2^52 + x.  What is 2^-69 of the top or
-  // less, masked tokens among it, counts as that, which rounds to 0.
+  // 720 = 3e-15.  n is read off the sum 1.5 2^52 + x.  What is e^-600 of the top or
+  // less, masked tokens among it, counts as that, which rounds to 0 in every bin and
+  // beside the top.
   constexpr double L = 0.6931471805599453 / 32, kRound = 0x1.8p52;
   const double top64 = (double)top, c32 = 32.0 / (0.6931471805599453 * (double)T);
-  const double least = -48.0 * (double)T;
+  const double least = -600.0 * (double)T;
   const bool wide = !(T < 1e36f);   // (nothing is that far below the top then: masked tokens by name)
-  double sum = 0x1p52;              // 2^52 + whole numbers: each addition rounds the weight to one
+  double sum = 0.0;
 #pragma unroll
   for (int half = 0; half < 2; half++) {
     double e[8], f2[8];
@@ -332,7 +343,7 @@ RLXQ_DEV void smp_hist_chunk(const rlxq_sample_args& a, int64_t row, int c, int 
       e[j] = __builtin_fma(e[j], f, L);
       e[j] = __builtin_fma(e[j], f, 1.0);
       const uint2 b = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pow2) + (n << 3 & 0xf8));
-      f2[j] = __hiloint2double((int)(b.y + ((n & ~31u) << 15)), (int)b.x);
+      f2[j] = __hiloint2double((int)(b.y + ((n & ~31u) << 15)), (int)b.x);   // (an exponent of 1071 - 866 at least)
     }
     if (wide) {
 #pragma unroll
@@ -342,8 +353,9 @@ RLXQ_DEV void smp_hist_chunk(const rlxq_sample_args& a, int64_t row, int c, int 
     if (bins) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const uint64_t w = (uint64_t)__double_as_longlong(__builtin_fma(e[j], f2[j], 0x1p52)) & 0xfffffffffffffull;
         const int d = smp_below(anchor, smp_bin(v[8 * half + j], scale));
+        const double f = __hiloint2double(__double2hiint(f2[j]) + ((d * fine & ~255) << 12), __double2loint(f2[j]));
+        const uint64_t w = (uint64_t)__double_as_longlong(__builtin_fma(e[j], f, 0x1p52)) & 0xfffffffffffffull;
         atomicAdd(&mass[d], (unsigned long long)w);
         if (by_k && v[8 * half + j] > -__builtin_inff()) atomicAdd(&count[d], 1u);
       }
@@ -353,14 +365,13 @@ RLXQ_DEV void smp_hist_chunk(const rlxq_sample_args& a, int64_t row, int c, int 
     }
   }
   if (!bins) {
-    uint64_t all = (uint64_t)(sum - 0x1p52);
 #pragma unroll
-    for (int off = 32; off; off >>= 1) all += __shfl_xor(all, off, 64);
-    if ((t & 63) == 0) r64[t >> 6] = all;
+    for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if ((t & 63) == 0) rd[t >> 6] = sum;
     __syncthreads();
     if (t == 0) {
-      for (int w = 1; w < TH / 64; w++) all += r64[w];
-      head->best = best, head->mass = all, head->bad = 0;
+      for (int w = 1; w < TH / 64; w++) sum += rd[w];
+      head->best = best, head->mass = sum, head->bad = 0;
     }
     return;
   }
@@ -370,17 +381,17 @@ RLXQ_DEV void smp_hist_chunk(const rlxq_sample_args& a, int64_t row, int c, int 
   const uint32_t n0 = count[2 * t], n1 = count[2 * t + 1];
   reinterpret_cast<ulonglong2*>(masses)[t] = make_ulonglong2(m0, m1);
   if (by_k) reinterpret_cast<uint32_t*>(counts)[t] = n0 | n1 << 16;
-  uint64_t gm = m0 + m1;
+  double gm = smp_bin_mass(m0, 2 * t, fine) + smp_bin_mass(m1, 2 * t + 1, fine);
   uint32_t gn = n0 + n1;
 #pragma unroll
   for (int off = 8; off; off >>= 1) gm += __shfl_xor(gm, off, 64), gn += __shfl_xor(gn, off, 64);
   if ((t & 15) == 0) head->group_mass[t >> 4] = gm, head->group_count[t >> 4] = gn;
 #pragma unroll
   for (int off = 32; off >= 16; off >>= 1) gm += __shfl_xor(gm, off, 64), gn += __shfl_xor(gn, off, 64);
-  if ((t & 63) == 0) r64[t >> 6] = gm, r32[t >> 6] = gn;
+  if ((t & 63) == 0) rd[t >> 6] = gm, r32[t >> 6] = gn;
   __syncthreads();
   if (t == 0) {
-    for (int w = 1; w < TH / 64; w++) gm += r64[w], gn += r32[w];
+    for (int w = 1; w < TH / 64; w++) gm += rd[w], gn += r32[w];
     head->best = best, head->mass = gm, head->bad = 0, head->count = gn;
   }
 }
@@ -391,7 +402,7 @@ RLXQ_DEV void smp_hist(const rlxq_sample_args& a) {
   __shared__ unsigned long long mass[kBins];
   __shared__ uint32_t count[kBins];
   __shared__ double pow2[32];
-  __shared__ uint64_t r64[TH / 64];
+  __shared__ double rd[TH / 64];
   __shared__ uint32_t r32[TH / 64];
   __shared__ float rf[TH / 64];
   __shared__ int at;
@@ -429,16 +440,17 @@ RLXQ_DEV void smp_hist(const rlxq_sample_args& a) {
     }
     if (c + 1 < c1 && inside(first + RLXQ_SAMPLE_CHUNK)) fetch(first + RLXQ_SAMPLE_CHUNK);
     if (c > c0) __syncthreads();   // (the last one's LDS is read)
-    smp_hist_chunk<BF>(a, row, c, first, v, T, by_k, bins, mass, count, pow2, r64, r32, rf, &at);
+    smp_hist_chunk<BF>(a, row, c, first, v, T, by_k, bins, mass, count, pow2, rd, r32, rf, &at);
   }
 }
 
 struct SmpPick {
   double scale[kSmpChunks], kept[kSmpChunks];   // chunks: their weights' scale in the row; their kept mass
   unsigned long long add[kSmpChunks];           // kept weights of listed elements, in 2^-50
-  uint64_t gmass[kSmpChunks][kGroups];          // the chunks' groups, as the first launch left them
+  double gmass[kSmpChunks][kGroups];            // the chunks' groups, as the first launch left them
   uint32_t gnum[kSmpChunks][kGroups];
   int shift[kSmpChunks];                        // groups from the row's top to the chunk's
+  int fine[kSmpChunks];                         // its bins' steps
   uint32_t some[kSmpChunks];                    // which bins of the group that smp_fine took hold something
   uint16_t flagged[kSmpChunks * kHistWaves];    // pieces to read again
   float tops[kSmpChunks][kHistWaves];           // their largest logits
@@ -481,7 +493,7 @@ RLXQ_DEV void smp_fine(const rlxq_sample_args& a, int64_t row, int j, bool by_k,
       const uint64_t any = __ballot(q[u] != 0 || qn[u] != 0 || (j == kGroups - 1 && b == kGroup - 1));
       if (c < C) {
         if (b == 0) g.some[c] = (uint32_t)(any >> (t & 32));
-        m += (double)q[u] * g.scale[c];
+        m += smp_bin_mass(q[u], (j - g.shift[c]) * kGroup + b, g.fine[c]) * g.scale[c];
         n += qn[u];
       }
     }
@@ -721,7 +733,8 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   const int64_t row = blockIdx.x;
   const int t = threadIdx.x, C = a.chunks, lane = t & 63, wave = t >> 6;
   const rlxq_sample_chunk* heads = a.heads + row * C;
-  uint64_t best = 0, my_best = 0, my_mass = 0;
+  uint64_t best = 0, my_best = 0;
+  double my_mass = 0.0;
   uint32_t bad = 0;
   if (t < C) my_best = heads[t].best, my_mass = heads[t].mass, bad = heads[t].bad;
   SmpRow r;
@@ -742,8 +755,10 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   if (t < C) {
     const float top = of_key((uint32_t)(my_best >> 32));
     g.scale[t] = my_best ? exp_neg(((double)top - (double)r.top) * r.inv_t) : 0.0;
-    g.shift[t] = my_best ? (int)fminf((anchor - smp_anchor(smp_bin(top, scale))) * (1.0f / kGroup), (float)kGroups) : kGroups;
-    g.kept[t] = (double)my_mass * 0x1p-48 * g.scale[t];
+    const float mine = smp_anchor(smp_bin(top, scale));
+    g.shift[t] = my_best ? (int)fminf((anchor - mine) * (1.0f / kGroup), (float)kGroups) : kGroups;
+    g.fine[t] = smp_fine_steps(mine);
+    g.kept[t] = my_mass * 0x1p-48 * g.scale[t];
     g.add[t] = 0;
     g.flag[t] = 0;
   }
@@ -759,7 +774,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
       for (int c = lane; c < C; c += 64) {
         const int jj = j - g.shift[c];
         if (j == kGroups - 1) m += g.kept[c], n += by_k ? heads[c].count : 0;
-        else if (jj >= 0) m += (double)g.gmass[c][jj] * 0x1p-48 * g.scale[c], n += g.gnum[c][jj];
+        else if (jj >= 0) m += g.gmass[c][jj] * 0x1p-48 * g.scale[c], n += g.gnum[c][jj];
       }
 #pragma unroll
       for (int off = 32; off; off >>= 1) m += __shfl_xor(m, off, 64), n += __shfl_xor(n, off, 64);
@@ -992,8 +1007,8 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
         const int c = c0 + (t >> 5), b = t & 31, jj = c < C ? d_lo / kGroup - g.shift[c] : -1;
         double m = 0.0;
         if (jj >= 0) {
-          if (b < d_lo % kGroup) m = (double)a.masses[(row * C + c) * kBins + jj * kGroup + b];
-          if (b < jj) m += (double)g.gmass[c][b];
+          if (b < d_lo % kGroup) m = smp_bin_mass(a.masses[(row * C + c) * kBins + jj * kGroup + b], jj * kGroup + b, g.fine[c]);
+          if (b < jj) m += g.gmass[c][b];
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) m += __shfl_xor(m, off, 32);

@@ -14,11 +14,11 @@
 /* What the first launch leaves of one chunk of one row. */
 typedef struct rlxq_sample_chunk {
   uint64_t best;      /* largest (key, falling index) of the chunk; 0: all masked */
-  uint64_t mass;      /* its weights over its own largest, in 2^-48            */
+  double mass;        /* its weights over its own largest, times 2^48          */
   uint32_t bad;       /* holds a NaN or +inf                                   */
   uint32_t count;     /* elements that are not masked (rows with top_k)        */
   float tops[4];      /* the largest logit of each quarter                     */
-  uint64_t group_mass[RLXQ_SAMPLE_GROUPS];    /* (rows with a border)          */
+  double group_mass[RLXQ_SAMPLE_GROUPS];      /* as mass (rows with a border)  */
   uint32_t group_count[RLXQ_SAMPLE_GROUPS];   /* (rows with top_k)             */
 } rlxq_sample_chunk;
 
@@ -35,7 +35,7 @@ typedef struct rlxq_sample_args {
   int32_t V, bf16;
   int32_t chunks, per;       /* of a row; of a workgroup                      */
   rlxq_sample_chunk* heads;  /* [M, chunks]                                   */
-  uint64_t* masses;          /* [M, chunks, BINS]                             */
+  uint64_t* masses;          /* [M, chunks, BINS], each in steps of its own   */
   uint16_t* counts;          /* [M, chunks, BINS]                             */
 } rlxq_sample_args;
 

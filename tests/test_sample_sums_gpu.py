@@ -73,3 +73,47 @@ def test_border_in_a_floor_past_the_list(srv, case, dt):
     tok, pr = _sample(srv, _row(v, heads, floor)[None], 1.0, dt, top_p=p, top_k=k, temperature=t)
     assert tok == [want]
     assert abs(pr[0] - float(w / mass)) <= 2.0 ** -23 * float(w / mass)
+
+
+# (vocabulary, likely tokens, floor, top-p, top-k, temperature): the floor's share of a
+# chunk that holds a likely token counts; the last three rows are listed as a whole
+CHUNKS = [(60000, [2], -26.0, 1 - 2.0 ** -23, 0, 1.0),
+          (163840, [4096 * i + 7 for i in range(8)], -25.875, 1 - 2.0 ** -24, 0, 1.0),
+          (163840, [4096 * i + 7 for i in range(20)], -24.875, 1 - 2.0 ** -24, 0, 1.0),
+          (151936, [4096 * i + 4000 for i in range(12)], -25.25, 1 - 2.0 ** -24, 150001, 1.0),
+          (60001, [4096 * i + 100 for i in range(3)], -12.9375, 1 - 2.0 ** -24, 0, 0.5),
+          (8001, [2], -25.25, 1 - 2.0 ** -24, 0, 1.0), (8001, [2, 900], -24.75, 1 - 2.0 ** -24, 0, 1.0),
+          (8001, [2, 900], -24.75, 1 - 2.0 ** -24, 7900, 1.0)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("case", CHUNKS, ids=lambda c: f"{c[0]}_{len(c[1])}_{c[2]}_{c[3]}_{c[4]}")
+def test_border_in_a_floor_of_chunks_with_likely_tokens(srv, case, dt):
+    v, heads, floor, p, k, t = case
+    announce(f"sample chunks {case} {dt}")
+    want, mass, w = border(v, heads, floor, p, k, t)
+    assert want > max(heads)
+    tok, pr = _sample(srv, _row(v, heads, floor)[None], 1.0, dt, top_p=p, top_k=k, temperature=t)
+    assert tok == [want]
+    assert abs(pr[0] - float(w / mass)) <= 2.0 ** -23 * float(w / mass)
+
+
+# (vocabulary, floor, u): a likely token at 0 over a floor, no border at all
+TOKENS = [(1 << 20, -30.0, 1 - 2.0 ** -24), (60000, -26.0, 1 - 2.0 ** -23), (60000, -25.5, 1 - 2.0 ** -22),
+          (4000, -24.625, 1 - 2.0 ** -24), (151936, -23.0, 1 - 2.0 ** -18)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("case", TOKENS, ids=lambda c: "_".join(map(str, c)))
+def test_token_in_a_floor(srv, case, dt):
+    """u M lies in the floor: index i, the first with 1 + i w > u M."""
+    v, floor, u = case
+    announce(f"sample token {case} {dt}")
+    w = _weight(floor)
+    mass = 1 + (v - 1) * w
+    x = (np.longdouble(np.float32(u)) * mass - 1) / w
+    away = abs(x - np.rint(x))
+    assert 1 < x < v - 1 and away > 0.01 and away > 8 * 2.0 ** -53 * mass / w
+    tok, pr = _sample(srv, _row(v, [0], floor)[None], u, dt)
+    assert tok == [int(np.floor(x)) + 1]
+    assert abs(pr[0] - float(w / mass)) <= 2.0 ** -23 * float(w / mass)

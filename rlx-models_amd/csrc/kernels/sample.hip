@@ -446,11 +446,12 @@ RLXQ_DEV void smp_hist(const rlxq_sample_args& a) {
 
 struct SmpPick {
   double scale[kSmpChunks], kept[kSmpChunks];   // chunks: their weights' scale in the row; their kept mass
-  unsigned long long add[kSmpChunks];           // kept weights of listed elements, in 2^-50
+  unsigned long long add[kSmpChunks];           // kept weights of listed elements, in 2^-51 of the chunk's top
   double gmass[kSmpChunks][kGroups];            // the chunks' groups, as the first launch left them
   uint32_t gnum[kSmpChunks][kGroups];
   int shift[kSmpChunks];                        // groups from the row's top to the chunk's
   int fine[kSmpChunks];                         // its bins' steps
+  float top[kSmpChunks];                        // its largest logit
   uint32_t some[kSmpChunks];                    // which bins of the group that smp_fine took hold something
   uint16_t flagged[kSmpChunks * kHistWaves];    // pieces to read again
   float tops[kSmpChunks][kHistWaves];           // their largest logits
@@ -758,6 +759,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
     const float mine = smp_anchor(smp_bin(top, scale));
     g.shift[t] = my_best ? (int)fminf((anchor - mine) * (1.0f / kGroup), (float)kGroups) : kGroups;
     g.fine[t] = smp_fine_steps(mine);
+    g.top[t] = top;
     g.kept[t] = my_mass * 0x1p-48 * g.scale[t];
     g.add[t] = 0;
     g.flag[t] = 0;
@@ -1017,10 +1019,10 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
       auto add = [&](uint64_t e) {
         const float x = of_key((uint32_t)(e >> 32));
         if (e < border || bin_at(x) < d_lo) return;
-        const double w = smp_w(r, x);
-        if (w < r.min_w) return;
-        const int idx = (int)~(uint32_t)e;
-        atomicAdd(&g.add[(idx + lead) / RLXQ_SAMPLE_CHUNK], (unsigned long long)(w * 0x1p50 + 0.5));
+        if (by_q && smp_w(r, x) < r.min_w) return;
+        // (beside the chunk's largest: 4096 of up to 2^51)
+        const int c = ((int)~(uint32_t)e + lead) / RLXQ_SAMPLE_CHUNK;
+        atomicAdd(&g.add[c], (unsigned long long)(exp_neg(((double)x - (double)g.top[c]) * r.inv_t) * 0x1p51 + 0.5));
       };
       if (n <= kSmpList)
         for (int i = t; i < n; i += kSmpThreads) add(g.list[i]);
@@ -1030,7 +1032,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
     __syncthreads();
   }
   // the chunk, then the element
-  const double m = t < C ? g.kept[t] + (double)g.add[t] * 0x1p-50 : 0.0;
+  const double m = t < C ? g.kept[t] + (double)g.add[t] * 0x1p-51 * g.scale[t] : 0.0;
   double total;
   const double incl = smp_scan<double>(m, s.rd, &total);
   const double target = (double)r.u * total;

@@ -77,7 +77,7 @@ def test_border_in_a_floor_past_the_list(srv, case, dt):
 
 # (vocabulary, likely tokens, floor, top-p, top-k, temperature): the floor's share of a
 # chunk that holds a likely token counts; the last three rows are listed as a whole
-CHUNKS = [(60000, [2], -26.0, 1 - 2.0 ** -23, 0, 1.0),
+CHUNKS = [(1 << 20, [2], -30.0, 1 - 2.0 ** -24, 0, 1.0), (60000, [2], -26.0, 1 - 2.0 ** -23, 0, 1.0),
           (163840, [4096 * i + 7 for i in range(8)], -25.875, 1 - 2.0 ** -24, 0, 1.0),
           (163840, [4096 * i + 7 for i in range(20)], -24.875, 1 - 2.0 ** -24, 0, 1.0),
           (151936, [4096 * i + 4000 for i in range(12)], -25.25, 1 - 2.0 ** -24, 150001, 1.0),
@@ -117,3 +117,44 @@ def test_token_in_a_floor(srv, case, dt):
     tok, pr = _sample(srv, _row(v, [0], floor)[None], u, dt)
     assert tok == [int(np.floor(x)) + 1]
     assert abs(pr[0] - float(w / mass)) <= 2.0 ** -23 * float(w / mass)
+
+
+def _floor_token(v, floor, k, u):
+    """The token of u, from one likely token at 0 over the first k - 1 of a floor."""
+    w = _weight(floor)
+    mass = 1 + (k - 1) * w
+    x = (np.longdouble(np.float32(u)) * mass - 1) / w
+    away = abs(x - np.rint(x))
+    assert 1 < x < k - 1 and away > 0.01 and away > 8 * 2.0 ** -53 * mass / w
+    return int(np.floor(x)) + 1, float(w / mass)
+
+
+# (vocabulary, floor, top-k, u): what top-k keeps of a floor, the last row listed
+KEPT = [(163840, -27.0, 150001, 1 - 2.0 ** -24), (60000, -26.25, 59001, 1 - 2.0 ** -24), (163840, -25.625, 120000, 1 - 2.0 ** -23),
+        (8001, -25.25, 7000, 1 - 2.0 ** -24)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("case", KEPT, ids=lambda c: "_".join(map(str, c)))
+def test_token_among_a_floor_that_is_kept(srv, case, dt):
+    v, floor, k, u = case
+    announce(f"sample kept {case} {dt}")
+    want, share = _floor_token(v, floor, k, u)
+    tok, pr = _sample(srv, _row(v, [0], floor)[None], u, dt, top_k=k)
+    assert tok == [want] and abs(pr[0] - share) <= 2.0 ** -23 * share
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [3000, 9001, 40000, 151936])
+def test_least_u_takes_the_first_that_is_kept(srv, v, dt):
+    """However little it weighs: sums of what lies ahead of the likely token are not
+    lost.  Rows differ in the floor; top-k leaves one of it out, min-p nothing."""
+    announce(f"sample least u v={v} {dt}")
+    floors = [-20.0, -40.0, -60.0, -88.0, -300.0]
+    likely, l = v - 100, np.stack([_row(v, [v - 100], f) for f in floors])
+    p = 1 - 2.0 ** -24
+    for kw, kept in (({}, floors), ({"top_k": v - 1}, floors), ({"top_k": v - 1, "top_p": p}, [f for f in floors if v * _weight(f) > 1 - p]),
+                     ({"min_p": 1e-38}, [f for f in floors if _weight(f) >= 1e-38])):
+        for u in (0.0, -1.0, 1.5e-45):
+            tok, _ = _sample(srv, l, u, dt, **kw)
+            assert tok == [0 if f in kept and _weight(f) > u else likely for f in floors], (kw, u)

@@ -63,6 +63,10 @@ RLXQ_DEV float smp_ld(const rlxq_sample_args& a, int64_t row, int i) {
 }
 RLXQ_DEV double smp_w(const SmpRow& r, float v) { return exp_neg(((double)v - (double)r.top) * r.inv_t); }
 
+// What the token's sum has to exceed: u times the kept mass, or (u from 1 up) what
+// no sum does, so that the last kept token is taken whatever the sums round to.
+RLXQ_DEV double smp_target(const SmpRow& r, double total) { return r.u < 1.0f ? (double)r.u * total : __builtin_inf(); }
+
 // The border as one number: key above, falling index below.  An element is
 // kept if its own is not smaller.
 RLXQ_DEV uint64_t smp_comp(uint32_t key, uint32_t idx) { return (uint64_t)key << 32 | (uint32_t)~idx; }
@@ -116,8 +120,8 @@ RLXQ_DEV void smp_choose(const rlxq_sample_args& a, const SmpRow& r, int64_t row
   double all;
   const double incl = before + smp_scan<double>(m, s.rd, &all);
   if (total < 0.0) total = all;
-  const double target = (double)r.u * total;
-  // the first thread whose sum exceeds the target, else (rounding, or u = 1) the
+  const double target = smp_target(r, total);
+  // the first thread whose sum exceeds the target, else (rounding, or u from 1 up) the
   // last that keeps anything
   const int t = threadIdx.x, wave = t >> 6;
   const uint64_t some = __ballot(last >= 0), past = __ballot(m > 0.0 && incl > target);
@@ -1035,7 +1039,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   const double m = t < C ? g.kept[t] + (double)g.add[t] * 0x1p-51 * g.scale[t] : 0.0;
   double total;
   const double incl = smp_scan<double>(m, s.rd, &total);
-  const double target = (double)r.u * total;
+  const double target = smp_target(r, total);
   if (t == 0) s.found = 0x7fffffff, s.last = -1;
   __syncthreads();
   const uint64_t some = __ballot(m > 0.0), past = __ballot(m > 0.0 && incl > target);

@@ -158,3 +158,22 @@ def test_least_u_takes_the_first_that_is_kept(srv, v, dt):
         for u in (0.0, -1.0, 1.5e-45):
             tok, _ = _sample(srv, l, u, dt, **kw)
             assert tok == [0 if f in kept and _weight(f) > u else likely for f in floors], (kw, u)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [300, 5000, 50257, 151936])
+def test_u_from_1_up_takes_the_last_that_is_kept(srv, v, dt):
+    """However little it weighs beside what the sums round to."""
+    announce(f"sample last v={v} {dt}")
+    import torch
+
+    rng = np.random.default_rng(v)
+    l = (3 * rng.standard_normal((12, v))).astype(np.float32)
+    top = l.max(1, keepdims=True)
+    l[:, v - 3:] = top - 38   # 2^-54 of the largest
+    l[:, 1:2] = top - 45      # (what top-k of v - 1 leaves out)
+    rounded = torch.from_numpy(l).to({"f32": torch.float32, "bf16": torch.bfloat16}[dt]).float().numpy()
+    best = [int(max(np.argsort(-r, kind="stable")[:200])) for r in rounded]
+    for kw, want in (({}, [v - 1] * 12), ({"top_k": v - 1}, [v - 1] * 12), ({"min_p": 1e-18}, [v - 1] * 12), ({"top_k": 200}, best)):
+        for u in (1.0, 5.0, np.inf):
+            assert _sample(srv, l, u, dt, **kw)[0] == want, (kw, u)

@@ -18,9 +18,10 @@ namespace rlxq {
 
 // exp(x) for x <= 0: 2^n 2^f with n the integer nearest x / ln 2; 2^f by its
 // Taylor series about 0, whose first term left out is below (ln 2 / 2)^13 / 13! =
-// 2e-16.  exp(0) is exactly 1.
+// 2e-16.  exp(0) is exactly 1; below 2^-1022 the result has the bits that a
+// denormal leaves it, below 2^-1075 it is 0.
 RLXQ_DEV double exp_neg(double x) {
-  if (x < -700.0) return 0.0;
+  if (x < -746.0) return 0.0;
   const double t = x * 1.4426950408889634, n = __builtin_rint(t), f = (t - n) * 0.6931471805599453;
   double p = 1.0 / 479001600;
   p = __builtin_fma(p, f, 1.0 / 39916800);

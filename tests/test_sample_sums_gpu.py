@@ -177,3 +177,18 @@ def test_u_from_1_up_takes_the_last_that_is_kept(srv, v, dt):
     for kw, want in (({}, [v - 1] * 12), ({"top_k": v - 1}, [v - 1] * 12), ({"min_p": 1e-18}, [v - 1] * 12), ({"top_k": 200}, best)):
         for u in (1.0, 5.0, np.inf):
             assert _sample(srv, l, u, dt, **kw)[0] == want, (kw, u)
+
+
+@pytest.mark.parametrize("v", [300, 3000, 40000])
+def test_least_u_and_the_smallest_weights(srv, v):
+    """A weight counts as long as f64 has it, denormals among them: e^-745 is one,
+    e^-750 is 0."""
+    announce(f"sample smallest weights v={v}")
+    floors = [-690.0, -701.0, -720.0, -744.0, -750.0, -2000.0]
+    l = np.stack([_row(v, [v - 100], f) for f in floors])
+    for dt in ("f32", "bf16"):
+        for kw in ({}, {"top_k": v - 1}, {"temperature": 0.5}):
+            t, x = kw.get("temperature", 1.0), l if dt == "f32" else np.round(l / 4) * 4   # (bf16: multiples of 4)
+            first = [0 if np.exp(np.float64(f) / t) > 0 else v - 100 for f in x[:, 0]]
+            assert _sample(srv, x, 0.0, dt, **kw)[0] == first, kw
+            assert _sample(srv, x, 1.0, dt, **kw)[0] == [v - 1 - ("top_k" in kw) if f == 0 else v - 100 for f in first], kw

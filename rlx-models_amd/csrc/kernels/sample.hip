@@ -231,10 +231,10 @@ RLXQ_DEV int smp_below(float anchor, float bin) { return (int)fminf(anchor - bin
 // Bin d of a chunk is summed in steps of 2^-(48 + s) of the chunk's largest weight,
 // s = d fine / 256 cut to a whole number: 23 / 256 is a little less than the 1 /
 // (16 ln 2) binary digits that weights fall by from bin to bin.  So each of a bin's
-// 4096 at most stays below 2^51 steps (up to 31 bins lie between the anchor and the
-// top, two more are rounding) and has 46 bits or more, in all bins but the last.
-// Where l / T is past 2^18 the bins' numbers round to more than that: 2^-48 in all.
-RLXQ_DEV int smp_fine_steps(float anchor) { return fabsf(anchor) < 0x1p22f ? 23 : 0; }
+// 4096 at most stays below 2^52 steps (up to 31 bins lie between the anchor and the
+// top, nine more are rounding) and has 46 bits or more, in all bins but the last.
+// Where l / T is past 2^23 the bins' numbers round to more than that: 2^-48 in all.
+RLXQ_DEV int smp_fine_steps(float anchor) { return fabsf(anchor) < 0x1p27f ? 23 : 0; }
 RLXQ_DEV double smp_bin_mass(uint64_t m, int d, int fine) { return __builtin_ldexp((double)m, -(d * fine >> 8)); }
 
 // The elements of 16 bytes.

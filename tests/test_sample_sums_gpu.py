@@ -192,3 +192,19 @@ def test_least_u_and_the_smallest_weights(srv, v):
             first = [0 if np.exp(np.float64(f) / t) > 0 else v - 100 for f in x[:, 0]]
             assert _sample(srv, x, 0.0, dt, **kw)[0] == first, kw
             assert _sample(srv, x, 1.0, dt, **kw)[0] == [v - 1 - ("top_k" in kw) if f == 0 else v - 100 for f in first], kw
+
+
+# (vocabulary, likely tokens, floor, top-p, temperature, the likely tokens' logit)
+FAR = [(163840, [4096 * i + 7 for i in range(8)], -25.875, 1 - 2.0 ** -24, 1.0, 1e6), (60001, [4096 * i + 100 for i in range(3)], -26.0, 1 - 2.0 ** -24, 1.0, -8e6),
+       (60001, [4096 * i + 100 for i in range(3)], -12.875, 1 - 2.0 ** -24, 0.5, 2.0 ** 20),
+       (163840, [4096 * i + 7 for i in range(20)], -24.75, 1 - 2.0 ** -24, 1.0, 3e5), (8001, [2, 900], -24.75, 1 - 2.0 ** -24, 1.0, -1e6)]
+
+
+@pytest.mark.parametrize("case", FAR, ids=lambda c: f"{c[0]}_{len(c[1])}_{c[2]}_{c[5]}")
+def test_border_in_a_floor_of_rows_far_from_0(srv, case):
+    v, heads, floor, p, t, at = case
+    announce(f"sample far {case}")
+    want, _, _ = border(v, heads, floor, p, 0, t)
+    l = _row(v, heads, floor) + np.float32(at)
+    assert l[0] - np.float32(at) == floor
+    assert _sample(srv, l[None], 1.0, top_p=p, temperature=t)[0] == [want]

@@ -143,7 +143,7 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   if (many && (rc = run_kernel(ctx, "rlxq_lora_sort", 1, 1024, (size_t)(num_adapters + 1) * 4, &g, stream))) return rc;
   std::snprintf(name, sizeof name, "rlxq_lora_shrink_%s_%s_%s", kDt[xb], kDt[ab], size);
   if ((rc = run_kernel(ctx, name, shrink, 256, 0, &g, stream))) return rc;
-  const size_t pieces = ab && !yb ? 3 : 2;   // of v, a lane (lr_expand)
+  const size_t pieces = ab ? 3 : 2;   // of v, a lane (lr_expand)
   const int steps = rank <= 32 ? 1 : (rank <= 64 ? 2 : (rank <= 128 ? 4 : 8));
   std::snprintf(name, sizeof name, "rlxq_lora_expand_%s_%s_%s_s%d", kDt[ab], kDt[yb], size, steps);
   return run_kernel(ctx, name, expand, 256, (size_t)((rank + 31) / 32) * (many ? RLXQ_LORA_ROWS / 16 : 1) * pieces * 1024, &g, stream);

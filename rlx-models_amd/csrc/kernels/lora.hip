@@ -13,9 +13,8 @@
 // y's columns are dealt to the tiles so that a lane holds 16 neighbouring ones.
 //
 // Types: the bf16 MFMA, f32 x and A as three bf16 terms each (all of their bits).
-// v stays f32; against bf16 B it takes part as bf16 terms,
-// three (all of its bits) for f32 y, two (2^-17 of it at most left out) for bf16
-// y, whose own rounding is 2^-9.  Sums are f32, y is rounded once.
+// v stays f32; against bf16 B it takes part as three bf16 terms, all of its bits
+// (base may cancel what two would round).  Sums are f32, y is rounded once.
 //
 // What bounds it: many adapters at few rows, their bytes (64 rows of 48 adapters of
 // rank 64, 4096 -> 24576: v 13.4 us for 50 MB, y 41.6 for 157, 3.7 TB/s); one
@@ -247,19 +246,6 @@ RLXQ_DEV void lr_shrink(const rlxq_lora_args& a) {
   }
 }
 
-// bf16 terms of eight floats: what the terms before it leave, rounded.
-RLXQ_DEV uint4 lr_term(float* v) {
-  uint4 q;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&q);
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-    v[2 * j] -= __uint_as_float(w[j] << 16);
-    v[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
-  }
-  return q;
-}
-
 // The column that row p of tile q of a wave's 64 columns stands for: chosen so that
 // a lane's results (rows 4 g .. 4 g + 3 of every tile, g = lane / 16) make 16-byte
 // pieces, neighbouring ones in neighbouring g.  Piece u of a lane starts at column
@@ -281,7 +267,7 @@ RLXQ_DEV int lr_piece(int u, int g) {
 template <bool BB, bool YB, bool LIST, int STEPS>
 RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
   constexpr int FR = LIST ? kLrFrags : 1;
-  constexpr int NT = BB ? (YB ? 2 : 3) : 2;   // 16-byte pieces of v a lane and 32 k (f32: the eight floats)
+  constexpr int NT = BB ? 3 : 2;   // 16-byte pieces of v a lane and 32 k (f32: the eight floats)
   constexpr bool AHEAD = STEPS <= 2;
   constexpr int P = YB ? 2 : 4, ES = YB ? 2 : 4;   // pieces of a lane's 16 columns
   extern __shared__ uint4 lds[];              // [steps][FR][NT][64]
@@ -360,12 +346,17 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
       for (int j = 0; j < 8; j++) v[j] = r + j < rank ? v[j] * scale : 0.f;
     }
     uint4* d = lds + (s * FR + f) * NT * 64 + l;
+    LrFrag<false> whole;
+    whole.q[0] = __builtin_bit_cast(uint4, make_float4(v[0], v[1], v[2], v[3]));
+    whole.q[1] = __builtin_bit_cast(uint4, make_float4(v[4], v[5], v[6], v[7]));
     if constexpr (BB) {
+      uint4 term[3];
+      lr_cut(whole, term);
 #pragma unroll
-      for (int q = 0; q < NT; q++) d[q * 64] = lr_term(v);
+      for (int q = 0; q < NT; q++) d[q * 64] = term[q];
     } else {
-      d[0] = __builtin_bit_cast(uint4, make_float4(v[0], v[1], v[2], v[3]));
-      d[64] = __builtin_bit_cast(uint4, make_float4(v[4], v[5], v[6], v[7]));
+      d[0] = whole.q[0];
+      d[64] = whole.q[1];
     }
   }
   __syncthreads();

@@ -796,14 +796,15 @@ class Serving:
         a [adapters, segments * rank, k], b [adapters, n, rank]; segments: the
         widths of the column ranges of a fused projection, each with its own
         rank rows of a.  A row whose id is outside [0, adapters) is base's.
-        Returns y (allocated if not given, of base's dtype, else f32); y may be base."""
+        Returns y (allocated if not given, of base's dtype, without base of y_dtype or
+        f32); y may be base.  A y_dtype that is not y's or base's is an error."""
         c, acts = self.ctx, self._acts
         dev = c.device
         try:
             (m, k), (e, n, rank) = x.shape, b.shape
             segs = 1 if segments is None else len(segments)
             yt = y.dtype if y is not None else base.dtype if base is not None else y_dtype or self._f32
-            fit = (x.dtype in acts and a.dtype in acts and yt in acts and (segments is None or (segs and min(segments) >= 0
+            fit = (x.dtype in acts and a.dtype in acts and yt in acts and y_dtype in (None, yt) and (segments is None or (segs and min(segments) >= 0
                    and sum(segments) == n)) and _fits(x, x.dtype, (m, k), dev) and _fits(ids, self._i32, (m,), dev)
                    and _fits(a, a.dtype, (e, segs * rank, k), dev) and _fits(b, a.dtype, (e, n, rank), dev)
                    and _fits(ranks, self._i32, (e,), dev) and _fits(scales, self._f32, (e,), dev)
@@ -812,6 +813,8 @@ class Serving:
             fit = False
         if not fit:
             check_lora_matmul(x, ids, a, b, ranks=ranks, scales=scales, segments=segments, base=base, y=y, device=dev)
+            if y_dtype not in (None, yt):
+                raise ValueError(f"lora_matmul: y_dtype is {y_dtype}, {'y' if y is not None else 'base'} {yt}")
             if yt not in acts:
                 raise ValueError(f"lora_matmul: y_dtype {yt} is not one of {[str(d) for d in acts]}")
         if y is None:
@@ -832,7 +835,8 @@ class Serving:
         pre_weight); returns (h, y).  block or resid None: zero; gate [groups, h]
         or None; post_weight None: block as it is; pre_weight None: no y.  h has
         resid's dtype (f32 without resid) and may be written over resid
-        (sum=resid); y has y_dtype, or h's dtype."""
+        (sum=resid); y, if not given, has y_dtype, or h's dtype (given, a y_dtype that is
+        not y's is an error)."""
         c, acts = self.ctx, self._acts
         dev = c.device
         first = block if block is not None else resid
@@ -842,7 +846,7 @@ class Serving:
             yt = y.dtype if y is not None else y_dtype or st
             w = pre_weight if pre_weight is not None else post_weight
             wt = w.dtype if w is not None else self._f32
-            fit = (st in acts and yt in acts and wt in acts and first.dtype in acts
+            fit = (st in acts and yt in acts and wt in acts and first.dtype in acts and (y is None or y_dtype in (None, yt))
                    and (block is not None or (gate is None and post_weight is None)) and (y is None or pre_weight is not None)
                    and _fits(block, first.dtype, (rows, hidden), dev) and _fits(resid, st, (rows, hidden), dev)
                    and _fits(pre_weight, wt, (hidden,), dev) and _fits(post_weight, wt, (hidden,), dev)
@@ -854,6 +858,8 @@ class Serving:
         if not fit:
             check_residual_norm(block, resid, pre_weight=pre_weight, post_weight=post_weight, gate=gate, sum=sum, y=y,
                                 device=dev)
+            if y is not None and y_dtype not in (None, yt):
+                raise ValueError(f"residual_norm: y_dtype is {y_dtype}, y {yt}")
             if pre_weight is not None and yt not in acts:
                 raise ValueError(f"residual_norm: y_dtype {yt} is not one of {[str(d) for d in acts]}")
         if sum is None or (y is None and pre_weight is not None):

@@ -334,10 +334,11 @@ int rlxq_swiglu(rlxq_ctx* ctx, const void* gu, int gu_dtype, int64_t rows,
  * [num_adapters] int32 (clamped to [0, rank]; what a and b hold past them is
  * not used) or NULL: rank; scales [num_adapters] f32 or NULL: 1; base and y
  * [m, n] of y_dtype.  seg_ends: host array of segs (1 to 4) column ends, rising
- * to n; NULL with segs = 1.  v and the sums are f32; y is rounded once.  A row of
- * x that is not finite, or its adapter's a, b or scale, or a v that overflows,
- * leaves the row of y not finite (NaN also where the sum would be an infinity) and
- * the others alone.
+ * to n; NULL with segs = 1.  v and the sums are f32, v is multiplied by its scale
+ * ahead of b; y is rounded once.  A row of x that is not finite, or its adapter's a,
+ * b or scale, or a v (times its scale) past the largest float, leaves the row of y
+ * not finite (NaN also where the sum would be an infinity) and the others alone;
+ * with ranks[e] = 0 nothing of the adapter is used and y = base.
  * k % 8 == 0, rank % 8 == 0 and at most 256; m, k, n up to 2^24;
  * num_adapters up to 16384; x, a, b 16-byte aligned.  With m = 0 or n = 0
  * nothing is read or written. */
@@ -382,8 +383,12 @@ int rlxq_residual_norm(rlxq_ctx* ctx, const void* block, int block_dtype,
  * (or NaN) are off.  u below 0 counts as 0, from 1 up as just below 1.  A logit of
  * -inf masks its token.  A row with a NaN or +inf logit, nothing but -inf, or a
  * NaN temperature or u gets token -1 and probability NaN.  probs may be NULL.
- * The weights and sums are f64: the same call gives the same tokens.  vocab up to
- * 2^20.  With rows = 0 nothing is read or written. */
+ * Weights are f64, denormals among them; sums are f64, or count whole steps of 2^-42
+ * or less of the largest weight in them: the same call gives the same tokens, those
+ * of the definition in 64 bits unless a sum comes as near to what it is compared with
+ * as such roundings.  (Where l / T passes 2^23 the steps are 2^-48 of the largest of
+ * 4096 neighbouring logits' weights, whatever the others weigh.)  vocab up to 2^20.
+ * With rows = 0 nothing is read or written. */
 int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype,
                 int64_t rows, int64_t vocab, const float* temperature,
                 const int32_t* top_k, const float* top_p, const float* min_p,

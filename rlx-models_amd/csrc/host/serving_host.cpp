@@ -106,9 +106,11 @@ int rlxq_lora_matmul(rlxq_ctx* ctx, const void* x, int x_dtype, const int32_t* i
   const int64_t tiles = many ? m / RLXQ_LORA_ROWS + std::min<int64_t>(num_adapters + 1, m) : m;
   g.max_tiles = (int32_t)tiles;
   // v: slices of K until there is a workgroup a CU (few rows, whose workgroups are
-  // small: six), of 512 elements at least (4096 rows 4096 -> 24576, rank 64, two slices
-  // 168 us, four 173; 1500 f32 rows of rank 256, one slice 259, two 227); no more than eight,
-  // which every workgroup of y adds up (33 rows 12288 -> 4096, 24 slices 19.6, 8 17.4)
+  // small: six), of 512 elements at least; no more than eight, which every workgroup of y
+  // adds up (33 rows 12288 -> 4096, 24 slices 19.6, 8 17.4).  A call with 1, 2, 4 and 8
+  // slices: 4096 bf16 rows 4096 -> 24576 of rank 64 168 us, 173, 180, 193 (the rule: 1);
+  // 1500 f32 rows 4096 -> 4096 of rank 256 124, 121, 121, 138 (2); 777 of rank 128 55, 41,
+  // 34, 36 (6: 37); 300 bf16 rows 4096 -> 6144 of rank 16 32, 23, 19, 19 (8)
   const int64_t sr = segs * rank;
   g.jblocks = (int32_t)((sr + (many ? 63 : 15)) / (many ? 64 : 16));
   const int64_t rows_wgs = many ? (m + RLXQ_LORA_ROWS - 1) / RLXQ_LORA_ROWS : used;
@@ -256,8 +258,10 @@ int rlxq_sample(rlxq_ctx* ctx, const void* logits, int logits_dtype, int64_t row
   g.counts = reinterpret_cast<uint16_t*>(g.masses + batch * g.chunks * RLXQ_SAMPLE_BINS);
   for (int64_t at = 0; at < rows; at += batch) {
     g.M = std::min(batch, rows - at);
-    // A chunk a workgroup, or up to three while there are six workgroups a CU (256
-    // rows of 128000: one 61 us, two 55, three 45, four 53, five 48).
+    // A chunk a workgroup, or up to three while there are six workgroups a CU.  It
+    // matters little; a call with 1, 2, 3, 4 and 6 chunks: 256 bf16 rows of 128000
+    // without borders 51 us, 44, 45, 44, 48 (the rule: 3); 1024 f32 rows of 50257 93, 92,
+    // 92, 100, 95 (3); 512 of 32000 40, 39, 41, 40, 46 (2); 64 of 151936 24, 25, 26, 26, 29 (1)
     g.per = (int32_t)std::max<int64_t>(1, std::min<int64_t>(3, g.M * g.chunks / (6 * cus)));
     g.logits = static_cast<const char*>(logits) + at * vocab * (bf ? 2 : 4);
     if (temperature) g.temperature = temperature + at;

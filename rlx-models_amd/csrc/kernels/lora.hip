@@ -17,9 +17,10 @@
 // (base may cancel what two would round).  Sums are f32, y is rounded once.
 //
 // What bounds it: many adapters at few rows, their bytes (64 rows of 48 adapters of
-// rank 64, 4096 -> 24576: v 13.4 us for 50 MB, y 41.6 for 157, 3.7 TB/s); one
-// adapter at one row, the two launches (4.0 and 6.6 us); prompts, base and y (4096
-// rows of 8 adapters, 4096 -> 24576: sort 8 us, v 31, y 134 for 458 MB, 3.4 TB/s).
+// rank 64, 4096 -> 24576: v 13.4 us for 50 MB, y 41.9 for 157, 3.7 TB/s); one
+// adapter at one row, the two launches (4.0 and 7.0 us); prompts, base and y (4096
+// rows of 8 adapters, 4096 -> 24576: sort 8 us, v 31, y 138 for 458 MB, 3.3 TB/s; 134
+// with two terms of v).
 // Tried on y of the last: tiles of 16, 64 and 128 rows (217, 172 and 193 us of the call
 // against 173; 777 f32 rows of rank 128, 64 rows 41.8, 32 35.9), B's sharers on one XCD
 // (145 us against 136: fewer columns at a time reach fewer memory channels), B's
@@ -260,10 +261,11 @@ RLXQ_DEV int lr_piece(int u, int g) {
 }
 
 // y of a tile's rows and a.cols columns of one segment, ranks up to 32 STEPS.  A
-// wave takes 64 columns at a time, their rows of B in registers (the next ones on
-// their way where two sets fit), and goes through the tile's rows 16 at a time
-// against them.  v lies in LDS as the MFMA takes it, made once for the workgroup
-// while the first of B and base are on their way.
+// wave takes 64 columns at a time, their rows of B in registers (the next ones asked
+// for where two sets fit), and goes through the tile's rows 16 at a time against
+// them.  v lies in LDS as the MFMA takes it, made once for the workgroup while the
+// first of B is on its way.  base is asked for in the step that adds it, after B's
+// next rows, and the build waits for both ahead of the step's first MFMA.
 template <bool BB, bool YB, bool LIST, int STEPS>
 RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
   constexpr int FR = LIST ? kLrFrags : 1;
@@ -329,7 +331,8 @@ RLXQ_DEV void lr_expand(const rlxq_lora_args& a) {
     if (row < count && r < rank) {
       const float* p = a.v + (int64_t)rows[row] * sr + seg * a.R + r;
       const int64_t step = a.M * sr;
-      // (slices in order, all on their way at once; past the last: the last, not added)
+      // (slices in order; past the last: the last, not added.  The build has a slice's
+      // loads behind the one before it: as many round trips as slices)
       float4 lo[RLXQ_LORA_SPLITS], hi[RLXQ_LORA_SPLITS];
 #pragma unroll
       for (int q = 0; q < RLXQ_LORA_SPLITS; q++) {

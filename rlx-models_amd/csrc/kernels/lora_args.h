@@ -32,7 +32,8 @@ typedef struct rlxq_lora_args {
   rlxq_lora_tile* tiles;   /* [max_tiles], unused ones with count 0           */
   int64_t M, K, N;
   int32_t R, E, S;
-  int32_t splits, kslice;  /* slices of K, a multiple of 32 each              */
+  int32_t splits, kslice;  /* slices of K, each a multiple of 128: four waves */
+                           /* of whole 32s                                    */
   int32_t jblocks;         /* shrink: workgroups over S * R                   */
   int32_t cols, cblocks;   /* expand: columns a workgroup, workgroups over N  */
   int32_t max_tiles;

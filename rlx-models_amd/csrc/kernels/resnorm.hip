@@ -138,7 +138,8 @@ RLXQ_DEV float rn_sum(float v, float (*red)[16], int& turn) {
 }
 
 // A row of whole 16-byte pieces a workgroup, in registers: CH pieces of eight a
-// thread, every load on its way before the first sum.
+// thread, all of block and resid on their way before the first sum; the weights and
+// the gate are loaded where they are used.
 template <int BB, int RB, int CH>
 RLXQ_DEV void rn_row(const rlxq_resnorm_args& a) {
   __shared__ float red[2][16];

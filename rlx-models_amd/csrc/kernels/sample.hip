@@ -196,8 +196,8 @@ RLXQ_DEV bool smp_row(const rlxq_sample_args& a, int64_t row, uint64_t best, uin
 //
 // The first reads the logits once: each workgroup a chunk of a row, in
 // registers, whose weights are taken relative to the chunk's own largest logit
-// and summed in fixed point, whole and by bins of l / T.  The bins of all chunks
-// lie on one grid, so the second launch adds them up (groups of 32 bins, then the
+// and summed, in f64 where the row has no border, else by bins of l / T in fixed
+// point.  The bins of all chunks lie on one grid, so the second launch adds them up (groups of 32 bins, then the
 // 32 of one group), finds the bin that each border falls into, and reads again
 // only the chunks that hold anything in those bins; what it finds there is
 // listed and settles the borders.  Where that is more than the list holds (rows as
@@ -205,9 +205,10 @@ RLXQ_DEV bool smp_row(const rlxq_sample_args& a, int64_t row, uint64_t best, uin
 // border to what can be listed, and again for the kept mass.
 //
 // What bounds it: the first launch the vector unit and the loads' latency (256
-// rows of 128000 bf16, no borders: 45 us, 30 instructions an element, half of the
-// time issuing; 64 of 151936 f32, most of them with borders: 25, with the bins; 512
-// threads a chunk took a sixth more, and held to fewer registers it spilled); the
+// rows of 128000 bf16, a quarter of them with borders: 47 us, 30 instructions an
+// element, half of the time issuing; 64 of 151936 f32, most of them with borders: 25,
+// 23 of them with one step for all bins; 512 threads a chunk took a sixth more, and
+// held to fewer registers it spilled); the
 // second a row's chain of dependent steps on one CU: 19 us for one row of 151936
 // with top-k 50; a row with min-p and 42 pieces 22 (settings and heads 3, groups and
 // bins 6, the pieces 6, their list, the border and the token 7); up to 50 where a
@@ -468,9 +469,9 @@ struct SmpPick {
   uint64_t list[kSmpList];
   uint64_t few[64], lo, hi;
   double few_w[64], sorted_w[kSmpSort];
-  uint32_t n, n_few, n_flag, kept_n;
+  uint32_t n, n_few, n_flag;
   int bin;
-  double before, base, total;
+  double before, base;
   uint32_t base_n, bin_n;
 };
 

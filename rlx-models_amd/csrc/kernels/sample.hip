@@ -72,9 +72,10 @@ RLXQ_DEV double smp_target(const SmpRow& r, double total) { return r.u < 1.0f ? 
 // kept if its own is not smaller.
 RLXQ_DEV uint64_t smp_comp(uint32_t key, uint32_t idx) { return (uint64_t)key << 32 | (uint32_t)~idx; }
 
-// Inclusive prefix sums over the workgroup's threads in thread order, and the total.
+// Sums over the workgroup's threads in thread order: down to the thread, ahead of it
+// (summed by itself: the difference would lose it beside a large v), and of all.
 template <class T>
-RLXQ_DEV T smp_scan(T v, T* red, T* total) {
+RLXQ_DEV T smp_scan(T v, T* red, T* ahead, T* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -90,6 +91,8 @@ RLXQ_DEV T smp_scan(T v, T* red, T* total) {
     all += red[w];
   }
   *total = all;
+  const T o = __shfl_up(v, 1, 64);
+  *ahead = lane ? before + o : before;
   return before + v;
 }
 
@@ -118,8 +121,8 @@ RLXQ_DEV double smp_kept(const SmpRow& r, uint64_t border, float v, int i) {
 template <class F>
 RLXQ_DEV void smp_choose(const rlxq_sample_args& a, const SmpRow& r, int64_t row, double m, int last, double before,
                          double total, SmpShared& s, F&& at) {
-  double all;
-  const double incl = before + smp_scan<double>(m, s.rd, &all);
+  double all, ahead;
+  const double incl = before + smp_scan<double>(m, s.rd, &ahead, &all);
   if (total < 0.0) total = all;
   const double target = smp_target(r, total);
   // the first thread whose sum exceeds the target, else (rounding, or u from 1 up) the
@@ -142,7 +145,7 @@ RLXQ_DEV void smp_choose(const rlxq_sample_args& a, const SmpRow& r, int64_t row
       if (a.probs) a.probs[row] = __builtin_nanf("");
     }
   } else if (t == (who >= 0 ? who : end)) {
-    const int tok = who >= 0 ? at(incl - m, target) : last;
+    const int tok = who >= 0 ? at(before + ahead, target) : last;
     a.tokens[row] = tok;
     if (a.probs) a.probs[row] = (float)(smp_w(r, smp_ld(a, row, tok)) / total);
   }
@@ -663,10 +666,11 @@ RLXQ_DEV uint64_t smp_select(bool by_rank, const SmpRow& r, SmpPick& g, SmpShare
     __syncthreads();
     const uint32_t c = s.count[t];
     const double w = (double)s.mass[t] * unit;
-    double wt;
-    uint32_t ct;
-    const double ahead = base + smp_scan<double>(w, s.rd, &wt) - w;
-    const uint32_t ahead_n = smp_scan<uint32_t>(c, s.r32, &ct) - c;
+    double ahead, wt;
+    uint32_t ahead_n, ct;
+    smp_scan<double>(w, s.rd, &ahead, &wt);
+    smp_scan<uint32_t>(c, s.r32, &ahead_n, &ct);
+    ahead += base;
     const bool in = c && (by_rank ? base_n + ahead_n < need : ahead_n == 0 || ahead < target);
     // the last bin that starts ahead of the border
     const uint64_t which = __ballot(in);
@@ -705,11 +709,11 @@ RLXQ_DEV void smp_small(const rlxq_sample_args& a, const SmpRow& r, int64_t row,
   __syncthreads();
   const int k = r.k < n ? r.k : n;
   const double mine = t < k ? g.sorted_w[t] : 0.0;
-  double mass_k;
-  const double incl = smp_scan<double>(mine, s.rd, &mass_k);
+  double ahead, mass_k;
+  smp_scan<double>(mine, s.rd, &ahead, &mass_k);
   const double target = r.p < 1.0f ? (r.p > 0.0f ? (double)r.p * mass_k : 0.0) : __builtin_inf();
   // of K's in order: what starts ahead of P's border and is not below min-p
-  const bool keep = t < k && (t == 0 || (incl - mine < target && mine >= r.min_w));
+  const bool keep = t < k && (t == 0 || (ahead < target && mine >= r.min_w));
   const uint64_t which = __ballot(keep);
   if ((t & 63) == 0) s.r32[t >> 6] = (uint32_t)__popcll(which);
   __syncthreads();
@@ -1039,8 +1043,8 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   }
   // the chunk, then the element
   const double m = t < C ? g.kept[t] + (double)g.add[t] * 0x1p-51 * g.scale[t] : 0.0;
-  double total;
-  const double incl = smp_scan<double>(m, s.rd, &total);
+  double ahead, total;
+  const double incl = smp_scan<double>(m, s.rd, &ahead, &total);
   const double target = smp_target(r, total);
   if (t == 0) s.found = 0x7fffffff, s.last = -1;
   __syncthreads();
@@ -1049,7 +1053,7 @@ RLXQ_DEV void smp_pick(const rlxq_sample_args& a) {
   if (lane == 0 && past) atomicMin(&s.found, t + __builtin_ctzll(past));
   __syncthreads();
   const int c = s.found != 0x7fffffff ? s.found : (s.last > 0 ? s.last : 0);
-  if (t == c) g.before = incl - m;
+  if (t == c) g.before = ahead;
   __syncthreads();
   constexpr int kPer = RLXQ_SAMPLE_CHUNK / kSmpThreads;
   const int first = c * RLXQ_SAMPLE_CHUNK - lead;

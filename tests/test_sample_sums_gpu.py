@@ -208,3 +208,26 @@ def test_border_in_a_floor_of_rows_far_from_0(srv, case):
     l = _row(v, heads, floor) + np.float32(at)
     assert l[0] - np.float32(at) == floor
     assert _sample(srv, l[None], 1.0, top_p=p, temperature=t)[0] == [want]
+
+
+# (vocabulary, the likely token, the token that u falls into, top-k): both in one chunk, most also in one thread's eight
+AHEAD = [(12288, 6000, 5000, 0), (12288, 5003, 5000, 12287), (60001, 39990, 39987, 0), (60001, 39990, 37001, 60000),
+         (300, 250, 120, 299), (300, 122, 120, 250), (4000, 498, 497, 500)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("case", AHEAD, ids=lambda c: "_".join(map(str, c)))
+def test_u_ahead_of_a_likely_token(srv, case, dt):
+    """What lies ahead of a likely token by index is summed by itself: u M in a floor of
+    2^-58 to 2^-130 of it, index i the first with (i + 1) w > u M."""
+    v, likely, token, k = case
+    announce(f"sample ahead {case} {dt}")
+    for floor in (-40.0, -58.0, -80.0):
+        w = _weight(floor)
+        mass = 1 + ((k if k else v) - 1) * w
+        u = np.float32((token + 0.5) * w / mass)
+        x = np.longdouble(u) * mass / w
+        assert abs(x - np.rint(x)) > 0.3 and int(x) == token
+        tok, pr = _sample(srv, _row(v, [likely], floor)[None], u, dt, top_k=k)
+        assert tok == [token], floor
+        assert abs(pr[0] - float(w / mass)) <= 2.0 ** -23 * float(w / mass) + 1e-45

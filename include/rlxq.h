@@ -34,6 +34,9 @@
  *     under stream capture must not need growth (the
  *     allocation fails under global capture): size the stream's scratch
  *     first with rlxq_reserve_workspace, or run the call once uncaptured.
+ *     A graph's calls use the scratch of the stream that they were captured
+ *     on, wherever it is replayed: two graphs captured on one stream, or such
+ *     a graph and calls on that stream, must not run at the same time.
  *     The MoE combine fused into the down launch (when selected) also
  *     takes 64 KB of per-stream counters, zeroed once when first used (or
  *     by rlxq_reserve_workspace) and left at zero by every call.
